@@ -154,6 +154,112 @@ int qwen2_cached_attention(const void* q, const void* k, const void* v, const vo
                            void* out, int64_t batch, int64_t length, int64_t past, int64_t num_heads,
                            int64_t num_kv_heads, int64_t head_dim, float scale, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged serving: batches of sequences whose cached keys and values lie in pages
+ * of one pool, several new positions per sequence and call.
+ *
+ * Rows (tokens) are packed: sequence b's new positions are rows cu_rows[b] ..
+ * cu_rows[b + 1] - 1, and they are the last ones of its lengths[b] cached
+ * positions: row i of n sits at position lengths[b] - n + i.  Position t of
+ * sequence b lies in page page_table[b][t / page_size], place t % page_size.
+ * cu_rows, lengths and page_table are read on the device; what they hold is
+ * bounded there: no access leaves the buffers whatever it is.
+ * ------------------------------------------------------------------------- */
+
+typedef struct qwen2_paged_cache {
+    void* k;                       /* key of position t, head h: k + page * k_page + h * k_head */
+    void* v;                       /*   + (t % page_size) * k_position; head_dim elements; v alike */
+    int64_t k_page, k_head, k_position; /* strides in elements, multiples of 8 (16 bytes) */
+    int64_t v_page, v_head, v_position;
+    int64_t num_pages;             /* in [1, 2^31) */
+    int64_t page_size;             /* a power of two in [16, 2^20] */
+    const int32_t* page_table;     /* [batch, table_width], rows table_stride apart */
+    int64_t table_width, table_stride;
+    const int32_t* cu_rows;        /* [batch + 1], not falling, from 0 */
+    const int32_t* lengths;        /* [batch], the new positions counted */
+    int64_t batch, kv_heads, head_dim;
+    int dtype;                     /* W4G64_DTYPE_BF16 or W4G64_DTYPE_F16: cache, q, k, v and outputs */
+} qwen2_paged_cache;
+
+/* Rows of a packed [rows, heads, head_dim] tensor: strides in elements. */
+typedef struct qwen2_rows {
+    void* data;                    /* 16-byte aligned */
+    int64_t row, head;             /* multiples of 8 */
+} qwen2_rows;
+
+/* Rotates the new positions' queries and keys and writes keys and values into
+ * their pages:
+ *   out[r, h]                      = R(p) q[r, h]
+ *   k of position p, head h        = R(p) k[r, h]
+ *   v of position p, head h        = v[r, h]
+ * where row r of sequence b has position p.  R(p) turns the first rotary_dim of
+ * the head_dim dimensions, in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
+ * with `interleaved`, by the angle p * inv_freq[i]:
+ *   (x, y) -> rotary_scale * (x cos - y sin, y cos + x sin);
+ * the angle in 64 bits, the rest in fp32, rounded once.  (Stretched contexts are
+ * a matter of inv_freq and rotary_scale.)  rotary_dim 0 turns nothing (inv_freq
+ * may then be NULL).  out may be q itself (same data and strides).
+ * A row whose page is not in the pool, or whose position is not in its table,
+ * is not written to the cache.  Rows behind the last sequence are left as they
+ * are, or zeroed in `out` with zero_rest.  Two rows of one call must not share
+ * a place in the cache (sequences may share pages, but not the ones written).
+ * head_dim and rotary_dim are multiples of 16, head_dim <= 256.
+ * Replaces: the rotary step and cache concatenation of QwenAttention.forward
+ *           (src/qwen_int4/model.py:17-31, :76-90) for packed sequences. */
+int qwen2_paged_append(const qwen2_paged_cache* cache, const qwen2_rows* q, const qwen2_rows* k, const qwen2_rows* v,
+                       const qwen2_rows* out, const float* inv_freq, int64_t rotary_dim, int interleaved,
+                       float rotary_scale, int64_t rows, int64_t heads, int zero_rest, void* stream);
+
+/* Attention of the new positions over the paged cache (theirs included: append
+ * first):
+ *   out[r, h] = softmax_t(scale * q[r, h] . k_t) v_t,   t = 0 .. p,
+ * p the row's position, query head h reading key/value head
+ * h / (heads / kv_heads); scores, softmax and sums in fp32, probabilities kept to
+ * 16 bits (two terms), rounded once.  The first shared_pages entries of every
+ * row of page_table must name the same pages (a prefix common to the batch): the
+ * first row's are read, once for all sequences.  A row without a position
+ * (lengths[b] too small) gives zeros; a row that reaches past its table, or to
+ * a page that is not in the pool, gives NaN.  Rows behind the last sequence are
+ * left as they are, or zeroed with zero_rest.  Keys and values at positions that
+ * a row does not see take no part, whatever they hold.
+ * head_dim is 64 or 128; heads a multiple of kv_heads; out must not overlap q.
+ * The workspace (16-byte aligned) holds fp32 partial results; nothing in it
+ * survives a call.  Calls sharing one must be ordered on one stream.
+ * Replaces: masking and attention of QwenAttention.forward
+ *           (src/qwen_int4/model.py:90-122) for packed sequences. */
+int64_t qwen2_paged_attention_workspace_bytes(const qwen2_paged_cache* cache, int64_t rows, int64_t heads,
+                                              int64_t shared_pages);
+int qwen2_paged_attention(const qwen2_paged_cache* cache, const qwen2_rows* q, const qwen2_rows* out, int64_t rows,
+                          int64_t heads, int64_t shared_pages, float scale, int zero_rest, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Which drafted tokens of a speculative step stand, and the token after them:
+ *   token i of sequence b stands iff all before it do and
+ *       uniforms[b, i] * q_i(x_i) < p_i(x_i),   x_i = draft_tokens[b, i],
+ *   n = accepted[b] tokens stand, of the k = draft_lengths[b] (NULL: drafts);
+ *   weights w = max(p_n - q_n, 0) for n < k, or p_k: the least v with
+ *       sum_{u <= v} w_u > uniforms[b, drafts] * sum w        is token n.
+ * p = target [batch, drafts + 1, vocab], q = draft [batch, drafts, vocab] of the
+ * same dtype (fp32, bf16 or fp16), or NULL: q_i is 1 at x_i and 0 elsewhere
+ * (tokens that no model drew).  Where max(p_n - q_n, 0) is zero everywhere the
+ * weights are p_n.  uniforms fp32 [batch, drafts + 1], in [0, 1) (in the sum's
+ * place a value outside counts as the nearest one inside, NaN as no choice).  A drafted id outside the
+ * vocabulary does not stand, and its q is 0 there.  All in 64 bits, so that a
+ * uniform next to a border falls where the definition says.
+ *   tokens[b, 0 .. n - 1] = the drafts that stand, tokens[b, n] the new token,
+ *   -1 behind it; tokens[b, n] = -1 where the weights' sum is zero, infinite or
+ *   NaN, or the uniform is NaN.  tokens int64 [batch, drafts + 1], accepted int32 [batch].
+ * target's and draft's rows are target_row (draft_row) elements apart, sequences
+ * target_batch (draft_batch).  The workspace (8-byte aligned) survives no call.
+ * Replaces: the greedy choice of a step (src/qwen_int4/generation.py:51) where
+ *           a step proposes several tokens. */
+int64_t qwen2_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
+int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target_row, const void* draft,
+                        int64_t draft_batch, int64_t draft_row, int dtype, const int64_t* draft_tokens,
+                        const int32_t* draft_lengths, const float* uniforms, int64_t* tokens, int32_t* accepted,
+                        int64_t batch, int64_t drafts, int64_t vocab, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* out[r, i] = silu(gate) * up in fp32, gate = gate_up[r, i], up = gate_up[r, I + i]
  * (bf16 inputs, the fused gate|up projection), silu(x) = x / (1 + exp(-x)).
  * Replaces: the SwiGLU product of QwenMLP.forward (src/qwen_int4/model.py:133-136). */

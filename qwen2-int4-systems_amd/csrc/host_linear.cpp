@@ -14,8 +14,7 @@
 //
 // What it measured: a call whose kernel takes 3 us cost 20.4 us of interpreter
 // and ctypes time one after the other (1 x 1536 x 1536), now 7.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
+#include "host_calls.h"
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
@@ -146,6 +145,10 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 PyMethodDef kMethods[] = {
     {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, "One W4G64 linear call; None: not of the plain form."},
+    {"paged_append", (PyCFunction)(void (*)(void))host_paged_append, METH_FASTCALL, "qwen_int4_hip.paged_append_hip"},
+    {"paged_attention", (PyCFunction)(void (*)(void))host_paged_attention, METH_FASTCALL,
+     "qwen_int4_hip.paged_attention_hip"},
+    {"verify_drafts", (PyCFunction)(void (*)(void))host_verify_drafts, METH_FASTCALL, "qwen_int4_hip.verify_drafts_hip"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

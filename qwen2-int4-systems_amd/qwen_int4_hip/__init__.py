@@ -17,6 +17,7 @@ from .kernels import (
     unpack_canonical_signed_int4_hip,
 )
 from .linear import QuantLinear
+from .paged import paged_append_hip, paged_attention_hip, verify_drafts_hip
 from .quantization import (
     PackingFormat,
     dequantize_groupwise,
@@ -42,6 +43,9 @@ __all__ = [
     "torch_w4g64_linear",
     "linear_canonical_w4g64_hip",
     "linear_kernel_name",
+    "paged_append_hip",
+    "paged_attention_hip",
+    "verify_drafts_hip",
     "unpack_canonical_signed_int4_hip",
     "validate_canonical_w4g64_inputs",
 ]

@@ -68,12 +68,33 @@ SIGNATURES = {
     "qwen2_prefill_attention_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "qwen2_prefill_attention": (_int, [_p] * 6 + [_i64] * 6 + [ctypes.c_float, _p, _i64, _p]),
     "qwen2_cached_attention": (_int, [_p] * 11 + [_i64] * 6 + [ctypes.c_float, _p]),
+    "qwen2_paged_append": (_int, [_p] * 6 + [_i64, _int, ctypes.c_float, _i64, _i64, _int, _p]),
+    "qwen2_paged_attention_workspace_bytes": (_i64, [_p, _i64, _i64, _i64]),
+    "qwen2_paged_attention": (_int, [_p] * 3 + [_i64] * 3 + [ctypes.c_float, _int, _p, _i64, _p]),
+    "qwen2_verify_drafts_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "qwen2_verify_drafts": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int] + [_p] * 5 + [_i64] * 3 + [_p, _i64, _p]),
     "qwen2_silu_mul": (_int, [_p, _p, _i64, _i64, _p]),
     "qwen2_lm_head_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "qwen2_lm_head": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p]),
     "qwen2_argmax_workspace_bytes": (_i64, [_i64, _i64]),
     "qwen2_argmax": (_int, [_p, _p, _i64, _i64, _p, _i64, _p]),
 }
+
+
+class PagedCache(ctypes.Structure):
+    """``qwen2_paged_cache`` of include/qwen2_decode.h."""
+
+    _fields_ = ([("k", _p), ("v", _p)] + [(name, _i64) for name in (
+        "k_page", "k_head", "k_position", "v_page", "v_head", "v_position", "num_pages", "page_size")]
+        + [("page_table", _p), ("table_width", _i64), ("table_stride", _i64), ("cu_rows", _p), ("lengths", _p)]
+        + [(name, _i64) for name in ("batch", "kv_heads", "head_dim")] + [("dtype", _int)])
+
+
+class Rows(ctypes.Structure):
+    """``qwen2_rows`` of include/qwen2_decode.h."""
+
+    _fields_ = [("data", _p), ("row", _i64), ("head", _i64)]
+
 
 _lock = threading.Lock()
 _library: ctypes.CDLL | None = None
@@ -124,6 +145,16 @@ def host_linear():
         else:
             _host_linear = _host.linear
     return _host_linear
+
+
+def host_module():
+    """The module ``_host``, for the operators that have no other route."""
+    load()
+    try:
+        from . import _host
+    except ImportError as e:
+        raise RuntimeError(f"HIP W4G64 host module is not usable ({e}); run __graft_entry__.build()") from e
+    return _host
 
 
 def check(status: int) -> None:

@@ -2,8 +2,8 @@
 and the CPython module ``_host.so`` that calls it.
 
 Compiles every ``csrc/*.hip`` translation unit with hipcc (in parallel) and
-links them into ``qwen_int4_hip/libw4g64_hip.so``; ``csrc/host_linear.cpp``
-(host code only) is compiled against torch's headers.  Always rebuilds: the
+links them into ``qwen_int4_hip/libw4g64_hip.so``; the ``csrc/host_*.cpp``
+(host code only) are compiled against torch's headers.  Always rebuilds: the
 caller (``__graft_entry__.build``) wants a fresh compile every time.
 
 ``build(timeline=True)`` compiles the same sources with ``-DW4G64_TIMELINE``
@@ -79,12 +79,12 @@ def build_host() -> Path:
            "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{root / 'include'}",
            f"-I{root / 'include/torch/csrc/api/include'}", f"-I{Path(hipcc()).resolve().parents[1] / 'include'}",
-           str(CSRC / "host_linear.cpp"), "-o", str(tmp), f"-L{root / 'lib'}",
+           *map(str, sorted(CSRC.glob("host_*.cpp"))), "-o", str(tmp), f"-L{root / 'lib'}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
            f"-L{PACKAGE_DIR}", f"-l:{LIBRARY.name}", "-Wl,-rpath,$ORIGIN"]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed for host_linear.cpp:\n{result.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed for the host module:\n{result.stderr}")
     os.replace(tmp, HOST_MODULE)
     return HOST_MODULE
 
