@@ -1,19 +1,20 @@
 // Verification of drafted tokens (qwen2_verify_drafts, include/qwen2_decode.h).
 //
-//   verify_sum_kernel   one workgroup per (sequence, 4096 entries of the
-//                       vocabulary): finds how many drafts stand (every
-//                       workgroup for itself: a few loads), then adds up its
-//                       entries' weights;
-//   verify_pick_kernel  one workgroup per sequence: the chunk in which the
+//   verify_sum_kernel   one wave per (sequence, span of 1024 entries of the
+//                       vocabulary): finds how many drafts stand (every wave
+//                       for itself: a few loads), then adds up its entries'
+//                       weights;
+//   verify_pick_kernel  one wave per sequence: the span in which the
 //                       running sum passes uniform * total, then the entry.
 //
 // Only one row of the target's (and the draft's) probabilities is read per
-// sequence.  A weight is a difference of two 24-bit numbers and the sums run
-// over the vocabulary, so they are held in 64 bits: the chosen entry is then
-// the definition's, not the summation order's.  Sums have one fixed order: 16
-// entries of a thread, the wave's threads pairwise, the waves, the chunks.
+// sequence, 16 bytes a lane.  A weight is a difference of two 24-bit numbers and
+// the sums run over the vocabulary, so they are held in 64 bits: the chosen
+// entry is then the definition's, not the summation order's.  Sums have one
+// fixed order.
 //
-// Bound by the rows' read from memory, and for few sequences by two launches.
+// Bound by the rows' read from memory, and for few sequences by its chain of
+// round trips (drafted id, its probabilities, the row, the launch between).
 #include <hip/hip_runtime.h>
 
 #include "qwen2_decode.h"
@@ -24,8 +25,9 @@ namespace w4g64 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;  // entries of a thread
-constexpr int kChunk = kThreads * kPer;
+constexpr int kWaves = kThreads / 64;
+constexpr int kSpan = 1024;   // entries of a sum, 16 of a lane
+constexpr int kMargin = 4096; // vocabularies end so far below 2^31
 
 struct VerifyArgs {
     const void* target;
@@ -36,8 +38,9 @@ struct VerifyArgs {
     const float* uniforms;
     int64_t* tokens;
     int32_t* accepted;
-    double* sums;  // [batch][chunks][2]: of the weights, and of the target alone
-    int drafts, vocab, chunks;
+    double* sums;      // [batch][spans][2]: of the weights, and of the target alone
+    int32_t* standing; // [batch]
+    int batch, drafts, vocab, spans;
 };
 
 template <int XK>
@@ -92,20 +95,53 @@ __device__ __forceinline__ Weights weights_of(const VerifyArgs& a, int b, int n,
     return w;
 }
 
-// The thread's entries chunk * 4096 + 16 tid .. + 15 (zero past the vocabulary).
-template <int XK>
-__device__ __forceinline__ void thread_weights(const Weights& w, int vocab, int chunk, int tid, double (&less)[kPer],
-                                               double (&plain)[kPer]) {
-    const int v0 = chunk * kChunk + kPer * tid;
+// Loads at an entry's alignment: one access, the target takes unaligned ones.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+// kCount (4 or 8) entries v .. of a row, zero past its end.
+template <int XK, int kCount>
+__device__ __forceinline__ void entries(const void* p, int64_t at, int v, int vocab, float (&x)[kCount]) {
+    if (v + kCount > vocab) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const int v = v0 + e;
-        const bool in = v < vocab;
-        const double p = in ? value<XK>(w.target, w.target_at + v) : 0.0;
-        double q = v == w.hot ? 1.0 : 0.0;
-        if (w.draft && in) q = value<XK>(w.draft, w.draft_at + v);
-        plain[e] = positive(p);
-        less[e] = positive(p - q);
+        for (int e = 0; e < kCount; ++e) x[e] = v + e < vocab ? (float)value<XK>(p, at + v + e) : 0.0f;
+    } else if constexpr (XK == kF32) {
+#pragma unroll
+        for (int i = 0; i < kCount; i += 4) {
+            // (bit cast as a whole: that of one element compiles to element 0 with this compiler)
+            const float4v w = __builtin_bit_cast(float4v, *(const u32x4_any*)((const float*)p + at + v + i));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] = w[e];
+        }
+    } else {
+        uint32_t w[kCount / 2];
+        if constexpr (kCount == 8) {
+            const u32x4 l = *(const u32x4_any*)((const uint16_t*)p + at + v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = l[e];
+        } else {
+            const u32x2 l = *(const u32x2_any*)((const uint16_t*)p + at + v);
+            w[0] = l[0], w[1] = l[1];
+        }
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            const uint16_t h = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+            x[e] = XK == kBF16 ? bf16_bits_to_float(h) : half_bits_to_float(h);
+        }
+    }
+}
+
+// The weights of entries whose probabilities are p (and q where w.draft), and
+// the target's alone.
+template <int kCount>
+__device__ __forceinline__ void weigh(const Weights& w, int v, const float (&p)[kCount], const float (&q)[kCount],
+                                      double (&less)[kCount], double (&plain)[kCount]) {
+#pragma unroll
+    for (int e = 0; e < kCount; ++e) {
+        const double x = (double)p[e];
+        const double y = w.draft ? (double)q[e] : (v + e == w.hot ? 1.0 : 0.0);
+        plain[e] = positive(x);
+        less[e] = positive(x - y);
     }
 }
 
@@ -117,144 +153,170 @@ __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
 
 template <int XK>
 __global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
-    __shared__ double part[2][kThreads / 64];
-    const int tid = threadIdx.x;
-    const int b = blockIdx.x / a.chunks;
-    const int chunk = blockIdx.x - b * a.chunks;
+    constexpr int kLoad = XK == kF32 ? 4 : 8;         // entries of a lane's load
+    constexpr int kLoads = kSpan / (64 * kLoad);
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (at >= (int64_t)a.batch * a.spans) return;
+    const int b = (int)(at / a.spans);
+    const int span = (int)(at - (int64_t)b * a.spans);
     int count;
-    const int n = standing<XK>(a, b, tid & 63, count);
+    const int n = standing<XK>(a, b, lane, count);
+    if (span == 0 && lane == 0) a.standing[b] = n;
     const Weights w = weights_of(a, b, n, count);
-    double less[kPer], plain[kPer];
-    thread_weights<XK>(w, a.vocab, chunk, tid, less, plain);
+    float p[kLoads][kLoad], q[kLoads][kLoad];
+    const int v0 = span * kSpan + kLoad * lane;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) entries<XK>(w.target, w.target_at, v0 + 64 * kLoad * i, a.vocab, p[i]);
+    if (w.draft)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) entries<XK>(w.draft, w.draft_at, v0 + 64 * kLoad * i, a.vocab, q[i]);
     double sl = 0.0, sp = 0.0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        sl += less[e];
-        sp += plain[e];
+    for (int i = 0; i < kLoads; ++i) {
+        double less[kLoad], plain[kLoad];
+        weigh(w, v0 + 64 * kLoad * i, p[i], q[i], less, plain);
+#pragma unroll
+        for (int e = 0; e < kLoad; ++e) {
+            sl += less[e];
+            sp += plain[e];
+        }
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         sl += shfl_xor_f64(sl, m);
         sp += shfl_xor_f64(sp, m);
     }
-    if ((tid & 63) == 0) {
-        part[0][tid >> 6] = sl;
-        part[1][tid >> 6] = sp;
-    }
-    __syncthreads();
-    if (tid < 2) {
-        double s = part[tid][0];
-        for (int i = 1; i < kThreads / 64; ++i) s += part[tid][i];
-        a.sums[2 * (int64_t)blockIdx.x + tid] = s;
+    if (lane == 0) {
+        a.sums[2 * at] = sl;
+        a.sums[2 * at + 1] = sp;
     }
 }
 
-// Sum of the values of the lower threads, in a workgroup of four waves.
-__device__ __forceinline__ double sum_before(double own, int tid, double* shared) {
-    const int lane = tid & 63;
-    double upto = own;
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, upto);
-        const uint32_t lo = __shfl_up((uint32_t)u, step), hi = __shfl_up((uint32_t)(u >> 32), step);
-        if (lane >= step) upto += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-    }
-    if (lane == 63) shared[tid >> 6] = upto;
-    __syncthreads();
-    double before = 0.0;
-    for (int i = 0; i < (tid >> 6); ++i) before += shared[i];
-    const uint64_t u = __builtin_bit_cast(uint64_t, upto);
-    const uint32_t lo = __shfl_up((uint32_t)u, 1), hi = __shfl_up((uint32_t)(u >> 32), 1);
-    if (lane) before += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-    return before;
+// Running sums over the wave's lanes, each lane's own value counted: within rows
+// of 16 lanes by shifts, then rows 1 and 3, then 2 and 3 take the last lane
+// before them.  (Lanes without a source receive 0.)
+template <int kControl, int kRows>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kControl, kRows, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kControl, kRows, 0xF, false);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double running_sum(double v) {
+    v += dpp_f64<0x111, 0xF>(v);
+    v += dpp_f64<0x112, 0xF>(v);
+    v += dpp_f64<0x114, 0xF>(v);
+    v += dpp_f64<0x118, 0xF>(v);
+    v += dpp_f64<0x142, 0xA>(v);
+    v += dpp_f64<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// One wave per sequence, no barrier: lane l has spans per l .. per l + per - 1,
+// then entries 16 l .. 16 l + 15 of the span.  (A workgroup of four waves over
+// LDS, with shuffles for its scans, took 10 us for any batch.)
 template <int XK>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ double totals[2];
-    __shared__ double shared[kThreads / 64];
-    __shared__ double base;
-    __shared__ int chosen_chunk, chosen, last;
-    const int tid = threadIdx.x;
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+    constexpr int kOwn = kSpan / 64;
+    const int lane = threadIdx.x;
     const int b = blockIdx.x;
-    int count;
-    const int n = standing<XK>(a, b, tid & 63, count);
-    const Weights w = weights_of(a, b, n, count);
-    const double* sums = a.sums + 2 * (int64_t)b * a.chunks;
-    if (tid < 2) {
-        double s = 0.0;
-        for (int c = 0; c < a.chunks; ++c) s += sums[2 * c + tid];
-        totals[tid] = s;
+    const double* sums = a.sums + 2 * (int64_t)b * a.spans;
+    const int per = (a.spans + 63) / 64;
+    const int first = per * lane;
+    double own[2] = {0.0, 0.0};
+    for (int i = 0; i < per && first + i < a.spans; ++i) {
+        own[0] += sums[2 * (first + i)];
+        own[1] += sums[2 * (first + i) + 1];
     }
-    if (tid == 0) chosen = 0x7FFFFFFF, last = -1;
-    __syncthreads();
-    // no entry where the draft falls short of the target: the target alone
-    const int which = totals[0] == 0.0;
-    const double total = totals[which];
+    int count = a.drafts;
+    if (a.draft_lengths) count = min(max(a.draft_lengths[b], 0), a.drafts);
+    const int n = a.standing[b];
     float u = a.uniforms[(int64_t)b * (a.drafts + 1) + a.drafts];
+    const Weights w = weights_of(a, b, n, count);
+    // the total; where the draft falls short of the target nowhere, the target's alone
+    int which = 0;
+    double end = running_sum(own[0]);
+    double total = lane_f64(end, 63);
+    if (total == 0.0) {
+        which = 1;
+        end = running_sum(own[1]);
+        total = lane_f64(end, 63);
+    }
     constexpr float kBelowOne = 0.999999940395355224609375f;  // 1 - 2^-24
     if (u > kBelowOne) u = kBelowOne;
     if (u < 0.0f) u = 0.0f;
     const double goal = (double)u * total;
-    const bool usable = total > 0.0 && total < __builtin_inf() && u == u;  // (uniform)
-    if (usable) {
-        if (tid == 0) {
-            double run = 0.0, at = 0.0;
-            int c = -1;  // the first chunk whose end passes the goal
-            for (int i = 0; i < a.chunks; ++i) {
-                const double next = run + sums[2 * i + which];
-                if (next > goal) {
-                    c = i, at = run;
-                    break;
-                }
-                run = next;
-            }
-            chosen_chunk = max(c, 0), base = at;  // (the last end is the total, past the goal)
+    int64_t token = -1;
+    if (total > 0.0 && total < __builtin_inf() && u == u) {  // (the same in every lane)
+        // the lane whose spans pass the goal (lane 63's end is the total), then the
+        // span: the last one of the lane's if its spans, added to what comes before
+        // them, stay a rounding below
+        const int at = __ffsll((unsigned long long)__ballot(end > goal)) - 1;
+        double run = at > 0 ? lane_f64(end, at - 1) : 0.0;
+        int span = min(per * at, a.spans - 1);
+        for (const int past = min(per * (at + 1), a.spans); span < past; ++span) {
+            const double next = run + sums[2 * span + which];
+            if (next > goal || span + 1 == past) break;
+            run = next;
         }
-        __syncthreads();
-        const int chunk = chosen_chunk;
-        double less[kPer], plain[kPer], own = 0.0;
-        thread_weights<XK>(w, a.vocab, chunk, tid, less, plain);
+        const int v0 = span * kSpan + kOwn * lane;
+        float p[kOwn / 4][4], q[kOwn / 4][4];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            less[e] = which ? plain[e] : less[e];
-            own += less[e];
-        }
-        double run = base + sum_before(own, tid, shared);
-        int found = 0x7FFFFFFF, some = -1;
+        for (int i = 0; i < kOwn / 4; ++i) entries<XK>(w.target, w.target_at, v0 + 4 * i, a.vocab, p[i]);
+        if (w.draft)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            run += less[e];
-            const int v = chunk * kChunk + kPer * tid + e;
-            if (less[e] > 0.0) {
-                some = v;
-                if (run > goal && found == 0x7FFFFFFF) found = v;
+            for (int i = 0; i < kOwn / 4; ++i) entries<XK>(w.draft, w.draft_at, v0 + 4 * i, a.vocab, q[i]);
+        double weight[kOwn], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < kOwn / 4; ++i) {
+            double less[4], plain[4];
+            weigh(w, v0 + 4 * i, p[i], q[i], less, plain);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                weight[4 * i + e] = which ? plain[e] : less[e];
+                mine += weight[4 * i + e];
             }
         }
-        if (found != 0x7FFFFFFF) atomicMin(&chosen, found);
-        if (some >= 0) atomicMax(&last, some);
-        __syncthreads();
+        const double upto = running_sum(mine);
+        const double before = __shfl_up(upto, 1);  // (by every lane: one that is off gives nothing)
+        double sum = run + (lane ? before : 0.0);
+        int found = -1, some = -1;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+            sum += weight[e];
+            if (weight[e] > 0.0) {
+                some = v0 + e;
+                if (sum > goal && found < 0) found = v0 + e;
+            }
+        }
+        // the first entry to pass; if all stay a rounding below, the last of any weight
+        const uint64_t passed = __ballot(found >= 0), any = __ballot(some >= 0);
+        if (passed) token = __shfl(found, __ffsll((unsigned long long)passed) - 1);
+        else if (any) token = __shfl(some, 63 - __clzll((unsigned long long)any));
     }
-    // (the chunk's sum passes the goal; where its entries, added in another order,
-    // stay a rounding below, it is the last of them)
-    const int64_t token = !usable ? -1 : (chosen != 0x7FFFFFFF ? chosen : last);
-    for (int i = tid; i <= a.drafts; i += kThreads) {
-        const int64_t at = (int64_t)b * (a.drafts + 1) + i;
-        a.tokens[at] = i < n ? a.draft_tokens[(int64_t)b * a.drafts + i] : (i == n ? token : -1);
+    for (int i = lane; i <= a.drafts; i += 64) {
+        const int64_t to = (int64_t)b * (a.drafts + 1) + i;
+        a.tokens[to] = i < n ? a.draft_tokens[(int64_t)b * a.drafts + i] : (i == n ? token : -1);
     }
-    if (tid == 0) a.accepted[b] = n;
+    if (lane == 0) a.accepted[b] = n;
 }
 
 template <int XK>
 hipError_t launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t stream) {
-    hipLaunchKernelGGL(verify_sum_kernel<XK>, dim3((unsigned)(batch * a.chunks)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(verify_sum_kernel<XK>, dim3((unsigned)((batch * a.spans + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(verify_pick_kernel<XK>, dim3((unsigned)batch), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(verify_pick_kernel<XK>, dim3((unsigned)batch), dim3(64), 0, stream, a);
     return hipGetLastError();
 }
 
-int64_t verify_chunks(int64_t vocab) { return (vocab + kChunk - 1) / kChunk; }
+int64_t verify_spans(int64_t vocab) { return (vocab + kSpan - 1) / kSpan; }
 
 }  // namespace
 }  // namespace w4g64
@@ -264,9 +326,9 @@ using namespace w4g64;
 extern "C" {
 
 int64_t qwen2_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
-    if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > 0x7FFFFFFF - kChunk || batch > 0x7FFFFFFF / verify_chunks(vocab))
+    if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > 0x7FFFFFFF - kMargin || batch > 0x7FFFFFFF / verify_spans(vocab))
         return 0;
-    return batch * verify_chunks(vocab) * 2 * (int64_t)sizeof(double);
+    return batch * verify_spans(vocab) * 2 * (int64_t)sizeof(double) + batch * (int64_t)sizeof(int32_t);
 }
 
 int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target_row, const void* draft,
@@ -276,7 +338,7 @@ int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target
                         void* stream) {
     if (dtype != W4G64_DTYPE_F32 && dtype != W4G64_DTYPE_BF16 && dtype != W4G64_DTYPE_F16)
         return set_error(W4G64_STATUS_INVALID_DTYPE, "verify_drafts probabilities must be fp32, bf16 or fp16, got code %d", dtype);
-    if (batch < 0 || drafts < 0 || drafts > 0xFFFF || vocab <= 0 || vocab > 0x7FFFFFFF - kChunk)
+    if (batch < 0 || drafts < 0 || drafts > 0xFFFF || vocab <= 0 || vocab > 0x7FFFFFFF - kMargin)
         return set_error(W4G64_STATUS_INVALID_VALUE,
                          "verify_drafts needs drafts in [0, 2^16) and vocab in [1, 2^31 - 4096), got %lld and %lld",
                          (long long)drafts, (long long)vocab);
@@ -292,7 +354,8 @@ int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target
         return set_error(W4G64_STATUS_WORKSPACE, "verify_drafts needs %lld workspace bytes, 8-byte aligned, got %lld",
                          (long long)need, (long long)(workspace ? workspace_bytes : 0));
     VerifyArgs a{target, draft, target_batch, target_row, draft_batch, draft_row, draft_tokens, draft_lengths, uniforms,
-                 tokens, accepted, (double*)workspace, (int)drafts, (int)vocab, (int)verify_chunks(vocab)};
+                 tokens, accepted, (double*)workspace, nullptr, (int)batch, (int)drafts, (int)vocab, (int)verify_spans(vocab)};
+    a.standing = (int32_t*)(a.sums + 2 * batch * a.spans);
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t err = dtype == W4G64_DTYPE_F32    ? launch_verify<kF32>(a, batch, s)
                            : dtype == W4G64_DTYPE_BF16 ? launch_verify<kBF16>(a, batch, s)
