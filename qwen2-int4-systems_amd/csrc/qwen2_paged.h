@@ -41,11 +41,11 @@ __host__ __device__ inline SequenceRows sequence_rows(const int32_t* cu_rows, co
 }
 
 // The page of a position, or -1: outside the table, or not a page of the pool.
+__host__ __device__ inline int checked_page(int page, int num_pages) { return page >= 0 && page < num_pages ? page : -1; }
 __host__ __device__ inline int page_of(const int32_t* table_row, int table_width, int page_shift, int num_pages,
                                        int64_t position) {
     if (position < 0 || (position >> page_shift) >= table_width) return -1;
-    const int page = table_row[position >> page_shift];
-    return page >= 0 && page < num_pages ? page : -1;
+    return checked_page(table_row[position >> page_shift], num_pages);
 }
 
 }  // namespace w4g64

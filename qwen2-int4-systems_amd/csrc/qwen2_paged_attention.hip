@@ -5,30 +5,41 @@
 // row m of a segment is token m / group, head m % group.  Two kinds of segment
 // share one launch:
 //   prefix    all rows of the batch against the shared pages of the table's
-//             first row: the keys are read once per 16 rows, not per sequence;
+//             first row: the keys are read once per tile of rows, not per sequence;
 //   own       one sequence's rows against the rest of its pages.
-// A workgroup takes 16 rows of a segment and one of several splits of its keys;
-// 32-key blocks are dealt round robin to the splits, then to the workgroup's
-// four waves, which work alone and meet in LDS at the end.  A second launch
-// joins the splits of both kinds.
+// A workgroup of four waves takes a tile of a segment's rows and one of several
+// splits of its keys, in one of two forms:
+//   narrow    16 rows.  The waves take different 32-key blocks, straight from
+//             memory into operands, two blocks in flight each, and meet in LDS at
+//             the end: for few rows, bound by the keys' and values' read.
+//   wide      128 rows, 32 of each wave.  The workgroup goes through 64-key tiles
+//             in LDS, the next one on its way (direct loads) while the waves work
+//             on this one: for many rows, bound by matrix and vector unit.
+// A second launch joins the splits of both kinds of segment.
 //
 // One pass over the keys: running maximum, sum and value sums per row.  MFMA
 // layout (v_mfma_f32_16x16x32; lane l = 16 q + j supplies row j of A and column
 // j of B with K slots 8 q .. 8 q + 7 and receives D[4 q + r][j]):
-//   scores  A = 16 keys, B = the 16 query rows: lane (j, q) gets row j's scores
-//           of keys 4 q + r;
+//   scores  A = 16 keys, B = 16 query rows: lane (j, q) gets row j's scores of
+//           keys 4 q + r;
 //   values  the lane's own 8 probabilities of a 32-key block are its 8 K slots;
-//           A = the values transposed: lane (j, q) loads kVd = D / 16 dimensions
+//           A = the values transposed: lane (j, q) reads kVd = D / 16 dimensions
 //           from kVd j of its 8 keys and pairs keys up by v_perm; dimension
 //           kVd j + dd is row j of the dd-th product.
 // A probability is kept as two 16-bit terms (16 bits or more of it): one term
 // alone would be as coarse as the output.
+//
+// The sums are rescaled only once a score passes their reference by kLazy units
+// of the base-2 exponent (from the floor on the first block); until then
+// probabilities reach 2^kLazy, which changes no relative rounding.
 //
 // Pages hold at least 16 positions, so that 16 aligned keys lie in one page and
 // the page's number is the wave's, not the lane's.  Every loaded address lies in
 // a page of the pool; what a block holds past the last visible key is replaced
 // by zeros, scores there by -inf.
 #include <math.h>
+
+#include <type_traits>
 
 #include "qwen2_attention.h"
 #include "qwen2_paged_device.h"
@@ -38,8 +49,10 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 16;   // rows of a workgroup
-constexpr int kBlock = 32;  // keys of a block
+constexpr int kNarrowRows = 16;  // rows of a workgroup
+constexpr int kWideRows = 128;
+constexpr int kBlock = 32;       // keys of a narrow block
+constexpr int kTileKeys = 64;    // keys of a wide tile
 constexpr int kMaxSplits = 64;
 
 struct PagedAttnArgs {
@@ -47,20 +60,50 @@ struct PagedAttnArgs {
     const uint16_t* q;
     uint16_t* out;
     int64_t q_row, q_head, out_row, out_head;
-    float* stats;     // [rows][heads][slots] (maximum, sum)
-    float* partials;  // [rows][heads][slots][D]
-    float scale2;     // scale * log2(e)
+    float* stats;         // [rows][heads][slots] (maximum, sum)
+    float* partials;      // [rows][heads][slots][D]
+    float scale2;         // |scale| * log2(e), above zero
+    uint32_t query_sign;  // both signs of a word of queries where the scale is negative
     int rows, heads, group;
-    int prefix;       // positions of the shared pages
+    int prefix;           // positions of the shared pages
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
+    int prefix_wide, own_wide;
     int zero_rest;
 };
 
-// Shift of the probabilities' exponent: fp16 ends at 2^-24, and a key far below
-// its row's maximum still counts if there are many; with 2^14 for the maximum
-// the terms reach down to 2^-38 of it.
+// Exponents of probabilities: fp16 ends at 2^-24 and at 2^16, and a key far below
+// its row's maximum still counts if there are many; with 2^11 for the reference
+// the terms reach down to 2^-35 of it.
 template <class E> constexpr float kProbShift = 0.0f;
-template <> constexpr float kProbShift<F16> = 14.0f;
+template <> constexpr float kProbShift<F16> = 11.0f;
+template <class E> constexpr float kLazy = 8.0f;
+template <> constexpr float kLazy<F16> = 4.0f;
+
+// An index array's entry at a wave's own index, through the scalar cache.
+__device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p + i);
+}
+
+// Over the 16 lanes of a row (quad swaps, half-row and row mirrors), and running
+// sums over the wave (shifts within rows, then their last lanes passed on).
+template <int kControl> __device__ __forceinline__ int dpp_row(int v) {
+    return __builtin_amdgcn_update_dpp(v, v, kControl, 0xF, 0xF, false);
+}
+__device__ __forceinline__ int row_max(int v) {
+    v = max(v, dpp_row<0xB1>(v));
+    v = max(v, dpp_row<0x4E>(v));
+    v = max(v, dpp_row<0x141>(v));
+    return max(v, dpp_row<0x140>(v));
+}
+__device__ __forceinline__ int running_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 
 __device__ __forceinline__ uint32_t keep_halves(uint32_t w, bool lo, bool hi) {
     return w & ((lo ? 0x0000FFFFu : 0u) | (hi ? 0xFFFF0000u : 0u));
@@ -69,31 +112,30 @@ template <class E> __device__ __forceinline__ uint32_t finite_halves(uint32_t w)
     return keep_halves(w, (w & E::kExponent) != E::kExponent, ((w >> 16) & E::kExponent) != E::kExponent);
 }
 
-// The sequence and place of own tile `tile` of 16 rows: the tiles of every
-// sequence counted up, 64 sequences at a time.  false: past the last one.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, int lane, int& sequence, int& local) {
+// The sequence, its rows and the place of own tile `tile` of `tile_rows` rows: the
+// tiles of every sequence counted up, 64 sequences at a time.  false: past the
+// last one.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile_rows, int tile, int lane, int& sequence,
+                                          int& local, SequenceRows& rows) {
     int before = 0;
     for (int base = 0; base < a.c.batch; base += 64) {
         const int i = base + lane;
-        int count = 0;
-        if (i < a.c.batch) {
-            const SequenceRows s = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
-            count = (int)(((int64_t)(s.end - s.begin) * a.group + kTile - 1) / kTile);
-        }
-        int upto = count;
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-            const int other = __shfl_up(upto, step);
-            if (lane >= step) upto += other;
-        }
-        const uint64_t past = __ballot(before + upto > tile);
+        SequenceRows s{0, 0, 0};
+        if (i < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
+        const int count = ((s.end - s.begin) * a.group + tile_rows - 1) / tile_rows;
+        const int upto = before + running_sum(count);
+        const uint64_t past = __ballot(upto > tile);
         if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
             sequence = base + at;
-            local = tile - before - __shfl(upto - count, at);
+            local = tile - __builtin_amdgcn_readlane(upto - count, at);
+            rows.begin = __builtin_amdgcn_readlane(s.begin, at);
+            rows.end = __builtin_amdgcn_readlane(s.end, at);
+            // (the length: at most 31 bits and a sign below the rows)
+            rows.first = (int64_t)__builtin_amdgcn_readlane((int)(s.first + (s.end - s.begin)), at) - (rows.end - rows.begin);
             return true;
         }
-        before += __shfl(upto, 63);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -109,270 +151,633 @@ __device__ __forceinline__ int sequence_by_halving(const int32_t* cu_rows, int b
     return lo;
 }
 
-template <class E, int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
-    constexpr int kVd = D / 16;           // dimensions of a value per lane
-    constexpr int kVw = kVd / 2;          // words of them
-    constexpr int kSteps = D / 32;        // K steps of a score
-    constexpr int kStride = D + 4;
-    typedef uint32_t vword __attribute__((ext_vector_type(kVw)));
-    __shared__ __attribute__((aligned(16))) float so[kWaves][kTile][kStride];
-    __shared__ float sm[kWaves][kTile];
-    __shared__ float sl[kWaves][kTile];
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int j = lane & 15;
-    const int q = lane >> 4;
+// What a workgroup works on.
+struct Segment {
+    bool shared;
+    bool sees_all;        // prefix: every row sees all of it
+    int split, splits, kvh, tile;
+    int first_token;
+    int count;            // rows
+    int64_t first;        // own: the first token's position
+    int key_lo;
+    int64_t key_end, held;
+    const int32_t* table;
+};
 
-    // rows behind the last sequence, where no second launch sees to them
-    if (a.slots == 1 && a.zero_rest) {
-        for (int r = max(a.c.cu_rows[a.c.batch], 0) + (int)blockIdx.x; r < a.rows; r += (int)gridDim.x)
-            for (int d = 8 * tid; d < a.heads * D; d += 8 * kThreads)
-                *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
-    }
-
-    // ---- which rows, which keys ----
+__device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, Segment& s) {
     const int prefix_work = a.prefix_tiles * a.c.kv_heads * a.prefix_splits;
-    const bool shared = (int)blockIdx.x < prefix_work;
-    const int work = shared ? (int)blockIdx.x : (int)blockIdx.x - prefix_work;
-    const int splits = shared ? a.prefix_splits : a.own_splits;
-    const int split = work % splits;
-    const int kvh = work / splits % a.c.kv_heads;
-    int tile = work / splits / a.c.kv_heads;
-    int first_token = 0, tokens = a.rows, sequence = 0;
-    if (!shared) {
-        int local;
-        if (!find_tile(a, tile, lane, sequence, local)) return;
-        sequence = __builtin_amdgcn_readfirstlane(sequence);
-        tile = __builtin_amdgcn_readfirstlane(local);
-        const SequenceRows s = sequence_rows(a.c.cu_rows, a.c.lengths, sequence, a.rows);
-        first_token = s.begin;
-        tokens = s.end - s.begin;
+    s.shared = (int)blockIdx.x < prefix_work;
+    const int work = s.shared ? (int)blockIdx.x : (int)blockIdx.x - prefix_work;
+    s.splits = s.shared ? a.prefix_splits : a.own_splits;
+    s.split = work % s.splits;
+    s.kvh = work / s.splits % a.c.kv_heads;
+    s.tile = work / s.splits / a.c.kv_heads;
+    s.held = (int64_t)a.c.table_width << a.c.page_shift;
+    s.sees_all = false;
+    if (s.shared) {
+        s.first_token = 0;
+        s.count = a.rows * a.group;
+        s.first = 0;
+        s.key_lo = 0;
+        s.key_end = a.prefix;
+        s.table = a.c.table;
+        // (the usual case, found out at once: all new positions lie behind the prefix)
+        bool behind = a.own_splits > 0;
+        for (int i = lane; i < a.c.batch; i += 64) {
+            const SequenceRows r = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
+            behind = behind && (r.end == r.begin || r.first >= a.prefix);
+        }
+        s.sees_all = __all(behind);
+        return true;
     }
-    const int64_t m = (int64_t)tile * kTile + j;  // this lane's row
-    const bool live = m < (int64_t)tokens * a.group;
-    const int64_t mc = live ? m : (int64_t)tokens * a.group - 1;
-    const int token = first_token + (int)(mc / a.group);
-    const int head = kvh * a.group + (int)(mc % a.group);
-    // the row's position; rows that no sequence has see nothing
-    int64_t position = -1;
-    bool known = live;
-    if (shared) {
-        const int b = sequence_by_halving(a.c.cu_rows, a.c.batch, token);
+    int sequence;
+    SequenceRows r;
+    const bool some = a.own_wide ? find_tile(a, kWideRows, s.tile, lane, sequence, s.tile, r)
+                                 : find_tile(a, kNarrowRows, s.tile, lane, sequence, s.tile, r);
+    if (!some) return false;
+    s.first_token = r.begin;
+    s.count = (r.end - r.begin) * a.group;
+    s.first = r.first;
+    s.key_lo = a.prefix;
+    s.key_end = s.held;
+    s.table = a.c.table + sequence * a.c.table_stride;
+    return true;
+}
+
+// A row of a segment, as a lane holds it.
+struct Row {
+    int token, head;
+    int limit;    // the last of the segment's keys that it sees, key_lo - 1 if none
+    bool live;    // there is such a row
+    bool beyond;  // it reaches past its table
+};
+
+__device__ __forceinline__ Row row_at(const PagedAttnArgs& a, const Segment& s, int m) {
+    Row r;
+    r.live = m < s.count;
+    m = r.live ? m : s.count - 1;
+    const int t = (uint32_t)m / (uint32_t)a.group;
+    r.token = s.first_token + t;
+    r.head = s.kvh * a.group + (m - t * a.group);
+    r.beyond = false;
+    if (s.sees_all) {
+        r.limit = r.live ? (int)s.key_end - 1 : s.key_lo - 1;
+        return r;
+    }
+    int64_t position = s.first + t;
+    bool known = r.live;
+    if (s.shared) {
+        const int b = sequence_by_halving(a.c.cu_rows, a.c.batch, r.token);
         known = known && b < a.c.batch;
         if (known) {
-            const SequenceRows s = sequence_rows(a.c.cu_rows, a.c.lengths, b, a.rows);
-            known = token >= s.begin && token < s.end;
-            position = s.first + (token - s.begin);
+            const SequenceRows q = sequence_rows(a.c.cu_rows, a.c.lengths, b, a.rows);
+            known = r.token >= q.begin && r.token < q.end;
+            position = q.first + (r.token - q.begin);
         }
-    } else {
-        const SequenceRows s = sequence_rows(a.c.cu_rows, a.c.lengths, sequence, a.rows);
-        position = s.first + (token - s.begin);
     }
-    if (!known) position = -1;
-    const int64_t held = (int64_t)a.c.table_width << a.c.page_shift;
-    const bool beyond = position >= held;  // reaches past its table
-    // last key of this segment that the row sees, below the segment's first if none
-    const int key_lo = shared ? 0 : a.prefix;
-    const int64_t key_end = shared ? a.prefix : held;
-    const int limit = (int)max(min(position, key_end - 1), (int64_t)(key_lo - 1));
-    int most = live ? limit : key_lo - 1, least = live ? limit : 0x7FFFFFFF;
-#pragma unroll
-    for (int step = 1; step < 16; step *= 2) {
-        most = max(most, __shfl_xor(most, step));
-        least = min(least, __shfl_xor(least, step));
-    }
-    most = __builtin_amdgcn_readfirstlane(most);
-    least = __builtin_amdgcn_readfirstlane(least);
-    const int blocks = (most - key_lo) / kBlock + (most >= key_lo ? 1 : 0);
+    if (!known) position = -1;  // (rows of no sequence see nothing)
+    r.beyond = position >= s.held;
+    r.limit = (int)max(min(position, s.key_end - 1), (int64_t)(s.key_lo - 1));
+    return r;
+}
 
-    const int32_t* table = a.c.table + (shared ? 0 : sequence * a.c.table_stride);
-    const uint16_t* kc = a.c.k + kvh * a.c.k_head;
-    const uint16_t* vc = a.c.v + kvh * a.c.v_head;
+// The page of a segment's 16 keys from t, the wave's own; keys that no row sees
+// (t > most): any page.
+__device__ __forceinline__ int segment_page(const PagedAttnArgs& a, const Segment& s, int t, int most) {
+    if (t > most) return 0;  // (most lies in the table)
+    return checked_page(scalar_load(s.table, t >> a.c.page_shift), a.c.num_pages);
+}
 
-    u32x4 qf[kSteps];
-    {
-        const uint16_t* from = a.q + token * a.q_row + head * a.q_head + 8 * q;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) qf[s] = *(const u32x4*)(from + 32 * s);
-    }
+// One lane's part of kTiles 16-row tiles: the running softmax and value sums of
+// row j of each, over the dimensions kVd (4 q + r) + dd.
+template <class E, int D, int kTiles>
+struct Attend {
+    static constexpr int kVd = D / 16;     // dimensions of a value per lane
+    static constexpr int kVw = kVd / 2;    // words of them
+    static constexpr int kSteps = D / 32;  // K steps of a score
+    typedef uint32_t vword __attribute__((ext_vector_type(kVw)));
 
-    float m_run = kScoreFloor, l_run = 0.0f;
-    bool seen = false;
-    float4v o[kVd];
-    u32x4 k[2][kSteps];
-    vword v[8];
-    int bad[2];
+    float m_run[kTiles], l_run[kTiles];
+    bool seen[kTiles];
+    float4v o[kTiles][kVd];
 
-    const int k_lane = j * (int)a.c.k_position + 8 * q;
-    const int v_lane = 4 * q * (int)a.c.v_position + kVd * j;
-    const int mask = (1 << a.c.page_shift) - 1;
-    auto load = [&](int block) {
+    __device__ __forceinline__ void start() {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int t = key_lo + block * kBlock + 16 * h;
-            // (16 keys that no row sees: any page)
-            int page = t > most ? 0 : page_of(table, a.c.table_width, a.c.page_shift, a.c.num_pages, t);
-            bad[h] = page < 0;
-            page = max(page, 0);
-            const uint16_t* kp = kc + page * a.c.k_page + (t & mask) * a.c.k_position;
-            const uint16_t* vp = vc + page * a.c.v_page + (t & mask) * a.c.v_position;
+        for (int u = 0; u < kTiles; ++u) {
+            m_run[u] = kScoreFloor, l_run[u] = 0.0f;
+            seen[u] = false;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) k[h][s] = *(const u32x4*)(kp + k_lane + 32 * s);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[4 * h + r] = *(const vword*)(vp + v_lane + r * (int)a.c.v_position);
+            for (int dd = 0; dd < kVd; ++dd) o[u][dd] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
-    };
-    auto compute = [&](int block, bool careful) {
-        const int t0 = key_lo + block * kBlock;
-        const bool edge = t0 + kBlock - 1 > least;
-        float s[8];
+    }
+
+    // Scores of kKeys keys from t0 (a lane's are t0 + 16 (e / 4) + 4 q + e % 4) become
+    // probabilities; the sums are rescaled where needed.
+    template <int kKeys>
+    __device__ __forceinline__ void soften(float (&s)[kTiles][kKeys / 4], u32x4 (&ph)[kTiles][kKeys / 32],
+                                           u32x4 (&pl)[kTiles][kKeys / 32], float scale2) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < kTiles; ++u) {
+            float top = s[u][0];
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u) acc = E::mfma(k[h][u], qf[u], acc);
+            for (int e = 1; e < kKeys / 4; ++e) top = fmaxf(top, s[u][e]);
+            const float mn = quarters_max(top) * scale2;
+            if (__any(mn - m_run[u] > kLazy<E>)) {
+                const float to = fmaxf(m_run[u], mn);
+                const float alpha = __builtin_amdgcn_exp2f(m_run[u] - to);  // (1 where it is another row's turn)
+                l_run[u] *= alpha;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[4 * h + r] = acc[r] * a.scale2;
-        }
-        if (edge) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int t = t0 + 16 * (e / 4) + 4 * q + e % 4;
-                if (t > limit) s[e] = -INFINITY;
-                if (t > most) v[e] = vword{};
+                for (int dd = 0; dd < kVd; ++dd) o[u][dd] *= alpha;
+                m_run[u] = to;
             }
+            const float ref = kProbShift<E> - m_run[u];
+#pragma unroll
+            for (int i = 0; i < kKeys / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][8 * i + 2 * e], scale2, ref));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][8 * i + 2 * e + 1], scale2, ref));
+                    l_run[u] += p0 + p1;
+                    ph[u][i][e] = E::pack(p0, p1);
+                    pl[u][i][e] = E::pack(p0 - E::lo(ph[u][i][e]), p1 - E::hi(ph[u][i][e]));
+                }
         }
-        seen = seen || t0 <= limit;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (bad[h] && t0 + 16 * h <= limit) l_run = __builtin_nanf("");
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e]);
-        const float to = fmaxf(m_run, quarters_max(top));
-        if (__any(to != m_run)) {
-            const float alpha = __builtin_amdgcn_exp2f(m_run - to);
-            l_run *= alpha;
-#pragma unroll
-            for (int dd = 0; dd < kVd; ++dd) o[dd] *= alpha;
-            m_run = to;
-        }
-        u32x4 ph, pl;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(s[2 * e] - to + kProbShift<E>);
-            const float p1 = __builtin_amdgcn_exp2f(s[2 * e + 1] - to + kProbShift<E>);
-            l_run += p0 + p1;
-            ph[e] = E::pack(p0, p1);
-            pl[e] = E::pack(p0 - E::lo(ph[e]), p1 - E::hi(ph[e]));
-        }
+    }
+
+    // The value sums of 32 keys from t0: v[e] is the lane's piece of key 16 (e / 4) + 4 q + e % 4.
+    template <bool kCareful>
+    __device__ __forceinline__ void gather(const vword (&v)[8], const u32x4 (&ph)[kTiles], const u32x4 (&pl)[kTiles],
+                                           const int (&limit)[kTiles], int t0, int j, int q) {
 #pragma unroll
         for (int dd = 0; dd < kVd; ++dd) {
             const uint32_t sel = (dd & 1) ? 0x07060302u : 0x05040100u;  // high or low halves
             u32x4 vt;
 #pragma unroll
             for (int e = 0; e < 4; ++e) vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][dd / 2], v[2 * e][dd / 2], sel);
-            if (!careful) {
-                o[dd] = E::mfma(vt, ph, o[dd]);
-                o[dd] = E::mfma(vt, pl, o[dd]);
-                continue;
-            }
-            // A value that is not finite must reach only the rows that see its key
-            // (0 * inf is NaN): the finite ones as always, the others column by
-            // column with what the column does not see at zero.
-            u32x4 plain, odd;
+            if constexpr (!kCareful) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                plain[e] = finite_halves<E>(vt[e]);
-                odd[e] = vt[e] & ~plain[e];
-            }
-            o[dd] = E::mfma(plain, ph, o[dd]);
-            o[dd] = E::mfma(plain, pl, o[dd]);
-            for (int c = 0; c < kTile; ++c) {
-                const int sees = __builtin_amdgcn_readlane(limit, c);
-                u32x4 part;
+                for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, ph[u], o[u][dd]);
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, pl[u], o[u][dd]);
+            } else {
+                // A value that is not finite must reach only the rows that see its key
+                // (0 * inf is NaN): the finite ones as always, the others column by
+                // column with what the column does not see at zero.
+                u32x4 plain, odd;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
-                    part[e] = keep_halves(odd[e], t <= sees, t + 1 <= sees);
+                    plain[e] = finite_halves<E>(vt[e]);
+                    odd[e] = vt[e] & ~plain[e];
                 }
-                const float4v more = E::mfma(part, ph, float4v{0.0f, 0.0f, 0.0f, 0.0f});
-                if (j == c) o[dd] += more;
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u) {
+                    o[u][dd] = E::mfma(plain, ph[u], o[u][dd]);
+                    o[u][dd] = E::mfma(plain, pl[u], o[u][dd]);
+                    for (int c = 0; c < 16; ++c) {
+                        const int sees = __builtin_amdgcn_readlane(limit[u], c);
+                        u32x4 part;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
+                            part[e] = keep_halves(odd[e], t <= sees, t + 1 <= sees);
+                        }
+                        const float4v more = E::mfma(part, ph[u], float4v{0.0f, 0.0f, 0.0f, 0.0f});
+                        if (j == c) o[u][dd] += more;
+                    }
+                }
             }
         }
-    };
-    // The second pass is for value sums that came out infinite or NaN.
-    for (int pass = 0; pass < 2; ++pass) {
-        m_run = kScoreFloor, l_run = 0.0f;
-        seen = false;
-#pragma unroll
-        for (int dd = 0; dd < kVd; ++dd) o[dd] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int block = split + splits * wave; block < blocks; block += splits * kWaves) {
-            load(block);
-            compute(block, pass != 0);
-        }
-        bool fine = true;
-#pragma unroll
-        for (int dd = 0; dd < kVd; ++dd)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[dd][r]) < INFINITY;
-        if (__all(fine)) break;
     }
 
-    // ---- the waves' results meet in LDS ----
-    float l_all = quarters_sum(l_run);
-    if (beyond && split == 0) {
-        l_all = __builtin_nanf("");
-        seen = true;
+    __device__ __forceinline__ bool finite() const {
+        bool fine = true;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+            for (int dd = 0; dd < kVd; ++dd)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[u][dd][r]) < INFINITY;
+        return fine;
     }
+
+    // Tile u's rows to their place: the output, or a slot of the partial results.
+    __device__ __forceinline__ void store(const PagedAttnArgs& a, const Segment& s, const Row& row, int u, float l,
+                                          float m, int q) const {
+        if (!row.live) return;
+        if (a.slots == 1) {
+            const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
+            uint16_t* to = a.out + row.token * a.out_row + row.head * a.out_head + 4 * kVd * q;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                uint32_t w[kVw];
 #pragma unroll
-        for (int dd = 0; dd < kVd; dd += 4)
-            *(float4v*)&so[wave][j][kVd * (4 * q + r) + dd] = float4v{o[dd][r], o[dd + 1][r], o[dd + 2][r], o[dd + 3][r]};
-    if (q == 0) {
-        sm[wave][j] = seen ? m_run : -INFINITY;  // -inf: no key seen
-        sl[wave][j] = l_all;
+                for (int i = 0; i < kVw; ++i) w[i] = E::pack(o[u][2 * i][r] * inv, o[u][2 * i + 1][r] * inv);
+                vword x;
+#pragma unroll
+                for (int i = 0; i < kVw; ++i) x[i] = w[i];
+                *(vword*)(to + kVd * r) = x;
+            }
+            return;
+        }
+        const int64_t slot = ((int64_t)row.token * a.heads + row.head) * a.slots + (s.shared ? 0 : a.prefix_splits) + s.split;
+        if (q == 0) *(float2v*)(a.stats + 2 * slot) = float2v{m, l};
+        if (m == -INFINITY) return;  // (the join does not read it)
+        float* to = a.partials + slot * D + 4 * kVd * q;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int dd = 0; dd < kVd; dd += 4)
+                *(float4v*)(to + kVd * r + dd) = float4v{o[u][dd][r], o[u][dd + 1][r], o[u][dd + 2][r], o[u][dd + 3][r]};
     }
-    __syncthreads();
-    // thread t: row t / 16, dimensions kVd (t % 16) ..
-    const int g = tid / 16;
-    const int d0 = kVd * (tid % 16);
-    const int64_t mg = (int64_t)tile * kTile + g;
-    if (mg >= (int64_t)tokens * a.group) return;
-    float top = sm[0][g];
+};
+
+// The queries of a row as MFMA operand pieces.
+template <int kSteps>
+__device__ __forceinline__ void load_queries(const PagedAttnArgs& a, const Row& row, int q, u32x4 (&qf)[kSteps]) {
+    const uint16_t* from = a.q + row.token * a.q_row + row.head * a.q_head + 8 * q;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][g]);
-    float sum[kVd] = {};
-    float l = 0.0f;
-    if (top > -INFINITY) {
+    for (int s = 0; s < kSteps; ++s) qf[s] = *(const u32x4*)(from + 32 * s) ^ a.query_sign;
+}
+
+// Least and largest limit over rows m0 .. m0 + count - 1 of a segment (those that
+// there are): an own segment's rise with the row; where a prefix is not all
+// seen, over the lanes of `row`, 16 rows.
+__device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s, const Row& row, int m0, int count,
+                                       int& least, int& most) {
+    const int last = min(m0 + count, s.count) - 1;
+    if (last < m0) {
+        least = 0x7FFFFFFF, most = s.key_lo - 1;
+    } else if (s.sees_all) {
+        least = most = (int)s.key_end - 1;
+    } else if (!s.shared) {
+        const int64_t first = s.first + (uint32_t)m0 / (uint32_t)a.group, end = s.first + (uint32_t)last / (uint32_t)a.group;
+        least = (int)max(min(first, s.key_end - 1), (int64_t)(s.key_lo - 1));
+        most = (int)max(min(end, s.key_end - 1), (int64_t)(s.key_lo - 1));
+    } else {
+        most = __builtin_amdgcn_readfirstlane(row_max(row.live ? row.limit : s.key_lo - 1));
+        least = -__builtin_amdgcn_readfirstlane(row_max(row.live ? -row.limit : -0x7FFFFFFF));
+    }
+}
+
+// ---- narrow ----
+
+template <class E, int D>
+struct KeyBlock {
+    u32x4 k[2][D / 32];                     // key 16 h + j, dimensions 32 s + 8 q ..
+    typename Attend<E, D, 1>::vword v[8];   // value of key 16 (e / 4) + 4 q + e % 4, dimensions kVd j ..
+    bool bad[2];
+};
+
+template <class E, int D>
+__device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s, int lane, int wave,
+                                       unsigned char* meet) {
+    typedef Attend<E, D, 1> A;
+    const int j = lane & 15;
+    const int q = lane >> 4;
+    const Row row = row_at(a, s, s.tile * kNarrowRows + j);
+    u32x4 qf[A::kSteps];
+    load_queries(a, row, q, qf);
+    int least, most;
+    limits(a, s, row, s.tile * kNarrowRows, kNarrowRows, least, most);
+    const int blocks = most >= s.key_lo ? (most - s.key_lo) / kBlock + 1 : 0;
+    const int stride = s.splits * kWaves;
+
+    const uint16_t* kc = a.c.k + s.kvh * a.c.k_head;
+    const uint16_t* vc = a.c.v + s.kvh * a.c.v_head;
+    const int k_lane = j * (int)a.c.k_position + 8 * q;
+    const int v_lane = 4 * q * (int)a.c.v_position + A::kVd * j;
+    const int mask = (1 << a.c.page_shift) - 1;
+    struct Pages {
+        int p[2];
+    };
+    auto look = [&](int block) {
+        const int t = s.key_lo + block * kBlock;
+        return Pages{{segment_page(a, s, t, most), segment_page(a, s, t + 16, most)}};
+    };
+    auto load = [&](KeyBlock<E, D>& b, int block, const Pages& pages) {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sm[w][g] - top);
-            if (f == 0.0f && sl[w][g] == sl[w][g]) continue;  // (no key, or none that counts; its sums may be infinite)
-            l = fmaf(sl[w][g], f, l);
+        for (int h = 0; h < 2; ++h) {
+            const int t = s.key_lo + block * kBlock + 16 * h;
+            b.bad[h] = pages.p[h] < 0;
+            const int64_t page = max(pages.p[h], 0);
+            const uint16_t* kp = kc + page * a.c.k_page + (t & mask) * a.c.k_position;
+            const uint16_t* vp = vc + page * a.c.v_page + (t & mask) * a.c.v_position;
 #pragma unroll
-            for (int i = 0; i < kVd; ++i) sum[i] = fmaf(so[w][g][d0 + i], f, sum[i]);
+            for (int i = 0; i < A::kSteps; ++i) b.k[h][i] = *(const u32x4*)(kp + k_lane + 32 * i);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                b.v[4 * h + r] = *(const typename A::vword*)(vp + v_lane + r * (int)a.c.v_position);
+        }
+    };
+    A state;
+    auto compute = [&](KeyBlock<E, D>& b, int block, auto careful) {
+        const int t0 = s.key_lo + block * kBlock;
+        float x[1][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < A::kSteps; ++i) acc = E::mfma(b.k[h][i], qf[i], acc);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[0][4 * h + r] = acc[r];
+        }
+        if (t0 + kBlock - 1 > least) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int t = t0 + 16 * (e / 4) + 4 * q + e % 4;
+                if (t > row.limit) x[0][e] = -INFINITY;
+                if (t > most) b.v[e] = typename A::vword{};
+            }
+        }
+        state.seen[0] = state.seen[0] || t0 <= row.limit;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (b.bad[h] && t0 + 16 * h <= row.limit) state.l_run[0] = __builtin_nanf("");
+        u32x4 ph[1][1], pl[1][1];
+        state.template soften<kBlock>(x, ph, pl, a.scale2);
+        const u32x4 h1[1] = {ph[0][0]}, l1[1] = {pl[0][0]};
+        const int limit[1] = {row.limit};
+        state.template gather<decltype(careful)::value>(b.v, h1, l1, limit, t0, j, q);
+    };
+    // Two blocks in flight, the pages of a third known.
+    state.start();
+    int block = s.split + s.splits * wave;
+    if (block < blocks) {
+        KeyBlock<E, D> buf[2];
+        load(buf[0], block, look(block));
+        Pages next = look(block + stride);
+        while (true) {
+            if (block + stride < blocks) load(buf[1], block + stride, next);
+            next = look(block + 2 * stride);
+            compute(buf[0], block, std::false_type{});
+            block += stride;
+            if (block >= blocks) break;
+            if (block + stride < blocks) load(buf[0], block + stride, next);
+            next = look(block + 2 * stride);
+            compute(buf[1], block, std::false_type{});
+            block += stride;
+            if (block >= blocks) break;
         }
     }
-    const int tg = first_token + (int)(mg / a.group);
-    const int hg = kvh * a.group + (int)(mg % a.group);
-    if (a.slots == 1) {
-        const float inv = top > -INFINITY ? 1.0f / l : 0.0f;
-        uint16_t* to = a.out + tg * a.out_row + hg * a.out_head + d0;
-#pragma unroll
-        for (int i = 0; i < kVd; i += 4)
-            *(u32x2*)(to + i) = u32x2{E::pack(sum[i] * inv, sum[i + 1] * inv), E::pack(sum[i + 2] * inv, sum[i + 3] * inv)};
-        return;
+    // (value sums that came out infinite or NaN: once more, with care)
+    if (!__all(state.finite())) {
+        state.start();
+        for (block = s.split + s.splits * wave; block < blocks; block += stride) {
+            KeyBlock<E, D> b;
+            load(b, block, look(block));
+            compute(b, block, std::true_type{});
+        }
     }
-    const int64_t slot = ((int64_t)tg * a.heads + hg) * a.slots + (shared ? split : a.prefix_splits * (a.prefix > 0) + split);
-    if (tid % 16 == 0) *(float2v*)(a.stats + 2 * slot) = float2v{top, l};
-    if (top == -INFINITY) return;  // (the join does not read it)
+
+    // ---- the waves' results meet in LDS: waves 2 and 3 give theirs to 0 and 1, then
+    // wave 1 to wave 0, which stores; a lane finds its own row and dimensions ----
+    float l = quarters_sum(state.l_run[0]);
+    float m = state.seen[0] ? state.m_run[0] : -INFINITY;  // -inf: no key seen
+    float4v(*so)[A::kVd][64] = (float4v(*)[A::kVd][64])meet;
+    float2v(*st)[64] = (float2v(*)[64])(meet + 2 * sizeof(float4v) * A::kVd * 64);
+    const int waves = min(kWaves, (blocks - s.split + s.splits - 1) / s.splits);  // those with a block
 #pragma unroll
-    for (int i = 0; i < kVd; i += 4)
-        *(float4v*)(a.partials + slot * D + d0 + i) = float4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
+    for (int half = 2; half > 0; half /= 2) {
+        if (waves <= half) continue;  // (the workgroup's)
+        if (half == 1) __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int dd = 0; dd < A::kVd; ++dd) so[wave - half][dd][lane] = state.o[0][dd];
+            st[wave - half][lane] = float2v{m, l};
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float2v other = st[wave][lane];
+            const float to = fmaxf(m, other[0]);
+            // (no key, or none that counts: factor zero, whatever its sums are; NaN is kept)
+            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
+            const float fo = other[0] > -INFINITY ? __builtin_amdgcn_exp2f(other[0] - to) : 0.0f;
+            const bool mine = f != 0.0f || l != l, its = fo != 0.0f || other[1] != other[1];
+            l = (mine ? l * f : 0.0f) + (its ? other[1] * fo : 0.0f);
+#pragma unroll
+            for (int dd = 0; dd < A::kVd; ++dd) {
+                const float4v x = so[wave][dd][lane];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float part = mine ? state.o[0][dd][r] * f : 0.0f;
+                    state.o[0][dd][r] = its ? fmaf(x[r], fo, part) : part;
+                }
+            }
+            m = to;
+        }
+    }
+    if (wave != 0) return;
+    if (row.beyond && s.split == 0) {
+        l = __builtin_nanf("");
+        m = fmaxf(m, kScoreFloor);
+    }
+    state.store(a, s, row, 0, l, m, q);
+}
+
+// ---- wide ----
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// All of this wave's loads into LDS and stores to it have landed, then all waves'.
+__device__ __forceinline__ void all_landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x7 << 4);  // vmcnt 0, lgkmcnt 0 (gfx9 encoding)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A tile's keys or values in LDS: 64 rows of D elements in 16-byte pieces, piece
+// c of row r in slot c ^ turn(r), so that reads of one piece of 16 rows meet
+// different banks.
+template <int D>
+struct Tile {
+    static constexpr int kPieces = D / 8;
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kBytes = kTileKeys * kRowBytes;
+    static constexpr int kRowsPerLoad = 64 / kPieces;  // rows that a wave's 16-byte load fills
+    static constexpr int kLoads = 16 / kRowsPerLoad;   // loads of 16 keys
+    static __device__ __forceinline__ int turn(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+};
+
+template <class E, int D>
+__device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
+                                     unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves]) {
+    typedef Attend<E, D, 2> A;
+    typedef Tile<D> T;
+    const int j = lane & 15;
+    const int q = lane >> 4;
+    const int m0 = s.tile * kWideRows + 32 * wave;
+    const Row row[2] = {row_at(a, s, m0 + j), row_at(a, s, m0 + 16 + j)};
+    const int limit[2] = {row[0].limit, row[1].limit};
+    u32x4 qf[2][A::kSteps];
+    load_queries(a, row[0], q, qf[0]);
+    load_queries(a, row[1], q, qf[1]);
+    // the wave's rows, then the workgroup's
+    int least, most, all_most, other;
+    limits(a, s, row[0], m0, 16, least, most);
+    limits(a, s, row[1], m0 + 16, 16, other, all_most);
+    least = min(least, other), most = max(most, all_most);
+    if (s.shared) all_most = (int)s.key_end - 1;
+    else limits(a, s, row[0], s.tile * kWideRows, kWideRows, other, all_most);
+    const int tiles = all_most >= s.key_lo ? (all_most - s.key_lo) / kTileKeys + 1 : 0;
+    const int per = (tiles + s.splits - 1) / s.splits;
+    const int begin = s.split * per;
+    const int end = min(tiles, begin + per);
+
+    // wave w brings keys 16 w .. 16 w + 15 of a tile
+    const uint16_t* kc = a.c.k + s.kvh * a.c.k_head;
+    const uint16_t* vc = a.c.v + s.kvh * a.c.v_head;
+    const int mask = (1 << a.c.page_shift) - 1;
+    int k_at[T::kLoads], v_at[T::kLoads];
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+        const int r = T::kRowsPerLoad * i + lane / T::kPieces;
+        const int piece = (lane % T::kPieces) ^ T::turn(r);
+        k_at[i] = 2 * r * (int)a.c.k_position + 16 * piece;
+        v_at[i] = 2 * r * (int)a.c.v_position + 16 * piece;
+    }
+    auto look = [&](int tile) { return segment_page(a, s, s.key_lo + tile * kTileKeys + 16 * wave, all_most); };
+    auto stage = [&](int tile, int page, unsigned char* keys, unsigned char* values, int* flags) {
+        const int t = s.key_lo + tile * kTileKeys + 16 * wave;
+        if (lane == 0) flags[wave] = page < 0;
+        const int64_t p = max(page, 0);
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(kc + p * a.c.k_page + (t & mask) * a.c.k_position), 0, (15 * (int)a.c.k_position + D) * 2, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(vc + p * a.c.v_page + (t & mask) * a.c.v_position), 0, (15 * (int)a.c.v_position + D) * 2, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr_t)(keys + 16 * wave * T::kRowBytes + 1024 * i), 16, k_at[i],
+                                                     0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(values + 16 * wave * T::kRowBytes + 1024 * i), 16,
+                                                     v_at[i], 0, 0, 0);
+    };
+    A state;
+    auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, const int* flags, auto careful) {
+        const int t0 = s.key_lo + tile * kTileKeys;
+        if (t0 > most) return;  // (the wave's)
+        float x[2][16];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            u32x4 kf[A::kSteps];
+#pragma unroll
+            for (int i = 0; i < A::kSteps; ++i)
+                kf[i] = *(const u32x4*)(keys + (16 * h + j) * T::kRowBytes + 16 * ((4 * i + q) ^ T::turn(j)));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < A::kSteps; ++i) acc = E::mfma(kf[i], qf[u][i], acc);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[u][4 * h + r] = acc[r];
+            }
+        }
+        const bool edge = t0 + kTileKeys - 1 > least;
+        if (edge) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (t0 + 16 * (e / 4) + 4 * q + e % 4 > limit[u]) x[u][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) state.seen[u] = state.seen[u] || t0 <= limit[u];
+        if (__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3])) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (flags[h] && t0 + 16 * h <= limit[u]) state.l_run[u] = __builtin_nanf("");
+        }
+        u32x4 ph[2][2], pl[2][2];
+        state.template soften<kTileKeys>(x, ph, pl, a.scale2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            typename A::vword v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = 32 * i + 16 * (e / 4) + 4 * q + e % 4;
+                if constexpr (D == 128)
+                    v[e] = *(const typename A::vword*)(values + r * T::kRowBytes + 16 * (j ^ T::turn(r)));
+                else
+                    v[e] = *(const typename A::vword*)(values + r * T::kRowBytes + 16 * ((j / 2) ^ T::turn(r)) + 8 * (j & 1));
+                if (edge && t0 + r > most) v[e] = typename A::vword{};
+            }
+            const u32x4 h2[2] = {ph[0][i], ph[1][i]}, l2[2] = {pl[0][i], pl[1][i]};
+            state.template gather<decltype(careful)::value>(v, h2, l2, limit, t0 + 32 * i, j, q);
+        }
+    };
+    // The next tile on its way while this one is worked on: its buffer was read
+    // before the barrier.
+    state.start();
+    if (begin < end) {
+        stage(begin, look(begin), k0, v0, bad[0]);
+        int next = look(begin + 1);
+        for (int tile = begin;;) {
+            all_landed();
+            if (tile + 1 < end) stage(tile + 1, next, k1, v1, bad[1]);
+            next = look(tile + 2);
+            compute(tile, k0, v0, bad[0], std::false_type{});
+            if (++tile >= end) break;
+            all_landed();
+            if (tile + 1 < end) stage(tile + 1, next, k0, v0, bad[0]);
+            next = look(tile + 2);
+            compute(tile, k1, v1, bad[1], std::false_type{});
+            if (++tile >= end) break;
+        }
+    }
+    // (value sums that came out infinite or NaN: once more, with care; all waves,
+    // for the tiles are brought by all)
+    if (__syncthreads_or(!state.finite())) {
+        state.start();
+        for (int tile = begin; tile < end; ++tile) {
+            stage(tile, look(tile), k0, v0, bad[0]);
+            all_landed();
+            compute(tile, k0, v0, bad[0], std::true_type{});
+            all_landed();
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        float l = quarters_sum(state.l_run[u]);
+        float m = state.seen[u] ? state.m_run[u] : -INFINITY;
+        if (row[u].beyond && s.split == 0) {
+            l = __builtin_nanf("");
+            m = fmaxf(m, kScoreFloor);
+        }
+        state.store(a, s, row[u], u, l, m, q);
+    }
+}
+
+// kWide: the prefix or the own segments go by wide tiles.
+template <class E, int D, bool kWide>
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
+    constexpr int kMeet = 2 * 64 * (D + 8);  // two narrow waves' sums and statistics
+    __shared__ __attribute__((aligned(16))) unsigned char k0[kMeet];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // rows behind the last sequence, where no second launch sees to them
+    if (a.slots == 1 && a.zero_rest) {
+        for (int r = max(a.c.cu_rows[a.c.batch], 0) + (int)blockIdx.x; r < a.rows; r += (int)gridDim.x)
+            for (int d = 8 * tid; d < a.heads * D; d += 8 * kThreads)
+                *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
+    }
+    Segment s;
+    if (!find_segment(a, lane, s)) return;
+    if constexpr (kWide) {
+        static_assert(kMeet >= Tile<D>::kBytes, "a tile's keys fit");
+        // (objects of their own: a read of one does not wait for loads into another)
+        __shared__ __attribute__((aligned(16))) unsigned char v0[Tile<D>::kBytes], k1[Tile<D>::kBytes], v1[Tile<D>::kBytes];
+        __shared__ int bad[2][kWaves];
+        if (s.shared ? a.prefix_wide : a.own_wide) {
+            wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad);
+            return;
+        }
+    }
+    narrow<E, D>(a, s, lane, wave, k0);
 }
 
 // One wave per (packed row, query head): lane l's D / 32 dimensions of the slots
@@ -380,11 +785,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnA
 template <class E, int D>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
     constexpr int kPer = D / 32;
+    typedef float fvec __attribute__((ext_vector_type(kPer)));
     const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (at >= (int64_t)a.rows * a.heads) return;
-    const int row = (int)(at / a.heads);
-    const int head = (int)(at - (int64_t)row * a.heads);
+    const int index = (int)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (index >= a.rows * a.heads) return;
+    const int row = (uint32_t)index / (uint32_t)a.heads;
+    const int head = index - row * a.heads;
+    const int64_t at = index;
     uint16_t* to = a.out + row * a.out_row + head * a.out_head;
     if (row >= a.c.cu_rows[a.c.batch]) {  // behind the last sequence
         if (a.zero_rest && lane < D / 8) *(u32x4*)(to + 8 * lane) = u32x4{0u, 0u, 0u, 0u};
@@ -398,14 +805,22 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
     const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
     const float l = wave_sum64(f != 0.0f || sum_l != sum_l ? sum_l * f : 0.0f);  // (NaN: a page that was not there)
     float sum[kPer] = {};
-    for (int i = 0; i < a.slots; i += 2) {
-        const int s = min(i + lane / 32, a.slots - 1);
-        float fs = __shfl(f, s);
-        if (i + lane / 32 >= a.slots) fs = 0.0f;
-        if (fs == 0.0f) continue;
-        const float* part = a.partials + (at * a.slots + s) * D + kPer * (lane % 32);
+    const float* part = a.partials + at * a.slots * D + kPer * (lane % 32);
+    const int half = lane / 32;
+    for (int first = 0; first < a.slots; first += 8) {  // eight slots' loads at once
+        fvec x[4];
+        float fs[4];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum[e] = fmaf(part[e], fs, sum[e]);
+        for (int i = 0; i < 4; ++i) {
+            const int slot = first + 2 * i + half;
+            fs[i] = __shfl(f, min(slot, 63));  // (0 past the slots)
+            x[i] = fvec{};
+            if (fs[i] != 0.0f) x[i] = *(const fvec*)(part + slot * D);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) sum[e] = fs[i] != 0.0f ? fmaf(x[i][e], fs[i], sum[e]) : sum[e];
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum[e] += __shfl_xor(sum[e], 32);
@@ -419,26 +834,32 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
 // How a call is cut up; the same from the same sizes, whatever the device holds.
 struct PagedPlan {
     int64_t prefix, prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
+    bool prefix_wide, own_wide;
 };
 
 PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t shared_pages) {
     PagedPlan p{};
     const int64_t group = heads / c.kv_heads;
+    const int64_t sequences = c.batch < rows ? c.batch : rows;
     p.prefix = shared_pages << c.page_shift;
     const int64_t own = ((int64_t)c.table_width - shared_pages) << c.page_shift;
-    auto splits = [&](int64_t workgroups, int64_t keys) {
-        const int64_t most = (keys + kBlock * kWaves - 1) / (kBlock * kWaves);  // a block per wave
+    auto splits = [&](int64_t workgroups, int64_t keys, int64_t least_keys) {
+        const int64_t most = (keys + least_keys - 1) / least_keys;
         int64_t s = (512 + workgroups - 1) / workgroups;
         s = s < most ? s : most;
         return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
     };
     if (p.prefix > 0) {
-        p.prefix_tiles = (rows * group + kTile - 1) / kTile;
-        p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix);
+        p.prefix_wide = rows * group >= 64;
+        const int64_t tile = p.prefix_wide ? kWideRows : kNarrowRows;
+        p.prefix_tiles = (rows * group + tile - 1) / tile;
+        p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix, kBlock * kWaves);
     }
     if (own > 0) {
-        p.own_tiles = rows * group / kTile + (c.batch < rows ? c.batch : rows);
-        p.own_splits = splits(p.own_tiles * c.kv_heads, own);
+        p.own_wide = rows * group >= 64 * sequences;
+        const int64_t tile = p.own_wide ? kWideRows : kNarrowRows;
+        p.own_tiles = rows * group / tile + sequences;
+        p.own_splits = splits(p.own_tiles * c.kv_heads, own, kBlock * kWaves);
     }
     p.slots = p.prefix_splits + p.own_splits;
     return p;
@@ -446,7 +867,10 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
 
 template <class E, int D>
 hipError_t launch_paged_attention(const PagedAttnArgs& a, int64_t workgroups, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_attention_kernel<E, D>), dim3((unsigned)workgroups), dim3(kThreads), 0, stream, a);
+    if (a.prefix_wide || a.own_wide)
+        hipLaunchKernelGGL((paged_attention_kernel<E, D, true>), dim3((unsigned)workgroups), dim3(kThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((paged_attention_kernel<E, D, false>), dim3((unsigned)workgroups), dim3(kThreads), 0, stream, a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess || a.slots == 1) return err;
     const int64_t joins = ((int64_t)a.rows * a.heads + kWaves - 1) / kWaves;
@@ -469,8 +893,8 @@ int attention_sizes(const qwen2_paged_cache* cache, PagedView* view, int64_t row
     if (shared_pages < 0 || shared_pages > cache->table_width)
         return set_error(W4G64_STATUS_INVALID_VALUE, "shared_pages must be in [0, table_width = %lld], got %lld",
                          (long long)cache->table_width, (long long)shared_pages);
-    if ((cache->table_width << view->page_shift) > 0x7FFFFF00)
-        return set_error(W4G64_STATUS_UNSUPPORTED, "paged_attention tables must hold fewer than 2^31 - 256 positions");
+    if ((cache->table_width << view->page_shift) > 0x7FF00000)
+        return set_error(W4G64_STATUS_UNSUPPORTED, "paged_attention tables must hold at most 2^31 - 2^20 positions");
     return W4G64_STATUS_OK;
 }
 
@@ -508,17 +932,21 @@ int qwen2_paged_attention(const qwen2_paged_cache* cache, const qwen2_rows* q, c
                          (long long)need, (long long)(workspace ? workspace_bytes : 0));
     const int64_t workgroups =
         (p.prefix_tiles * p.prefix_splits + p.own_tiles * p.own_splits) * cache->kv_heads;
-    if (workgroups > 0x7FFFFFFF || rows * heads > 0x7FFFFFFF)
+    if (workgroups > 0x7FFFFFFF || rows * heads > 0x7FF00000)
         return set_error(W4G64_STATUS_UNSUPPORTED, "paged_attention call is too large: %lld workgroups", (long long)workgroups);
     a.q = (const uint16_t*)q->data, a.q_row = q->row, a.q_head = q->head;
     a.out = (uint16_t*)out->data, a.out_row = out->row, a.out_head = out->head;
     a.partials = (float*)workspace;  // (D floats per slot: 16-byte aligned)
     a.stats = a.partials + rows * heads * p.slots * cache->head_dim;
-    a.scale2 = scale * 1.44269504088896340736f;
+    // (a scale of zero: as small as there is, so that a hidden key's -inf stays -inf)
+    const float scale2 = fabsf(scale) * 1.44269504088896340736f;
+    a.scale2 = scale2 > 0.0f ? fminf(scale2, 3.402823466e+38f) : 1.401298464324817e-45f;
+    a.query_sign = scale < 0.0f ? 0x80008000u : 0u;
     a.rows = (int)rows, a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads);
     a.prefix = (int)p.prefix;
     a.prefix_tiles = (int)p.prefix_tiles, a.prefix_splits = (int)p.prefix_splits;
     a.own_tiles = (int)p.own_tiles, a.own_splits = (int)p.own_splits, a.slots = (int)p.slots;
+    a.prefix_wide = p.prefix_wide, a.own_wide = p.own_wide;
     a.zero_rest = zero_rest;
     const hipStream_t s = (hipStream_t)stream;
     hipError_t err;
