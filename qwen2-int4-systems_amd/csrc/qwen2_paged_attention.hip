@@ -23,9 +23,10 @@
 //   scores  A = 16 keys, B = 16 query rows: lane (j, q) gets row j's scores of
 //           keys 4 q + r;
 //   values  the lane's own 8 probabilities of a 32-key block are its 8 K slots;
-//           A = the values transposed: lane (j, q) reads kVd = D / 16 dimensions
-//           from kVd j of its 8 keys and pairs keys up by v_perm; dimension
-//           kVd j + dd is row j of the dd-th product.
+//           A = the values transposed.  Narrow: lane (j, q) loads kVd = D / 16
+//           dimensions from kVd j of its 8 keys and pairs keys up by v_perm;
+//           dimension kVd j + dd is row j of the dd-th product.  Wide: LDS reads
+//           that transpose; dimension 16 dd + j is row j of the dd-th product.
 // A probability is kept as two 16-bit terms (16 bits or more of it): one term
 // alone would be as coarse as the output.
 //
@@ -241,16 +242,17 @@ __device__ __forceinline__ Row row_at(const PagedAttnArgs& a, const Segment& s, 
     return r;
 }
 
-// The page of a segment's 16 keys from t, the wave's own; keys that no row sees
-// (t > most): any page.
-__device__ __forceinline__ int segment_page(const PagedAttnArgs& a, const Segment& s, int t, int most) {
-    if (t > most) return 0;  // (most lies in the table)
-    return checked_page(scalar_load(s.table, t >> a.c.page_shift), a.c.num_pages);
+// What the table says of a segment's 16 keys from t, the wave's own; keys that no
+// row sees (t > most): any page.  (checked_page comes with the use, one round
+// later: the load is not waited for here.)
+__device__ __forceinline__ int table_entry(const PagedAttnArgs& a, const Segment& s, int t, int most) {
+    return t > most ? 0 : scalar_load(s.table, t >> a.c.page_shift);  // (most lies in the table)
 }
 
 // One lane's part of kTiles 16-row tiles: the running softmax and value sums of
-// row j of each, over the dimensions kVd (4 q + r) + dd.
-template <class E, int D, int kTiles>
+// row j of each, o[u][dd][r] over the dimensions kVd (4 q + r) + dd (narrow), or 16
+// dd + 4 q + r (wide, kTransposed).
+template <class E, int D, int kTiles, bool kTransposed>
 struct Attend {
     static constexpr int kVd = D / 16;     // dimensions of a value per lane
     static constexpr int kVw = kVd / 2;    // words of them
@@ -304,47 +306,41 @@ struct Attend {
         }
     }
 
-    // The value sums of 32 keys from t0: v[e] is the lane's piece of key 16 (e / 4) + 4 q + e % 4.
+    // Product dd of the value sums of 32 keys from t0: vt holds, for the product's row
+    // j, the values of the lane's keys 16 (e / 4) + 4 q + e % 4.
     template <bool kCareful>
-    __device__ __forceinline__ void gather(const vword (&v)[8], const u32x4 (&ph)[kTiles], const u32x4 (&pl)[kTiles],
+    __device__ __forceinline__ void gather(int dd, const u32x4& vt, const u32x4 (&ph)[kTiles], const u32x4 (&pl)[kTiles],
                                            const int (&limit)[kTiles], int t0, int j, int q) {
+        if constexpr (!kCareful) {
 #pragma unroll
-        for (int dd = 0; dd < kVd; ++dd) {
-            const uint32_t sel = (dd & 1) ? 0x07060302u : 0x05040100u;  // high or low halves
-            u32x4 vt;
+            for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, ph[u], o[u][dd]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][dd / 2], v[2 * e][dd / 2], sel);
-            if constexpr (!kCareful) {
+            for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, pl[u], o[u][dd]);
+            return;
+        }
+        // A value that is not finite must reach only the rows that see its key (0 * inf
+        // is NaN): the finite ones as always, the others column by column with what the
+        // column does not see at zero.
+        u32x4 plain, odd;
 #pragma unroll
-                for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, ph[u], o[u][dd]);
+        for (int e = 0; e < 4; ++e) {
+            plain[e] = finite_halves<E>(vt[e]);
+            odd[e] = vt[e] & ~plain[e];
+        }
 #pragma unroll
-                for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, pl[u], o[u][dd]);
-            } else {
-                // A value that is not finite must reach only the rows that see its key
-                // (0 * inf is NaN): the finite ones as always, the others column by
-                // column with what the column does not see at zero.
-                u32x4 plain, odd;
+        for (int u = 0; u < kTiles; ++u) {
+            o[u][dd] = E::mfma(plain, ph[u], o[u][dd]);
+            o[u][dd] = E::mfma(plain, pl[u], o[u][dd]);
+            for (int c = 0; c < 16; ++c) {
+                const int sees = __builtin_amdgcn_readlane(limit[u], c);
+                u32x4 part;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    plain[e] = finite_halves<E>(vt[e]);
-                    odd[e] = vt[e] & ~plain[e];
+                    const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
+                    part[e] = keep_halves(odd[e], t <= sees, t + 1 <= sees);
                 }
-#pragma unroll
-                for (int u = 0; u < kTiles; ++u) {
-                    o[u][dd] = E::mfma(plain, ph[u], o[u][dd]);
-                    o[u][dd] = E::mfma(plain, pl[u], o[u][dd]);
-                    for (int c = 0; c < 16; ++c) {
-                        const int sees = __builtin_amdgcn_readlane(limit[u], c);
-                        u32x4 part;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
-                            part[e] = keep_halves(odd[e], t <= sees, t + 1 <= sees);
-                        }
-                        const float4v more = E::mfma(part, ph[u], float4v{0.0f, 0.0f, 0.0f, 0.0f});
-                        if (j == c) o[u][dd] += more;
-                    }
-                }
+                const float4v more = E::mfma(part, ph[u], float4v{0.0f, 0.0f, 0.0f, 0.0f});
+                if (j == c) o[u][dd] += more;
             }
         }
     }
@@ -366,30 +362,48 @@ struct Attend {
         if (!row.live) return;
         if (a.slots == 1) {
             const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
-            uint16_t* to = a.out + row.token * a.out_row + row.head * a.out_head + 4 * kVd * q;
+            uint16_t* to = a.out + row.token * a.out_row + row.head * a.out_head;
+            if constexpr (kTransposed) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                uint32_t w[kVw];
+                for (int dd = 0; dd < kVd; ++dd) {
+                    const float4v x = o[u][dd];
+                    *(u32x2*)(to + 16 * dd + 4 * q) = u32x2{E::pack(x[0] * inv, x[1] * inv), E::pack(x[2] * inv, x[3] * inv)};
+                }
+            } else {
 #pragma unroll
-                for (int i = 0; i < kVw; ++i) w[i] = E::pack(o[u][2 * i][r] * inv, o[u][2 * i + 1][r] * inv);
-                vword x;
+                for (int r = 0; r < 4; ++r) {
+                    vword x;
 #pragma unroll
-                for (int i = 0; i < kVw; ++i) x[i] = w[i];
-                *(vword*)(to + kVd * r) = x;
+                    for (int i = 0; i < kVw; ++i) x[i] = E::pack(o[u][2 * i][r] * inv, o[u][2 * i + 1][r] * inv);
+                    *(vword*)(to + kVd * (4 * q + r)) = x;
+                }
             }
             return;
         }
         const int64_t slot = ((int64_t)row.token * a.heads + row.head) * a.slots + (s.shared ? 0 : a.prefix_splits) + s.split;
         if (q == 0) *(float2v*)(a.stats + 2 * slot) = float2v{m, l};
         if (m == -INFINITY) return;  // (the join does not read it)
-        float* to = a.partials + slot * D + 4 * kVd * q;
+        float* to = a.partials + slot * D;
+        if constexpr (kTransposed) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int dd = 0; dd < kVd; ++dd) *(float4v*)(to + 16 * dd + 4 * q) = o[u][dd];
+        } else {
 #pragma unroll
-            for (int dd = 0; dd < kVd; dd += 4)
-                *(float4v*)(to + kVd * r + dd) = float4v{o[u][dd][r], o[u][dd + 1][r], o[u][dd + 2][r], o[u][dd + 3][r]};
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int dd = 0; dd < kVd; dd += 4)
+                    *(float4v*)(to + kVd * (4 * q + r) + dd) =
+                        float4v{o[u][dd][r], o[u][dd + 1][r], o[u][dd + 2][r], o[u][dd + 3][r]};
+        }
     }
 };
+
+// A value that a rare branch works with: keeps the compiler from running the
+// branch's instructions always.
+__device__ __forceinline__ int rare(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // The queries of a row as MFMA operand pieces.
 template <int kSteps>
@@ -424,14 +438,14 @@ __device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s,
 template <class E, int D>
 struct KeyBlock {
     u32x4 k[2][D / 32];                     // key 16 h + j, dimensions 32 s + 8 q ..
-    typename Attend<E, D, 1>::vword v[8];   // value of key 16 (e / 4) + 4 q + e % 4, dimensions kVd j ..
+    typename Attend<E, D, 1, false>::vword v[8];   // value of key 16 (e / 4) + 4 q + e % 4, dimensions kVd j ..
     bool bad[2];
 };
 
 template <class E, int D>
 __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s, int lane, int wave,
                                        unsigned char* meet) {
-    typedef Attend<E, D, 1> A;
+    typedef Attend<E, D, 1, false> A;
     const int j = lane & 15;
     const int q = lane >> 4;
     const Row row = row_at(a, s, s.tile * kNarrowRows + j);
@@ -452,14 +466,15 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
     };
     auto look = [&](int block) {
         const int t = s.key_lo + block * kBlock;
-        return Pages{{segment_page(a, s, t, most), segment_page(a, s, t + 16, most)}};
+        return Pages{{table_entry(a, s, t, most), table_entry(a, s, t + 16, most)}};
     };
     auto load = [&](KeyBlock<E, D>& b, int block, const Pages& pages) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int t = s.key_lo + block * kBlock + 16 * h;
-            b.bad[h] = pages.p[h] < 0;
-            const int64_t page = max(pages.p[h], 0);
+            const int entry = checked_page(pages.p[h], a.c.num_pages);
+            b.bad[h] = entry < 0;
+            const int64_t page = max(entry, 0);
             const uint16_t* kp = kc + page * a.c.k_page + (t & mask) * a.c.k_position;
             const uint16_t* vp = vc + page * a.c.v_page + (t & mask) * a.c.v_position;
 #pragma unroll
@@ -482,11 +497,12 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
             for (int r = 0; r < 4; ++r) x[0][4 * h + r] = acc[r];
         }
         if (t0 + kBlock - 1 > least) {
+            const int sees = rare(row.limit - t0), held = rare(most - t0);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int t = t0 + 16 * (e / 4) + 4 * q + e % 4;
-                if (t > row.limit) x[0][e] = -INFINITY;
-                if (t > most) b.v[e] = typename A::vword{};
+                const int t = 16 * (e / 4) + 4 * q + e % 4;
+                if (t > sees) x[0][e] = -INFINITY;
+                if (t > held) b.v[e] = typename A::vword{};
             }
         }
         state.seen[0] = state.seen[0] || t0 <= row.limit;
@@ -497,7 +513,14 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         state.template soften<kBlock>(x, ph, pl, a.scale2);
         const u32x4 h1[1] = {ph[0][0]}, l1[1] = {pl[0][0]};
         const int limit[1] = {row.limit};
-        state.template gather<decltype(careful)::value>(b.v, h1, l1, limit, t0, j, q);
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; ++dd) {
+            const uint32_t sel = (dd & 1) ? 0x07060302u : 0x05040100u;  // high or low halves
+            u32x4 vt;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vt[e] = __builtin_amdgcn_perm(b.v[2 * e + 1][dd / 2], b.v[2 * e][dd / 2], sel);
+            state.template gather<decltype(careful)::value>(dd, vt, h1, l1, limit, t0, j, q);
+        }
     };
     // Two blocks in flight, the pages of a third known.
     state.start();
@@ -577,7 +600,15 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
 // ---- wide ----
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v* lds_halves_t;
 
+// This wave's loads into LDS have landed.
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));  // vmcnt 0 (gfx9 encoding)
+    asm volatile("" ::: "memory");
+}
 // All of this wave's loads into LDS and stores to it have landed, then all waves'.
 __device__ __forceinline__ void all_landed() {
     asm volatile("" ::: "memory");
@@ -587,8 +618,11 @@ __device__ __forceinline__ void all_landed() {
 }
 
 // A tile's keys or values in LDS: 64 rows of D elements in 16-byte pieces, piece
-// c of row r in slot c ^ turn(r), so that reads of one piece of 16 rows meet
-// different banks.
+// c of row r in slot c ^ turn(r).  Keys are read one piece of 16 rows at a time:
+// the turns are all different (D 64: where the rows' banks are the same).  Values
+// are read transposed, 32 bytes of 4 rows by 16 lanes (ds_read_b64_tr_b16: lane t
+// brings elements 4 (t % 4) .. of row t / 4 and gets element t of the four
+// rows): there the pairs of pieces are turned.
 template <int D>
 struct Tile {
     static constexpr int kPieces = D / 8;
@@ -596,13 +630,14 @@ struct Tile {
     static constexpr int kBytes = kTileKeys * kRowBytes;
     static constexpr int kRowsPerLoad = 64 / kPieces;  // rows that a wave's 16-byte load fills
     static constexpr int kLoads = 16 / kRowsPerLoad;   // loads of 16 keys
-    static __device__ __forceinline__ int turn(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+    static __device__ __forceinline__ int key_turn(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+    static __device__ __forceinline__ int value_turn(int row) { return D == 128 ? 2 * (row & 7) : row & 6; }
 };
 
 template <class E, int D>
 __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
                                      unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves]) {
-    typedef Attend<E, D, 2> A;
+    typedef Attend<E, D, 2, true> A;
     typedef Tile<D> T;
     const int j = lane & 15;
     const int q = lane >> 4;
@@ -632,12 +667,12 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) {
         const int r = T::kRowsPerLoad * i + lane / T::kPieces;
-        const int piece = (lane % T::kPieces) ^ T::turn(r);
-        k_at[i] = 2 * r * (int)a.c.k_position + 16 * piece;
-        v_at[i] = 2 * r * (int)a.c.v_position + 16 * piece;
+        k_at[i] = 2 * r * (int)a.c.k_position + 16 * ((lane % T::kPieces) ^ T::key_turn(r));
+        v_at[i] = 2 * r * (int)a.c.v_position + 16 * ((lane % T::kPieces) ^ T::value_turn(r));
     }
-    auto look = [&](int tile) { return segment_page(a, s, s.key_lo + tile * kTileKeys + 16 * wave, all_most); };
-    auto stage = [&](int tile, int page, unsigned char* keys, unsigned char* values, int* flags) {
+    auto look = [&](int tile) { return table_entry(a, s, s.key_lo + tile * kTileKeys + 16 * wave, all_most); };
+    auto stage = [&](int tile, int entry, unsigned char* keys, unsigned char* values, int* flags) {
+        const int page = checked_page(entry, a.c.num_pages);
         const int t = s.key_lo + tile * kTileKeys + 16 * wave;
         if (lane == 0) flags[wave] = page < 0;
         const int64_t p = max(page, 0);
@@ -654,6 +689,19 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
             __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(values + 16 * wave * T::kRowBytes + 1024 * i), 16,
                                                      v_at[i], 0, 0, 0);
     };
+    // Before the barrier: values past the last visible key become zeros (their
+    // probabilities are, but what lies there may not be finite).
+    auto settle = [&](int tile, unsigned char* values) {
+        const int held = all_most - (s.key_lo + tile * kTileKeys + 16 * wave);  // last of the wave's 16 keys
+        if (held >= 15) return;
+        wait_loads();
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i) {
+            const int r = T::kRowsPerLoad * i + lane / T::kPieces;
+            if (r > held)
+                *(u32x4*)(values + (16 * wave + r) * T::kRowBytes + 16 * (lane % T::kPieces)) = u32x4{0u, 0u, 0u, 0u};
+        }
+    };
     A state;
     auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, const int* flags, auto careful) {
         const int t0 = s.key_lo + tile * kTileKeys;
@@ -664,23 +712,25 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
             u32x4 kf[A::kSteps];
 #pragma unroll
             for (int i = 0; i < A::kSteps; ++i)
-                kf[i] = *(const u32x4*)(keys + (16 * h + j) * T::kRowBytes + 16 * ((4 * i + q) ^ T::turn(j)));
+                kf[i] = *(const u32x4*)(keys + (16 * h + j) * T::kRowBytes + 16 * ((4 * i + q) ^ T::key_turn(j)));
+            float4v acc[2] = {};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < A::kSteps; ++i)
 #pragma unroll
-                for (int i = 0; i < A::kSteps; ++i) acc = E::mfma(kf[i], qf[u][i], acc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[u][4 * h + r] = acc[r];
-            }
-        }
-        const bool edge = t0 + kTileKeys - 1 > least;
-        if (edge) {
+                for (int u = 0; u < 2; ++u) acc[u] = E::mfma(kf[i], qf[u][i], acc[u]);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
+                for (int r = 0; r < 4; ++r) x[u][4 * h + r] = acc[u][r];
+        }
+        if (t0 + kTileKeys - 1 > least) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int sees = rare(limit[u] - t0);
+#pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (t0 + 16 * (e / 4) + 4 * q + e % 4 > limit[u]) x[u][e] = -INFINITY;
+                    if (16 * (e / 4) + 4 * q + e % 4 > sees) x[u][e] = -INFINITY;
+            }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) state.seen[u] = state.seen[u] || t0 <= limit[u];
@@ -695,18 +745,21 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         state.template soften<kTileKeys>(x, ph, pl, a.scale2);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            typename A::vword v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int r = 32 * i + 16 * (e / 4) + 4 * q + e % 4;
-                if constexpr (D == 128)
-                    v[e] = *(const typename A::vword*)(values + r * T::kRowBytes + 16 * (j ^ T::turn(r)));
-                else
-                    v[e] = *(const typename A::vword*)(values + r * T::kRowBytes + 16 * ((j / 2) ^ T::turn(r)) + 8 * (j & 1));
-                if (edge && t0 + r > most) v[e] = typename A::vword{};
-            }
             const u32x4 h2[2] = {ph[0][i], ph[1][i]}, l2[2] = {pl[0][i], pl[1][i]};
-            state.template gather<decltype(careful)::value>(v, h2, l2, limit, t0 + 32 * i, j, q);
+            // the lane's part of the four rows 4 q ..: row 4 q + j / 4, elements 4 (j % 4) ..
+            const int r = 32 * i + 4 * q + j / 4;
+#pragma unroll
+            for (int dd = 0; dd < A::kVd; ++dd) {
+                u32x4 vt;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {  // (rows 16 apart turn alike)
+                    const unsigned char* at = values + (r + 16 * g) * T::kRowBytes +
+                                              16 * ((2 * dd + (j & 3) / 2) ^ T::value_turn(r)) + 8 * (j & 1);
+                    const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_halves_t)at));
+                    vt[2 * g] = w[0], vt[2 * g + 1] = w[1];
+                }
+                state.template gather<decltype(careful)::value>(dd, vt, h2, l2, limit, t0 + 32 * i, j, q);
+            }
         }
     };
     // The next tile on its way while this one is worked on: its buffer was read
@@ -716,11 +769,13 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         stage(begin, look(begin), k0, v0, bad[0]);
         int next = look(begin + 1);
         for (int tile = begin;;) {
+            settle(tile, v0);
             all_landed();
             if (tile + 1 < end) stage(tile + 1, next, k1, v1, bad[1]);
             next = look(tile + 2);
             compute(tile, k0, v0, bad[0], std::false_type{});
             if (++tile >= end) break;
+            settle(tile, v1);
             all_landed();
             if (tile + 1 < end) stage(tile + 1, next, k0, v0, bad[0]);
             next = look(tile + 2);
@@ -734,6 +789,7 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         state.start();
         for (int tile = begin; tile < end; ++tile) {
             stage(tile, look(tile), k0, v0, bad[0]);
+            settle(tile, v0);
             all_landed();
             compute(tile, k0, v0, bad[0], std::true_type{});
             all_landed();
@@ -845,7 +901,7 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
     const int64_t own = ((int64_t)c.table_width - shared_pages) << c.page_shift;
     auto splits = [&](int64_t workgroups, int64_t keys, int64_t least_keys) {
         const int64_t most = (keys + least_keys - 1) / least_keys;
-        int64_t s = (512 + workgroups - 1) / workgroups;
+        int64_t s = 512 > workgroups ? 512 / workgroups : 1;
         s = s < most ? s : most;
         return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
     };
