@@ -273,36 +273,36 @@ struct Attend {
         }
     }
 
-    // Scores of kKeys keys from t0 (a lane's are t0 + 16 (e / 4) + 4 q + e % 4) become
-    // probabilities; the sums are rescaled where needed.
-    template <int kKeys>
-    __device__ __forceinline__ void soften(float (&s)[kTiles][kKeys / 4], u32x4 (&ph)[kTiles][kKeys / 32],
-                                           u32x4 (&pl)[kTiles][kKeys / 32], float scale2) {
+    // Before a lane's kCount scores of tile u become probabilities: the sums rescaled
+    // where needed.
+    template <int kCount>
+    __device__ __forceinline__ void settle(int u, const float (&s)[kCount], float scale2) {
+        float top = s[0];
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u) {
-            float top = s[u][0];
+        for (int e = 1; e < kCount; ++e) top = fmaxf(top, s[e]);
+        const float mn = quarters_max(top) * scale2;
+        if (__any(mn - m_run[u] > kLazy<E>)) {
+            const float to = fmaxf(m_run[u], mn);
+            const float alpha = __builtin_amdgcn_exp2f(m_run[u] - to);  // (1 where it is another row's turn)
+            l_run[u] *= alpha;
 #pragma unroll
-            for (int e = 1; e < kKeys / 4; ++e) top = fmaxf(top, s[u][e]);
-            const float mn = quarters_max(top) * scale2;
-            if (__any(mn - m_run[u] > kLazy<E>)) {
-                const float to = fmaxf(m_run[u], mn);
-                const float alpha = __builtin_amdgcn_exp2f(m_run[u] - to);  // (1 where it is another row's turn)
-                l_run[u] *= alpha;
+            for (int dd = 0; dd < kVd; ++dd) o[u][dd] *= alpha;
+            m_run[u] = to;
+        }
+    }
+
+    // Eight scores of tile u as probabilities, in two 16-bit terms.
+    template <int kCount>
+    __device__ __forceinline__ void soften(int u, const float (&s)[kCount], int from, u32x4& ph, u32x4& pl,
+                                           float scale2) {
+        const float ref = kProbShift<E> - m_run[u];
 #pragma unroll
-                for (int dd = 0; dd < kVd; ++dd) o[u][dd] *= alpha;
-                m_run[u] = to;
-            }
-            const float ref = kProbShift<E> - m_run[u];
-#pragma unroll
-            for (int i = 0; i < kKeys / 32; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][8 * i + 2 * e], scale2, ref));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][8 * i + 2 * e + 1], scale2, ref));
-                    l_run[u] += p0 + p1;
-                    ph[u][i][e] = E::pack(p0, p1);
-                    pl[u][i][e] = E::pack(p0 - E::lo(ph[u][i][e]), p1 - E::hi(ph[u][i][e]));
-                }
+        for (int e = 0; e < 4; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[from + 2 * e], scale2, ref));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[from + 2 * e + 1], scale2, ref));
+            l_run[u] += p0 + p1;
+            ph[e] = E::pack(p0, p1);
+            pl[e] = E::pack(p0 - E::lo(ph[e]), p1 - E::hi(ph[e]));
         }
     }
 
@@ -487,21 +487,21 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
     A state;
     auto compute = [&](KeyBlock<E, D>& b, int block, auto careful) {
         const int t0 = s.key_lo + block * kBlock;
-        float x[1][8];
+        float x[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < A::kSteps; ++i) acc = E::mfma(b.k[h][i], qf[i], acc);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[0][4 * h + r] = acc[r];
+            for (int r = 0; r < 4; ++r) x[4 * h + r] = acc[r];
         }
         if (t0 + kBlock - 1 > least) {
-            const int sees = rare(row.limit - t0), held = rare(most - t0);
+            const int sees = rare(row.limit - t0 - 4 * q), held = rare(most - t0 - 4 * q);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int t = 16 * (e / 4) + 4 * q + e % 4;
-                if (t > sees) x[0][e] = -INFINITY;
+                const int t = 16 * (e / 4) + e % 4;
+                if (t > sees) x[e] = -INFINITY;
                 if (t > held) b.v[e] = typename A::vword{};
             }
         }
@@ -509,9 +509,9 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             if (b.bad[h] && t0 + 16 * h <= row.limit) state.l_run[0] = __builtin_nanf("");
-        u32x4 ph[1][1], pl[1][1];
-        state.template soften<kBlock>(x, ph, pl, a.scale2);
-        const u32x4 h1[1] = {ph[0][0]}, l1[1] = {pl[0][0]};
+        u32x4 h1[1], l1[1];
+        state.settle(0, x, a.scale2);
+        state.soften(0, x, 0, h1[0], l1[0], a.scale2);
         const int limit[1] = {row.limit};
 #pragma unroll
         for (int dd = 0; dd < A::kVd; ++dd) {
@@ -642,18 +642,23 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
     const int j = lane & 15;
     const int q = lane >> 4;
     const int m0 = s.tile * kWideRows + 32 * wave;
-    const Row row[2] = {row_at(a, s, m0 + j), row_at(a, s, m0 + 16 + j)};
-    const int limit[2] = {row[0].limit, row[1].limit};
     u32x4 qf[2][A::kSteps];
-    load_queries(a, row[0], q, qf[0]);
-    load_queries(a, row[1], q, qf[1]);
+    int limit[2];
     // the wave's rows, then the workgroup's
-    int least, most, all_most, other;
-    limits(a, s, row[0], m0, 16, least, most);
-    limits(a, s, row[1], m0 + 16, 16, other, all_most);
-    least = min(least, other), most = max(most, all_most);
-    if (s.shared) all_most = (int)s.key_end - 1;
-    else limits(a, s, row[0], s.tile * kWideRows, kWideRows, other, all_most);
+    int least = 0x7FFFFFFF, most = s.key_lo - 1, all_most = (int)s.key_end - 1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const Row row = row_at(a, s, m0 + 16 * u + j);
+        limit[u] = row.limit;
+        load_queries(a, row, q, qf[u]);
+        int one, other;
+        limits(a, s, row, m0 + 16 * u, 16, one, other);
+        least = min(least, one), most = max(most, other);
+    }
+    if (!s.shared) {
+        int other;
+        limits(a, s, Row{}, s.tile * kWideRows, kWideRows, other, all_most);
+    }
     const int tiles = all_most >= s.key_lo ? (all_most - s.key_lo) / kTileKeys + 1 : 0;
     const int per = (tiles + s.splits - 1) / s.splits;
     const int begin = s.split * per;
@@ -707,17 +712,23 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         const int t0 = s.key_lo + tile * kTileKeys;
         if (t0 > most) return;  // (the wave's)
         float x[2][16];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            u32x4 kf[A::kSteps];
+        // keys of the next product on their way while this one's are used
+        u32x4 kf[2][A::kSteps];
+        auto load_keys = [&](int h) {
 #pragma unroll
             for (int i = 0; i < A::kSteps; ++i)
-                kf[i] = *(const u32x4*)(keys + (16 * h + j) * T::kRowBytes + 16 * ((4 * i + q) ^ T::key_turn(j)));
+                kf[h & 1][i] = *(const u32x4*)(keys + (16 * h + j) * T::kRowBytes + 16 * ((4 * i + q) ^ T::key_turn(j)));
+        };
+        load_keys(0);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            if (h < 3) load_keys(h + 1);
+            __builtin_amdgcn_sched_barrier(0);
             float4v acc[2] = {};
 #pragma unroll
             for (int i = 0; i < A::kSteps; ++i)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) acc[u] = E::mfma(kf[i], qf[u][i], acc[u]);
+                for (int u = 0; u < 2; ++u) acc[u] = E::mfma(kf[h & 1][i], qf[u][i], acc[u]);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -726,10 +737,10 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         if (t0 + kTileKeys - 1 > least) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int sees = rare(limit[u] - t0);
+                const int sees = rare(limit[u] - t0 - 4 * q);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (16 * (e / 4) + 4 * q + e % 4 > sees) x[u][e] = -INFINITY;
+                    if (16 * (e / 4) + e % 4 > sees) x[u][e] = -INFINITY;
             }
         }
 #pragma unroll
@@ -741,24 +752,33 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
                 for (int u = 0; u < 2; ++u)
                     if (flags[h] && t0 + 16 * h <= limit[u]) state.l_run[u] = __builtin_nanf("");
         }
-        u32x4 ph[2][2], pl[2][2];
-        state.template soften<kTileKeys>(x, ph, pl, a.scale2);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) state.settle(u, x[u], a.scale2);
+        // the lane's part of the four rows 4 q ..: row 4 q + j / 4, elements 4 (j % 4) ..
+        u32x4 vt[2];
+        auto load_values = [&](int i, int dd) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {  // (rows 16 apart turn alike)
+                const int r = 4 * q + j / 4;
+                const unsigned char* at = values + r * T::kRowBytes +
+                                          16 * ((2 * dd + (j & 3) / 2) ^ T::value_turn(r)) + 8 * (j & 1) +
+                                          (32 * i + 16 * g) * T::kRowBytes;
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_halves_t)at));
+                vt[dd & 1][2 * g] = w[0], vt[dd & 1][2 * g + 1] = w[1];
+            }
+        };
+        load_values(0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const u32x4 h2[2] = {ph[0][i], ph[1][i]}, l2[2] = {pl[0][i], pl[1][i]};
-            // the lane's part of the four rows 4 q ..: row 4 q + j / 4, elements 4 (j % 4) ..
-            const int r = 32 * i + 4 * q + j / 4;
+            u32x4 ph[2], pl[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) state.soften(u, x[u], 8 * i, ph[u], pl[u], a.scale2);
 #pragma unroll
             for (int dd = 0; dd < A::kVd; ++dd) {
-                u32x4 vt;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {  // (rows 16 apart turn alike)
-                    const unsigned char* at = values + (r + 16 * g) * T::kRowBytes +
-                                              16 * ((2 * dd + (j & 3) / 2) ^ T::value_turn(r)) + 8 * (j & 1);
-                    const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_halves_t)at));
-                    vt[2 * g] = w[0], vt[2 * g + 1] = w[1];
-                }
-                state.template gather<decltype(careful)::value>(dd, vt, h2, l2, limit, t0 + 32 * i, j, q);
+                if (dd + 1 < A::kVd) load_values(i, dd + 1);
+                else if (i == 0) load_values(1, 0);
+                __builtin_amdgcn_sched_barrier(0x7);  // (no LDS read past this; arithmetic as it likes)
+                state.template gather<decltype(careful)::value>(dd, vt[dd & 1], ph, pl, limit, t0 + 32 * i, j, q);
             }
         }
     };
@@ -799,11 +819,12 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
     for (int u = 0; u < 2; ++u) {
         float l = quarters_sum(state.l_run[u]);
         float m = state.seen[u] ? state.m_run[u] : -INFINITY;
-        if (row[u].beyond && s.split == 0) {
+        const Row row = row_at(a, s, rare(m0 + 16 * u + j));  // (again: not kept in registers over the keys)
+        if (row.beyond && s.split == 0) {
             l = __builtin_nanf("");
             m = fmaxf(m, kScoreFloor);
         }
-        state.store(a, s, row[u], u, l, m, q);
+        state.store(a, s, row, u, l, m, q);
     }
 }
 
@@ -903,7 +924,10 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
         const int64_t most = (keys + least_keys - 1) / least_keys;
         int64_t s = 512 > workgroups ? 512 / workgroups : 1;
         s = s < most ? s : most;
-        return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
+        s = s < kMaxSplits / 2 ? s : kMaxSplits / 2;
+        // tiles of the same keys on one XCD (workgroups go to the eight in turn)
+        const int64_t turn = c.kv_heads % 8 == 0 ? 1 : c.kv_heads % 4 == 0 ? 2 : c.kv_heads % 2 == 0 ? 4 : 8;
+        return s > turn ? s - s % turn : s;
     };
     if (p.prefix > 0) {
         p.prefix_wide = rows * group >= 64;
