@@ -56,6 +56,22 @@ constexpr int kBlock = 32;       // keys of a narrow block
 constexpr int kTileKeys = 64;    // keys of a wide tile
 constexpr int kMaxSplits = 64;
 
+// Division of numbers below 2^31 by a divisor that the host knows: the usual
+// multiplication by 2^(32 + shift) / divisor, less its leading one.
+struct Divisor {
+    uint32_t magic, shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return (int)((__umulhi((uint32_t)n, magic) + (uint32_t)n) >> shift);
+    }
+};
+Divisor divisor(int64_t d) {
+    Divisor r{0, 0};
+    d = d > 0 ? d : 1;
+    while ((int64_t(1) << r.shift) < d) ++r.shift;
+    r.magic = (uint32_t)((((uint64_t(1) << r.shift) - (uint64_t)d) << 32) / (uint64_t)d + (r.shift ? 1 : 0));
+    return r;
+}
+
 struct PagedAttnArgs {
     PagedView c;
     const uint16_t* q;
@@ -70,6 +86,7 @@ struct PagedAttnArgs {
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
     int prefix_wide, own_wide;
     int zero_rest;
+    Divisor by_group, by_heads, by_kv_heads, by_prefix_splits, by_own_splits;
 };
 
 // Exponents of probabilities: fp16 ends at 2^-24 and at 2^16, and a key far below
@@ -79,6 +96,21 @@ template <class E> constexpr float kProbShift = 0.0f;
 template <> constexpr float kProbShift<F16> = 11.0f;
 template <class E> constexpr float kLazy = 8.0f;
 template <> constexpr float kLazy<F16> = 4.0f;
+
+// The kernel's arguments, read anew: what only the end of a kernel needs is not
+// held in scalar registers (and spilled) over its loop.
+__device__ __forceinline__ PagedAttnArgs late_arguments() {
+    typedef const __attribute__((address_space(4))) uint32_t* words_t;
+    words_t p = (words_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    uint32_t w[sizeof(PagedAttnArgs) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(w) / 4); ++i) w[i] = p[i];
+    PagedAttnArgs a;
+    static_assert(sizeof(w) == sizeof(a), "whole words");
+    __builtin_memcpy(&a, w, sizeof(a));
+    return a;
+}
 
 // An index array's entry at a wave's own index, through the scalar cache.
 __device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
@@ -113,17 +145,24 @@ template <class E> __device__ __forceinline__ uint32_t finite_halves(uint32_t w)
     return keep_halves(w, (w & E::kExponent) != E::kExponent, ((w >> 16) & E::kExponent) != E::kExponent);
 }
 
-// The sequence, its rows and the place of own tile `tile` of `tile_rows` rows: the
-// tiles of every sequence counted up, 64 sequences at a time.  false: past the
-// last one.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile_rows, int tile, int lane, int& sequence,
-                                          int& local, SequenceRows& rows) {
+// Whether a sequence's own rows go by wide tiles, where the call has any.
+constexpr int kWideFrom = 64;
+__device__ __forceinline__ bool wide_rows(const PagedAttnArgs& a, int tokens) {
+    return a.own_wide && tokens * a.group > kWideFrom;
+}
+
+// The sequence, its rows and the place of own tile `tile`: the tiles of every
+// sequence counted up, 64 sequences at a time.  false: past the last one.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, int lane, int& sequence, int& local,
+                                          SequenceRows& rows) {
     int before = 0;
     for (int base = 0; base < a.c.batch; base += 64) {
         const int i = base + lane;
         SequenceRows s{0, 0, 0};
         if (i < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
-        const int count = ((s.end - s.begin) * a.group + tile_rows - 1) / tile_rows;
+        const int tokens = s.end - s.begin;
+        const int count = wide_rows(a, tokens) ? (tokens * a.group + kWideRows - 1) / kWideRows
+                                               : (tokens * a.group + kNarrowRows - 1) / kNarrowRows;
         const int upto = before + running_sum(count);
         const uint64_t past = __ballot(upto > tile);
         if (past) {
@@ -133,7 +172,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile_rows,
             rows.begin = __builtin_amdgcn_readlane(s.begin, at);
             rows.end = __builtin_amdgcn_readlane(s.end, at);
             // (the length: at most 31 bits and a sign below the rows)
-            rows.first = (int64_t)__builtin_amdgcn_readlane((int)(s.first + (s.end - s.begin)), at) - (rows.end - rows.begin);
+            rows.first = (int64_t)__builtin_amdgcn_readlane((int)(s.first + tokens), at) - (rows.end - rows.begin);
             return true;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
@@ -154,7 +193,7 @@ __device__ __forceinline__ int sequence_by_halving(const int32_t* cu_rows, int b
 
 // What a workgroup works on.
 struct Segment {
-    bool shared;
+    bool shared, wide;
     bool sees_all;        // prefix: every row sees all of it
     int split, splits, kvh, tile;
     int first_token;
@@ -170,12 +209,14 @@ __device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, S
     s.shared = (int)blockIdx.x < prefix_work;
     const int work = s.shared ? (int)blockIdx.x : (int)blockIdx.x - prefix_work;
     s.splits = s.shared ? a.prefix_splits : a.own_splits;
-    s.split = work % s.splits;
-    s.kvh = work / s.splits % a.c.kv_heads;
-    s.tile = work / s.splits / a.c.kv_heads;
+    const int slot = s.shared ? a.by_prefix_splits(work) : a.by_own_splits(work);  // tile * kv_heads + kvh
+    s.split = work - slot * s.splits;
+    s.tile = a.by_kv_heads(slot);
+    s.kvh = slot - s.tile * a.c.kv_heads;
     s.held = (int64_t)a.c.table_width << a.c.page_shift;
     s.sees_all = false;
     if (s.shared) {
+        s.wide = a.prefix_wide;
         s.first_token = 0;
         s.count = a.rows * a.group;
         s.first = 0;
@@ -193,9 +234,8 @@ __device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, S
     }
     int sequence;
     SequenceRows r;
-    const bool some = a.own_wide ? find_tile(a, kWideRows, s.tile, lane, sequence, s.tile, r)
-                                 : find_tile(a, kNarrowRows, s.tile, lane, sequence, s.tile, r);
-    if (!some) return false;
+    if (!find_tile(a, s.tile, lane, sequence, s.tile, r)) return false;
+    s.wide = wide_rows(a, r.end - r.begin);
     s.first_token = r.begin;
     s.count = (r.end - r.begin) * a.group;
     s.first = r.first;
@@ -217,7 +257,7 @@ __device__ __forceinline__ Row row_at(const PagedAttnArgs& a, const Segment& s, 
     Row r;
     r.live = m < s.count;
     m = r.live ? m : s.count - 1;
-    const int t = (uint32_t)m / (uint32_t)a.group;
+    const int t = a.by_group(m);
     r.token = s.first_token + t;
     r.head = s.kvh * a.group + (m - t * a.group);
     r.beyond = false;
@@ -249,10 +289,15 @@ __device__ __forceinline__ int table_entry(const PagedAttnArgs& a, const Segment
     return t > most ? 0 : scalar_load(s.table, t >> a.c.page_shift);  // (most lies in the table)
 }
 
+// Where a row's partial results of this workgroup's split go.
+__device__ __forceinline__ int64_t slot_of(const PagedAttnArgs& a, const Segment& s, const Row& row) {
+    return ((int64_t)row.token * a.heads + row.head) * a.slots + (s.shared ? 0 : a.prefix_splits) + s.split;
+}
+
 // One lane's part of kTiles 16-row tiles: the running softmax and value sums of
 // row j of each, o[u][dd][r] over the dimensions kVd (4 q + r) + dd (narrow), or 16
-// dd + 4 q + r (wide, kTransposed).
-template <class E, int D, int kTiles, bool kTransposed>
+// dd + 4 q + r (wide).
+template <class E, int D, int kTiles>
 struct Attend {
     static constexpr int kVd = D / 16;     // dimensions of a value per lane
     static constexpr int kVw = kVd / 2;    // words of them
@@ -355,47 +400,6 @@ struct Attend {
                 for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[u][dd][r]) < INFINITY;
         return fine;
     }
-
-    // Tile u's rows to their place: the output, or a slot of the partial results.
-    __device__ __forceinline__ void store(const PagedAttnArgs& a, const Segment& s, const Row& row, int u, float l,
-                                          float m, int q) const {
-        if (!row.live) return;
-        if (a.slots == 1) {
-            const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
-            uint16_t* to = a.out + row.token * a.out_row + row.head * a.out_head;
-            if constexpr (kTransposed) {
-#pragma unroll
-                for (int dd = 0; dd < kVd; ++dd) {
-                    const float4v x = o[u][dd];
-                    *(u32x2*)(to + 16 * dd + 4 * q) = u32x2{E::pack(x[0] * inv, x[1] * inv), E::pack(x[2] * inv, x[3] * inv)};
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    vword x;
-#pragma unroll
-                    for (int i = 0; i < kVw; ++i) x[i] = E::pack(o[u][2 * i][r] * inv, o[u][2 * i + 1][r] * inv);
-                    *(vword*)(to + kVd * (4 * q + r)) = x;
-                }
-            }
-            return;
-        }
-        const int64_t slot = ((int64_t)row.token * a.heads + row.head) * a.slots + (s.shared ? 0 : a.prefix_splits) + s.split;
-        if (q == 0) *(float2v*)(a.stats + 2 * slot) = float2v{m, l};
-        if (m == -INFINITY) return;  // (the join does not read it)
-        float* to = a.partials + slot * D;
-        if constexpr (kTransposed) {
-#pragma unroll
-            for (int dd = 0; dd < kVd; ++dd) *(float4v*)(to + 16 * dd + 4 * q) = o[u][dd];
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int dd = 0; dd < kVd; dd += 4)
-                    *(float4v*)(to + kVd * (4 * q + r) + dd) =
-                        float4v{o[u][dd][r], o[u][dd + 1][r], o[u][dd + 2][r], o[u][dd + 3][r]};
-        }
-    }
 };
 
 // A value that a rare branch works with: keeps the compiler from running the
@@ -424,7 +428,7 @@ __device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s,
     } else if (s.sees_all) {
         least = most = (int)s.key_end - 1;
     } else if (!s.shared) {
-        const int64_t first = s.first + (uint32_t)m0 / (uint32_t)a.group, end = s.first + (uint32_t)last / (uint32_t)a.group;
+        const int64_t first = s.first + a.by_group(m0), end = s.first + a.by_group(last);
         least = (int)max(min(first, s.key_end - 1), (int64_t)(s.key_lo - 1));
         most = (int)max(min(end, s.key_end - 1), (int64_t)(s.key_lo - 1));
     } else {
@@ -438,14 +442,14 @@ __device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s,
 template <class E, int D>
 struct KeyBlock {
     u32x4 k[2][D / 32];                     // key 16 h + j, dimensions 32 s + 8 q ..
-    typename Attend<E, D, 1, false>::vword v[8];   // value of key 16 (e / 4) + 4 q + e % 4, dimensions kVd j ..
+    typename Attend<E, D, 1>::vword v[8];   // value of key 16 (e / 4) + 4 q + e % 4, dimensions kVd j ..
     bool bad[2];
 };
 
 template <class E, int D>
 __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s, int lane, int wave,
-                                       unsigned char* meet) {
-    typedef Attend<E, D, 1, false> A;
+                                       unsigned char* meet0, unsigned char* meet1) {
+    typedef Attend<E, D, 1> A;
     const int j = lane & 15;
     const int q = lane >> 4;
     const Row row = row_at(a, s, s.tile * kNarrowRows + j);
@@ -552,49 +556,63 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         }
     }
 
-    // ---- the waves' results meet in LDS: waves 2 and 3 give theirs to 0 and 1, then
-    // wave 1 to wave 0, which stores; a lane finds its own row and dimensions ----
+    // ---- the waves' results meet in LDS ----
+    constexpr int kStride = D + 4;
+    typedef float Line[kStride];  // a row's sums
+    constexpr int kLines = 16 * kStride * (int)sizeof(float);
+    auto lines = [&](int w) { return (Line*)((w < 2 ? meet0 : meet1) + (w & 1) * kLines); };
+    auto stats = [&](int w) { return (float2v*)((w < 2 ? meet0 : meet1) + 2 * kLines + (w & 1) * 16 * sizeof(float2v)); };
     float l = quarters_sum(state.l_run[0]);
-    float m = state.seen[0] ? state.m_run[0] : -INFINITY;  // -inf: no key seen
-    float4v(*so)[A::kVd][64] = (float4v(*)[A::kVd][64])meet;
-    float2v(*st)[64] = (float2v(*)[64])(meet + 2 * sizeof(float4v) * A::kVd * 64);
-    const int waves = min(kWaves, (blocks - s.split + s.splits - 1) / s.splits);  // those with a block
-#pragma unroll
-    for (int half = 2; half > 0; half /= 2) {
-        if (waves <= half) continue;  // (the workgroup's)
-        if (half == 1) __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int dd = 0; dd < A::kVd; ++dd) so[wave - half][dd][lane] = state.o[0][dd];
-            st[wave - half][lane] = float2v{m, l};
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float2v other = st[wave][lane];
-            const float to = fmaxf(m, other[0]);
-            // (no key, or none that counts: factor zero, whatever its sums are; NaN is kept)
-            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 0.0f;
-            const float fo = other[0] > -INFINITY ? __builtin_amdgcn_exp2f(other[0] - to) : 0.0f;
-            const bool mine = f != 0.0f || l != l, its = fo != 0.0f || other[1] != other[1];
-            l = (mine ? l * f : 0.0f) + (its ? other[1] * fo : 0.0f);
-#pragma unroll
-            for (int dd = 0; dd < A::kVd; ++dd) {
-                const float4v x = so[wave][dd][lane];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float part = mine ? state.o[0][dd][r] * f : 0.0f;
-                    state.o[0][dd][r] = its ? fmaf(x[r], fo, part) : part;
-                }
-            }
-            m = to;
-        }
-    }
-    if (wave != 0) return;
     if (row.beyond && s.split == 0) {
         l = __builtin_nanf("");
-        m = fmaxf(m, kScoreFloor);
+        state.seen[0] = true;
     }
-    state.store(a, s, row, 0, l, m, q);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; dd += 4)
+            *(float4v*)&lines(wave)[j][A::kVd * (4 * q + r) + dd] =
+                float4v{state.o[0][dd][r], state.o[0][dd + 1][r], state.o[0][dd + 2][r], state.o[0][dd + 3][r]};
+    if (q == 0) stats(wave)[j] = float2v{state.seen[0] ? state.m_run[0] : -INFINITY, l};  // -inf: no key seen
+    __syncthreads();
+    // thread t: row t / 16, dimensions kVd (t % 16) ..
+    const int tid = 64 * wave + lane;
+    const int g = tid / 16;
+    const int d0 = A::kVd * (tid % 16);
+    const PagedAttnArgs late = late_arguments();
+    const Row mine = row_at(late, s, s.tile * kNarrowRows + g);
+    if (!mine.live) return;
+    float2v st[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) st[w] = stats(w)[g];
+    const float top = fmaxf(fmaxf(st[0][0], st[1][0]), fmaxf(st[2][0], st[3][0]));
+    float sum[A::kVd] = {};
+    l = 0.0f;
+    if (top > -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(st[w][0] - top);
+            // (no key, or none that counts: left out, whatever its sums are; NaN is kept)
+            if (f == 0.0f && st[w][1] == st[w][1]) continue;
+            l = fmaf(st[w][1], f, l);
+#pragma unroll
+            for (int i = 0; i < A::kVd; ++i) sum[i] = fmaf(lines(w)[g][d0 + i], f, sum[i]);
+        }
+    }
+    if (late.slots == 1) {
+        const float inv = top > -INFINITY ? 1.0f / l : 0.0f;
+        typename A::vword x;
+#pragma unroll
+        for (int i = 0; i < A::kVw; ++i) x[i] = E::pack(sum[2 * i] * inv, sum[2 * i + 1] * inv);
+        *(typename A::vword*)(late.out + mine.token * late.out_row + mine.head * late.out_head + d0) = x;
+        return;
+    }
+    const int64_t slot = slot_of(late, s, mine);
+    if (tid % 16 == 0) *(float2v*)(late.stats + 2 * slot) = float2v{top, l};
+    if (top == -INFINITY) return;  // (the join does not read it)
+#pragma unroll
+    for (int i = 0; i < A::kVd; i += 4)
+        *(float4v*)(late.partials + slot * D + d0 + i) = float4v{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
 }
 
 // ---- wide ----
@@ -637,7 +655,7 @@ struct Tile {
 template <class E, int D>
 __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
                                      unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves]) {
-    typedef Attend<E, D, 2, true> A;
+    typedef Attend<E, D, 2> A;
     typedef Tile<D> T;
     const int j = lane & 15;
     const int q = lane >> 4;
@@ -815,24 +833,42 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
             all_landed();
         }
     }
+    const PagedAttnArgs late = late_arguments();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         float l = quarters_sum(state.l_run[u]);
         float m = state.seen[u] ? state.m_run[u] : -INFINITY;
-        const Row row = row_at(a, s, rare(m0 + 16 * u + j));  // (again: not kept in registers over the keys)
+        const Row row = row_at(late, s, rare(m0 + 16 * u + j));  // (again: not kept in registers over the keys)
+        if (!row.live) continue;
         if (row.beyond && s.split == 0) {
             l = __builtin_nanf("");
             m = fmaxf(m, kScoreFloor);
         }
-        state.store(a, s, row, u, l, m, q);
+        if (late.slots == 1) {
+            const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
+            uint16_t* to = late.out + row.token * late.out_row + row.head * late.out_head + 4 * q;
+#pragma unroll
+            for (int dd = 0; dd < A::kVd; ++dd) {
+                const float4v x = state.o[u][dd];
+                *(u32x2*)(to + 16 * dd) = u32x2{E::pack(x[0] * inv, x[1] * inv), E::pack(x[2] * inv, x[3] * inv)};
+            }
+            continue;
+        }
+        const int64_t slot = slot_of(late, s, row);
+        if (q == 0) *(float2v*)(late.stats + 2 * slot) = float2v{m, l};
+        if (m == -INFINITY) continue;  // (the join does not read it)
+        float* to = late.partials + slot * D + 4 * q;
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; ++dd) *(float4v*)(to + 16 * dd) = state.o[u][dd];
     }
 }
 
 // kWide: the prefix or the own segments go by wide tiles.
 template <class E, int D, bool kWide>
 __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
-    constexpr int kMeet = 2 * 64 * (D + 8);  // two narrow waves' sums and statistics
-    __shared__ __attribute__((aligned(16))) unsigned char k0[kMeet];
+    constexpr int kMeet = 2 * 16 * (4 * (D + 4) + 8);  // two narrow waves' sums and statistics
+    static_assert(kMeet >= Tile<D>::kBytes, "or a wide tile's keys");
+    __shared__ __attribute__((aligned(16))) unsigned char k0[kMeet], k1[kMeet];
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -845,16 +881,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnA
     Segment s;
     if (!find_segment(a, lane, s)) return;
     if constexpr (kWide) {
-        static_assert(kMeet >= Tile<D>::kBytes, "a tile's keys fit");
         // (objects of their own: a read of one does not wait for loads into another)
-        __shared__ __attribute__((aligned(16))) unsigned char v0[Tile<D>::kBytes], k1[Tile<D>::kBytes], v1[Tile<D>::kBytes];
+        __shared__ __attribute__((aligned(16))) unsigned char v0[Tile<D>::kBytes], v1[Tile<D>::kBytes];
         __shared__ int bad[2][kWaves];
-        if (s.shared ? a.prefix_wide : a.own_wide) {
+        if (s.wide) {
             wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad);
             return;
         }
     }
-    narrow<E, D>(a, s, lane, wave, k0);
+    narrow<E, D>(a, s, lane, wave, k0, k1);
 }
 
 // One wave per (packed row, query head): lane l's D / 32 dimensions of the slots
@@ -866,38 +901,40 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
     const int lane = threadIdx.x & 63;
     const int index = (int)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (index >= a.rows * a.heads) return;
-    const int row = (uint32_t)index / (uint32_t)a.heads;
+    const int row = a.by_heads(index);
     const int head = index - row * a.heads;
     const int64_t at = index;
     uint16_t* to = a.out + row * a.out_row + head * a.out_head;
-    if (row >= a.c.cu_rows[a.c.batch]) {  // behind the last sequence
-        if (a.zero_rest && lane < D / 8) *(u32x4*)(to + 8 * lane) = u32x4{0u, 0u, 0u, 0u};
-        return;
-    }
     const float* stats = a.stats + 2 * at * a.slots;
     const bool has = lane < a.slots;
-    const float m = has ? stats[2 * lane] : -INFINITY;
-    const float sum_l = has ? stats[2 * lane + 1] : 0.0f;
-    const float top = wave_max64(m);
-    const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-    const float l = wave_sum64(f != 0.0f || sum_l != sum_l ? sum_l * f : 0.0f);  // (NaN: a page that was not there)
     float sum[kPer] = {};
     const float* part = a.partials + at * a.slots * D + kPer * (lane % 32);
     const int half = lane / 32;
-    for (int first = 0; first < a.slots; first += 8) {  // eight slots' loads at once
-        fvec x[4];
-        float fs[4];
+    // Eight slots' loads at once, the first ones before the statistics arrive: a slot
+    // that nobody wrote has a factor of zero and is left out, whatever it holds.
+    fvec x[4];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *(const fvec*)(part + min(first + 2 * i + half, a.slots - 1) * D);
+    };
+    load(0);
+    const float m = has ? stats[2 * lane] : -INFINITY;
+    const float sum_l = has ? stats[2 * lane + 1] : 0.0f;
+    if (row >= scalar_load(a.c.cu_rows, a.c.batch)) {  // behind the last sequence
+        if (a.zero_rest && lane < D / 8) *(u32x4*)(to + 8 * lane) = u32x4{0u, 0u, 0u, 0u};
+        return;
+    }
+    const float top = wave_max64(m);
+    const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
+    const float l = wave_sum64(f != 0.0f || sum_l != sum_l ? sum_l * f : 0.0f);  // (NaN: a page that was not there)
+    for (int first = 0; first < a.slots; first += 8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int slot = first + 2 * i + half;
-            fs[i] = __shfl(f, min(slot, 63));  // (0 past the slots)
-            x[i] = fvec{};
-            if (fs[i] != 0.0f) x[i] = *(const fvec*)(part + slot * D);
+            const float fs = __shfl(f, min(first + 2 * i + half, 63));  // (0 past the slots)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) sum[e] = fs != 0.0f ? fmaf(x[i][e], fs, sum[e]) : sum[e];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) sum[e] = fs[i] != 0.0f ? fmaf(x[i][e], fs[i], sum[e]) : sum[e];
+        if (first + 8 < a.slots) load(first + 8);
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum[e] += __shfl_xor(sum[e], 32);
@@ -924,21 +961,20 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
         const int64_t most = (keys + least_keys - 1) / least_keys;
         int64_t s = 512 > workgroups ? 512 / workgroups : 1;
         s = s < most ? s : most;
-        s = s < kMaxSplits / 2 ? s : kMaxSplits / 2;
-        // tiles of the same keys on one XCD (workgroups go to the eight in turn)
-        const int64_t turn = c.kv_heads % 8 == 0 ? 1 : c.kv_heads % 4 == 0 ? 2 : c.kv_heads % 2 == 0 ? 4 : 8;
-        return s > turn ? s - s % turn : s;
+        return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
     };
     if (p.prefix > 0) {
-        p.prefix_wide = rows * group >= 64;
+        p.prefix_wide = rows * group > kWideFrom;
         const int64_t tile = p.prefix_wide ? kWideRows : kNarrowRows;
         p.prefix_tiles = (rows * group + tile - 1) / tile;
         p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix, kBlock * kWaves);
     }
     if (own > 0) {
-        p.own_wide = rows * group >= 64 * sequences;
-        const int64_t tile = p.own_wide ? kWideRows : kNarrowRows;
-        p.own_tiles = rows * group / tile + sequences;
+        // (on the average; the sequences with few rows among them go by narrow tiles
+        // all the same: at most four each)
+        p.own_wide = rows * group > kWideFrom * sequences;
+        p.own_tiles = p.own_wide ? rows * group / kWideRows + kWideFrom / kNarrowRows * sequences
+                                 : rows * group / kNarrowRows + sequences;
         p.own_splits = splits(p.own_tiles * c.kv_heads, own, kBlock * kWaves);
     }
     p.slots = p.prefix_splits + p.own_splits;
@@ -1027,6 +1063,8 @@ int qwen2_paged_attention(const qwen2_paged_cache* cache, const qwen2_rows* q, c
     a.prefix_tiles = (int)p.prefix_tiles, a.prefix_splits = (int)p.prefix_splits;
     a.own_tiles = (int)p.own_tiles, a.own_splits = (int)p.own_splits, a.slots = (int)p.slots;
     a.prefix_wide = p.prefix_wide, a.own_wide = p.own_wide;
+    a.by_group = divisor(a.group), a.by_heads = divisor(heads), a.by_kv_heads = divisor(cache->kv_heads);
+    a.by_prefix_splits = divisor(p.prefix_splits), a.by_own_splits = divisor(p.own_splits);
     a.zero_rest = zero_rest;
     const hipStream_t s = (hipStream_t)stream;
     hipError_t err;
