@@ -138,11 +138,21 @@ __device__ __forceinline__ int running_sum(int v) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t keep_halves(uint32_t w, bool lo, bool hi) {
-    return w & ((lo ? 0x0000FFFFu : 0u) | (hi ? 0xFFFF0000u : 0u));
+// Values that are not finite (an infinity or a NaN, met in the sums of a first
+// pass) must reach the rows that see their keys and no others, where a product
+// with a probability of zero would give NaN.  Three more passes tell: two that
+// count, for every row and dimension, the visible keys with +inf or NaN and with
+// -inf or NaN (ones in place of probabilities and of such values), and one over
+// the finite values alone.
+enum Pass { kOrdinary, kCountUp, kCountDown, kFinite };
+template <class E> __device__ __forceinline__ uint32_t pass_half(uint32_t h, Pass pass) {
+    const bool odd = (h & E::kExponent) == E::kExponent;
+    if (pass == kFinite) return odd ? 0u : h;
+    const bool nan = (h & 0x7FFFu) > E::kExponent, down = (h & 0x8000u) != 0;
+    return odd && (nan || down == (pass == kCountDown)) ? E::kOne : 0u;
 }
-template <class E> __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
-    return keep_halves(w, (w & E::kExponent) != E::kExponent, ((w >> 16) & E::kExponent) != E::kExponent);
+template <class E> __device__ __forceinline__ uint32_t pass_word(uint32_t w, Pass pass) {
+    return pass_half<E>(w & 0xFFFFu, pass) | (pass_half<E>(w >> 16, pass) << 16);
 }
 
 // Whether a sequence's own rows go by wide tiles, where the call has any.
@@ -351,43 +361,47 @@ struct Attend {
         }
     }
 
-    // Product dd of the value sums of 32 keys from t0: vt holds, for the product's row
-    // j, the values of the lane's keys 16 (e / 4) + 4 q + e % 4.
-    template <bool kCareful>
-    __device__ __forceinline__ void gather(int dd, const u32x4& vt, const u32x4 (&ph)[kTiles], const u32x4 (&pl)[kTiles],
-                                           const int (&limit)[kTiles], int t0, int j, int q) {
-        if constexpr (!kCareful) {
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, ph[u], o[u][dd]);
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, pl[u], o[u][dd]);
-            return;
-        }
-        // A value that is not finite must reach only the rows that see its key (0 * inf
-        // is NaN): the finite ones as always, the others column by column with what the
-        // column does not see at zero.
-        u32x4 plain, odd;
+    // Eight of tile u's keys from t0 as ones where the row sees them.
+    __device__ __forceinline__ static void show(int limit, int t0, int q, u32x4& ph, u32x4& pl) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            plain[e] = finite_halves<E>(vt[e]);
-            odd[e] = vt[e] & ~plain[e];
+            const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
+            ph[e] = (t <= limit ? E::kOne : 0u) | (t + 1 <= limit ? E::kOne << 16 : 0u);
+            pl[e] = 0u;
         }
+    }
+
+    // Product dd of the value sums of 32 keys: vt holds, for the product's row j, the
+    // values of the lane's keys 16 (e / 4) + 4 q + e % 4.
+    __device__ __forceinline__ void gather(int dd, const u32x4& vt, const u32x4 (&ph)[kTiles], const u32x4 (&pl)[kTiles]) {
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u) {
-            o[u][dd] = E::mfma(plain, ph[u], o[u][dd]);
-            o[u][dd] = E::mfma(plain, pl[u], o[u][dd]);
-            for (int c = 0; c < 16; ++c) {
-                const int sees = __builtin_amdgcn_readlane(limit[u], c);
-                u32x4 part;
+        for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, ph[u], o[u][dd]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + 16 * (e / 2) + 4 * q + 2 * (e % 2);
-                    part[e] = keep_halves(odd[e], t <= sees, t + 1 <= sees);
+        for (int u = 0; u < kTiles; ++u) o[u][dd] = E::mfma(vt, pl[u], o[u][dd]);
+    }
+
+    // After a counting pass: which sums are not zero, a bit each; and what they say.
+    __device__ __forceinline__ uint64_t marks() const {
+        uint64_t m = 0;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+            for (int dd = 0; dd < kVd; ++dd)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m |= (uint64_t)(o[u][dd][r] != 0.0f) << ((u * kVd + dd) * 4 + r);
+        return m;
+    }
+    __device__ __forceinline__ void mark(uint64_t up, uint64_t down) {
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+            for (int dd = 0; dd < kVd; ++dd)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int bit = (u * kVd + dd) * 4 + r;
+                    const float plus = (up >> bit) & 1 ? INFINITY : 0.0f, minus = (down >> bit) & 1 ? INFINITY : 0.0f;
+                    o[u][dd][r] += plus - minus;  // (both: NaN)
                 }
-                const float4v more = E::mfma(part, ph[u], float4v{0.0f, 0.0f, 0.0f, 0.0f});
-                if (j == c) o[u][dd] += more;
-            }
-        }
     }
 
     __device__ __forceinline__ bool finite() const {
@@ -446,19 +460,24 @@ struct KeyBlock {
     bool bad[2];
 };
 
+// A workgroup's 32-key blocks of its segment: begin, begin + step, ... below end.
+struct KeyRange {
+    int begin, step, end;
+};
+
 template <class E, int D>
-__device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s, int lane, int wave,
-                                       unsigned char* meet0, unsigned char* meet1) {
+__device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s, int tile, const KeyRange& keys, int lane,
+                                       int wave, unsigned char* meet0, unsigned char* meet1) {
     typedef Attend<E, D, 1> A;
     const int j = lane & 15;
     const int q = lane >> 4;
-    const Row row = row_at(a, s, s.tile * kNarrowRows + j);
+    const Row row = row_at(a, s, tile * kNarrowRows + j);
     u32x4 qf[A::kSteps];
     load_queries(a, row, q, qf);
     int least, most;
-    limits(a, s, row, s.tile * kNarrowRows, kNarrowRows, least, most);
-    const int blocks = most >= s.key_lo ? (most - s.key_lo) / kBlock + 1 : 0;
-    const int stride = s.splits * kWaves;
+    limits(a, s, row, tile * kNarrowRows, kNarrowRows, least, most);
+    const int blocks = min(most >= s.key_lo ? (most - s.key_lo) / kBlock + 1 : 0, keys.end);
+    const int first = keys.begin + keys.step * wave, stride = keys.step * kWaves;
 
     const uint16_t* kc = a.c.k + s.kvh * a.c.k_head;
     const uint16_t* vc = a.c.v + s.kvh * a.c.v_head;
@@ -489,7 +508,7 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         }
     };
     A state;
-    auto compute = [&](KeyBlock<E, D>& b, int block, auto careful) {
+    auto compute = [&](KeyBlock<E, D>& b, int block, auto ordinary, Pass pass) {
         const int t0 = s.key_lo + block * kBlock;
         float x[8];
 #pragma unroll
@@ -514,21 +533,27 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         for (int h = 0; h < 2; ++h)
             if (b.bad[h] && t0 + 16 * h <= row.limit) state.l_run[0] = __builtin_nanf("");
         u32x4 h1[1], l1[1];
-        state.settle(0, x, a.scale2);
-        state.soften(0, x, 0, h1[0], l1[0], a.scale2);
-        const int limit[1] = {row.limit};
+        if (ordinary || pass == kFinite) {
+            state.settle(0, x, a.scale2);
+            state.soften(0, x, 0, h1[0], l1[0], a.scale2);
+        } else {
+            A::show(row.limit, t0, q, h1[0], l1[0]);
+        }
 #pragma unroll
         for (int dd = 0; dd < A::kVd; ++dd) {
             const uint32_t sel = (dd & 1) ? 0x07060302u : 0x05040100u;  // high or low halves
             u32x4 vt;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vt[e] = __builtin_amdgcn_perm(b.v[2 * e + 1][dd / 2], b.v[2 * e][dd / 2], sel);
-            state.template gather<decltype(careful)::value>(dd, vt, h1, l1, limit, t0, j, q);
+            for (int e = 0; e < 4; ++e) {
+                vt[e] = __builtin_amdgcn_perm(b.v[2 * e + 1][dd / 2], b.v[2 * e][dd / 2], sel);
+                if constexpr (!ordinary) vt[e] = pass_word<E>(vt[e], pass);
+            }
+            state.gather(dd, vt, h1, l1);
         }
     };
     // Two blocks in flight, the pages of a third known.
     state.start();
-    int block = s.split + s.splits * wave;
+    int block = first;
     if (block < blocks) {
         KeyBlock<E, D> buf[2];
         load(buf[0], block, look(block));
@@ -536,24 +561,31 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         while (true) {
             if (block + stride < blocks) load(buf[1], block + stride, next);
             next = look(block + 2 * stride);
-            compute(buf[0], block, std::false_type{});
+            compute(buf[0], block, std::true_type{}, kOrdinary);
             block += stride;
             if (block >= blocks) break;
             if (block + stride < blocks) load(buf[0], block + stride, next);
             next = look(block + 2 * stride);
-            compute(buf[1], block, std::false_type{});
+            compute(buf[1], block, std::true_type{}, kOrdinary);
             block += stride;
             if (block >= blocks) break;
         }
     }
-    // (value sums that came out infinite or NaN: once more, with care)
-    if (!__all(state.finite())) {
-        state.start();
-        for (block = s.split + s.splits * wave; block < blocks; block += stride) {
-            KeyBlock<E, D> b;
-            load(b, block, look(block));
-            compute(b, block, std::true_type{});
+    if (!__all(state.finite())) {  // (the wave's)
+        uint64_t up = 0, down = 0;
+#pragma unroll 1
+        for (int pass = kCountUp; pass <= kFinite; ++pass) {
+            state.start();
+#pragma unroll 1
+            for (block = first; block < blocks; block += stride) {
+                KeyBlock<E, D> b;
+                load(b, block, look(block));
+                compute(b, block, std::false_type{}, (Pass)pass);
+            }
+            if (pass == kCountUp) up = state.marks();
+            if (pass == kCountDown) down = state.marks();
         }
+        state.mark(up, down);
     }
 
     // ---- the waves' results meet in LDS ----
@@ -580,7 +612,7 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
     const int g = tid / 16;
     const int d0 = A::kVd * (tid % 16);
     const PagedAttnArgs late = late_arguments();
-    const Row mine = row_at(late, s, s.tile * kNarrowRows + g);
+    const Row mine = row_at(late, s, tile * kNarrowRows + g);
     if (!mine.live) return;
     float2v st[kWaves];
 #pragma unroll
@@ -652,9 +684,12 @@ struct Tile {
     static __device__ __forceinline__ int value_turn(int row) { return D == 128 ? 2 * (row & 7) : row & 6; }
 };
 
+// false, with nothing stored, where a value sum came out infinite or NaN: the
+// rows are then left to narrow(), over the keys given back.
 template <class E, int D>
-__device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
-                                     unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves]) {
+__device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
+                                     unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves],
+                                     KeyRange& keys) {
     typedef Attend<E, D, 2> A;
     typedef Tile<D> T;
     const int j = lane & 15;
@@ -726,7 +761,7 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
         }
     };
     A state;
-    auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, const int* flags, auto careful) {
+    auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, const int* flags) {
         const int t0 = s.key_lo + tile * kTileKeys;
         if (t0 > most) return;  // (the wave's)
         float x[2][16];
@@ -796,7 +831,7 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
                 if (dd + 1 < A::kVd) load_values(i, dd + 1);
                 else if (i == 0) load_values(1, 0);
                 __builtin_amdgcn_sched_barrier(0x7);  // (no LDS read past this; arithmetic as it likes)
-                state.template gather<decltype(careful)::value>(dd, vt[dd & 1], ph, pl, limit, t0 + 32 * i, j, q);
+                state.gather(dd, vt[dd & 1], ph, pl);
             }
         }
     };
@@ -811,27 +846,19 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
             all_landed();
             if (tile + 1 < end) stage(tile + 1, next, k1, v1, bad[1]);
             next = look(tile + 2);
-            compute(tile, k0, v0, bad[0], std::false_type{});
+            compute(tile, k0, v0, bad[0]);
             if (++tile >= end) break;
             settle(tile, v1);
             all_landed();
             if (tile + 1 < end) stage(tile + 1, next, k0, v0, bad[0]);
             next = look(tile + 2);
-            compute(tile, k1, v1, bad[1], std::false_type{});
+            compute(tile, k1, v1, bad[1]);
             if (++tile >= end) break;
         }
     }
-    // (value sums that came out infinite or NaN: once more, with care; all waves,
-    // for the tiles are brought by all)
-    if (__syncthreads_or(!state.finite())) {
-        state.start();
-        for (int tile = begin; tile < end; ++tile) {
-            stage(tile, look(tile), k0, v0, bad[0]);
-            settle(tile, v0);
-            all_landed();
-            compute(tile, k0, v0, bad[0], std::true_type{});
-            all_landed();
-        }
+    if (__syncthreads_or(!state.finite())) {  // (the workgroup's)
+        keys = KeyRange{kTileKeys / kBlock * begin, 1, kTileKeys / kBlock * end};
+        return false;
     }
     const PagedAttnArgs late = late_arguments();
 #pragma unroll
@@ -861,6 +888,7 @@ __device__ __forceinline__ void wide(const PagedAttnArgs& a, const Segment& s, i
 #pragma unroll
         for (int dd = 0; dd < A::kVd; ++dd) *(float4v*)(to + 16 * dd) = state.o[u][dd];
     }
+    return true;
 }
 
 // kWide: the prefix or the own segments go by wide tiles.
@@ -880,16 +908,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnA
     }
     Segment s;
     if (!find_segment(a, lane, s)) return;
+    int tile = s.tile, past = tile + 1;
+    KeyRange keys{s.split, s.splits, 0x7FFFFFFF};
     if constexpr (kWide) {
         // (objects of their own: a read of one does not wait for loads into another)
         __shared__ __attribute__((aligned(16))) unsigned char v0[Tile<D>::kBytes], v1[Tile<D>::kBytes];
         __shared__ int bad[2][kWaves];
         if (s.wide) {
-            wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad);
-            return;
+            if (wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad, keys)) return;
+            tile *= kWideRows / kNarrowRows;
+            past = tile + kWideRows / kNarrowRows;
         }
     }
-    narrow<E, D>(a, s, lane, wave, k0, k1);
+    while (true) {
+        narrow<E, D>(a, s, tile, keys, lane, wave, k0, k1);
+        if (++tile >= past) break;
+        __syncthreads();  // (LDS is free again)
+    }
 }
 
 // One wave per (packed row, query head): lane l's D / 32 dimensions of the slots

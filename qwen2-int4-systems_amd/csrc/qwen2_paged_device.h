@@ -15,6 +15,7 @@ struct Bf16 {
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
     static constexpr uint32_t kExponent = 0x7F80u;  // all ones: an infinity or NaN
+    static constexpr uint32_t kOne = 0x3F80u;
     static __device__ __forceinline__ float4v mfma(const u32x4& a, const u32x4& b, const float4v& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -28,6 +29,7 @@ struct F16 {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{a, b}, half2v));
     }
     static constexpr uint32_t kExponent = 0x7C00u;
+    static constexpr uint32_t kOne = 0x3C00u;
     static __device__ __forceinline__ float4v mfma(const u32x4& a, const u32x4& b, const float4v& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
                                                       0, 0);

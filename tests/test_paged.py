@@ -436,6 +436,35 @@ def test_what_a_row_does_not_see_takes_no_part(dtype, shared, bad):
 
 
 @gpu
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("shared", [0, 9])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_values_that_are_not_finite_among_many_rows(dtype, dim, shared, bad):
+    """Sequences of 40, one and 30 rows, 6 query heads each: whole values at one new
+    position, and one element that all rows see, in the prefix or at the start."""
+    p = Paged([40, 1, 30], [21, 70, 3], shared=shared, dtype=dtype, heads=12, dim=dim)
+    want, slack = p.reference()
+    spot = shared * 16 + 21 + 17
+    page, place = p.used[0][spot // 16], spot % 16
+    kept = p.v_pages[page, :, place].clone()
+    p.v_pages[page, :, place] = bad
+    got = p.attention()
+    _near(got[:17], want[:17], slack[:17])
+    _near(got[40:], want[40:], slack[40:])
+    assert bool((got[17:40].isnan() if math.isnan(bad) else got[17:40] == bad).all())
+    p.v_pages[page, :, place] = kept
+    p.v_pages[p.used[0][0], 1, 3, 7] = bad  # (key/value head 1: query heads 6 ..)
+    got = p.attention()
+    touched = torch.zeros_like(got, dtype=torch.bool)
+    touched[:71 if shared else 40, 6:, 7] = True
+    seen = got[touched]
+    assert bool((seen.isnan() if math.isnan(bad) else seen == bad).all())
+    _near(torch.where(touched, 0, got), torch.where(touched, 0.0, want), slack)
+    p.v_pages[p.used[0][0], 1, 4, 7] = -bad  # (another key's: their sum has no value)
+    assert bool(p.attention()[touched].isnan().all())
+
+
+@gpu
 @pytest.mark.parametrize("shared", [0, 2])
 def test_pages_that_are_not_there_give_nan(shared):
     p = Paged([3, 2, 1], [40, 2, 100], shared=shared, heads=6)
