@@ -551,24 +551,14 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
             state.gather(dd, vt, h1, l1);
         }
     };
-    // Two blocks in flight, the pages of a third known.
     state.start();
-    int block = first;
-    if (block < blocks) {
-        KeyBlock<E, D> buf[2];
-        load(buf[0], block, look(block));
-        Pages next = look(block + stride);
-        while (true) {
-            if (block + stride < blocks) load(buf[1], block + stride, next);
-            next = look(block + 2 * stride);
-            compute(buf[0], block, std::true_type{}, kOrdinary);
-            block += stride;
-            if (block >= blocks) break;
-            if (block + stride < blocks) load(buf[0], block + stride, next);
-            next = look(block + 2 * stride);
-            compute(buf[1], block, std::true_type{}, kOrdinary);
-            block += stride;
-            if (block >= blocks) break;
+    {
+        Pages next = look(first);
+        for (int block = first; block < blocks; block += stride) {
+            KeyBlock<E, D> b;
+            load(b, block, next);
+            next = look(block + stride);
+            compute(b, block, std::true_type{}, kOrdinary);
         }
     }
     if (!__all(state.finite())) {  // (the wave's)
@@ -577,7 +567,7 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         for (int pass = kCountUp; pass <= kFinite; ++pass) {
             state.start();
 #pragma unroll 1
-            for (block = first; block < blocks; block += stride) {
+            for (int block = first; block < blocks; block += stride) {
                 KeyBlock<E, D> b;
                 load(b, block, look(block));
                 compute(b, block, std::false_type{}, (Pass)pass);
@@ -893,7 +883,7 @@ __device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, i
 
 // kWide: the prefix or the own segments go by wide tiles.
 template <class E, int D, bool kWide>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, kWide ? 2 : 3) void paged_attention_kernel(PagedAttnArgs a) {
     constexpr int kMeet = 2 * 16 * (4 * (D + 4) + 8);  // two narrow waves' sums and statistics
     static_assert(kMeet >= Tile<D>::kBytes, "or a wide tile's keys");
     __shared__ __attribute__((aligned(16))) unsigned char k0[kMeet], k1[kMeet];
@@ -992,25 +982,28 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
     const int64_t sequences = c.batch < rows ? c.batch : rows;
     p.prefix = shared_pages << c.page_shift;
     const int64_t own = ((int64_t)c.table_width - shared_pages) << c.page_shift;
-    auto splits = [&](int64_t workgroups, int64_t keys, int64_t least_keys) {
-        const int64_t most = (keys + least_keys - 1) / least_keys;
-        int64_t s = 512 > workgroups ? 512 / workgroups : 1;
+    // as many as the chip holds at once (two workgroups of a CU with wide tiles, three
+    // without), but a block for each wave
+    auto splits = [&](int64_t workgroups, int64_t keys) {
+        const int64_t hold = 256 * (p.prefix_wide || p.own_wide ? 2 : 3);
+        const int64_t most = (keys + kBlock * kWaves - 1) / (kBlock * kWaves);
+        int64_t s = hold > workgroups ? hold / workgroups : 1;
         s = s < most ? s : most;
         return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
     };
+    // (own: on the average; the sequences with few rows among them go by narrow tiles
+    // all the same, at most four each)
+    p.prefix_wide = p.prefix > 0 && rows * group > kWideFrom;
+    p.own_wide = own > 0 && rows * group > kWideFrom * sequences;
     if (p.prefix > 0) {
-        p.prefix_wide = rows * group > kWideFrom;
         const int64_t tile = p.prefix_wide ? kWideRows : kNarrowRows;
         p.prefix_tiles = (rows * group + tile - 1) / tile;
-        p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix, kBlock * kWaves);
+        p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix);
     }
     if (own > 0) {
-        // (on the average; the sequences with few rows among them go by narrow tiles
-        // all the same: at most four each)
-        p.own_wide = rows * group > kWideFrom * sequences;
         p.own_tiles = p.own_wide ? rows * group / kWideRows + kWideFrom / kNarrowRows * sequences
                                  : rows * group / kNarrowRows + sequences;
-        p.own_splits = splits(p.own_tiles * c.kv_heads, own, kBlock * kWaves);
+        p.own_splits = splits(p.own_tiles * c.kv_heads, own);
     }
     p.slots = p.prefix_splits + p.own_splits;
     return p;
