@@ -117,17 +117,8 @@ __device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
     return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p + i);
 }
 
-// Over the 16 lanes of a row (quad swaps, half-row and row mirrors), and running
-// sums over the wave (shifts within rows, then their last lanes passed on).
-template <int kControl> __device__ __forceinline__ int dpp_row(int v) {
-    return __builtin_amdgcn_update_dpp(v, v, kControl, 0xF, 0xF, false);
-}
-__device__ __forceinline__ int row_max(int v) {
-    v = max(v, dpp_row<0xB1>(v));
-    v = max(v, dpp_row<0x4E>(v));
-    v = max(v, dpp_row<0x141>(v));
-    return max(v, dpp_row<0x140>(v));
-}
+// Running sums over the wave (shifts within rows of 16 lanes, then their last lanes
+// passed on).
 __device__ __forceinline__ int running_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
@@ -432,22 +423,19 @@ __device__ __forceinline__ void load_queries(const PagedAttnArgs& a, const Row& 
 }
 
 // Least and largest limit over rows m0 .. m0 + count - 1 of a segment (those that
-// there are): an own segment's rise with the row; where a prefix is not all
-// seen, over the lanes of `row`, 16 rows.
-__device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s, const Row& row, int m0, int count,
-                                       int& least, int& most) {
+// there are): an own segment's rise with the row; where a prefix is not all seen,
+// the widest they can be.
+__device__ __forceinline__ void limits(const PagedAttnArgs& a, const Segment& s, int m0, int count, int& least, int& most) {
     const int last = min(m0 + count, s.count) - 1;
     if (last < m0) {
         least = 0x7FFFFFFF, most = s.key_lo - 1;
-    } else if (s.sees_all) {
-        least = most = (int)s.key_end - 1;
-    } else if (!s.shared) {
+    } else if (s.shared) {
+        most = (int)s.key_end - 1;
+        least = s.sees_all ? most : s.key_lo - 1;
+    } else {
         const int64_t first = s.first + a.by_group(m0), end = s.first + a.by_group(last);
         least = (int)max(min(first, s.key_end - 1), (int64_t)(s.key_lo - 1));
         most = (int)max(min(end, s.key_end - 1), (int64_t)(s.key_lo - 1));
-    } else {
-        most = __builtin_amdgcn_readfirstlane(row_max(row.live ? row.limit : s.key_lo - 1));
-        least = -__builtin_amdgcn_readfirstlane(row_max(row.live ? -row.limit : -0x7FFFFFFF));
     }
 }
 
@@ -471,11 +459,8 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
     typedef Attend<E, D, 1> A;
     const int j = lane & 15;
     const int q = lane >> 4;
-    const Row row = row_at(a, s, tile * kNarrowRows + j);
-    u32x4 qf[A::kSteps];
-    load_queries(a, row, q, qf);
     int least, most;
-    limits(a, s, row, tile * kNarrowRows, kNarrowRows, least, most);
+    limits(a, s, tile * kNarrowRows, kNarrowRows, least, most);
     const int blocks = min(most >= s.key_lo ? (most - s.key_lo) / kBlock + 1 : 0, keys.end);
     const int first = keys.begin + keys.step * wave, stride = keys.step * kWaves;
 
@@ -507,6 +492,13 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
                 b.v[4 * h + r] = *(const typename A::vword*)(vp + v_lane + r * (int)a.c.v_position);
         }
     };
+    // the first block is on its way before the rows and their queries are looked up
+    KeyBlock<E, D> b;
+    if (first < blocks) load(b, first, look(first));
+    Pages next = look(first + stride);
+    const Row row = row_at(a, s, tile * kNarrowRows + j);
+    u32x4 qf[A::kSteps];
+    load_queries(a, row, q, qf);
     A state;
     auto compute = [&](KeyBlock<E, D>& b, int block, auto ordinary, Pass pass) {
         const int t0 = s.key_lo + block * kBlock;
@@ -552,14 +544,11 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
         }
     };
     state.start();
-    {
-        Pages next = look(first);
-        for (int block = first; block < blocks; block += stride) {
-            KeyBlock<E, D> b;
-            load(b, block, next);
-            next = look(block + stride);
-            compute(b, block, std::true_type{}, kOrdinary);
-        }
+    for (int block = first; block < blocks;) {
+        compute(b, block, std::true_type{}, kOrdinary);
+        block += stride;
+        if (block < blocks) load(b, block, next);
+        next = look(block + stride);
     }
     if (!__all(state.finite())) {  // (the wave's)
         uint64_t up = 0, down = 0;
@@ -568,7 +557,6 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
             state.start();
 #pragma unroll 1
             for (int block = first; block < blocks; block += stride) {
-                KeyBlock<E, D> b;
                 load(b, block, look(block));
                 compute(b, block, std::false_type{}, (Pass)pass);
             }
@@ -679,29 +667,16 @@ struct Tile {
 template <class E, int D>
 __device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, int lane, int wave, unsigned char* k0,
                                      unsigned char* v0, unsigned char* k1, unsigned char* v1, int (*bad)[kWaves],
-                                     KeyRange& keys) {
+                                     int* odd, KeyRange& keys) {
     typedef Attend<E, D, 2> A;
     typedef Tile<D> T;
     const int j = lane & 15;
     const int q = lane >> 4;
     const int m0 = s.tile * kWideRows + 32 * wave;
-    u32x4 qf[2][A::kSteps];
-    int limit[2];
     // the wave's rows, then the workgroup's
-    int least = 0x7FFFFFFF, most = s.key_lo - 1, all_most = (int)s.key_end - 1;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const Row row = row_at(a, s, m0 + 16 * u + j);
-        limit[u] = row.limit;
-        load_queries(a, row, q, qf[u]);
-        int one, other;
-        limits(a, s, row, m0 + 16 * u, 16, one, other);
-        least = min(least, one), most = max(most, other);
-    }
-    if (!s.shared) {
-        int other;
-        limits(a, s, Row{}, s.tile * kWideRows, kWideRows, other, all_most);
-    }
+    int least, most, all_least, all_most;
+    limits(a, s, m0, 32, least, most);
+    limits(a, s, s.tile * kWideRows, kWideRows, all_least, all_most);
     const int tiles = all_most >= s.key_lo ? (all_most - s.key_lo) / kTileKeys + 1 : 0;
     const int per = (tiles + s.splits - 1) / s.splits;
     const int begin = s.split * per;
@@ -750,6 +725,17 @@ __device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, i
                 *(u32x4*)(values + (16 * wave + r) * T::kRowBytes + 16 * (lane % T::kPieces)) = u32x4{0u, 0u, 0u, 0u};
         }
     };
+    // the first tile is on its way before the rows and their queries are looked up
+    if (begin < end) stage(begin, look(begin), k0, v0, bad[0]);
+    int next = look(begin + 1);
+    u32x4 qf[2][A::kSteps];
+    int limit[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const Row row = row_at(a, s, m0 + 16 * u + j);
+        limit[u] = row.limit;
+        load_queries(a, row, q, qf[u]);
+    }
     A state;
     auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, const int* flags) {
         const int t0 = s.key_lo + tile * kTileKeys;
@@ -829,8 +815,6 @@ __device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, i
     // before the barrier.
     state.start();
     if (begin < end) {
-        stage(begin, look(begin), k0, v0, bad[0]);
-        int next = look(begin + 1);
         for (int tile = begin;;) {
             settle(tile, v0);
             all_landed();
@@ -846,7 +830,11 @@ __device__ __forceinline__ bool wide(const PagedAttnArgs& a, const Segment& s, i
             if (++tile >= end) break;
         }
     }
-    if (__syncthreads_or(!state.finite())) {  // (the workgroup's)
+    if (lane == 0) odd[wave] = 0;
+    if (!__all(state.finite()) && lane == 0) odd[wave] = 1;
+    __syncthreads();
+    if (odd[0] | odd[1] | odd[2] | odd[3]) {
+        __syncthreads();  // (LDS is free)
         keys = KeyRange{kTileKeys / kBlock * begin, 1, kTileKeys / kBlock * end};
         return false;
     }
@@ -903,9 +891,9 @@ __global__ __launch_bounds__(kThreads, kWide ? 2 : 3) void paged_attention_kerne
     if constexpr (kWide) {
         // (objects of their own: a read of one does not wait for loads into another)
         __shared__ __attribute__((aligned(16))) unsigned char v0[Tile<D>::kBytes], v1[Tile<D>::kBytes];
-        __shared__ int bad[2][kWaves];
+        __shared__ int bad[2][kWaves], odd[kWaves];
         if (s.wide) {
-            if (wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad, keys)) return;
+            if (wide<E, D>(a, s, lane, wave, k0, v0, k1, v1, bad, odd, keys)) return;
             tile *= kWideRows / kNarrowRows;
             past = tile + kWideRows / kNarrowRows;
         }
