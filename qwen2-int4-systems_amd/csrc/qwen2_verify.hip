@@ -1,11 +1,14 @@
 // Verification of drafted tokens (qwen2_verify_drafts, include/qwen2_decode.h).
 //
+//   verify_one_kernel   one workgroup per sequence does all of what follows;
 //   verify_sum_kernel   one wave per (sequence, span of 1024 entries of the
 //                       vocabulary): finds how many drafts stand (every wave
 //                       for itself: a few loads), then adds up its entries'
 //                       weights;
 //   verify_pick_kernel  one wave per sequence: the span in which the
 //                       running sum passes uniform * total, then the entry.
+// Where max(p - q, 0) is zero everywhere, the picking wave goes through the
+// target's row by itself.
 //
 // Only one row of the target's (and the draft's) probabilities is read per
 // sequence, 16 bytes a lane.  A weight is a difference of two 24-bit numbers and
@@ -13,8 +16,11 @@
 // entry is then the definition's, not the summation order's.  Sums have one
 // fixed order.
 //
-// Bound by the rows' read from memory, and for few sequences by its chain of
-// round trips (drafted id, its probabilities, the row, the launch between).
+// Bound by the rows' read from memory (64 x 4 drafts of 151936 fp32: 77.8 MB in
+// 13.9 us of the sums, 17 the call), and for few sequences by its chain of round
+// trips (drafted id, its probabilities, the row) and the host's launches, some 4 us
+// each.  First forms, us: 64 x 4 147 with single entries per lane and both sums in
+// every workgroup, 19.6 with 16-byte loads and the pick by one wave.
 #include <hip/hip_runtime.h>
 
 #include "qwen2_decode.h"
@@ -38,7 +44,7 @@ struct VerifyArgs {
     const float* uniforms;
     int64_t* tokens;
     int32_t* accepted;
-    double* sums;      // [batch][spans][2]: of the weights, and of the target alone
+    double* sums;      // [batch][spans]
     int32_t* standing; // [batch]
     int batch, drafts, vocab, spans;
 };
@@ -49,9 +55,6 @@ __device__ __forceinline__ double value(const void* p, int64_t i) {
     if constexpr (XK == kBF16) return (double)bf16_bits_to_float(((const uint16_t*)p)[i]);
     return (double)half_bits_to_float(((const uint16_t*)p)[i]);
 }
-
-// max(x, 0), NaN kept.
-__device__ __forceinline__ double positive(double x) { return x > 0.0 || x != x ? x : 0.0; }
 
 // How many drafts of the sequence stand; `count` is how many there are.
 template <int XK>
@@ -131,18 +134,19 @@ __device__ __forceinline__ void entries(const void* p, int64_t at, int v, int vo
     }
 }
 
-// The weights of entries whose probabilities are p (and q where w.draft), and
-// the target's alone.
-template <int kCount>
-__device__ __forceinline__ void weigh(const Weights& w, int v, const float (&p)[kCount], const float (&q)[kCount],
-                                      double (&less)[kCount], double (&plain)[kCount]) {
-#pragma unroll
-    for (int e = 0; e < kCount; ++e) {
-        const double x = (double)p[e];
-        const double y = w.draft ? (double)q[e] : (v + e == w.hot ? 1.0 : 0.0);
-        plain[e] = positive(x);
-        less[e] = positive(x - y);
-    }
+// How a span's weights come about: the target alone, less the draft's, or less one
+// at `hot` (the one span that holds it).
+enum Less { kNothing, kDraft, kHot };
+
+// The weight max(p - q, 0) of an entry; `odd` remembers a NaN, which the maximum
+// drops.
+template <int kLess>
+__device__ __forceinline__ double weight(const Weights& w, int v, float p, float q, bool& odd) {
+    double x = (double)p;
+    if constexpr (kLess == kDraft) x -= (double)q;
+    if constexpr (kLess == kHot) x -= v == w.hot ? 1.0 : 0.0;
+    odd = odd || x != x;
+    return __builtin_fmax(x, 0.0);
 }
 
 __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
@@ -151,10 +155,39 @@ __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-template <int XK>
-__global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
+// The sum of one span's weights, in every lane; NaN if one of them is.
+template <int XK, int kLess>
+__device__ __forceinline__ double span_sum(const Weights& w, int vocab, int span, int lane) {
     constexpr int kLoad = XK == kF32 ? 4 : 8;         // entries of a lane's load
     constexpr int kLoads = kSpan / (64 * kLoad);
+    float p[kLoads][kLoad], q[kLoads][kLoad];
+    const int v0 = span * kSpan + kLoad * lane;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) entries<XK>(w.target, w.target_at, v0 + 64 * kLoad * i, vocab, p[i]);
+    if constexpr (kLess == kDraft) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) entries<XK>(w.draft, w.draft_at, v0 + 64 * kLoad * i, vocab, q[i]);
+    }
+    double sum = 0.0;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int e = 0; e < kLoad; ++e)
+            sum += weight<kLess>(w, v0 + 64 * kLoad * i + e, p[i][e], kLess == kDraft ? q[i][e] : 0.0f, odd);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum += shfl_xor_f64(sum, m);
+    return __any(odd) ? __builtin_nan("") : sum;
+}
+template <int XK>
+__device__ __forceinline__ double span_sum(const Weights& w, int vocab, int span, int lane) {
+    if (w.draft) return span_sum<XK, kDraft>(w, vocab, span, lane);
+    if (w.hot >= 0 && w.hot / kSpan == span) return span_sum<XK, kHot>(w, vocab, span, lane);
+    return span_sum<XK, kNothing>(w, vocab, span, lane);
+}
+
+template <int XK>
+__global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t at = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (at >= (int64_t)a.batch * a.spans) return;
@@ -163,34 +196,8 @@ __global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
     int count;
     const int n = standing<XK>(a, b, lane, count);
     if (span == 0 && lane == 0) a.standing[b] = n;
-    const Weights w = weights_of(a, b, n, count);
-    float p[kLoads][kLoad], q[kLoads][kLoad];
-    const int v0 = span * kSpan + kLoad * lane;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) entries<XK>(w.target, w.target_at, v0 + 64 * kLoad * i, a.vocab, p[i]);
-    if (w.draft)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) entries<XK>(w.draft, w.draft_at, v0 + 64 * kLoad * i, a.vocab, q[i]);
-    double sl = 0.0, sp = 0.0;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        double less[kLoad], plain[kLoad];
-        weigh(w, v0 + 64 * kLoad * i, p[i], q[i], less, plain);
-#pragma unroll
-        for (int e = 0; e < kLoad; ++e) {
-            sl += less[e];
-            sp += plain[e];
-        }
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        sl += shfl_xor_f64(sl, m);
-        sp += shfl_xor_f64(sp, m);
-    }
-    if (lane == 0) {
-        a.sums[2 * at] = sl;
-        a.sums[2 * at + 1] = sp;
-    }
+    const double sum = span_sum<XK>(weights_of(a, b, n, count), a.vocab, span, lane);
+    if (lane == 0) a.sums[at] = sum;
 }
 
 // Running sums over the wave's lanes, each lane's own value counted: within rows
@@ -218,70 +225,65 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-// One wave per sequence, no barrier: lane l has spans per l .. per l + per - 1,
-// then entries 16 l .. 16 l + 15 of the span.  (A workgroup of four waves over
-// LDS, with shuffles for its scans, took 10 us for any batch.)
+// The choice of sequence b by one wave, no barrier: lane l has spans per l .. per l +
+// per - 1, then entries 16 l .. 16 l + 15 of the span.  (A workgroup of four waves
+// over LDS, with shuffles for its scans, took 10 us for any batch.)
 template <int XK>
-__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+__device__ __forceinline__ void pick(const VerifyArgs& a, int b, int lane, const double* sums, int n, int count) {
     constexpr int kOwn = kSpan / 64;
-    const int lane = threadIdx.x;
-    const int b = blockIdx.x;
-    const double* sums = a.sums + 2 * (int64_t)b * a.spans;
     const int per = (a.spans + 63) / 64;
     const int first = per * lane;
-    double own[2] = {0.0, 0.0};
-    for (int i = 0; i < per && first + i < a.spans; ++i) {
-        own[0] += sums[2 * (first + i)];
-        own[1] += sums[2 * (first + i) + 1];
-    }
-    int count = a.drafts;
-    if (a.draft_lengths) count = min(max(a.draft_lengths[b], 0), a.drafts);
-    const int n = a.standing[b];
+    double own = 0.0;
+    for (int i = 0; i < per && first + i < a.spans; ++i) own += sums[first + i];
     float u = a.uniforms[(int64_t)b * (a.drafts + 1) + a.drafts];
-    const Weights w = weights_of(a, b, n, count);
-    // the total; where the draft falls short of the target nowhere, the target's alone
-    int which = 0;
-    double end = running_sum(own[0]);
-    double total = lane_f64(end, 63);
-    if (total == 0.0) {
-        which = 1;
-        end = running_sum(own[1]);
-        total = lane_f64(end, 63);
-    }
+    Weights w = weights_of(a, b, n, count);
     constexpr float kBelowOne = 0.999999940395355224609375f;  // 1 - 2^-24
     if (u > kBelowOne) u = kBelowOne;
     if (u < 0.0f) u = 0.0f;
-    const double goal = (double)u * total;
-    int64_t token = -1;
-    if (total > 0.0 && total < __builtin_inf() && u == u) {  // (the same in every lane)
+    const double end = running_sum(own);
+    double total = lane_f64(end, 63), run = 0.0, goal;
+    int span = 0;
+    if (total != 0.0) {
         // the lane whose spans pass the goal (lane 63's end is the total), then the
         // span: the last one of the lane's if its spans, added to what comes before
         // them, stay a rounding below
-        const int at = __ffsll((unsigned long long)__ballot(end > goal)) - 1;
-        double run = at > 0 ? lane_f64(end, at - 1) : 0.0;
-        int span = min(per * at, a.spans - 1);
-        for (const int past = min(per * (at + 1), a.spans); span < past; ++span) {
-            const double next = run + sums[2 * span + which];
-            if (next > goal || span + 1 == past) break;
+        goal = (double)u * total;
+        const uint64_t past = __ballot(end > goal);
+        const int at = past ? __ffsll((unsigned long long)past) - 1 : 0;  // (none: no number)
+        run = at > 0 ? lane_f64(end, at - 1) : 0.0;
+        span = min(per * at, a.spans - 1);
+        for (const int stop = min(per * (at + 1), a.spans); span + 1 < stop; ++span) {
+            const double next = run + sums[span];
+            if (next > goal) break;
             run = next;
         }
+    } else {
+        // the draft falls short of the target nowhere: the target alone, by this wave
+        w.draft = nullptr, w.hot = -1;
+        for (int i = 0; i < a.spans; ++i) total += span_sum<XK>(w, a.vocab, i, lane);
+        goal = (double)u * total;
+        for (; span + 1 < a.spans; ++span) {
+            const double next = run + span_sum<XK>(w, a.vocab, span, lane);
+            if (next > goal) break;
+            run = next;
+        }
+    }
+    int64_t token = -1;
+    if (total > 0.0 && total < __builtin_inf() && u == u) {  // (the same in every lane)
         const int v0 = span * kSpan + kOwn * lane;
-        float p[kOwn / 4][4], q[kOwn / 4][4];
+        float p[kOwn / 4][4], q[kOwn / 4][4] = {};
 #pragma unroll
         for (int i = 0; i < kOwn / 4; ++i) entries<XK>(w.target, w.target_at, v0 + 4 * i, a.vocab, p[i]);
         if (w.draft)
 #pragma unroll
             for (int i = 0; i < kOwn / 4; ++i) entries<XK>(w.draft, w.draft_at, v0 + 4 * i, a.vocab, q[i]);
-        double weight[kOwn], mine = 0.0;
+        double each[kOwn], mine = 0.0;
 #pragma unroll
-        for (int i = 0; i < kOwn / 4; ++i) {
-            double less[4], plain[4];
-            weigh(w, v0 + 4 * i, p[i], q[i], less, plain);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                weight[4 * i + e] = which ? plain[e] : less[e];
-                mine += weight[4 * i + e];
-            }
+        for (int e = 0; e < kOwn; ++e) {
+            // (of the two, one is not there and takes nothing off)
+            const double less = (double)q[e / 4][e % 4] + (v0 + e == w.hot ? 1.0 : 0.0);
+            each[e] = __builtin_fmax((double)p[e / 4][e % 4] - less, 0.0);
+            mine += each[e];
         }
         const double upto = running_sum(mine);
         const double before = __shfl_up(upto, 1);  // (by every lane: one that is off gives nothing)
@@ -289,8 +291,8 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
         int found = -1, some = -1;
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
-            sum += weight[e];
-            if (weight[e] > 0.0) {
+            sum += each[e];
+            if (each[e] > 0.0) {
                 some = v0 + e;
                 if (sum > goal && found < 0) found = v0 + e;
             }
@@ -308,7 +310,49 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
 }
 
 template <int XK>
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+    const int b = blockIdx.x;
+    int count = a.drafts;
+    if (a.draft_lengths) count = min(max(a.draft_lengths[b], 0), a.drafts);
+    pick<XK>(a, b, threadIdx.x, a.sums + (int64_t)b * a.spans, a.standing[b], count);
+}
+
+// Both in one launch, a workgroup of 16 waves per sequence: the spans' sums meet in
+// LDS.
+constexpr int kOneWaves = 16;
+constexpr int kOneSpans = 512;
+template <int XK>
+__global__ __launch_bounds__(64 * kOneWaves) void verify_one_kernel(VerifyArgs a) {
+    __shared__ double sums[kOneSpans];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x;
+    int count;
+    const int n = standing<XK>(a, b, lane, count);
+    const Weights w = weights_of(a, b, n, count);
+    for (int span = wave; span < a.spans; span += kOneWaves) {
+        const double sum = span_sum<XK>(w, a.vocab, span, lane);
+        if (lane == 0) sums[span] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) pick<XK>(a, b, lane, sums, n, count);
+}
+
+// One launch where its workgroup has two spans a wave at most, or where there are
+// sequences for every CU.  us per call, one launch / two: 1 x 8000 fp32 with a
+// draft model 6.5 / 8.5, 1 x 32000 7.4 / 8.5, 96 x 32000 9.3 / 10.8, 1 x 50257 8.4 /
+// 8.5, its bf16 9.7 / 8.5, 96 x 50257 bf16 13.4 / 11.6, 1 x 151936 bf16 19.8 / 8.4,
+// but 256 x 50257 15.0 / 17.4 and 256 x 151936 35.8 / 39.7.
+bool verify_in_one(const VerifyArgs& a) {
+    return a.spans <= 2 * kOneWaves || (a.spans <= kOneSpans && a.batch >= 256);
+}
+
+template <int XK>
 hipError_t launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t stream) {
+    if (verify_in_one(a)) {
+        hipLaunchKernelGGL(verify_one_kernel<XK>, dim3((unsigned)batch), dim3(64 * kOneWaves), 0, stream, a);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(verify_sum_kernel<XK>, dim3((unsigned)((batch * a.spans + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
@@ -328,7 +372,7 @@ extern "C" {
 int64_t qwen2_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
     if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > 0x7FFFFFFF - kMargin || batch > 0x7FFFFFFF / verify_spans(vocab))
         return 0;
-    return batch * verify_spans(vocab) * 2 * (int64_t)sizeof(double) + batch * (int64_t)sizeof(int32_t);
+    return batch * verify_spans(vocab) * (int64_t)sizeof(double) + batch * (int64_t)sizeof(int32_t);
 }
 
 int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target_row, const void* draft,
@@ -355,7 +399,7 @@ int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target
                          (long long)need, (long long)(workspace ? workspace_bytes : 0));
     VerifyArgs a{target, draft, target_batch, target_row, draft_batch, draft_row, draft_tokens, draft_lengths, uniforms,
                  tokens, accepted, (double*)workspace, nullptr, (int)batch, (int)drafts, (int)vocab, (int)verify_spans(vocab)};
-    a.standing = (int32_t*)(a.sums + 2 * batch * a.spans);
+    a.standing = (int32_t*)(a.sums + batch * a.spans);
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t err = dtype == W4G64_DTYPE_F32    ? launch_verify<kF32>(a, batch, s)
                            : dtype == W4G64_DTYPE_BF16 ? launch_verify<kBF16>(a, batch, s)

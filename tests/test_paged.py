@@ -758,7 +758,7 @@ def _same(got, want):
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("batch, drafts, vocab", [(1, 1, 1), (1, 4, 151936), (3, 2, 4096), (2, 7, 4097), (17, 3, 5001),
-                                                  (5, 0, 300), (2, 130, 77), (66, 1, 16)])
+                                                  (5, 0, 300), (2, 130, 77), (66, 1, 16), (2, 2, 32768), (2, 3, 32769), (257, 1, 40001)])
 @pytest.mark.parametrize("copied", [False, True])
 def test_verify_is_the_formula(dtype, batch, drafts, vocab, copied):
     gen = torch.Generator(device="cuda").manual_seed(batch * 1000 + drafts)
@@ -788,6 +788,21 @@ def test_verify_on_borders():
             uniforms = torch.tensor([[i / 8, i / 8]], device="cuda")
             for q in (draft, None):
                 _same(verify_drafts_hip(target, tokens, uniforms, draft_probs=q), _verified(target, tokens, uniforms, q))
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [3, 5000, 40000])
+def test_verify_falls_back_to_the_target(vocab):
+    """A draft that is nowhere below the target, refused: drawn from the target."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    target = torch.softmax(torch.randn(4, 2, vocab, generator=gen, device="cuda"), -1)
+    draft = 1.25 * target[:, :1]
+    tokens = torch.randint(0, vocab, (4, 1), generator=gen, device="cuda")
+    uniforms = torch.rand(4, 2, generator=gen, device="cuda")
+    uniforms[:, 0] = 0.9  # (past 0.8: refused)
+    got = verify_drafts_hip(target, tokens, uniforms, draft_probs=draft)
+    _same(got, _verified(target, tokens, uniforms, draft))
+    assert got[1].tolist() == [0] * 4 and int(got[0][:, 0].min()) >= 0
 
 
 @gpu
