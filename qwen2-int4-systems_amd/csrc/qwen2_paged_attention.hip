@@ -146,8 +146,12 @@ template <class E> __device__ __forceinline__ uint32_t pass_word(uint32_t w, Pas
     return pass_half<E>(w & 0xFFFFu, pass) | (pass_half<E>(w >> 16, pass) << 16);
 }
 
+// Rows of a segment from which wide tiles are taken.  Main kernel, us, narrow /
+// wide, 12/2 heads of 128: a prefix of 1 K by 96 rows 10.0 / 12.1, by 240 17.4 / 15.1,
+// of 4 K by 96 17.3 / 22.3, by 192 16.0 / 15.2, by 240 31.0 / 25.0; own segments of
+// 240 rows over up to 1 K 13.2 / 13.8.
+constexpr int kWideFrom = 128;
 // Whether a sequence's own rows go by wide tiles, where the call has any.
-constexpr int kWideFrom = 64;
 __device__ __forceinline__ bool wide_rows(const PagedAttnArgs& a, int tokens) {
     return a.own_wide && tokens * a.group > kWideFrom;
 }
@@ -980,7 +984,7 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
         return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
     };
     // (own: on the average; the sequences with few rows among them go by narrow tiles
-    // all the same, at most four each)
+    // all the same, at most eight each)
     p.prefix_wide = p.prefix > 0 && rows * group > kWideFrom;
     p.own_wide = own > 0 && rows * group > kWideFrom * sequences;
     if (p.prefix > 0) {
@@ -991,7 +995,10 @@ PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t sh
     if (own > 0) {
         p.own_tiles = p.own_wide ? rows * group / kWideRows + kWideFrom / kNarrowRows * sequences
                                  : rows * group / kNarrowRows + sequences;
-        p.own_splits = splits(p.own_tiles * c.kv_heads, own);
+        // (by the tiles of sequences of the average length, not by the most there can be)
+        const int64_t tile = p.own_wide ? kWideRows : kNarrowRows;
+        const int64_t usual = sequences * ((rows * group + sequences * tile - 1) / (sequences * tile));
+        p.own_splits = splits(usual * c.kv_heads, own);
     }
     p.slots = p.prefix_splits + p.own_splits;
     return p;
