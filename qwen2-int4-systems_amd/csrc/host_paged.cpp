@@ -139,6 +139,17 @@ bool same_view(const at::Tensor& a, const at::Tensor& b) {
     return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
 }
 
+// Whether the rows of two views of one buffer (parts of a fused projection) lie
+// apart: rows equally far from each other, and within a row one behind the other.
+bool rows_apart(const at::Tensor& a, const at::Tensor& b) {
+    if (!overlap(a, b)) return true;
+    const at::Tensor& x = a.const_data_ptr() <= b.const_data_ptr() ? a : b;
+    const at::Tensor& y = &x == &a ? b : a;
+    const int64_t between = ((const char*)y.const_data_ptr() - (const char*)x.const_data_ptr()) / x.element_size();
+    auto extent = [](const at::Tensor& t) { return (t.size(1) - 1) * step(t, 1) + t.size(2); };
+    return x.size(0) > 1 && x.stride(0) == y.stride(0) && between >= extent(x) && between + extent(y) <= x.stride(0);
+}
+
 void check_output(const at::Tensor& out, const at::Tensor& q) {
     if (out.scalar_type() != q.scalar_type()) refuse(PyExc_TypeError, "out must have q's dtype");
     if (out.sizes() != q.sizes()) refuse(PyExc_ValueError, "out must have q's shape");
@@ -204,6 +215,7 @@ struct Cache {
 qwen2_rows rows_of(const at::Tensor& t) { return qwen2_rows{const_cast<void*>(t.const_data_ptr()), step(t, 0), step(t, 1)}; }
 
 double number(PyObject* obj, const char* name) {
+    if (THPVariable_Check(obj)) refuse(PyExc_TypeError, "%s must be a number, not a tensor", name);
     const double v = PyFloat_AsDouble(obj);
     if (v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
@@ -213,8 +225,11 @@ double number(PyObject* obj, const char* name) {
 }
 
 int64_t whole(PyObject* obj, const char* name) {
-    if (!PyLong_Check(obj) || PyBool_Check(obj)) refuse(PyExc_TypeError, "%s must be an integer", name);
-    const long long v = PyLong_AsLongLong(obj);
+    if (!PyIndex_Check(obj) || PyBool_Check(obj) || THPVariable_Check(obj))  // (a tensor's would wait for the GPU)
+        refuse(PyExc_TypeError, "%s must be an integer", name);
+    PyObject* index = PyNumber_Index(obj);
+    const long long v = index ? PyLong_AsLongLong(index) : -1;
+    Py_XDECREF(index);
     if (v == -1 && PyErr_Occurred()) {
         PyErr_Clear();
         refuse(PyExc_ValueError, "%s is out of range", name);
@@ -284,6 +299,8 @@ PyObject* host_paged_append(PyObject*, PyObject* const* args, Py_ssize_t count) 
         }
         if (given && !same_view(*given, q) && (overlap(*given, q) || overlap(*given, k) || overlap(*given, v)))
             refuse(PyExc_ValueError, "out must be q itself or share no memory with q, k and v");
+        if (given && (!rows_apart(q, k) || !rows_apart(q, v)))
+            refuse(PyExc_ValueError, "q must not share its rows with k and v where it is rotated in place");
         const c10::DeviceGuard guard(device);
         if (!cache.c.batch || !rows) return THPVariable_Wrap(given ? *given : at::zeros(q.sizes(), q.options().requires_grad(false)));
         cache.bind();

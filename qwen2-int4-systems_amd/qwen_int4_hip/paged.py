@@ -62,7 +62,8 @@ def paged_append_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages:
     64 bits; ``rotary_scale`` multiplies what is turned.  Contexts stretched past
     the trained length are a matter of these two.  Results are rounded once.
 
-    ``out`` may be ``q`` itself.  Rows behind the last sequence are left as they
+    ``out`` may be ``q`` itself (whose rows then lie apart from k's and v's, as in a
+    fused projection).  head_dim is a multiple of 16 up to 256.  Rows behind the last sequence are left as they
     are in ``out``, and zeros in a new tensor.  Two rows of one call must not
     share a place in the cache."""
     return _calls().paged_append(q, k, v, k_pages, v_pages, page_table, cu_rows, lengths, inv_freq, interleaved,
@@ -83,8 +84,8 @@ def paged_attention_hip(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
 
     Keys and values that a row does not see take no part, whatever they hold.  A
     row without a position gives zeros.  Rows behind the last sequence are left
-    as they are in ``out``, and zeros in a new tensor.  Softmax and sums are fp32;
-    each (row, head) is summed in an order that the sizes alone decide."""
+    as they are in ``out``, and zeros in a new tensor.  Softmax and sums are fp32,
+    in a fixed order: the same inputs give the same bits."""
     return _calls().paged_attention(q, k_pages, v_pages, page_table, cu_rows, lengths, shared_pages, scale, out)
 
 

@@ -129,6 +129,9 @@ def test_append_and_attention_refuse_their_own():
         with pytest.raises(error, match=said):
             paged_append_hip(**(append | change))
     for change, error, said in [({"shared_pages": 1.0}, TypeError, "shared_pages must be an integer"),
+                                ({"shared_pages": torch.tensor(1)}, TypeError, "shared_pages must be an integer"),
+                                ({"shared_pages": 2 ** 70}, ValueError, "shared_pages is out of range"),
+                                ({"scale": torch.tensor(1.0)}, TypeError, "scale must be a number"),
                                 ({"shared_pages": True}, TypeError, "shared_pages must be an integer"),
                                 ({"scale": None, "q": torch.zeros(5, 4, 64, dtype=BF16).requires_grad_()}, RuntimeError,
                                  "has no gradient"),
@@ -344,6 +347,10 @@ ATTENTION = [
     ([1] * 70, [b % 40 for b in range(70)], {"shared": 2, "heads": 3, "kv_heads": 1}),
     ([64] * 3, [100, 0, 1], {"shared": 66, "heads": 12, "dim": 128}),
     ([1], [4100], {"heads": 32, "kv_heads": 1, "dim": 128, "page": 1024}),
+    ([150, 1, 1, 40], [0, 700, 33, 200], {"heads": 12, "dim": 128}),
+    ([90, 30], [64, 7], {"shared": 21, "heads": 16, "kv_heads": 2, "dim": 64, "page": 32, "token_major": True}),
+    ([300], [17], {"shared": 1, "heads": 7, "kv_heads": 1, "dtype": F16, "page": 256}),
+    ([5] * 40, [3 * b for b in range(40)], {"shared": 130, "heads": 12, "dim": 128}),
 ]
 
 
@@ -402,6 +409,27 @@ def test_rows_without_a_position_give_zeros(shared):
     assert not got[0].any() and not got[3:].any() and bool(got[1:3].any())
     p.lengths.fill_(-(2 ** 31))
     assert not p.attention().any()
+
+
+@gpu
+@pytest.mark.parametrize("rows, heads", [([3, 2, 1], 4), ([60, 50, 3], 12)])
+def test_sequences_that_end_inside_the_shared_prefix(rows, heads):
+    """One of them sees a part of the prefix, one all of it but one position, one more."""
+    p = Paged(rows, [0, 0, 9], shared=6, heads=heads, dim=128)
+    p.lengths_list = [rows[0] + 7, 95, p.lengths_list[2]]
+    p.lengths.copy_(torch.tensor(p.lengths_list))
+    _near(p.attention(), *p.reference())
+
+
+@gpu
+def test_lengths_change_between_calls_of_one_shape():
+    """The same tables and sizes, every length from one position to the table's end."""
+    p = Paged([2], [126], heads=12, dim=128)
+    whole = p.lengths_list[0]
+    for length in list(range(1, 70)) + [whole - 1, whole]:
+        p.lengths_list = [length]
+        p.lengths.fill_(length)
+        _near(p.attention(), *p.reference())
 
 
 @gpu
@@ -709,6 +737,10 @@ def test_append_copies_rows_it_cannot_read_in_place():
     with pytest.raises(ValueError, match="out must be q itself"):
         paged_append_hip(base[:20].view(5, 4, 64), k, v, p.k_pages, p.v_pages, p.table, p.cu, p.lengths, inv,
                          out=base[4:].view(5, 4, 64))
+    one = torch.zeros(5, 2, 64, dtype=BF16, device="cuda")  # queries and keys of one tensor
+    assert torch.equal(paged_append_hip(one, one, one, p.k_pages, p.v_pages, p.table, p.cu, p.lengths, inv), one)
+    with pytest.raises(ValueError, match="must not share its rows"):
+        paged_append_hip(one, one, one, p.k_pages, p.v_pages, p.table, p.cu, p.lengths, inv, out=one)
     with pytest.raises(ValueError, match="the cache must not share memory"):
         paged_append_hip(p.q, p.k_pages[:5, :, 0], v, p.k_pages, p.v_pages, p.table, p.cu, p.lengths, inv)
 
@@ -980,6 +1012,10 @@ def test_calls_on_several_streams_and_modes():
         p.attention()
     with pytest.raises(RuntimeError, match="function transform"):
         torch.func.vmap(lambda x: p.attention(q=x))(p.q.unsqueeze(0))
+    import torch.autograd.forward_ad as fwAD
+
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="has no gradient"):
+        p.attention(q=fwAD.make_dual(p.q, torch.ones_like(p.q)))
     version = p.k_pages._version
     paged_append_hip(p.q, p.randn(6, 2, 128), p.randn(6, 2, 128), p.k_pages, p.v_pages, p.table, p.cu, p.lengths, None)
     assert p.k_pages._version > version
