@@ -968,38 +968,40 @@ struct PagedPlan {
     bool prefix_wide, own_wide;
 };
 
-PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t shared_pages) {
+PagedPlan paged_plan(const PagedView& c, int64_t rows, int64_t heads, int64_t head_dim, int64_t shared_pages) {
     PagedPlan p{};
     const int64_t group = heads / c.kv_heads;
     const int64_t sequences = c.batch < rows ? c.batch : rows;
     p.prefix = shared_pages << c.page_shift;
     const int64_t own = ((int64_t)c.table_width - shared_pages) << c.page_shift;
-    // as many as the chip holds at once (two workgroups of a CU with wide tiles, three
-    // without), but a block for each wave
-    auto splits = [&](int64_t workgroups, int64_t keys) {
-        const int64_t hold = 256 * (p.prefix_wide || p.own_wide ? 2 : 3);
-        const int64_t most = (keys + kBlock * kWaves - 1) / (kBlock * kWaves);
-        int64_t s = hold > workgroups ? hold / workgroups : 1;
-        s = s < most ? s : most;
-        return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
-    };
     // (own: on the average; the sequences with few rows among them go by narrow tiles
     // all the same, at most eight each)
     p.prefix_wide = p.prefix > 0 && rows * group > kWideFrom;
     p.own_wide = own > 0 && rows * group > kWideFrom * sequences;
-    if (p.prefix > 0) {
-        const int64_t tile = p.prefix_wide ? kWideRows : kNarrowRows;
-        p.prefix_tiles = (rows * group + tile - 1) / tile;
-        p.prefix_splits = splits(p.prefix_tiles * c.kv_heads, p.prefix);
-    }
+    const int64_t prefix_tile = p.prefix_wide ? kWideRows : kNarrowRows, own_tile = p.own_wide ? kWideRows : kNarrowRows;
+    int64_t usual = 0;  // own tiles if all sequences have the average rows
+    if (p.prefix > 0) p.prefix_tiles = (rows * group + prefix_tile - 1) / prefix_tile;
     if (own > 0) {
+        usual = sequences * ((rows * group + sequences * own_tile - 1) / (sequences * own_tile));
         p.own_tiles = p.own_wide ? rows * group / kWideRows + kWideFrom / kNarrowRows * sequences
                                  : rows * group / kNarrowRows + sequences;
-        // (by the tiles of sequences of the average length, not by the most there can be)
-        const int64_t tile = p.own_wide ? kWideRows : kNarrowRows;
-        const int64_t usual = sequences * ((rows * group + sequences * tile - 1) / (sequences * tile));
-        p.own_splits = splits(usual * c.kv_heads, own);
     }
+    // Splits: as many workgroups as the chip holds at once, dealt out by the time that
+    // the two kinds of segment take (a key costs a wide tile some four times a narrow
+    // one's; tables are half full), but no more than leave a block for each wave.
+    const bool wide = p.prefix_wide || p.own_wide;
+    const int64_t hold = 256 * (head_dim == 64 ? (wide ? 3 : 5) : (wide ? 2 : 3));
+    const double prefix_time = (double)p.prefix_tiles * p.prefix * (p.prefix_wide ? 4 : 1);
+    const double own_time = (double)usual * own / 2 * (p.own_wide ? 4 : 1);
+    const int64_t prefix_hold = (int64_t)(hold * (prefix_time / (prefix_time + own_time)));
+    auto splits = [&](int64_t hold, int64_t tiles, int64_t keys) {
+        const int64_t workgroups = tiles * c.kv_heads, most = (keys + kBlock * kWaves - 1) / (kBlock * kWaves);
+        int64_t s = hold > workgroups ? hold / workgroups : 1;
+        s = s < most ? s : most;
+        return s < kMaxSplits / 2 ? s : kMaxSplits / 2;
+    };
+    if (p.prefix > 0) p.prefix_splits = splits(prefix_hold, p.prefix_tiles, p.prefix);
+    if (own > 0) p.own_splits = splits(hold - prefix_hold, usual, own);
     p.slots = p.prefix_splits + p.own_splits;
     return p;
 }
@@ -1048,7 +1050,7 @@ int64_t qwen2_paged_attention_workspace_bytes(const qwen2_paged_cache* cache, in
                                               int64_t shared_pages) {
     PagedView view{};
     if (attention_sizes(cache, &view, rows, heads, shared_pages) || rows == 0) return 0;
-    const PagedPlan p = paged_plan(view, rows, heads, shared_pages);
+    const PagedPlan p = paged_plan(view, rows, heads, cache->head_dim, shared_pages);
     return p.slots == 1 ? 0 : rows * heads * p.slots * (cache->head_dim + 2) * (int64_t)sizeof(float) + 16;
 }
 
@@ -1064,7 +1066,7 @@ int qwen2_paged_attention(const qwen2_paged_cache* cache, const qwen2_rows* q, c
         if (!r || !r->data || ((uintptr_t)r->data & 15) || r->row % 8 || r->head % 8)
             return set_error(W4G64_STATUS_INVALID_VALUE,
                              "q and out must be non-null, 16-byte aligned, with strides that are multiples of 8 elements");
-    const PagedPlan p = paged_plan(a.c, rows, heads, shared_pages);
+    const PagedPlan p = paged_plan(a.c, rows, heads, cache->head_dim, shared_pages);
     const int64_t need = qwen2_paged_attention_workspace_bytes(cache, rows, heads, shared_pages);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return set_error(W4G64_STATUS_WORKSPACE, "paged_attention needs %lld workspace bytes, 16-byte aligned, got %lld",
