@@ -10,12 +10,28 @@
 // A workgroup of four waves takes a tile of a segment's rows and one of several
 // splits of its keys, in one of two forms:
 //   narrow    16 rows.  The waves take different 32-key blocks, straight from
-//             memory into operands, two blocks in flight each, and meet in LDS at
-//             the end: for few rows, bound by the keys' and values' read.
+//             memory into operands, and meet in LDS at the end: for few rows.
 //   wide      128 rows, 32 of each wave.  The workgroup goes through 64-key tiles
 //             in LDS, the next one on its way (direct loads) while the waves work
-//             on this one: for many rows, bound by matrix and vector unit.
+//             on this one: for many rows.
 // A second launch joins the splits of both kinds of segment.
+//
+// What bounds it.  Narrow: the keys' and values' read (64 sequences of 1 K
+// positions, 2 key/value heads of 128: 65 MB in 15.5 us, 4.2 TB/s) and, where that is
+// little, 5-6 us of dependent loads, serial instructions and the join's 2-4.  Three
+// workgroups a CU with one block in flight beat two with two (24 sequences of up
+// to 2 K: 11.7 and 12.6 us).  Wide: matrix and vector unit, which overlap by a third
+// only (two waves of a SIMD, 8 products and 32 additions each 64 and 70 ns alone, 100
+// together; exponentials hide): 96 products and some 320 vector instructions a wave
+// and tile.  1920 rows a key/value head over 16 K positions take 50 us beyond some 10
+// for start and end, 640 TFLOP/s, at 1.9 to 2.0 GHz.  On the way, 64 x 5 rows, 12/2
+// heads, 16 K shared and up to 1 K own positions, us per call: 160 narrow alone, 106 wide,
+// 75 with values read transposed from LDS instead of permuted and masks in branches
+// of their own, 69 with LDS reads issued ahead and the workgroups dealt out by time.
+// Measured and dropped: 32-key wide tiles at three waves per SIMD (61 -> 64), wave
+// priorities around the products and splits that keep a tile's keys on one XCD
+// (no change), all keys in one workgroup of twelve waves instead of a join (1 x 576
+// 8.7 -> 10.9; a CU draws some 60 GB/s).
 //
 // One pass over the keys: running maximum, sum and value sums per row.  MFMA
 // layout (v_mfma_f32_16x16x32; lane l = 16 q + j supplies row j of A and column
