@@ -529,6 +529,34 @@ def test_pages_that_are_not_there_give_nan(shared):
 
 
 @gpu
+@pytest.mark.parametrize("shared", [0, 2])
+def test_pages_that_are_not_there_among_many_rows(shared):
+    """Sixty rows of six heads at own positions 40 .. 99; the page of 80 .. 95, then one
+    of the prefix, then the table's end."""
+    p = Paged([60, 45], [40, 2], shared=shared, heads=12, dim=128)
+    want, slack = p.reference()
+    table = p.table.clone()
+    table[0, shared + 5] = -1
+    got = paged_attention_hip(p.q, p.k_pages, p.v_pages, table, p.cu, p.lengths, shared_pages=shared)
+    assert bool(got[40:60].isnan().all())
+    _near(got[:40], want[:40], slack[:40])
+    _near(got[60:], want[60:], slack[60:])
+    if shared:
+        table = p.table.clone()
+        table[0, 1] = p.k_pages.shape[0]
+        assert bool(paged_attention_hip(p.q, p.k_pages, p.v_pages, table, p.cu, p.lengths,
+                                        shared_pages=shared).isnan().all())
+    reach = p.table.shape[1] * 16
+    for cache in (p.k_pages, p.v_pages):  # (all that the table names is written)
+        cache[p.used[0]] = cache[p.used[0]].nan_to_num(0.5)
+    lengths = p.lengths.clone()
+    lengths[0] = reach + 10
+    got = paged_attention_hip(p.q, p.k_pages, p.v_pages, p.table, p.cu, lengths, shared_pages=shared)
+    assert bool(got[50:60].isnan().all()) and bool(got[:50].isfinite().all())
+    _near(got[60:], want[60:], slack[60:])
+
+
+@gpu
 @pytest.mark.parametrize("values", [[-7, 90, 2, -1], [5, 5, 5, 5], [0, 2 ** 31 - 1, -(2 ** 31), 4]])
 def test_row_bounds_that_fall_or_lead_out_stay_in_the_buffers(values):
     """What cu_rows should not hold: nothing is promised but that nothing faults
