@@ -40,6 +40,17 @@ __host__ __device__ inline SequenceRows sequence_rows(const int32_t* cu_rows, co
     return s;
 }
 
+// The end of the last sequence's rows, bounded by [0, rows] whatever cu_rows
+// holds, and the row behind it that is a workgroup's first one (in 64 bits: the
+// sum of two bounds of 31).
+__host__ __device__ inline int rows_end(const int32_t* cu_rows, int batch, int rows) {
+    const int end = cu_rows[batch];
+    return end < 0 ? 0 : (end > rows ? rows : end);
+}
+__host__ __device__ inline int64_t rest_row(const int32_t* cu_rows, int batch, int rows, unsigned workgroup) {
+    return (int64_t)rows_end(cu_rows, batch, rows) + workgroup;
+}
+
 // The page of a position, or -1: outside the table, or not a page of the pool.
 __host__ __device__ inline int checked_page(int page, int num_pages) { return page >= 0 && page < num_pages ? page : -1; }
 __host__ __device__ inline int page_of(const int32_t* table_row, int table_width, int page_shift, int num_pages,

@@ -900,7 +900,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 2 : 3) void paged_attention_kerne
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // rows behind the last sequence, where no second launch sees to them
     if (a.slots == 1 && a.zero_rest) {
-        for (int r = max(a.c.cu_rows[a.c.batch], 0) + (int)blockIdx.x; r < a.rows; r += (int)gridDim.x)
+        for (int64_t r = rest_row(a.c.cu_rows, a.c.batch, a.rows, blockIdx.x); r < a.rows; r += gridDim.x)
             for (int d = 8 * tid; d < a.heads * D; d += 8 * kThreads)
                 *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
     }

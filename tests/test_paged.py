@@ -67,6 +67,36 @@ def test_indices_from_device_memory_stay_in_bounds(tmp_path):
         ["3", "8", "-10", "/", "2", "2", "-5"]]  # a length below its rows: negative positions
 
 
+REST_PROGRAM = r"""
+#define __host__
+#define __device__
+#include "qwen2_paged.h"
+#include <cstdio>
+using namespace w4g64;
+int main() {
+    const int32_t ends[] = {0, 3, 8, 9, 2147483647, -1, -2147483647 - 1};
+    for (int32_t end : ends) {
+        const int32_t cu[3] = {0, 0, end};
+        printf("%d", rows_end(cu, 2, 8));
+        for (unsigned workgroup : {0u, 1u, 5u, 2147483646u}) {  // rows behind the last sequence, of all 8
+            const int64_t r = rest_row(cu, 2, 8, workgroup);
+            if (r < 8) printf(" %lld", (long long)r);
+        }
+        printf("|");
+    }
+}
+"""
+
+
+def test_rows_behind_the_last_sequence_stay_in_bounds(tmp_path):
+    source, program = tmp_path / "rest.cpp", tmp_path / "rest"
+    source.write_text(REST_PROGRAM)
+    subprocess.run(["g++", "-std=c++17", f"-I{CSRC}", str(source), "-o", str(program)], check=True)
+    said = subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout
+    assert [part.split() for part in said.split("|")[:-1]] == [
+        ["0", "0", "1", "5"], ["3", "3", "4"], ["8"], ["8"], ["8"], ["0", "0", "1", "5"], ["0", "0", "1", "5"]]
+
+
 def _arguments(device="cpu", dtype=BF16, rows=5, heads=4, kv_heads=2, dim=64, page=16, pages=6, batch=2, width=3):
     def t(*shape, dtype=dtype):
         return torch.zeros(shape, dtype=dtype, device=device)
@@ -1047,3 +1077,61 @@ def test_calls_on_several_streams_and_modes():
     version = p.k_pages._version
     paged_append_hip(p.q, p.randn(6, 2, 128), p.randn(6, 2, 128), p.k_pages, p.v_pages, p.table, p.cu, p.lengths, None)
     assert p.k_pages._version > version
+
+
+# ---- what the device's own bounds hold back ----
+
+class Guarded:
+    """A buffer filled with one value, of which ``t`` is the middle."""
+
+    def __init__(self, *shape, dtype=BF16, value=9.0, margin=4096):
+        count = math.prod(shape)
+        self.all = torch.full((count + 2 * margin,), value, dtype=dtype, device="cuda")
+        self.t, self.value, self.margin = self.all[margin:margin + count].view(shape), value, margin
+
+    def kept(self):
+        return bool((self.all[:self.margin] == self.value).all() and (self.all[-self.margin:] == self.value).all())
+
+
+def _c_cache(p, table, cu, lengths):
+    k, v = p.k_pages, p.v_pages
+    return _lib.PagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k.shape[0], k.shape[2],
+                           table.data_ptr(), table.shape[1], table.stride(0), cu.data_ptr(), lengths.data_ptr(),
+                           table.shape[0], k.shape[1], k.shape[3], {F16: 1, BF16: 2}[k.dtype])
+
+
+def _c_attention(p, out, *, cu, zero_rest, table=None, lengths=None, shared=0):
+    """The C entry point, so that rows behind the last sequence can be zeroed in a buffer of the test's."""
+    lib = _lib.load()
+    cache = _c_cache(p, p.table if table is None else table, cu, p.lengths if lengths is None else lengths)
+    rows = [_lib.Rows(t.data_ptr(), t.stride(0), t.stride(1)) for t in (p.q, out)]
+    need = lib.qwen2_paged_attention_workspace_bytes(ctypes.byref(cache), p.q.shape[0], p.heads, shared)
+    workspace = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.qwen2_paged_attention(ctypes.byref(cache), *map(ctypes.byref, rows), p.q.shape[0], p.heads, shared,
+                                         p.dim ** -0.5, zero_rest, workspace.data_ptr(), need, _stream()))
+    return need
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+@gpu
+@pytest.mark.parametrize("last", [2 ** 31 - 1, 2 ** 31 - 2, 5, 3, -1, -(2 ** 31)])
+@pytest.mark.parametrize("zero_rest", [0, 1])
+def test_a_last_bound_outside_the_rows(last, zero_rest):
+    """One split (the call's own stores see to the rows behind the last sequence), three
+    rows: whatever the last bound is, only rows behind it (all, where it is negative)
+    are zeroed, and nothing outside them is written."""
+    p = Paged([2, 1], [3, 40], heads=4)
+    cu = torch.tensor([0, 2, last], dtype=torch.int64).to(torch.int32).to(p.q.device)
+    out = Guarded(3, 4, 64)
+    assert _c_attention(p, out.t, cu=cu, zero_rest=zero_rest) == 0  # (no workspace: one split)
+    assert out.kept()
+    want, slack = p.reference()
+    if last >= 3:
+        _near(out.t, want, slack)
+    elif zero_rest:
+        assert not out.t[2].any()
+    else:
+        assert bool((out.t[2] == 9.0).all())
