@@ -78,7 +78,8 @@ int main() {
     for (int32_t end : ends) {
         const int32_t cu[3] = {0, 0, end};
         printf("%d", rows_end(cu, 2, 8));
-        for (unsigned workgroup : {0u, 1u, 5u, 2147483646u}) {  // rows behind the last sequence, of all 8
+        const unsigned workgroups[] = {0, 1, 5, 2147483646};
+        for (unsigned workgroup : workgroups) {  // rows behind the last sequence, of all 8
             const int64_t r = rest_row(cu, 2, 8, workgroup);
             if (r < 8) printf(" %lld", (long long)r);
         }
