@@ -239,7 +239,9 @@ __device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, S
     if (s.shared) {
         s.wide = a.prefix_wide;
         s.first_token = 0;
-        s.count = a.rows * a.group;
+        // (rows behind the last sequence are not this kernel's to write)
+        s.count = rows_end(a.c.cu_rows, a.c.batch, a.rows) * a.group;
+        if ((int64_t)s.tile * (s.wide ? kWideRows : kNarrowRows) >= s.count) return false;
         s.first = 0;
         s.key_lo = 0;
         s.key_end = a.prefix;

@@ -1136,3 +1136,32 @@ def test_a_last_bound_outside_the_rows(last, zero_rest):
         assert not out.t[2].any()
     else:
         assert bool((out.t[2] == 9.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [[2, 1], [17, 9], [60, 45], [1, 0]])
+@pytest.mark.parametrize("pages", [1, 8, 40])
+@pytest.mark.parametrize("tail", [1, 130])
+def test_rows_behind_the_last_sequence_of_a_prefix_alone(rows, pages, tail):
+    """All pages shared, so that no sequence has keys of its own: tables of one split and
+    of several, 16-row and 128-row tiles, padding that fills tiles of its own."""
+    p = Paged(rows, [0, 0], heads=12, tail=tail)
+    p.k_pages, p.v_pages = (p.randn(pages, 2, 16, 64) for _ in range(2))
+    p.table = torch.arange(pages, dtype=torch.int32, device=p.q.device).expand(2, pages)
+    p.used, p.shared = [list(range(pages))] * 2, pages
+    p.lengths_list = [max(16 * pages - 5, rows[0]), max(16 * pages - 11, rows[1])]
+    if pages == 1:  # (no row past the table; those before the sequence's start give zeros)
+        p.lengths_list = [min(n, 16) for n in p.lengths_list]
+    p.lengths.copy_(torch.tensor(p.lengths_list))
+    want, slack = p.reference()
+    got = p.attention()
+    _near(got[:p.total], want[:p.total], slack[:p.total])
+    assert not got[p.total:].any()
+    out = Guarded(*p.q.shape, value=7.0)
+    p.attention(out=out.t)
+    assert torch.equal(out.t[:p.total], got[:p.total])
+    assert bool((out.t[p.total:] == 7.0).all()) and out.kept()
+    p.cu.zero_()  # no rows at all
+    out.t.fill_(7.0)
+    p.attention(out=out.t)
+    assert bool((out.t == 7.0).all()) and not p.attention().any()
