@@ -12,9 +12,10 @@
 //
 // Only one row of the target's (and the draft's) probabilities is read per
 // sequence, 16 bytes a lane.  A weight is a difference of two 24-bit numbers and
-// the sums run over the vocabulary, so they are held in 64 bits: the chosen
-// entry is then the definition's, not the summation order's.  Sums have one
-// fixed order.
+// the sums run over the vocabulary, so they are held in 64 bits, in one fixed
+// order: the chosen entry is the definition's unless the uniform's share of the
+// total lies within roundings of 2^-53 of a border between two entries (then it
+// may be a neighbour of weight), and never one without weight.
 //
 // Bound by the rows' read from memory (64 x 4 drafts of 151936 fp32: 77.8 MB in
 // 13.9 us of the sums, 17 the call), and for few sequences by its chain of round
@@ -244,18 +245,27 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, int b, int lane, const
     double total = lane_f64(end, 63), run = 0.0, goal;
     int span = 0;
     if (total != 0.0) {
-        // the lane whose spans pass the goal (lane 63's end is the total), then the
-        // span: the last one of the lane's if its spans, added to what comes before
-        // them, stay a rounding below
+        // every lane goes through its own spans from where the lanes before it end: the
+        // first span of any weight at which the running sum passes the goal, of the first
+        // lane that has one; if all stay a rounding below, the last span of any weight
+        // (the lanes' ends are added up in different orders: one can lie above the one
+        // before it though its spans are empty, so that it alone does not choose)
         goal = (double)u * total;
-        const uint64_t past = __ballot(end > goal);
-        const int at = past ? __ffsll((unsigned long long)past) - 1 : 0;  // (none: no number)
-        run = at > 0 ? lane_f64(end, at - 1) : 0.0;
-        span = min(per * at, a.spans - 1);
-        for (const int stop = min(per * (at + 1), a.spans); span + 1 < stop; ++span) {
-            const double next = run + sums[span];
-            if (next > goal) break;
-            run = next;
+        const double up = __shfl_up(end, 1);  // (by every lane: one that is off gives nothing)
+        double sum = lane ? up : 0.0, before = 0.0;
+        int found = -1, some = -1;
+        for (int i = 0; i < per && first + i < a.spans && found < 0; ++i) {
+            const double own_sum = sums[first + i];
+            if (!(own_sum > 0.0)) continue;
+            some = first + i, before = sum;
+            sum += own_sum;
+            if (sum > goal) found = some;
+        }
+        const uint64_t passed = __ballot(found >= 0), any = __ballot(some >= 0);
+        if (passed | any) {
+            const int at = passed ? __ffsll((unsigned long long)passed) - 1 : 63 - __clzll((unsigned long long)any);
+            span = __builtin_amdgcn_readlane(some, at);  // (where one was found, the walk ended at it)
+            run = lane_f64(before, at);
         }
     } else {
         // the draft falls short of the target nowhere: the target alone, by this wave

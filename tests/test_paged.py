@@ -1165,3 +1165,55 @@ def test_rows_behind_the_last_sequence_of_a_prefix_alone(rows, pages, tail):
     out.t.fill_(7.0)
     p.attention(out=out.t)
     assert bool((out.t == 7.0).all()) and not p.attention().any()
+
+
+# ---- verification over rows of few entries ----
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [4097, 33000, 151936])
+def test_verify_on_a_border_before_spans_without_weight(vocab, dtype):
+    """Two entries of 2^-54 before two halves, 1024 apart, and a share of one half: the
+    first half's running sum, 2^-53 above it, passes.  (The lanes' sums in other orders
+    are 0.5 and, over the empty span behind it, 0.5 + 2^-53.)  Then entries of one lane's
+    several spans, and each entry alone."""
+    target = torch.zeros(1, 1, vocab, dtype=dtype, device="cuda")
+    target[0, 0, [0, 1024]] = 2.0 ** -54
+    target[0, 0, [2048, 4096]] = 0.5
+    none = torch.zeros(1, 0, dtype=torch.int64, device="cuda")
+    for u in (0.5, 0.5 - 2.0 ** -24, 0.5 + 2.0 ** -24, 0.0, 2.0 ** -60, 1.0):
+        share = torch.full((1, 1), u, device="cuda")
+        _same(verify_drafts_hip(target, none, share), _verified(target, none, share, None))
+    for at in [*range(0, vocab, 1021), vocab - 1]:
+        target.zero_()
+        target[0, 0, at] = 2.0 ** -20
+        for u in (0.0, 1.0 - 2.0 ** -24):
+            got = verify_drafts_hip(target, none, torch.full((1, 1), u, device="cuda"))
+            assert got[0].tolist() == [[at]], (at, u)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("batch, vocab", [(5, 5000), (3, 40000), (2, 151936), (260, 32000)])
+@pytest.mark.parametrize("kept", [1, 2, 20])
+def test_verify_of_rows_cut_to_their_largest(dtype, batch, vocab, kept):
+    """Probabilities cut to the largest few of a row, most spans empty, with a draft cut
+    to others; uniforms at zero, next to one, and between."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab + kept)
+
+    def cut(rows):
+        x = torch.rand(batch, rows, kept, generator=gen, device="cuda") + 0.05
+        at = torch.rand(batch, rows, vocab, generator=gen, device="cuda").topk(kept, -1).indices
+        return torch.zeros(batch, rows, vocab, device="cuda").scatter_(-1, at, x / x.sum(-1, True)).to(dtype), at
+
+    target, at = cut(3)
+    draft, drafted = cut(2)
+    tokens = torch.where(torch.rand(batch, 2, generator=gen, device="cuda") < 0.5, at[:, :2, 0], drafted[:, :, 0])
+    uniforms = torch.rand(batch, 3, generator=gen, device="cuda")
+    uniforms[::3, 2], uniforms[1::3, 2] = 0.0, 1.0 - 2.0 ** -24
+    for q in (draft, None):
+        got = verify_drafts_hip(target, tokens, uniforms, draft_probs=q)
+        _same(got, _verified(target, tokens, uniforms, q))
+        chosen = got[0].gather(1, got[1].long().view(-1, 1))
+        weight = target[torch.arange(batch, device=target.device), got[1].long()].gather(1, chosen)
+        assert bool((chosen >= 0).all() and (weight > 0).all())
