@@ -429,6 +429,12 @@ struct Attend {
     }
 };
 
+// What sums whose weight came out as zero still say: infinities and NaN, which the
+// formula's weight, small as it is, does not take away.
+__device__ __forceinline__ void add_odd(float& sum, float x) {
+    if (!(fabsf(x) < INFINITY)) sum += x;
+}
+
 // A value that a rare branch works with: keeps the compiler from running the
 // branch's instructions always.
 __device__ __forceinline__ int rare(int v) {
@@ -624,8 +630,16 @@ __device__ __forceinline__ void narrow(const PagedAttnArgs& a, const Segment& s,
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float f = __builtin_amdgcn_exp2f(st[w][0] - top);
-            // (no key, or none that counts: left out, whatever its sums are; NaN is kept)
-            if (f == 0.0f && st[w][1] == st[w][1]) continue;
+            if (f == 0.0f) {
+                // no key, or keys of no weight beside the others': nothing, unless a value that
+                // the row sees was not finite
+                if (st[w][0] > -INFINITY) {
+                    if (st[w][1] != st[w][1]) l = st[w][1];
+#pragma unroll
+                    for (int i = 0; i < A::kVd; ++i) add_odd(sum[i], lines(w)[g][d0 + i]);
+                }
+                continue;
+            }
             l = fmaf(st[w][1], f, l);
 #pragma unroll
             for (int i = 0; i < A::kVd; ++i) sum[i] = fmaf(lines(w)[g][d0 + i], f, sum[i]);
@@ -970,6 +984,13 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
             for (int e = 0; e < kPer; ++e) sum[e] = fs != 0.0f ? fmaf(x[i][e], fs, sum[e]) : sum[e];
         }
         if (first + 8 < a.slots) load(first + 8);
+    }
+    // slots of no weight beside the others': their values that were not finite
+    for (uint64_t low = __ballot(m > -INFINITY && f == 0.0f); low; low &= low - 1) {
+        const fvec odd = *(const fvec*)(part + (__ffsll((unsigned long long)low) - 1) * D);
+        if (half == 0)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) add_odd(sum[e], odd[e]);
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum[e] += __shfl_xor(sum[e], 32);

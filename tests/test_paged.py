@@ -1217,3 +1217,30 @@ def test_verify_of_rows_cut_to_their_largest(dtype, batch, vocab, kept):
         chosen = got[0].gather(1, got[1].long().view(-1, 1))
         weight = target[torch.arange(batch, device=target.device), got[1].long()].gather(1, chosen)
         assert bool((chosen >= 0).all() and (weight > 0).all())
+
+
+# ---- values that are not finite, at keys of hardly any weight ----
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("rows, past, shared, spots", [
+    ([1], [100], 0, [40]), ([2], [900], 0, [0, 500]), ([1, 1], [300, 40], 9, [3, 150]), ([60, 1], [2000, 7], 0, [64, 1033]),
+    ([40], [100], 40, [100, 600])])
+def test_values_that_are_not_finite_at_keys_of_little_weight(dtype, bad, rows, past, shared, spots):
+    """Scores of the 64 keys around a spot some 10^-125 below the others: whichever wave
+    or split has them alone, an infinity or NaN among their values reaches the rows that
+    see it (the formula's weight is not zero), and its dimension only."""
+    p = Paged(rows, past, heads=12, dim=64, shared=shared, dtype=dtype)
+    p.q.copy_(1.0 + p.randn(*p.q.shape) / 16)
+    for b, length in enumerate(p.lengths_list):
+        where = torch.tensor(p.used[b], device=p.q.device)[:-(-length // 16)]
+        p.k_pages[where] = 4.0 + p.randn(len(where), 2, 16, 64) / 16
+    for spot in spots:
+        first = max(0, spot // 32 * 32 - 32)
+        for t in range(first, min(first + 96, p.lengths_list[0] - rows[0])):
+            p.k_pages[p.used[0][t // 16], :, t % 16] = -32.0
+        p.v_pages[p.used[0][spot // 16], :, spot % 16, 9] = bad
+    want, slack = p.reference()
+    assert not want[:rows[0], :, 9].isfinite().any()
+    _near(p.attention(), want, slack)
