@@ -220,8 +220,8 @@ int qwen2_paged_append(const qwen2_paged_cache* cache, const qwen2_rows* q, cons
  * first row's are read, once for all sequences.  A row without a position
  * (lengths[b] too small) gives zeros; a row that reaches past its table, or to
  * a page that is not in the pool, gives NaN.  (Values are summed before the sum is
- * divided: 2^8 times the keys' number times their size has to stay in fp32.)  Rows behind the last sequence are
- * left as they are, or zeroed with zero_rest.  Keys and values at positions that
+ * divided: the keys' number times the values' size has to stay in fp32.)  Rows behind the
+ * last sequence are left as they are, or zeroed with zero_rest.  Keys and values at positions that
  * a row does not see take no part, whatever they hold.
  * head_dim is 64 or 128; heads a multiple of kv_heads; out must not overlap q.
  * The workspace (16-byte aligned) holds fp32 partial results; nothing in it

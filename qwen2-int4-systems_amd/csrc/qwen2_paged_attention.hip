@@ -48,7 +48,8 @@
 //
 // The sums are rescaled only once a score passes their reference by kLazy units
 // of the base-2 exponent (from the floor on the first block); until then
-// probabilities reach 2^kLazy, which changes no relative rounding.
+// probabilities reach 2^kLazy times the reference's, which changes no relative
+// rounding.
 //
 // Pages hold at least 16 positions, so that 16 aligned keys lie in one page and
 // the page's number is the wave's, not the lane's.  Every loaded address lies in
@@ -105,10 +106,13 @@ struct PagedAttnArgs {
     Divisor by_group, by_heads, by_kv_heads, by_prefix_splits, by_own_splits;
 };
 
-// Exponents of probabilities: fp16 ends at 2^-24 and at 2^16, and a key far below
-// its row's maximum still counts if there are many; with 2^11 for the reference
-// the terms reach down to 2^-35 of it.
-template <class E> constexpr float kProbShift = 0.0f;
+// Exponents of probabilities.  bf16: they reach 2^kLazy before the sums are
+// rescaled, and stay at one or below with 2^-kLazy for the reference, so that values
+// add up as far as fp32 holds the keys' number times their size.  fp16 ends at
+// 2^-24 and at 2^16, and a key far below its row's maximum still counts if there are
+// many; with 2^11 for the reference the terms reach down to 2^-35 of it (and its
+// values times their number stay far inside fp32).
+template <class E> constexpr float kProbShift = -8.0f;
 template <> constexpr float kProbShift<F16> = 11.0f;
 template <class E> constexpr float kLazy = 8.0f;
 template <> constexpr float kLazy<F16> = 4.0f;

@@ -84,8 +84,11 @@ def paged_attention_hip(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
 
     Keys and values that a row does not see take no part, whatever they hold.  A
     row without a position gives zeros.  Rows behind the last sequence are left
-    as they are in ``out``, and zeros in a new tensor.  Softmax and sums are fp32,
-    in a fixed order: the same inputs give the same bits."""
+    as they are in ``out``, and zeros in a new tensor.  Scores, softmax and sums are
+    fp32, in a fixed order: the same inputs give the same bits.  Probabilities enter
+    the value products as two terms of the tensors' type (16 bits or more of them), and
+    values are summed before the sum is divided: the keys' number times the values'
+    size has to stay in fp32.  The result is rounded once."""
     return _calls().paged_attention(q, k_pages, v_pages, page_table, cu_rows, lengths, shared_pages, scale, out)
 
 

@@ -1244,3 +1244,33 @@ def test_values_that_are_not_finite_at_keys_of_little_weight(dtype, bad, rows, p
     want, slack = p.reference()
     assert not want[:rows[0], :, 9].isfinite().any()
     _near(p.attention(), want, slack)
+
+
+# ---- values of any size ----
+
+@gpu
+@pytest.mark.parametrize("rows, past, batch, shared", [
+    ([1], [1023], 400, 0), ([2], [1022], 1, 0), ([260], [900], 1, 0), ([70], [30], 2, 64)])
+@pytest.mark.parametrize("size", [2.0 ** 117, 2.0 ** -110])
+def test_values_of_any_size(rows, past, batch, shared, size):
+    """Scores that rise by nearly eight units of the base-2 exponent after every wave's
+    first keys, and values whose sum over the keys fp32 just holds (2^117 times a
+    thousand to two thousand), then small ones.  Many sequences over the same pages:
+    one split."""
+    p = Paged(rows, past, heads=12, dim=64, shared=shared)
+    p.q.fill_(1.0)
+    length = p.lengths_list[0]
+    where = torch.tensor(p.used[0], device=p.q.device)
+    p.k_pages[where] = 0.6  # (0.6 * 64 / 8 = 4.8: 6.9 units of the base-2 exponent)
+    for first in range(0, length, 1024):
+        p.k_pages[where[first // 16:(first + 128) // 16]] = 0.0
+    p.v_pages[where] = ((1.0 + torch.rand(len(where), 2, 16, 64, device=p.q.device) / 2) * size).to(BF16)
+    want, slack = p.reference()
+    assert bool(want.isfinite().all())
+    if batch > 1:
+        p.q = p.q.repeat(batch, 1, 1)
+        p.table = p.table.expand(batch, -1)
+        p.cu = torch.arange(batch + 1, dtype=torch.int32, device=p.q.device) * rows[0]
+        p.lengths = p.lengths.repeat(batch)
+        want, slack = want.repeat(batch, 1, 1), slack.repeat(batch, 1, 1)
+    _near(p.attention(), want, slack)
