@@ -135,6 +135,43 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
     return x.first < y.second && y.first < x.second;
 }
 
+// Whether an entry of one view is one of the other: two addresses meet where the
+// offset is a sum of strides, each as often as its dimension's indices can differ
+// (a.size - 1 to -(b.size - 1)).  Dimensions go by falling strides; what is left
+// after one has to lie within what the smaller ones span.
+struct Dim {
+    int64_t stride, up, down;
+};
+bool meets(const Dim* dim, int count, int64_t offset) {
+    if (!count) return offset == 0;
+    int64_t up = 0, down = 0;  // of the smaller strides
+    for (int i = 1; i < count; ++i) up += dim[i].stride * dim[i].up, down += dim[i].stride * dim[i].down;
+    const int64_t s = dim->stride;
+    auto below = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };  // (rounded down)
+    const int64_t from = std::max(-below(up - offset, s), -dim->down), to = std::min(below(offset + down, s), dim->up);
+    if (to - from > 8) return true;  // (strides that do not nest: not told apart)
+    for (int64_t n = from; n <= to; ++n)
+        if (meets(dim + 1, count - 1, offset - n * s)) return true;
+    return false;
+}
+
+// Whether two views may share memory: told exactly where they have the same strides
+// (parts of one buffer), else by their ranges.
+bool share(const at::Tensor& a, const at::Tensor& b) {
+    if (!overlap(a, b)) return false;
+    const int64_t bytes = (const char*)b.const_data_ptr() - (const char*)a.const_data_ptr();
+    if (a.dim() != b.dim() || a.dim() > 4 || a.scalar_type() != b.scalar_type() || bytes % a.element_size()) return true;
+    Dim dims[4];
+    int count = 0;
+    for (int64_t d = 0; d < a.dim(); ++d) {
+        const int64_t x = step(a, d), y = step(b, d);
+        if (a.size(d) > 1 && b.size(d) > 1 && x != y) return true;
+        if (x + y) dims[count++] = Dim{std::max(x, y), a.size(d) - 1, b.size(d) - 1};
+    }
+    std::sort(dims, dims + count, [](const Dim& l, const Dim& r) { return l.stride > r.stride; });
+    return meets(dims, count, bytes / a.element_size());
+}
+
 bool same_view(const at::Tensor& a, const at::Tensor& b) {
     return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
 }
@@ -189,7 +226,7 @@ struct Cache {
             if (t->numel() && (!readable(*t) || !distinct(*t)))
                 refuse(PyExc_ValueError, "%s must be 16-byte aligned with a contiguous last dimension, other strides "
                        "multiples of 8, and no two entries in one place", t == &k ? "k_pages" : "v_pages");
-        if (k.numel() && k.const_data_ptr() == v.const_data_ptr())
+        if (share(k, v))
             refuse(PyExc_ValueError, "k_pages and v_pages must not share memory");
         c.num_pages = k.size(0), c.kv_heads = k.size(1), c.page_size = k.size(2), c.head_dim = k.size(3);
         c.k_page = step(k, 0), c.k_head = step(k, 1), c.k_position = step(k, 2);

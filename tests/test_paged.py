@@ -171,6 +171,41 @@ def test_append_and_attention_refuse_their_own():
             paged_attention_hip(**(attention | change))
 
 
+def _pools():
+    """(k_pages, v_pages of [6, 2, 16, 64], whether they lie apart) of one buffer each."""
+    def z(*shape):
+        return torch.zeros(shape, dtype=BF16)
+
+    yield *z(2, 6, 2, 16, 64).unbind(0), True
+    yield *z(6, 2, 2, 16, 64).unbind(1), True          # side by side in a page
+    yield *z(6, 2, 2, 16, 64).unbind(2), True          # in a head
+    yield *z(6, 2, 16, 2, 64).unbind(3), True          # in a position
+    yield *z(6, 2, 16, 128).split(64, 3), True
+    yield *(t.transpose(1, 2) for t in z(6, 16, 4, 64).split(2, 2)), True
+    pool = z(16, 2, 16, 64)
+    yield pool[0:12:2], pool[3:15:2], True             # even pages, odd pages
+    yield pool[3:15:2], pool[0:12:2], True
+    yield pool[0:12:2], pool[4:16:2], False
+    yield pool[:6], pool[5:11], False                  # one page of both
+    yield pool[5:11], pool[:6], False
+    yield pool[:6], pool[:6], False
+    row = z(6 * 2 * 16 * 64 + 8 * 64)
+    yield row[:12288].view(6, 2, 16, 64), row[512:].view(6, 2, 16, 64), False  # a position eight further
+    wide = z(6, 2, 16, 128)
+    yield wide[..., :64], wide[..., 32:96], False      # half of each vector
+    yield wide[..., 64:], wide[..., :64], True
+    yield pool[:6], pool[:12].view(6, 2, 2, 16, 64)[:, 1], False  # other strides: by their ranges
+
+
+@built
+@pytest.mark.parametrize("k_pages, v_pages, apart", list(_pools()))
+def test_pools_that_share_memory_are_refused(k_pages, v_pages, apart):
+    append, attention = _arguments()
+    for call, arguments in ((paged_append_hip, append), (paged_attention_hip, attention)):
+        with pytest.raises(ValueError, match="must be a GPU tensor" if apart else "must not share memory"):
+            call(**(arguments | {"k_pages": k_pages, "v_pages": v_pages}))
+
+
 @built
 def test_verify_refuses_before_launch():
     good = {"target_probs": torch.zeros(2, 4, 9), "draft_tokens": torch.zeros(2, 3, dtype=torch.int64),
