@@ -1275,9 +1275,10 @@ def test_values_that_are_not_finite_at_keys_of_little_weight(dtype, bad, rows, p
         first = max(0, spot // 32 * 32 - 32)
         for t in range(first, min(first + 96, p.lengths_list[0] - rows[0])):
             p.k_pages[p.used[0][t // 16], :, t % 16] = -32.0
+    want, slack = p.reference()  # (finite: a library product with an infinity may give NaN)
+    for spot in spots:
         p.v_pages[p.used[0][spot // 16], :, spot % 16, 9] = bad
-    want, slack = p.reference()
-    assert not want[:rows[0], :, 9].isfinite().any()
+    want[:None if spots[0] < 16 * shared else rows[0], :, 9] = bad
     _near(p.attention(), want, slack)
 
 
