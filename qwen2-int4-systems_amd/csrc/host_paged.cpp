@@ -176,10 +176,11 @@ bool same_view(const at::Tensor& a, const at::Tensor& b) {
     return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
 }
 
-// Whether the rows of two views of one buffer (parts of a fused projection) lie
-// apart: rows equally far from each other, and within a row one behind the other.
-bool rows_apart(const at::Tensor& a, const at::Tensor& b) {
-    if (!overlap(a, b)) return true;
+// Whether two row tensors lie apart: told by share(), or, where their heads lie at
+// other strides (parts of a fused projection), rows equally far from each other and
+// within a row one behind the other.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+    if (!share(a, b)) return true;
     const at::Tensor& x = a.const_data_ptr() <= b.const_data_ptr() ? a : b;
     const at::Tensor& y = &x == &a ? b : a;
     const int64_t between = ((const char*)y.const_data_ptr() - (const char*)x.const_data_ptr()) / x.element_size();
@@ -334,10 +335,12 @@ PyObject* host_paged_append(PyObject*, PyObject* const* args, Py_ssize_t count) 
             if (overlap(*t, q) || overlap(*t, k) || overlap(*t, v) || (given && overlap(*t, *given)))
                 refuse(PyExc_ValueError, "the cache must not share memory with q, k, v or out");
         }
-        if (given && !same_view(*given, q) && (overlap(*given, q) || overlap(*given, k) || overlap(*given, v)))
+        if (given && same_view(*given, q)) {
+            if (!apart(q, k) || !apart(q, v))
+                refuse(PyExc_ValueError, "q must not share its rows with k and v where it is rotated in place");
+        } else if (given && (!apart(*given, q) || !apart(*given, k) || !apart(*given, v))) {
             refuse(PyExc_ValueError, "out must be q itself or share no memory with q, k and v");
-        if (given && (!rows_apart(q, k) || !rows_apart(q, v)))
-            refuse(PyExc_ValueError, "q must not share its rows with k and v where it is rotated in place");
+        }
         const c10::DeviceGuard guard(device);
         if (!cache.c.batch || !rows) return THPVariable_Wrap(given ? *given : at::zeros(q.sizes(), q.options().requires_grad(false)));
         cache.bind();
@@ -377,7 +380,7 @@ PyObject* host_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t coun
         const c10::Device device = device_of({{&q, "q"}, {&cache.k, "k_pages"}, {&cache.v, "v_pages"},
             {&cache.table_arg, "page_table"}, {&cache.cu_arg, "cu_rows"}, {&cache.lengths_arg, "lengths"},
             {given ? given : &q, "out"}});
-        if (given && (overlap(*given, q) || overlap(*given, cache.k) || overlap(*given, cache.v)))
+        if (given && (!apart(*given, q) || overlap(*given, cache.k) || overlap(*given, cache.v)))
             refuse(PyExc_ValueError, "out must share no memory with q and the cache");
         const c10::DeviceGuard guard(device);
         if (!cache.c.batch || !rows) return THPVariable_Wrap(given ? *given : at::zeros(q.sizes(), q.options().requires_grad(false)));

@@ -1310,3 +1310,62 @@ def test_values_of_any_size(rows, past, batch, shared, size):
         p.lengths = p.lengths.repeat(batch)
         want, slack = want.repeat(batch, 1, 1), slack.repeat(batch, 1, 1)
     _near(p.attention(), want, slack)
+
+
+# ---- outputs beside their inputs ----
+
+@gpu
+def test_append_into_outputs_beside_its_inputs():
+    """What lies apart is taken, wherever it lies: an output of its own for queries and
+    keys of one tensor, heads of q, k and v in turn, an output between the queries' heads,
+    keys and values in turn behind the queries."""
+    p = Paged([3, 2], [7, 0], heads=2)
+    inv = torch.rand(32, device="cuda")
+
+    def append(q, k, v, out=None):
+        return paged_append_hip(q, k, v, p.k_pages, p.v_pages, p.table, p.cu, p.lengths, inv, out=out)
+
+    def caches():
+        return [c.view(torch.int16).clone() for c in (p.k_pages, p.v_pages)]
+
+    def same(got, q, k, v):
+        """The call's outputs against those for copies of its inputs."""
+        left = caches()
+        assert torch.equal(got, append(q.clone(), k.clone(), v.clone()))
+        assert all(torch.equal(a, b) for a, b in zip(left, caches()))
+
+    one = p.randn(5, 2, 64)
+    kept = one.clone()
+    same(append(one, one, one, torch.empty_like(one)), one, one, one)
+    assert torch.equal(one, kept)
+    for fused in (p.randn(5, 2, 3, 64), p.randn(5, 3, 2, 64).transpose(1, 2)):
+        q, k, v = (fused[:, :, i] for i in range(3))
+        before = q.clone()
+        got = append(q, k, v, q)
+        assert got.data_ptr() == q.data_ptr()
+        same(got, before, k, v)
+        before, other = k.clone(), v.clone()
+        same(append(q, k, k, v), q, k, k)  # (over v's place)
+        assert torch.equal(k, before) and not torch.equal(v, other)
+    rows = p.randn(5, 6, 64)
+    q, k, v = rows[:, :2], rows[:, 2::2], rows[:, 3::2]
+    before = q.clone()
+    same(append(q, k, v, q), before, k, v)
+    rows = p.randn(5, 6, 64)
+    for out in (rows[:, 1:3], rows[:, 1:5:2], rows[:, 3:5]):
+        with pytest.raises(ValueError, match="out must be q itself"):
+            append(rows[:, :2], rows[:, 2:4], rows[:, 4:], out)
+    with pytest.raises(ValueError, match="must not share its rows"):
+        append(rows[:, :2], rows[:, 1:3], rows[:, 4:], rows[:, :2])
+
+
+@gpu
+def test_attention_into_an_output_between_the_queries():
+    p = Paged([3, 1], [20, 5], heads=4, shared=1)
+    want = p.attention()
+    both = torch.zeros(4, 4, 2, 64, dtype=BF16, device="cuda")
+    both[:, :, 0] = p.q
+    p.attention(q=both[:, :, 0], out=both[:, :, 1])
+    assert torch.equal(both[:, :, 1], want) and torch.equal(both[:, :, 0], p.q)
+    with pytest.raises(ValueError, match="share no memory"):
+        p.attention(q=both[:, :, 0], out=both.view(4, 8, 64)[:, 2:6])
