@@ -43,9 +43,12 @@ struct Refusal {
 
 void check_status(int status) {
     if (status == W4G64_STATUS_OK) return;
+    // (what these operators do not support is a matter of shapes and strides)
     PyObject* type = status == W4G64_STATUS_INVALID_DTYPE ? PyExc_TypeError
-                     : status == W4G64_STATUS_INVALID_VALUE || status == W4G64_STATUS_WORKSPACE ? PyExc_ValueError
-                                                                                                 : PyExc_RuntimeError;
+                     : status == W4G64_STATUS_INVALID_VALUE || status == W4G64_STATUS_WORKSPACE ||
+                             status == W4G64_STATUS_UNSUPPORTED
+                         ? PyExc_ValueError
+                         : PyExc_RuntimeError;
     throw Refusal{type, w4g64_last_error()};
 }
 

@@ -1369,3 +1369,30 @@ def test_attention_into_an_output_between_the_queries():
     assert torch.equal(both[:, :, 1], want) and torch.equal(both[:, :, 0], p.q)
     with pytest.raises(ValueError, match="share no memory"):
         p.attention(q=both[:, :, 0], out=both.view(4, 8, 64)[:, 2:6])
+
+
+# ---- limits of shapes ----
+
+@gpu
+def test_limits_of_shapes_are_value_errors():
+    def z(*shape, dtype=BF16):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    cu, lengths = torch.tensor([0, 2], dtype=torch.int32, device="cuda"), z(1, dtype=torch.int32)
+    for dim in (32, 72, 80, 256):
+        with pytest.raises(ValueError, match="head_dim of 64 or 128"):
+            paged_attention_hip(z(2, 4, dim), z(3, 2, 16, dim), z(3, 2, 16, dim), z(1, 3, dtype=torch.int32), cu, lengths)
+    for dim in (72, 272):
+        with pytest.raises(ValueError, match="head_dim that is a multiple of 16 up to 256"):
+            paged_append_hip(z(2, 4, dim), z(2, 2, dim), z(2, 2, dim), z(3, 2, 16, dim), z(3, 2, 16, dim),
+                             z(1, 3, dtype=torch.int32), cu, lengths, None)
+    pool = [z(1, 1, 1 << 20, 64) for _ in range(2)]
+    with pytest.raises(ValueError, match="at most 2.31 - 2.20 positions"):
+        paged_attention_hip(z(2, 1, 64), *pool, z(1, 2048, dtype=torch.int32), cu, lengths)
+    with pytest.raises(ValueError, match="page_size must be a power of two"):
+        paged_attention_hip(z(2, 1, 64), z(1, 1, 24, 64), z(1, 1, 24, 64), z(1, 2, dtype=torch.int32), cu, lengths)
+    with pytest.raises(ValueError, match="shared_pages must be in"):
+        paged_attention_hip(z(2, 1, 64), *pool, z(1, 2, dtype=torch.int32), cu, lengths, shared_pages=3)
+    far = torch.empty(15 * (1 << 25) + 64, dtype=BF16, device="cuda").as_strided((1, 1, 16, 64), (0, 0, 1 << 25, 1))
+    with pytest.raises(ValueError, match="position strides must be at most 2.24"):
+        paged_attention_hip(z(2, 1, 64), far, z(1, 1, 16, 64), z(1, 2, dtype=torch.int32), cu, lengths)
