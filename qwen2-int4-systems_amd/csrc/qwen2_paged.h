@@ -26,6 +26,7 @@ struct PagedView {
 
 // The rows of one sequence, bounded by [0, rows] whatever cu_rows holds, and
 // the position of its first one (negative where lengths says less than n).
+// The kernels give rows_end() for `rows`: no sequence reaches past the last one.
 struct SequenceRows {
     int begin, end;
     int64_t first;

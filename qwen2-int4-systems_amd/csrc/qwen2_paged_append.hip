@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(AppendArgs a)
     const int units = (a.heads + 2 * a.c.kv_heads) * per;
     const int seq = sequence_of(a.c.cu_rows, a.c.batch, row, lane);
     SequenceRows s{0, 0, 0};
-    if (seq < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, seq, a.rows);
+    if (seq < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, seq, rows_end(a.c.cu_rows, a.c.batch, a.rows));
     if (row < s.begin || row >= s.end) {  // no sequence's row
         if (!a.zero_rest) return;
         for (int u = 64 * part + lane; u < a.heads * per; u += 64 * a.parts) {

@@ -181,10 +181,11 @@ __device__ __forceinline__ bool wide_rows(const PagedAttnArgs& a, int tokens) {
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int tile, int lane, int& sequence, int& local,
                                           SequenceRows& rows) {
     int before = 0;
+    const int all = rows_end(a.c.cu_rows, a.c.batch, a.rows);
     for (int base = 0; base < a.c.batch; base += 64) {
         const int i = base + lane;
         SequenceRows s{0, 0, 0};
-        if (i < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
+        if (i < a.c.batch) s = sequence_rows(a.c.cu_rows, a.c.lengths, i, all);
         const int tokens = s.end - s.begin;
         const int count = wide_rows(a, tokens) ? (tokens * a.group + kWideRows - 1) / kWideRows
                                                : (tokens * a.group + kNarrowRows - 1) / kNarrowRows;
@@ -244,7 +245,8 @@ __device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, S
         s.wide = a.prefix_wide;
         s.first_token = 0;
         // (rows behind the last sequence are not this kernel's to write)
-        s.count = rows_end(a.c.cu_rows, a.c.batch, a.rows) * a.group;
+        const int all = rows_end(a.c.cu_rows, a.c.batch, a.rows);
+        s.count = all * a.group;
         if ((int64_t)s.tile * (s.wide ? kWideRows : kNarrowRows) >= s.count) return false;
         s.first = 0;
         s.key_lo = 0;
@@ -253,7 +255,7 @@ __device__ __forceinline__ bool find_segment(const PagedAttnArgs& a, int lane, S
         // (the usual case, found out at once: all new positions lie behind the prefix)
         bool behind = a.own_splits > 0;
         for (int i = lane; i < a.c.batch; i += 64) {
-            const SequenceRows r = sequence_rows(a.c.cu_rows, a.c.lengths, i, a.rows);
+            const SequenceRows r = sequence_rows(a.c.cu_rows, a.c.lengths, i, all);
             behind = behind && (r.end == r.begin || r.first >= a.prefix);
         }
         s.sees_all = __all(behind);
@@ -298,7 +300,7 @@ __device__ __forceinline__ Row row_at(const PagedAttnArgs& a, const Segment& s, 
         const int b = sequence_by_halving(a.c.cu_rows, a.c.batch, r.token);
         known = known && b < a.c.batch;
         if (known) {
-            const SequenceRows q = sequence_rows(a.c.cu_rows, a.c.lengths, b, a.rows);
+            const SequenceRows q = sequence_rows(a.c.cu_rows, a.c.lengths, b, rows_end(a.c.cu_rows, a.c.batch, a.rows));
             known = r.token >= q.begin && r.token < q.end;
             position = q.first + (r.token - q.begin);
         }

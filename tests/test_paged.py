@@ -1396,3 +1396,39 @@ def test_limits_of_shapes_are_value_errors():
     far = torch.empty(15 * (1 << 25) + 64, dtype=BF16, device="cuda").as_strided((1, 1, 16, 64), (0, 0, 1 << 25, 1))
     with pytest.raises(ValueError, match="position strides must be at most 2.24"):
         paged_attention_hip(z(2, 1, 64), far, z(1, 1, 16, 64), z(1, 2, dtype=torch.int32), cu, lengths)
+
+
+# ---- row bounds that fall or lead out, with everything around the buffers watched ----
+
+@gpu
+@pytest.mark.parametrize("values", [[-7, 90, 2, -1], [5, 5, 5, 5], [0, 2 ** 31 - 1, -(2 ** 31), 4], [0, 2, 3, 2 ** 31 - 1],
+                                    [0, 0, 0, -(2 ** 31)], [2 ** 31 - 1] * 4, [0, 4, 0, 4], [3, 2, 1, 0]])
+@pytest.mark.parametrize("rows, shared", [([2, 1, 1], 2), ([2, 1, 1], 0), ([60, 1, 50], 0), ([60, 1, 50], 9)])
+def test_row_bounds_that_fall_or_lead_out_write_nothing_else(values, rows, shared):
+    """Whatever cu_rows holds: rows behind its last entry keep what they hold, and nothing
+    around the output, the pools and the rotated queries is written, nor a page that no
+    table entry names."""
+    p = Paged(rows, [3, 40, 9], shared=shared, heads=12)
+    scale = p.total // 4  # (bounds inside the rows at both sizes)
+    p.cu.copy_(torch.tensor([v * scale if 0 < v < 100 else v for v in values], dtype=torch.int64).to(torch.int32))
+    pools = [Guarded(*c.shape, value=5.0) for c in (p.k_pages, p.v_pages)]
+    for pool, cache in zip(pools, (p.k_pages, p.v_pages)):
+        pool.t.copy_(cache.nan_to_num(0.25))
+    before = [pool.t.clone() for pool in pools]
+    end = max(int(p.cu[-1]), 0)
+    k, v = p.randn(p.total, 2, 64), p.randn(p.total, 2, 64)
+    turned = Guarded(*p.q.shape, value=7.0)
+    paged_append_hip(p.q, k, v, pools[0].t, pools[1].t, p.table, p.cu, p.lengths, None, out=turned.t)
+    assert turned.kept() and bool((turned.t[end:] == 7.0).all())
+    named = torch.zeros(p.k_pages.shape[0], dtype=torch.bool, device="cuda")
+    named[[page for used in p.used for page in used]] = True
+    for pool, old in zip(pools, before):
+        assert pool.kept() and torch.equal(pool.t[~named], old[~named])
+    after = [pool.t.clone() for pool in pools]
+    out = Guarded(*p.q.shape, value=7.0)
+    paged_attention_hip(p.q, pools[0].t, pools[1].t, p.table, p.cu, p.lengths, shared_pages=shared, out=out.t)
+    assert out.kept() and bool((out.t[end:] == 7.0).all())
+    fresh = paged_attention_hip(p.q, pools[0].t, pools[1].t, p.table, p.cu, p.lengths, shared_pages=shared)
+    assert not fresh[end:].any()
+    for pool, old in zip(pools, after):
+        assert pool.kept() and torch.equal(pool.t, old)
