@@ -234,8 +234,15 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, int b, int lane, const
     constexpr int kOwn = kSpan / 64;
     const int per = (a.spans + 63) / 64;
     const int first = per * lane;
-    double own = 0.0;
-    for (int i = 0; i < per && first + i < a.spans; ++i) own += sums[first + i];
+    // (the usual vocabulary's spans of a lane are held: their loads go out together)
+    constexpr int kHeld = 3;
+    const int mine_spans = min(per, a.spans - first);
+    double held[kHeld], own = 0.0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = i < mine_spans ? sums[first + i] : 0.0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) own += held[i];
+    for (int i = kHeld; i < mine_spans; ++i) own += sums[first + i];
     float u = a.uniforms[(int64_t)b * (a.drafts + 1) + a.drafts];
     Weights w = weights_of(a, b, n, count);
     constexpr float kBelowOne = 0.999999940395355224609375f;  // 1 - 2^-24
@@ -254,13 +261,15 @@ __device__ __forceinline__ void pick(const VerifyArgs& a, int b, int lane, const
         const double up = __shfl_up(end, 1);  // (by every lane: one that is off gives nothing)
         double sum = lane ? up : 0.0, before = 0.0;
         int found = -1, some = -1;
-        for (int i = 0; i < per && first + i < a.spans && found < 0; ++i) {
-            const double own_sum = sums[first + i];
-            if (!(own_sum > 0.0)) continue;
+        auto pass = [&](int i, double weight) {
+            if (found >= 0 || !(weight > 0.0)) return;
             some = first + i, before = sum;
-            sum += own_sum;
+            sum += weight;
             if (sum > goal) found = some;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) pass(i, held[i]);
+        for (int i = kHeld; i < mine_spans; ++i) pass(i, sums[first + i]);
         const uint64_t passed = __ballot(found >= 0), any = __ballot(some >= 0);
         if (passed | any) {
             const int at = passed ? __ffsll((unsigned long long)passed) - 1 : 63 - __clzll((unsigned long long)any);
