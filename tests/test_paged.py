@@ -1432,3 +1432,33 @@ def test_row_bounds_that_fall_or_lead_out_write_nothing_else(values, rows, share
     assert not fresh[end:].any()
     for pool, old in zip(pools, after):
         assert pool.kept() and torch.equal(pool.t, old)
+
+
+# ---- tables wider than the sequences, long sequences ----
+
+@gpu
+@pytest.mark.parametrize("columns", [1, 60, 2000])
+@pytest.mark.parametrize("rows, past, more", [
+    ([1, 1, 1], [3, 200, 31], {"dim": 128, "heads": 12}),
+    ([1] * 5, [0, 2, 15, 16, 300], {"shared": 9, "heads": 8, "dtype": F16}),
+    ([70, 1, 33], [0, 400, 5], {"heads": 12, "dim": 128, "page": 32}),
+    ([60, 30], [64, 7], {"shared": 21, "heads": 12, "dim": 64}),
+])
+def test_tables_wider_than_their_sequences(rows, past, more, columns):
+    """Columns behind the longest sequence, as a captured graph's table has them: what they
+    hold (no page, or any) is not looked at."""
+    p = Paged(rows, past, **more)
+    want, slack = p.reference()
+    spare = torch.full((len(rows), columns), -1, dtype=torch.int32, device="cuda")
+    spare[:, ::3] = 2 ** 31 - 1
+    spare[:, 1::3] = 0
+    p.table = torch.cat((p.table, spare), 1)
+    _near(p.attention(), want, slack)
+
+
+@gpu
+@pytest.mark.parametrize("rows, past, heads, dim, dtype", [(1, 20000, 12, 128, BF16), (3, 33333, 8, 64, F16),
+                                                           (30, 9000, 12, 64, BF16)])
+def test_attention_over_one_long_sequence(rows, past, heads, dim, dtype):
+    p = Paged([rows], [past], heads=heads, dim=dim, page=128, dtype=dtype)
+    _near(p.attention(), *p.reference())
