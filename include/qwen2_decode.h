@@ -163,7 +163,8 @@ int qwen2_cached_attention(const void* q, const void* k, const void* v, const vo
  * positions: row i of n sits at position lengths[b] - n + i.  Position t of
  * sequence b lies in page page_table[b][t / page_size], place t % page_size.
  * cu_rows, lengths and page_table are read on the device; what they hold is
- * bounded there: no access leaves the buffers whatever it is.
+ * bounded there: no access leaves the buffers whatever it is, and no row from
+ * cu_rows[batch] on is written but to be zeroed.
  * ------------------------------------------------------------------------- */
 
 typedef struct qwen2_paged_cache {
@@ -223,7 +224,12 @@ int qwen2_paged_append(const qwen2_paged_cache* cache, const qwen2_rows* q, cons
  * divided: the keys' number times the values' size has to stay in fp32.)  Rows behind the
  * last sequence are left as they are, or zeroed with zero_rest.  Keys and values at positions that
  * a row does not see take no part, whatever they hold.
+ * An infinity or NaN among the values of a key that a row sees reaches the row
+ * however small the key's weight.
  * head_dim is 64 or 128; heads a multiple of kv_heads; out must not overlap q.
+ * A call is cut into workgroups by table_width and shared_pages, not by the lengths
+ * (they are on the device): columns far behind the longest sequence do not change
+ * the result but cost time.
  * The workspace (16-byte aligned) holds fp32 partial results; nothing in it
  * survives a call.  Calls sharing one must be ordered on one stream.
  * Replaces: masking and attention of QwenAttention.forward

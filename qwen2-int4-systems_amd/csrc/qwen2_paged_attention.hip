@@ -168,8 +168,12 @@ template <class E> __device__ __forceinline__ uint32_t pass_word(uint32_t w, Pas
 
 // Rows of a segment from which wide tiles are taken.  Main kernel, us, narrow /
 // wide, 12/2 heads of 128: a prefix of 1 K by 96 rows 10.0 / 12.1, by 240 17.4 / 15.1,
-// of 4 K by 96 17.3 / 22.3, by 192 16.0 / 15.2, by 240 31.0 / 25.0; own segments of
-// 240 rows over up to 1 K 13.2 / 13.8.
+// of 4 K by 96 17.3 / 22.3, by 192 16.0 / 15.2, by 240 31.0 / 25.0.  The bound is the
+// prefix's.  Own segments go by it too, and lose by it between 128 and some 1000 rows
+// a sequence (each form with its own splits, us per call): one sequence of 144 rows
+// after 1 K positions 9.5 / 14.4, 240 11.8 / 15.5, 960 16.6 / 19.4; 2400 rows 15.0 / 17.7 after
+// none, 35.0 / 27.7 after 1.6 K; 12000 rows 68.7 / 54.0 after none, 372 / 163 after 6 K; six
+// sequences of 240 rows after 1 K 19.4 / 21.9, of 1200 after 700 36.5 / 30.9.
 constexpr int kWideFrom = 128;
 // Whether a sequence's own rows go by wide tiles, where the call has any.
 __device__ __forceinline__ bool wide_rows(const PagedAttnArgs& a, int tokens) {

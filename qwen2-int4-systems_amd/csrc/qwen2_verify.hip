@@ -18,7 +18,7 @@
 // may be a neighbour of weight), and never one without weight.
 //
 // Bound by the rows' read from memory (64 x 4 drafts of 151936 fp32: 77.8 MB in
-// 13.9 us of the sums, 17 the call), and for few sequences by its chain of round
+// 14.1 us of the sums, 17.5 the call), and for few sequences by its chain of round
 // trips (drafted id, its probabilities, the row) and the host's launches, some 4 us
 // each.  First forms, us: 64 x 4 147 with single entries per lane and both sums in
 // every workgroup, 19.6 with 16-byte loads and the pick by one wave.

@@ -82,8 +82,14 @@ def paged_attention_hip(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     the same pages (a prompt common to the batch).  They are taken from the first
     row and read once for all sequences; the result is the same.
 
-    Keys and values that a row does not see take no part, whatever they hold.  A
-    row without a position gives zeros.  Rows behind the last sequence are left
+    The call is cut into workgroups by the width of ``page_table``, for the lengths are
+    on the GPU: columns behind the longest sequence change no result, but a table much
+    wider than the sequences leaves too few workgroups to a shared prefix (32 rows over
+    4096 common positions, 12 and 2 heads of 128: 18.7 us with a table of their
+    length, 25.9 with one of 32768 positions, 68.1 with one of 131072).
+
+    Keys and values that a row does not see take no part, whatever they hold; an
+    infinity or NaN that it sees reaches it, however small the key's weight.  A row without a position gives zeros.  Rows behind the last sequence are left
     as they are in ``out``, and zeros in a new tensor.  Scores, softmax and sums are
     fp32, in a fixed order: the same inputs give the same bits.  Probabilities enter
     the value products as two terms of the tensors' type (16 bits or more of them), and
