@@ -89,11 +89,12 @@ def paged_attention_hip(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     length, 25.9 with one of 32768 positions, 68.1 with one of 131072).
 
     Keys and values that a row does not see take no part, whatever they hold; an
-    infinity or NaN that it sees reaches it, however small the key's weight.  A row without a position gives zeros.  Rows behind the last sequence are left
-    as they are in ``out``, and zeros in a new tensor.  Scores, softmax and sums are
-    fp32, in a fixed order: the same inputs give the same bits.  Probabilities enter
-    the value products as two terms of the tensors' type (16 bits or more of them), and
-    values are summed before the sum is divided: the keys' number times the values'
+    infinity or NaN that it sees reaches it, however small the key's weight.  A row
+    without a position gives zeros.  Rows behind the last sequence are left as they
+    are in ``out``, and zeros in a new tensor.  Scores, softmax and sums are fp32, in a
+    fixed order: the same inputs give the same bits.  Probabilities enter the value
+    products as two terms of the tensors' type (16 bits or more of them), and values
+    are summed before the sum is divided: the keys' number times the values'
     size has to stay in fp32.  The result is rounded once."""
     return _calls().paged_attention(q, k_pages, v_pages, page_table, cu_rows, lengths, shared_pages, scale, out)
 
@@ -114,5 +115,6 @@ def verify_drafts_hip(target_probs: torch.Tensor, draft_tokens: torch.Tensor, un
     ``max(p - q, 0)`` at row n (from p, if all stand): the least entry at which the
     running sum passes the uniform's share of the total, all in 64 bits.  Returns
     (tokens int64 [B, K + 1]: the n, the new one, then -1; accepted int32 [B]: n).
-    The new token is -1 where the weights' sum is zero, infinite or NaN."""
+    The new token is -1 where the weights' sum is zero, infinite or NaN, and an entry
+    of weight otherwise."""
     return _calls().verify_drafts(target_probs, draft_tokens, uniforms, draft_probs, draft_lengths)
