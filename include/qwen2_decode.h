@@ -252,7 +252,8 @@ int qwen2_paged_attention(const qwen2_paged_cache* cache, const qwen2_rows* q, c
  * weights are p_n.  uniforms fp32 [batch, drafts + 1], in [0, 1) (in the sum's
  * place a value outside counts as the nearest one inside, NaN as no choice).  A drafted id outside the
  * vocabulary does not stand, and its q is 0 there.  All in 64 bits, so that a
- * uniform next to a border falls where the definition says.
+ * uniform next to a border falls where the definition says, but for roundings of
+ * 2^-53 of the sums; what is drawn has weight.
  *   tokens[b, 0 .. n - 1] = the drafts that stand, tokens[b, n] the new token,
  *   -1 behind it; tokens[b, n] = -1 where the weights' sum is zero, infinite or
  *   NaN, or the uniform is NaN.  tokens int64 [batch, drafts + 1], accepted int32 [batch].

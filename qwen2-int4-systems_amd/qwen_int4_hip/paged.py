@@ -115,6 +115,6 @@ def verify_drafts_hip(target_probs: torch.Tensor, draft_tokens: torch.Tensor, un
     ``max(p - q, 0)`` at row n (from p, if all stand): the least entry at which the
     running sum passes the uniform's share of the total, all in 64 bits.  Returns
     (tokens int64 [B, K + 1]: the n, the new one, then -1; accepted int32 [B]: n).
-    The new token is -1 where the weights' sum is zero, infinite or NaN, and an entry
-    of weight otherwise."""
+    The new token is -1 where the weights' sum is zero, infinite or NaN or the uniform is
+    NaN, and an entry of weight otherwise."""
     return _calls().verify_drafts(target_probs, draft_tokens, uniforms, draft_probs, draft_lengths)
