@@ -268,6 +268,103 @@ int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target
                         int64_t batch, int64_t drafts, int64_t vocab, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* Causal attention over whole prompts of different lengths, packed:
+ *   out[r, h] = softmax_t(scale * q[r, h] . k[t, g]) v[t, g],   t = first row of r's sequence .. r,
+ * query head h reading key/value head g = h / (heads / kv_heads); sequence b's rows
+ * are cu_rows[b] .. cu_rows[b + 1] - 1 (a device array of batch + 1, not falling, from
+ * 0; what it holds is bounded there as the paged operators' is).  q, out [rows, heads,
+ * head_dim], k, v [rows, kv_heads, head_dim]: parts of a fused projection are read in
+ * place.  Scores, softmax and sums in fp32; a probability is rounded once to dtype
+ * before it meets its value, and it is the rounded ones that the sum adds up; the result
+ * is rounded once.  Rows behind the last sequence are left as they are, or zeroed with
+ * zero_rest.  Keys and values that a row does not see take no part, whatever they hold;
+ * an infinity or NaN among the values that it sees reaches it, however small the key's
+ * weight.  (Values are summed before the sum is divided: the keys' number times the
+ * values' size has to stay in fp32.)
+ * head_dim is 64 or 128; heads a multiple of kv_heads; dtype W4G64_DTYPE_BF16 or
+ * W4G64_DTYPE_F16; out must not overlap q, k and v.  No workspace.
+ * Replaces: masking and attention of QwenAttention.forward over a prompt
+ *           (src/qwen_int4/model.py:90-122) for packed sequences. */
+int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, const qwen2_rows* v, const qwen2_rows* out,
+                           const int32_t* cu_rows, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
+                           int64_t head_dim, int dtype, float scale, int zero_rest, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The pages of a paged cache: giving them out, forking sequences, compacting.
+ *
+ * page_users[p] (int32, num_pages) counts what names page p: entries of page
+ * tables, and whatever else keeps it (a prefix cached without a sequence).  A page is
+ * free where it is 0.  A table's entry names a page where it lies in [0, num_pages);
+ * -1 is written where it names none.  Index arrays are device arrays; answers go to
+ * arrays of their own, which must share no memory with what is read, so that a step
+ * that has to be given up leaves its state whole.  All is bounded on the device: no
+ * access leaves the buffers whatever lengths, entries and parents hold.  Whole
+ * numbers alone decide, in a fixed order.  batch (and children) at most 2^20, num_pages
+ * at most 2^24, batch * table_width below 2^31.  Workspaces are 4-byte aligned; nothing
+ * in one survives a call, and calls that share one must be ordered on one stream.
+ * ------------------------------------------------------------------------- */
+
+/* Every row of the table gets the pages that its length needs: entry c of row b,
+ * c < ceil(max(lengths[b], 0) / page_size), keeps the page that it names, or is given
+ * the lowest free page, row after row and column after column; all others are -1 and
+ * their pages given up (a length of 0 frees a sequence).  Pages given up in a call are
+ * free from the next one on.
+ *   new_table [batch, table_width], new_users[p] = page_users[p] - entries given up
+ *   + entries given, missing[b] = pages that row b still lacks (its table's width or
+ *   the pool too small; the last columns of the last rows go without first).
+ * page_table's rows lie table_stride apart.  page_size: a power of two in [16, 2^20].
+ * Replaces: the growth of the cache in QwenAttention.forward (model.py:83-90),
+ *           where keys and values lie in pages. */
+int64_t qwen2_paged_resize_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages);
+int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* page_users,
+                       int32_t* new_table, int32_t* new_users, int32_t* missing, int64_t batch, int64_t table_width,
+                       int64_t num_pages, int64_t page_size, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Pools of `layers` layers whose pages one table names: the key of page p, position
+ * t, head h of layer l is k + l * k_layer + p * k_page + h * k_head + t * k_position, v
+ * alike.  Strides in elements of 16 bits, multiples of 8; 16-byte aligned. */
+typedef struct qwen2_page_pool {
+    void* k;
+    void* v;
+    int64_t k_layer, k_page, k_head, k_position;
+    int64_t v_layer, v_page, v_head, v_position;
+    int64_t layers, num_pages, kv_heads;
+    int64_t page_size;             /* a power of two in [16, 2^20] */
+    int64_t head_dim;              /* a multiple of 8 up to 1024 */
+} qwen2_page_pool;
+
+/* The next batch of sequences, made of copies of this one's (samples of one prompt,
+ * beams, a batch in another order): row i of the answer is sequence parents[i], or
+ * none (length 0) where that is outside [0, batch).  A row holds the pages of its
+ * length; full pages are shared, and of a last page that is not full the sequence's first
+ * row (the lowest i) keeps the page itself, if page_users is 1 there, and every other one
+ * is given the lowest free page, row after row, with the filled positions' keys and
+ * values copied to it.  So no row's next position lies in a page that something else
+ * names.  Sequences that no row descends from give up their pages, all give up what lies
+ * behind their length; those are free from the next call on.
+ *   new_table [children, table_width], new_lengths [children],
+ *   new_users[p] = page_users[p] - entries of page_table + entries of new_table,
+ *   missing[i] = 1 where a copy found no free page (its entry is -1), else 0.
+ * Replaces: nothing of the reference's: its batches decode greedily
+ *           (src/qwen_int4/generation.py:10-115). */
+int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t num_pages);
+int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride, const int32_t* lengths,
+                     const int32_t* page_users, const int32_t* parents, int32_t* new_table, int32_t* new_lengths,
+                     int32_t* new_users, int32_t* missing, int64_t batch, int64_t children, int64_t table_width,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The n pages in use move to the pool's first n: those behind them, from the lowest
+ * on, to the free ones among the first n, from the lowest on.
+ *   moved_to[p] = where page p lies now, -1 for a free one; new_table [batch,
+ *   table_width]: page_table's entries renamed by it; new_users[moved_to[p]] =
+ *   page_users[p], 0 for all others.
+ * Pages behind the first n keep what they hold, and may be given back.
+ * Replaces: nothing of the reference's (one cache per batch). */
+int64_t qwen2_paged_compact_workspace_bytes(int64_t num_pages);
+int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride,
+                        const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* moved_to, int64_t batch,
+                        int64_t table_width, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* out[r, i] = silu(gate) * up in fp32, gate = gate_up[r, i], up = gate_up[r, I + i]
  * (bf16 inputs, the fused gate|up projection), silu(x) = x / (1 + exp(-x)).
  * Replaces: the SwiGLU product of QwenMLP.forward (src/qwen_int4/model.py:133-136). */

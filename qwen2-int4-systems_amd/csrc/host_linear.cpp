@@ -149,6 +149,11 @@ PyMethodDef kMethods[] = {
     {"paged_attention", (PyCFunction)(void (*)(void))host_paged_attention, METH_FASTCALL,
      "qwen_int4_hip.paged_attention_hip"},
     {"verify_drafts", (PyCFunction)(void (*)(void))host_verify_drafts, METH_FASTCALL, "qwen_int4_hip.verify_drafts_hip"},
+    {"packed_attention", (PyCFunction)(void (*)(void))host_packed_attention, METH_FASTCALL,
+     "qwen_int4_hip.packed_attention_hip"},
+    {"paged_resize", (PyCFunction)(void (*)(void))host_paged_resize, METH_FASTCALL, "qwen_int4_hip.paged_resize_hip"},
+    {"paged_fork", (PyCFunction)(void (*)(void))host_paged_fork, METH_FASTCALL, "qwen_int4_hip.paged_fork_hip"},
+    {"paged_compact", (PyCFunction)(void (*)(void))host_paged_compact, METH_FASTCALL, "qwen_int4_hip.paged_compact_hip"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

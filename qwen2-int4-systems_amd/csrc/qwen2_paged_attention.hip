@@ -73,22 +73,6 @@ constexpr int kBlock = 32;       // keys of a narrow block
 constexpr int kTileKeys = 64;    // keys of a wide tile
 constexpr int kMaxSplits = 64;
 
-// Division of numbers below 2^31 by a divisor that the host knows: the usual
-// multiplication by 2^(32 + shift) / divisor, less its leading one.
-struct Divisor {
-    uint32_t magic, shift;
-    __device__ __forceinline__ int operator()(int n) const {
-        return (int)((__umulhi((uint32_t)n, magic) + (uint32_t)n) >> shift);
-    }
-};
-Divisor divisor(int64_t d) {
-    Divisor r{0, 0};
-    d = d > 0 ? d : 1;
-    while ((int64_t(1) << r.shift) < d) ++r.shift;
-    r.magic = (uint32_t)((((uint64_t(1) << r.shift) - (uint64_t)d) << 32) / (uint64_t)d + (r.shift ? 1 : 0));
-    return r;
-}
-
 struct PagedAttnArgs {
     PagedView c;
     const uint16_t* q;
@@ -105,17 +89,6 @@ struct PagedAttnArgs {
     int zero_rest;
     Divisor by_group, by_heads, by_kv_heads, by_prefix_splits, by_own_splits;
 };
-
-// Exponents of probabilities.  bf16: they reach 2^kLazy before the sums are
-// rescaled, and stay at one or below with 2^-kLazy for the reference, so that values
-// add up as far as fp32 holds the keys' number times their size.  fp16 ends at
-// 2^-24 and at 2^16, and a key far below its row's maximum still counts if there are
-// many; with 2^11 for the reference the terms reach down to 2^-35 of it (and its
-// values times their number stay far inside fp32).
-template <class E> constexpr float kProbShift = -8.0f;
-template <> constexpr float kProbShift<F16> = 11.0f;
-template <class E> constexpr float kLazy = 8.0f;
-template <> constexpr float kLazy<F16> = 4.0f;
 
 // The kernel's arguments, read anew: what only the end of a kernel needs is not
 // held in scalar registers (and spilled) over its loop.
@@ -147,23 +120,6 @@ __device__ __forceinline__ int running_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
-}
-
-// Values that are not finite (an infinity or a NaN, met in the sums of a first
-// pass) must reach the rows that see their keys and no others, where a product
-// with a probability of zero would give NaN.  Three more passes tell: two that
-// count, for every row and dimension, the visible keys with +inf or NaN and with
-// -inf or NaN (ones in place of probabilities and of such values), and one over
-// the finite values alone.
-enum Pass { kOrdinary, kCountUp, kCountDown, kFinite };
-template <class E> __device__ __forceinline__ uint32_t pass_half(uint32_t h, Pass pass) {
-    const bool odd = (h & E::kExponent) == E::kExponent;
-    if (pass == kFinite) return odd ? 0u : h;
-    const bool nan = (h & 0x7FFFu) > E::kExponent, down = (h & 0x8000u) != 0;
-    return odd && (nan || down == (pass == kCountDown)) ? E::kOne : 0u;
-}
-template <class E> __device__ __forceinline__ uint32_t pass_word(uint32_t w, Pass pass) {
-    return pass_half<E>(w & 0xFFFFu, pass) | (pass_half<E>(w >> 16, pass) << 16);
 }
 
 // Rows of a segment from which wide tiles are taken.  Main kernel, us, narrow /
@@ -438,12 +394,6 @@ struct Attend {
         return fine;
     }
 };
-
-// What sums whose weight came out as zero still say: infinities and NaN, which the
-// formula's weight, small as it is, does not take away.
-__device__ __forceinline__ void add_odd(float& sum, float x) {
-    if (!(fabsf(x) < INFINITY)) sum += x;
-}
 
 // A value that a rare branch works with: keeps the compiler from running the
 // branch's instructions always.

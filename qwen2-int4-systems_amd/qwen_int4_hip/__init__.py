@@ -17,7 +17,9 @@ from .kernels import (
     unpack_canonical_signed_int4_hip,
 )
 from .linear import QuantLinear
+from .packed import packed_attention_hip
 from .paged import paged_append_hip, paged_attention_hip, verify_drafts_hip
+from .pages import paged_compact_hip, paged_fork_hip, paged_resize_hip
 from .quantization import (
     PackingFormat,
     dequantize_groupwise,
@@ -43,8 +45,12 @@ __all__ = [
     "torch_w4g64_linear",
     "linear_canonical_w4g64_hip",
     "linear_kernel_name",
+    "packed_attention_hip",
     "paged_append_hip",
     "paged_attention_hip",
+    "paged_compact_hip",
+    "paged_fork_hip",
+    "paged_resize_hip",
     "verify_drafts_hip",
     "unpack_canonical_signed_int4_hip",
     "validate_canonical_w4g64_inputs",

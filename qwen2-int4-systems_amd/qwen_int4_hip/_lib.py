@@ -73,6 +73,13 @@ SIGNATURES = {
     "qwen2_paged_attention": (_int, [_p] * 3 + [_i64] * 3 + [ctypes.c_float, _int, _p, _i64, _p]),
     "qwen2_verify_drafts_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "qwen2_verify_drafts": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int] + [_p] * 5 + [_i64] * 3 + [_p, _i64, _p]),
+    "qwen2_packed_attention": (_int, [_p] * 5 + [_i64] * 5 + [_int, ctypes.c_float, _int, _p]),
+    "qwen2_paged_resize_workspace_bytes": (_i64, [_i64] * 3),
+    "qwen2_paged_resize": (_int, [_p, _i64] + [_p] * 5 + [_i64] * 4 + [_p, _i64, _p]),
+    "qwen2_paged_fork_workspace_bytes": (_i64, [_i64] * 3),
+    "qwen2_paged_fork": (_int, [_p, _p, _i64] + [_p] * 7 + [_i64] * 3 + [_p, _i64, _p]),
+    "qwen2_paged_compact_workspace_bytes": (_i64, [_i64]),
+    "qwen2_paged_compact": (_int, [_p, _p, _i64] + [_p] * 4 + [_i64] * 2 + [_p, _i64, _p]),
     "qwen2_silu_mul": (_int, [_p, _p, _i64, _i64, _p]),
     "qwen2_lm_head_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "qwen2_lm_head": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p]),
@@ -94,6 +101,14 @@ class Rows(ctypes.Structure):
     """``qwen2_rows`` of include/qwen2_decode.h."""
 
     _fields_ = [("data", _p), ("row", _i64), ("head", _i64)]
+
+
+class PagePool(ctypes.Structure):
+    """``qwen2_page_pool`` of include/qwen2_decode.h."""
+
+    _fields_ = [("k", _p), ("v", _p)] + [(name, _i64) for name in (
+        "k_layer", "k_page", "k_head", "k_position", "v_layer", "v_page", "v_head", "v_position", "layers", "num_pages",
+        "kv_heads", "page_size", "head_dim")]
 
 
 _lock = threading.Lock()

@@ -1,0 +1,382 @@
+"""The sources of the packed prompt attention and of the page operators compiled for
+the CPU (tests/lanes, tests/lanes_more), every buffer in a mapping of its own with
+nothing mapped around it, as test_paged_lanes does for the paged kernels: an access
+outside a buffer ends the process, whatever lengths, entries, parents and row bounds
+hold."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import re
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+REPO = Path(__file__).resolve().parents[1]
+for _path in (REPO / "tests", REPO / "qwen2-int4-systems_amd"):
+    if str(_path) not in sys.path:
+        sys.path.insert(0, str(_path))
+
+from test_paged_lanes import CSRC, INTERNAL, LANES, Memory, _compiler  # noqa: E402
+
+MORE = Path(__file__).resolve().parent / "lanes_more"
+SOURCES = ("qwen2_packed_attention", "qwen2_pages")
+BF16, F16, I32 = torch.bfloat16, torch.float16, torch.int32
+WILD = [2 ** 31 - 1, -(2 ** 31)]
+
+
+@pytest.fixture(scope="module")
+def lanes_library(tmp_path_factory):
+    root = tmp_path_factory.mktemp("lanes_more")
+    for path in [*CSRC.glob("*.h"), *(CSRC / f"{name}.hip" for name in SOURCES)]:
+        text = path.read_text()
+        # (GPU registers and address spaces are the only words of the language that the CPU lacks)
+        text = re.sub(r'asm volatile\("" : "\+[sv]"\((\w)\)\);', r'asm volatile("" : "+r"(\1));', text)
+        text = re.sub(r"__attribute__\(\(address_space\(\d+\)\)\)", "", text)
+        (root / path.name).write_text(text)
+    (root / "w4g64_internal.h").write_text(INTERNAL)
+    flags = ["-std=c++17", "-O2", "-fPIC", "-ffp-contract=off", "-mf16c", "-mfma", "-w", f"-I{LANES}", f"-I{root}",
+             f"-I{REPO / 'include'}", f"-I{MORE}"]
+    compiler = _compiler()
+    more = ["-include", str(MORE / "more.h")]
+    jobs = [subprocess.Popen([compiler, *flags, *(more if source.suffix == ".hip" else []), "-x", "c++", "-c", str(source),
+                              "-o", str(root / f"{source.stem}.o")], stderr=subprocess.PIPE, text=True)
+            for source in [LANES / "lanes.cpp", *(root / f"{name}.hip" for name in SOURCES)]]
+    for job in jobs:
+        said = job.communicate()[1]
+        assert job.returncode == 0, said
+    library = root / "lanes.so"
+    subprocess.run([compiler, "-shared", *map(str, root.glob("*.o")), "-o", str(library)], check=True)
+    return library
+
+
+# ---------------------------------------------------------------------------
+# In the process of a check
+# ---------------------------------------------------------------------------
+
+class Kernels:
+    def __init__(self, library, side):
+        from qwen_int4_hip import _lib
+
+        self.abi, self.lib, memory = _lib, ctypes.CDLL(library), Memory(side)
+        # (what is empty lies in a mapping of one element)
+        self.memory = lambda t: memory(t) if t.numel() else memory(t.new_zeros(1))[:0].view(t.shape)
+        for name, (result, arguments) in _lib.SIGNATURES.items():
+            if name.startswith(("qwen2_packed", "qwen2_paged_resize", "qwen2_paged_fork", "qwen2_paged_compact")):
+                getattr(self.lib, name).restype, getattr(self.lib, name).argtypes = result, arguments
+        self.lib.lanes_error.restype = ctypes.c_char_p
+
+    def check(self, status):
+        assert status == 0, (status, self.lib.lanes_error())
+
+    def ints(self, values):
+        return self.memory(torch.tensor(values, dtype=torch.int64).to(I32))
+
+    def rows(self, t):
+        return ctypes.byref(self.abi.Rows(t.data_ptr(), t.stride(0), t.stride(1)))
+
+    def attention(self, q, k, v, cu, zero_rest=1, fill=0.0, scale=None):
+        out = self.memory(torch.full_like(q, fill))
+        self.check(self.lib.qwen2_packed_attention(
+            *map(self.rows, (q, k, v, out)), cu.data_ptr(), len(cu) - 1, *q.shape[:2], k.shape[1], q.shape[2],
+            {F16: 1, BF16: 2}[q.dtype], q.shape[2] ** -0.5 if scale is None else scale, zero_rest, None))
+        return out
+
+    def pool(self, k, v):
+        return ctypes.byref(self.abi.PagePool(k.data_ptr(), v.data_ptr(), *k.stride()[:4], *v.stride()[:4], k.shape[0],
+                                              k.shape[1], k.shape[2], k.shape[3], k.shape[4]))
+
+    def empty(self, *shape):
+        return self.memory(torch.full(shape, 77777, dtype=I32))
+
+    def resize(self, table, lengths, users, page):
+        (batch, width), pages = table.shape, len(users)
+        answers = self.empty(batch, width), self.empty(pages), self.empty(batch)
+        need = self.lib.qwen2_paged_resize_workspace_bytes(batch, width, pages)
+        workspace = self.memory(torch.full((need,), 0xA5, dtype=torch.uint8))
+        self.check(self.lib.qwen2_paged_resize(
+            table.data_ptr(), width, lengths.data_ptr(), users.data_ptr(), *(t.data_ptr() for t in answers), batch, width,
+            pages, page, workspace.data_ptr(), need, None))
+        return answers
+
+    def fork(self, k, v, table, lengths, users, parents):
+        (batch, width), pages, children = table.shape, len(users), len(parents)
+        answers = self.empty(children, width), self.empty(children), self.empty(pages), self.empty(children)
+        need = self.lib.qwen2_paged_fork_workspace_bytes(batch, children, pages)
+        workspace = self.memory(torch.full((need,), 0xA5, dtype=torch.uint8))
+        self.check(self.lib.qwen2_paged_fork(
+            self.pool(k, v), table.data_ptr(), width, lengths.data_ptr(), users.data_ptr(), parents.data_ptr(),
+            *(t.data_ptr() for t in answers), batch, children, width, workspace.data_ptr(), need, None))
+        return answers
+
+    def compact(self, k, v, table, users):
+        (batch, width), pages = table.shape, len(users)
+        answers = self.empty(batch, width), self.empty(pages), self.empty(pages)
+        need = self.lib.qwen2_paged_compact_workspace_bytes(pages)
+        workspace = self.memory(torch.full((need,), 0xA5, dtype=torch.uint8))
+        self.check(self.lib.qwen2_paged_compact(
+            self.pool(k, v), table.data_ptr(), width, users.data_ptr(), *(t.data_ptr() for t in answers), batch, width,
+            workspace.data_ptr(), need, None))
+        return answers
+
+
+def formula(q, k, v, cu, scale=None):
+    """Attended rows in 64 bits."""
+    out, group = torch.zeros(q.shape, dtype=torch.float64, device=q.device), q.shape[1] // k.shape[1]
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    cu = cu.tolist()
+    for first, end in zip(cu, cu[1:]):
+        for r in range(first, end):
+            for h in range(q.shape[1]):
+                w = torch.softmax(k[first:r + 1, h // group].double() @ q[r, h].double() * scale, 0)
+                out[r, h] = w @ v[first:r + 1, h // group].double()
+    return out
+
+
+def _packed(kernels, lengths, heads, kv_heads, dim, dtype=BF16, tail=0):
+    gen = torch.Generator().manual_seed(sum(lengths))
+    rows = sum(lengths) + tail
+    q, k, v = (kernels.memory(torch.randn(rows, n, dim, generator=gen).to(dtype)) for n in (heads, kv_heads, kv_heads))
+    return q, k, v, kernels.ints([sum(lengths[:i]) for i in range(len(lengths) + 1)])
+
+
+PROMPTS = [
+    ([1], 2, 1, 64, BF16),
+    ([3, 0, 40], 4, 2, 64, F16),
+    ([70], 6, 1, 128, BF16),
+    ([33, 1, 5], 3, 3, 128, F16),
+    ([140], 1, 1, 64, BF16),
+]
+
+
+def _prompts(kernels, name):
+    for lengths, heads, kv_heads, dim, dtype in PROMPTS:
+        q, k, v, cu = args = _packed(kernels, lengths, heads, kv_heads, dim, dtype, tail=2)
+        out = kernels.attention(*args)
+        # (a half step of the output and of each probability, values of a few units)
+        assert float((out.double() - formula(*args)).abs().amax()) < 4 * torch.finfo(dtype).eps, (lengths, dim)
+        assert not out[sum(lengths):].any()
+        kept = kernels.attention(*args, zero_rest=0, fill=7.0)
+        assert torch.equal(kept[:sum(lengths)], out[:sum(lengths)]) and bool((kept[sum(lengths):] == 7.0).all())
+        # an infinite value at the last row of the first sequence, whole
+        last = lengths[0] - 1
+        v[last] = -math.inf
+        out = kernels.attention(*args)
+        assert bool((out[last] == -math.inf).all())
+        out[last] = 0
+        assert bool(out.isfinite().all()), lengths
+
+
+def _bounds(kernels, name):
+    for lengths in ([2, 3], [40, 30], [150, 9]):
+        q, k, v, cu = args = list(_packed(kernels, lengths, 4, 2, 64, tail=3))
+        for values in [[0, 2, 2 ** 31 - 1], [0, *WILD], [-7, 90, 2], [3, 1, 0], [0, 0, -1], [0, 3, 3], [2 ** 31 - 1] * 3,
+                       [-(2 ** 31)] * 3]:
+            args[3] = kernels.ints(values)
+            end = min(max(values[-1], 0), q.shape[0])
+            for zero_rest in (0, 1):
+                out = kernels.attention(*args, zero_rest, fill=7.0)
+                assert bool((out[end:] == (0.0 if zero_rest else 7.0)).all()), values
+
+
+def resized(table, lengths, users, page):
+    """The operator's answers, entry by entry."""
+    table, users, missing = [list(r) for r in table], list(users), []
+    free = iter([p for p, n in enumerate(users) if n == 0])
+    for row, length in zip(table, lengths):
+        need = -(-max(length, 0) // page)
+        for c, e in enumerate(row):
+            named = 0 <= e < len(users)
+            if c >= need:
+                if named:
+                    users[e] -= 1
+                row[c] = -1
+            elif not named:
+                row[c] = next(free, -1)
+                if row[c] >= 0:
+                    users[row[c]] += 1
+        missing.append(need - sum(e >= 0 for e in row))
+    return table, users, missing
+
+
+def forked(table, lengths, users, parents, page):
+    """The operator's answers and its copies (source, target, positions)."""
+    pages, width = len(users), len(table[0]) if table else 0
+    free = iter([p for p, n in enumerate(users) if n == 0])
+    after, rows, sizes, missing, copies, taken = list(users), [], [], [], [], set()
+    for row in table:
+        for e in row:
+            if 0 <= e < pages:
+                after[e] -= 1
+    for parent in parents:
+        row, length, lacks = [-1] * width, 0, 0
+        if 0 <= parent < len(table):
+            length = max(lengths[parent], 0)
+            row = [e if c < -(-length // page) and 0 <= e < pages else -1 for c, e in enumerate(table[parent])]
+            at, rest = divmod(length, page)
+            if rest and at < width and row[at] >= 0:
+                if parent in taken or users[row[at]] != 1:
+                    source, row[at] = row[at], next(free, -1)
+                    if row[at] >= 0:
+                        copies.append((source, row[at], rest))
+                    lacks = int(row[at] < 0)
+                taken.add(parent)
+        for e in row:
+            if e >= 0:
+                after[e] += 1
+        rows.append(row)
+        sizes.append(length)
+        missing.append(lacks)
+    return rows, sizes, after, missing, copies
+
+
+def compacted(table, users):
+    """The operator's answers."""
+    live = [p for p, n in enumerate(users) if n]
+    holes = iter([p for p, n in enumerate(users) if not n and p < len(live)])
+    to = [-1] * len(users)
+    for p in live:
+        to[p] = p if p < len(live) else next(holes)
+    after = [0] * len(users)
+    for p in live:
+        after[to[p]] = users[p]
+    return [[to[e] if 0 <= e < len(users) else -1 for e in row] for row in table], after, to
+
+
+def state_of(seed, batch, width, pages, page, *, spare=0, wild=False):
+    """Tables, lengths and users of a pool in use, as lists; `spare` pages pinned without a
+    table; `wild`: entries and lengths that no program should have."""
+    gen = torch.Generator().manual_seed(seed)
+
+    def below(n, *shape):
+        return torch.randint(0, max(n, 1), shape, generator=gen).tolist()
+
+    order = torch.randperm(pages, generator=gen).tolist()
+    pinned, order = order[:spare], order[spare:]
+    lengths, table = below(width * page + 1, batch), []
+    for b in range(batch):
+        need = min(-(-lengths[b] // page), len(order))
+        row, order = order[:need], order[need:]
+        if b and need and b % 3 == 0:  # full pages shared with another sequence
+            other = [e for e in table[b - 1][:need - 1] if e >= 0]
+            order += row[:len(other)]
+            row = other + row[len(other):]
+        lengths[b] = min(lengths[b], need * page)
+        table.append(row + [-1] * (width - len(row)))
+    users = [0] * pages
+    for row in table:
+        for e in row:
+            if e >= 0:
+                users[e] += 1
+    for p in pinned:
+        users[p] += 1
+    if wild:
+        for b in range(0, batch, 2):
+            lengths[b] = (2 ** 31 - 1, -(2 ** 31), -1, width * page + 1)[b // 2 % 4]
+            table[b][below(width, 1)[0]] = (2 ** 31 - 1, -(2 ** 31), pages, -7)[b // 2 % 4]
+    return table, lengths, users
+
+
+POOLS = [  # batch, width, pages, page
+    (1, 1, 1, 16), (1, 5, 6, 16), (3, 4, 9, 16), (7, 9, 70, 32), (20, 70, 700, 16), (65, 3, 300, 64), (5, 300, 900, 16),
+    (3, 2, 257, 16), (2, 2, 512, 16),
+]
+
+
+def _lists(*tensors):
+    return tuple(t.tolist() for t in tensors)
+
+
+def _resize(kernels, name):
+    for seed, (batch, width, pages, page) in enumerate(POOLS):
+        for wild in (False, True):
+            table, lengths, users = state_of(seed, batch, width, pages, page, spare=min(pages // 7, 9), wild=wild)
+            gen = torch.Generator().manual_seed(seed)
+            for wanted in (lengths, [0] * batch, [width * page] * batch,
+                           torch.randint(0, width * page + 20, (batch,), generator=gen).tolist()):
+                got = kernels.resize(kernels.ints(table), kernels.ints(wanted), kernels.ints(users), page)
+                assert _lists(*got) == resized(table, wanted, users, page), (batch, width, pages, wild)
+
+
+def _pages_of(kernels, pages, page, seed, layers=2, heads=2, dim=8):
+    gen = torch.Generator().manual_seed(seed)
+    return [kernels.memory(torch.randn(layers, pages, heads, page, dim, generator=gen).to(BF16)) for _ in range(2)]
+
+
+def _fork(kernels, name):
+    for seed, (batch, width, pages, page) in enumerate(POOLS):
+        for wild in (False, True):
+            table, lengths, users = state_of(seed, batch, width, pages, page, spare=min(pages // 7, 9), wild=wild)
+            gen = torch.Generator().manual_seed(seed)
+            for parents in (list(range(batch)), [0] * 5, [], torch.randint(-1, batch + 1, (2 * batch,), generator=gen).tolist(),
+                            [*WILD, batch, -1]):
+                k, v = _pages_of(kernels, pages, page, seed)
+                want_k, want_v = k.clone(), v.clone()
+                got = kernels.fork(k, v, kernels.ints(table), kernels.ints(lengths), kernels.ints(users), kernels.ints(parents))
+                *want, copies = forked(table, lengths, users, parents, page)
+                assert _lists(*got) == tuple(want), (batch, width, pages, wild, parents)
+                for source, target, count in copies:
+                    for pool in (want_k, want_v):
+                        pool[:, target, :, :count] = pool[:, source, :, :count]
+                assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+def _compact(kernels, name):
+    for seed, (batch, width, pages, page) in enumerate(POOLS):
+        for wild in (False, True):
+            table, lengths, users = state_of(seed, batch, width, pages, page, spare=min(pages // 7, 9), wild=wild)
+            for counts in (users, [0] * pages, [1] * pages, [n if p % 3 else 0 for p, n in enumerate(users)],
+                           [int(p >= pages // 2) for p in range(pages)], [int(p < pages // 2) for p in range(pages)]):
+                k, v = _pages_of(kernels, pages, page, seed)
+                before_k, before_v = k.clone(), v.clone()
+                got = kernels.compact(k, v, kernels.ints(table), kernels.ints(counts))
+                want = compacted(table, counts)
+                assert _lists(*got) == want, (batch, width, pages, wild)
+                for p, to in enumerate(want[2]):
+                    if to >= 0:
+                        assert torch.equal(k[:, to], before_k[:, p]) and torch.equal(v[:, to], before_v[:, p])
+
+
+def _many(kernels, name):
+    """Pools and tables past what one workgroup goes through."""
+    pages, batch, width, page = 65536 + 300, 40, 900, 16
+    table, lengths, users = state_of(5, batch, width, pages, page, spare=500)
+    wanted = [width * page - 7 if b % 3 else 0 for b in range(batch)]
+    got = kernels.resize(kernels.ints(table), kernels.ints(wanted), kernels.ints(users), page)
+    assert _lists(*got) == resized(table, wanted, users, page)
+    k, v = _pages_of(kernels, pages, page, 0, layers=1, heads=1)
+    want_k = k.clone()
+    parents = [b // 2 for b in range(batch)] + [-1]
+    got = kernels.fork(k, v, kernels.ints(table), kernels.ints(lengths), kernels.ints(users), kernels.ints(parents))
+    *want, copies = forked(table, lengths, users, parents, page)
+    assert _lists(*got) == tuple(want)
+    for source, target, count in copies:
+        want_k[:, target, :, :count] = want_k[:, source, :, :count]
+    assert torch.equal(k, want_k)
+    got = kernels.compact(k, v, kernels.ints(table), kernels.ints(users))
+    want = compacted(table, users)
+    assert _lists(*got) == want
+    to = torch.tensor(want[2])
+    moved = (to >= 0).nonzero().view(-1)
+    assert torch.equal(k[:, to[moved]], want_k[:, moved])
+
+
+CHECKS = {"prompts": _prompts, "bounds": _bounds, "resize": _resize, "fork": _fork, "compact": _compact, "many": _many}
+
+
+@pytest.mark.parametrize("side", ["end", "start"])
+@pytest.mark.parametrize("name", CHECKS)
+def test_every_access_lies_in_its_buffer(lanes_library, name, side):
+    result = subprocess.run([sys.executable, __file__, str(lanes_library), name, side], capture_output=True, text=True,
+                            timeout=300)
+    assert result.returncode == 0 and result.stdout.endswith("done\n"), (result.returncode, result.stderr[-2000:])
+
+
+if __name__ == "__main__":
+    torch.set_num_threads(1)
+    CHECKS[sys.argv[2]](Kernels(sys.argv[1], sys.argv[3]), sys.argv[2])
+    print("done")
