@@ -4,12 +4,9 @@
 // Work.  A "row" here is a (token, query head) pair of one sequence and key/value
 // head: row m is token m / group, head m % group of the group, so that heads that
 // share keys fill a tile together and a short prompt's tile is not mostly empty.  A
-// workgroup of four waves takes a tile of rows in one of two forms:
-//   narrow    32 rows.  The waves take different 32-key blocks, straight from memory
-//             into operands, and meet in LDS at the end.
-//   wide      128 rows, 32 of each wave.  The workgroup goes through 64-key tiles in
-//             LDS, the next one on its way (direct loads) while the waves work on this
-//             one.
+// workgroup goes through tiles of keys in LDS, the next one on its way (direct loads)
+// while the waves work on this one.  kSplit waves share 32 rows, each with kBlocks * 32
+// of every tile's keys, and meet in LDS at the end.
 //
 // One pass over the keys: running maximum, sum and value sums per row.  MFMA layout
 // (v_mfma_f32_32x32x16; lane l = 32 h + j supplies row j of A and column j of B with K
@@ -17,11 +14,9 @@
 //   scores  A = 32 keys, B = 32 query rows: a lane holds 16 of its row's 32 scores,
 //           the lane 32 further the others;
 //   values  the lane's scores as they are, eight by eight, are its K slots of B: slot e
-//           is key 8 (e / 4) + 4 h + e % 4 of 16.  A = the values transposed, in that
-//           order of the keys.  Narrow: lane (j, h) loads kVd = D / 32 dimensions from
-//           kVd j of its keys and pairs keys up by v_perm; dimension kVd j + dd is row
-//           j of the dd-th product.  Wide: LDS reads that transpose; dimension 32 dd +
-//           j is row j of the dd-th product.
+//           is key 8 (e / 4) + 4 h + e % 4 of 16.  A = the values in that order of the
+//           keys, by LDS reads that transpose; dimension 32 dd + j is row j of the dd-th
+//           product.
 //
 // A probability is rounded once, to the tensors' type, before it meets its value: half
 // a step of it (2^-9 of its size in bf16) for each key, which the result's own rounding
@@ -42,10 +37,7 @@
 namespace w4g64 {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kNarrowRows = 32;
-constexpr int kBlock = 32;     // keys of a narrow block
+constexpr int kWaveRows = 32;
 
 struct PackedArgs {
     const uint16_t* q;
@@ -69,9 +61,15 @@ template <> __device__ __forceinline__ float16v mfma32<F16>(const u32x4& a, cons
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// c plus both halves of a word.
-template <class E> __device__ __forceinline__ float add_pair(uint32_t w, float c) {
-    return c + (E::lo(w) + E::hi(w));
+// c plus both halves of a word, in one instruction.  It cuts sums off where an addition
+// rounds them (2^-24 of the sum at a time, always down), so it adds up a tile's
+// probabilities, not all of them.
+template <class E> __device__ __forceinline__ float add_pair(uint32_t w, float c);
+template <> __device__ __forceinline__ float add_pair<Bf16>(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, w), __builtin_bit_cast(bf16x2v, 0x3F803F80u), c, false);
+}
+template <> __device__ __forceinline__ float add_pair<F16>(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w), __builtin_bit_cast(half2v, 0x3C003C00u), c, false);
 }
 
 // Over the two lanes j, j + 32.
@@ -99,32 +97,49 @@ struct Piece {
     int kvh;
 };
 
-// Tile `index`: the tiles of every sequence counted up, 64 sequences at a time; those
-// of a sequence from its end, where the most keys are.
+// Piece `index`.  Up to 64 sequences: tiles in the order of their keys' number, the most
+// first (a tile's place in its sequence goes by it), so that no workgroup begins a long
+// one when the others are done.  More: sequence after sequence, the last tile first.
 template <int kRows>
 __device__ __forceinline__ bool find_piece(const PackedArgs& a, int index, int lane, Piece& s) {
     int before = 0;
-    const int all = rows_end(a.cu_rows, a.batch, a.rows);
     for (int base = 0; base < a.batch; base += 64) {
         const int b = base + lane;
-        PackedRows r{0, 0};
-        if (b < a.batch) r = packed_rows(a.cu_rows, b, all);
-        const int count = (r.end - r.begin) * a.group;
+        // (both bounds and the last one on their way together)
+        const PackedRows r = packed_rows(a.cu_rows, min(b, a.batch - 1), rows_end(a.cu_rows, a.batch, a.rows));
+        const int count = b < a.batch ? (r.end - r.begin) * a.group : 0;
         const int tiles = (count + kRows - 1) / kRows;
-        int upto = tiles;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int other = __shfl_up(upto, d);
-            if (lane >= d) upto += other;
+        int at = 0;
+        if (a.batch == 1) {
+            s.tile = __builtin_amdgcn_readfirstlane(tiles) - 1 - index;
+            if (s.tile < 0) return false;
+        } else {
+            const int upto = running_sum(tiles), sum = __builtin_amdgcn_readlane(upto, 63);
+            if (index >= before + sum) {
+                before += sum;
+                continue;
+            }
+            if (a.batch > 64) {
+                at = __ffsll((unsigned long long)__ballot(before + upto > index)) - 1;
+                s.tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - index;
+            } else {
+                // more than `index` tiles have the place `low` in their sequence or a later one,
+                // `fewer`, and not more, the place `high`
+                int low = 0, high = (a.rows * a.group + kRows - 1) / kRows, fewer = 0;
+                while (high - low > 1) {
+                    const int mid = (low + high) / 2;
+                    const int from = __builtin_amdgcn_readlane(running_sum(max(tiles - mid, 0)), 63);
+                    if (from > index) low = mid;
+                    else high = mid, fewer = from;
+                }
+                s.tile = low;
+                const int has = tiles > low, rank = running_sum(has);  // (of all lanes)
+                at = __ffsll((unsigned long long)__ballot(has && rank == index - fewer + 1)) - 1;
+            }
         }
-        const uint64_t past = __ballot(before + upto > index);
-        if (past) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            s.begin = __builtin_amdgcn_readlane(r.begin, at);
-            s.count = __builtin_amdgcn_readlane(count, at);
-            s.tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - index;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        s.begin = __builtin_amdgcn_readlane(r.begin, at);
+        s.count = __builtin_amdgcn_readlane(count, at);
+        return true;
     }
     return false;
 }
@@ -145,20 +160,19 @@ __device__ __forceinline__ Row row_at(const PackedArgs& a, const Piece& s, int m
 }
 
 template <int kSteps>
-__device__ __forceinline__ void load_queries(const PackedArgs& a, const Piece& s, const Row& row, int h, u32x4 (&qf)[kSteps]) {
+__device__ __forceinline__ void load_queries(const PackedArgs& a, const Piece& s, const Row& row, int h,
+                                             u32x4 (&qf)[kSteps]) {
     const uint16_t* from = a.q + (int64_t)(s.begin + row.token) * a.q_row + row.head * a.q_head + 8 * h;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = *(const u32x4*)(from + 16 * i) ^ a.query_sign;
 }
 
-// One lane's part of 32 rows: the running softmax and value sums of row j; o[dd][i]
-// is row 8 (i / 4) + 4 h + i % 4 of the dd-th product.
+// One lane's part of 32 rows: the running softmax and value sums of row j; o[dd][i] is
+// dimension 32 dd + 8 (i / 4) + 4 h + i % 4.
 template <class E, int D>
 struct Attend {
-    static constexpr int kVd = D / 32;
-    static constexpr int kVw = kVd / 2;
+    static constexpr int kVd = D / 32;     // products of the values
     static constexpr int kSteps = D / 16;  // K steps of a score
-    typedef uint32_t vword __attribute__((ext_vector_type(kVw)));
 
     float m_run, l_run;
     float16v o[kVd];
@@ -186,27 +200,16 @@ struct Attend {
         }
     }
 
-    // Eight scores as probabilities.
+    // Eight scores as probabilities, which `sum` adds up.
     template <int kCount>
-    __device__ __forceinline__ u32x4 soften(const float (&s)[kCount], int from, float scale2) {
+    __device__ __forceinline__ u32x4 soften(const float (&s)[kCount], int from, float scale2, float& sum) const {
         const float ref = kProbShift<E> - m_run;
         u32x4 p;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             p[e] = E::pack(__builtin_amdgcn_exp2f(fmaf(s[from + 2 * e], scale2, ref)),
                            __builtin_amdgcn_exp2f(fmaf(s[from + 2 * e + 1], scale2, ref)));
-            l_run = add_pair<E>(p[e], l_run);
-        }
-        return p;
-    }
-
-    // Eight keys' ones where the row sees them (keys 8 (e / 4) + 4 h + e % 4 from t0).
-    static __device__ __forceinline__ u32x4 show(int limit, int t0, int h) {
-        u32x4 p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = t0 + 8 * (e / 2) + 4 * h + 2 * (e % 2);
-            p[e] = (t <= limit ? E::kOne : 0u) | (t + 1 <= limit ? E::kOne << 16 : 0u);
+            sum = add_pair<E>(p[e], sum);
         }
         return p;
     }
@@ -231,163 +234,60 @@ struct Attend {
             }
     }
     __device__ __forceinline__ bool finite() const {
-        bool fine = true;
+        float nothing[4] = {};  // 0 times what is not finite is NaN
 #pragma unroll
         for (int dd = 0; dd < kVd; ++dd)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) fine = fine && fabsf(o[dd][i]) < INFINITY;
-        return fine;
+            for (int i = 0; i < 16; ++i) nothing[i % 4] = fmaf(o[dd][i], 0.0f, nothing[i % 4]);
+        return (nothing[0] + nothing[1]) + (nothing[2] + nothing[3]) == 0.0f;
     }
 };
 
-// ---- narrow ----
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v* lds_halves_t;
 
-template <class E, int D>
-struct KeyBlock {
-    u32x4 k[D / 16];                    // key j, dimensions 16 i + 8 h ..
-    typename Attend<E, D>::vword v[16];  // value of key 16 (e / 8) + 8 (e % 8 / 4) + 4 h + e % 4, dimensions kVd j ..
-};
-
-// The lane's value sums of each wave in LDS: 64 lanes of 16 D / 32 floats, so that a
-// wave's piece is one tile of 64 keys.
-template <int D> constexpr int kMeetBytes = 64 * 16 * (D / 32) * (int)sizeof(float);
-
-template <class E, int D>
-__device__ __forceinline__ void narrow(const PackedArgs& a, const Piece& s, int tile, int lane, int wave,
-                                       unsigned char* meet0, unsigned char* meet1, unsigned char* meet2,
-                                       unsigned char* meet3, float2v (*stats)[64]) {
-    typedef Attend<E, D> A;
-    const int j = lane & 31;
-    const int h = lane >> 5;
-    const int m0 = tile * kNarrowRows;
-    const int least = a.by_group(m0), most = a.by_group(min(m0 + kNarrowRows, s.count) - 1);
-    const int blocks = most / kBlock + 1;
-    const uint16_t* kc = a.k + s.begin * a.k_row + s.kvh * a.k_head + 8 * h;
-    const uint16_t* vc = a.v + s.begin * a.v_row + s.kvh * a.v_head + A::kVd * j;
-    // (a key past the last visible one: that one again, of no weight)
-    auto load = [&](KeyBlock<E, D>& b, int block) {
-        const int t0 = block * kBlock;
-        const uint16_t* kp = kc + (int64_t)min(t0 + j, most) * a.k_row;
-#pragma unroll
-        for (int i = 0; i < A::kSteps; ++i) b.k[i] = *(const u32x4*)(kp + 16 * i);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            b.v[e] = *(const typename A::vword*)(vc + (int64_t)min(t0 + 8 * (e / 4) + 4 * h + e % 4, most) * a.v_row);
-    };
-    KeyBlock<E, D> b;
-    if (wave < blocks) load(b, wave);
-    const Row row = row_at(a, s, m0 + j);
-    u32x4 qf[A::kSteps];
-    load_queries(a, s, row, h, qf);
-    A state;
-    auto compute = [&](const KeyBlock<E, D>& b, int block, auto ordinary, Pass pass) {
-        const int t0 = block * kBlock;
-        float16v acc = {};
-#pragma unroll
-        for (int i = 0; i < A::kSteps; ++i) acc = mfma32<E>(b.k[i], qf[i], acc);
-        float x[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = acc[e];
-        if (t0 + kBlock - 1 > least) {
-            const int sees = rare(row.token - t0 - 4 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (8 * (e / 4) + e % 4 > sees) x[e] = -INFINITY;
-        }
-        if (ordinary || pass == kFinite) state.settle(x, a.scale2);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const u32x4 p = ordinary || pass == kFinite ? state.soften(x, 8 * half, a.scale2)
-                                                        : A::show(row.token, t0 + 16 * half, h);
-#pragma unroll
-            for (int dd = 0; dd < A::kVd; ++dd) {
-                const uint32_t select = (dd & 1) ? 0x07060302u : 0x05040100u;  // high or low halves
-                u32x4 vt;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    vt[e] = __builtin_amdgcn_perm(b.v[8 * half + 2 * e + 1][dd / 2], b.v[8 * half + 2 * e][dd / 2], select);
-                    if constexpr (!ordinary) vt[e] = pass_word<E>(vt[e], pass);
-                }
-                state.o[dd] = mfma32<E>(vt, p, state.o[dd]);
-            }
-        }
-    };
-    state.start();
-    for (int block = wave; block < blocks;) {
-        compute(b, block, std::true_type{}, kOrdinary);
-        block += kWaves;
-        if (block < blocks) load(b, block);
-    }
-    if (!__all(state.finite())) {  // (the wave's)
-        uint64_t up = 0, down = 0;
-#pragma unroll 1
-        for (int pass = kCountUp; pass <= kFinite; ++pass) {
-            state.start();
-#pragma unroll 1
-            for (int block = wave; block < blocks; block += kWaves) {
-                load(b, block);
-                compute(b, block, std::false_type{}, (Pass)pass);
-            }
-            if (pass == kCountUp) up = state.marks();
-            if (pass == kCountDown) down = state.marks();
-        }
-        state.mark(up, down);
-    }
-
-    // ---- the waves' results meet in LDS: register i of product dd at (16 dd + i) * 64 + lane ----
-    auto meet = [&](int w) { return (float*)(w < 2 ? (w ? meet1 : meet0) : (w > 2 ? meet3 : meet2)); };
-#pragma unroll
-    for (int dd = 0; dd < A::kVd; ++dd)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) meet(wave)[(16 * dd + i) * 64 + lane] = state.o[dd][i];
-    // (-inf: no key in the wave's blocks)
-    stats[wave][lane] = float2v{row.token >= wave * kBlock ? state.m_run : -INFINITY, halves_sum(state.l_run)};
-    __syncthreads();
-    // this wave's registers 4 wave .. 4 wave + 3 of every product
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][lane][0]);
-    float l = 0.0f, sum[4][A::kVd] = {};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        const float2v st = stats[w][lane];
-        const float f = __builtin_amdgcn_exp2f(st[0] - top);
-        const float* from = meet(w) + (4 * wave) * 64 + lane;
-        if (f != 0.0f) {
-            l = fmaf(st[1], f, l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int dd = 0; dd < A::kVd; ++dd) sum[i][dd] = fmaf(from[(16 * dd + i) * 64], f, sum[i][dd]);
-        } else if (st[0] > -INFINITY) {
-            // keys of no weight beside the others': nothing, unless a value that the row
-            // sees was not finite
-            if (st[1] != st[1]) l = st[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int dd = 0; dd < A::kVd; ++dd) add_odd(sum[i][dd], from[(16 * dd + i) * 64]);
-        }
-    }
-    if (!row.live) return;
-    const float inv = 1.0f / l;
-    uint16_t* to = a.out + (int64_t)(s.begin + row.token) * a.out_row + row.head * a.out_head + A::kVd * (8 * wave + 4 * h);
-    uint32_t word[2 * A::kVd];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int dd = 0; dd < A::kVd; dd += 2) word[(A::kVd * i + dd) / 2] = E::pack(sum[i][dd] * inv, sum[i][dd + 1] * inv);
-#pragma unroll
-    for (int i = 0; i < 2 * A::kVd; i += 4) *(u32x4*)(to + 2 * i) = u32x4{word[i], word[i + 1], word[i + 2], word[i + 3]};
+// All of this wave's loads into LDS have landed, then all waves'.
+__device__ __forceinline__ void all_landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x7 << 4);  // vmcnt 0, lgkmcnt 0 (gfx9 encoding)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-template <class E, int D>
-__global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(PackedArgs a) {
-    __shared__ __attribute__((aligned(16))) unsigned char k0[kMeetBytes<D>], v0[kMeetBytes<D>], k1[kMeetBytes<D>], v1[kMeetBytes<D>];
+// A tile's keys or values in LDS: kKeys rows of D elements in 16-byte pieces, piece c of
+// row r in slot c ^ turn(r).  Keys are read one piece of 32 rows at a time: the turns of
+// 16 rows are all different (D 64: where the rows' banks are the same).  Values are read
+// transposed (ds_read_b64_tr_b16: of 16 lanes, lane t brings elements 4 (t % 4) .. of
+// row t / 4 and gets element t of the four rows), 64 bytes of 4 rows by 32 lanes: there
+// the groups of four pieces are turned.
+template <int D, int kWaves, int kKeys>
+struct Tile {
+    static constexpr int kPieces = D / 8;
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kBytes = kKeys * kRowBytes;
+    static constexpr int kWaveKeys = kKeys / kWaves;       // that a wave brings
+    static constexpr int kRowsPerLoad = 64 / kPieces;      // rows that a wave's 16-byte load fills
+    static constexpr int kLoads = kWaveKeys / kRowsPerLoad;
+    static __device__ __forceinline__ int key_turn(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+    static __device__ __forceinline__ int value_turn(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+};
+
+template <class E, int D, int kWaves, int kSplit, int kBlocks>
+__device__ __forceinline__ void attend_piece(const PackedArgs& a) {
+    constexpr int kThreads = 64 * kWaves, kKeys = 32 * kBlocks * kSplit;
+    typedef Attend<E, D> A;
+    typedef Tile<D, kWaves, kKeys> T;
+    constexpr int kRows = kWaves / kSplit * kWaveRows;  // of the workgroup
+    // (objects of their own: a read of one does not wait for loads into another)
+    __shared__ __attribute__((aligned(16))) unsigned char k0[T::kBytes], v0[T::kBytes], k1[T::kBytes], v1[T::kBytes];
     __shared__ float2v stats[kWaves][64];
+    __shared__ int odd;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j = lane & 31;
+    const int h = lane >> 5;
     if (a.zero_rest) {
         for (int64_t r = rest_row(a.cu_rows, a.batch, a.rows, blockIdx.x); r < a.rows; r += gridDim.x)
             for (int d = 8 * tid; d < a.heads * D; d += 8 * kThreads)
@@ -396,14 +296,260 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(PackedArg
     Piece s;
     const int index = a.by_kv_heads((int)blockIdx.x);
     s.kvh = (int)blockIdx.x - index * a.kv_heads;
-    if (!find_piece<kNarrowRows>(a, index, lane, s)) return;
-    narrow<E, D>(a, s, s.tile, lane, wave, k0, v0, k1, v1, stats);
+    if (!find_piece<kRows>(a, index, lane, s)) return;
+
+    const int part = wave % kSplit;  // of every tile's keys
+    const int m0 = s.tile * kRows + kWaveRows * (wave / kSplit);
+    // the wave's rows, then the workgroup's (rows past the last one are that one again)
+    const int least = a.by_group(min(m0, s.count - 1)), most = a.by_group(min(m0 + kWaveRows, s.count) - 1);
+    const int all_most = a.by_group(min((s.tile + 1) * kRows, s.count) - 1);
+    const int tiles = all_most / kKeys + 1;
+
+    const uint16_t* kc = a.k + s.begin * a.k_row + s.kvh * a.k_head;
+    const uint16_t* vc = a.v + s.begin * a.v_row + s.kvh * a.v_head;
+    int k_at[T::kLoads], v_at[T::kLoads];
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+        const int r = T::kRowsPerLoad * i + lane / T::kPieces;
+        k_at[i] = 2 * r * (int)a.k_row + 16 * ((lane % T::kPieces) ^ T::key_turn(r));
+        v_at[i] = 2 * r * (int)a.v_row + 16 * ((lane % T::kPieces) ^ T::value_turn(r));
+    }
+    auto stage = [&](int tile, unsigned char* keys, unsigned char* values) {
+        // (a key past the last visible one: that one again, of no weight)
+        const int t = min(tile * kKeys + T::kWaveKeys * wave, all_most), past = min(all_most - t, T::kWaveKeys - 1);
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kc + t * a.k_row), 0,
+                                                                            (past * (int)a.k_row + D) * 2, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vc + t * a.v_row), 0,
+                                                                            (past * (int)a.v_row + D) * 2, 0x00020000);
+        unsigned char* k_to = keys + T::kWaveKeys * wave * T::kRowBytes;
+        unsigned char* v_to = values + T::kWaveKeys * wave * T::kRowBytes;
+        if (past < T::kWaveKeys - 1) {
+#pragma unroll
+            for (int i = 0; i < T::kLoads; ++i) {
+                const int r = rare(T::kRowsPerLoad * i + lane / T::kPieces), back = max(r - past, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr_t)(k_to + 1024 * i), 16,
+                                                         k_at[i] - 2 * back * (int)a.k_row, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(v_to + 1024 * i), 16,
+                                                         v_at[i] - 2 * back * (int)a.v_row, 0, 0, 0);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr_t)(k_to + 1024 * i), 16, k_at[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(v_to + 1024 * i), 16, v_at[i], 0, 0, 0);
+    };
+    if (tid == 0) odd = 0;
+    stage(0, k0, v0);
+    const Row row = row_at(a, s, m0 + j);
+    u32x4 qf[A::kSteps];
+    load_queries(a, s, row, h, qf);
+    A state;
+    auto compute = [&](int tile, const unsigned char* keys, const unsigned char* values, auto ordinary, Pass pass) {
+        const int t0 = tile * kKeys + 32 * kBlocks * part;
+        if (t0 > most) return;  // (the wave's)
+        float x[16 * kBlocks];
+        u32x4 kf[2][A::kSteps];
+        auto load_keys = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < A::kSteps; ++i)
+                kf[b & 1][i] = *(const u32x4*)(keys + (32 * (kBlocks * part + b) + j) * T::kRowBytes + 16 * ((2 * i + h) ^ T::key_turn(j)));
+        };
+        load_keys(0);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            if (b + 1 < kBlocks) load_keys(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            float16v acc = {};
+#pragma unroll
+            for (int i = 0; i < A::kSteps; ++i) acc = mfma32<E>(kf[b & 1][i], qf[i], acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[16 * b + e] = acc[e];
+        }
+        if (t0 + 32 * kBlocks - 1 > least) {
+            const int sees = rare(row.token - t0 - 4 * h);
+#pragma unroll
+            for (int e = 0; e < 16 * kBlocks; ++e)
+                if (8 * (e / 4) + e % 4 > sees) x[e] = -INFINITY;
+        }
+        if (ordinary || pass == kFinite) state.settle(x, a.scale2);
+        const int t = lane & 15, block = (lane >> 4) & 1;
+        float sum = 0.0f;
+        u32x4 vt[2];
+        auto load_values = [&](int half, int dd) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int r = 32 * kBlocks * part + 16 * half + 8 * g + 4 * h + t / 4;
+                const unsigned char* at = values + r * T::kRowBytes +
+                                          16 * ((4 * dd + 2 * block + (t & 3) / 2) ^ T::value_turn(t / 4)) + 8 * (t & 1);
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_halves_t)at));
+                vt[dd & 1][2 * g] = w[0], vt[dd & 1][2 * g + 1] = w[1];
+            }
+        };
+        load_values(0, 0);
+#pragma unroll
+        for (int half = 0; half < 2 * kBlocks; ++half) {
+            u32x4 p;
+            if (ordinary || pass == kFinite) {
+                p = state.soften(x, 8 * half, a.scale2, sum);
+            } else {  // ones where the row sees the keys
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = t0 + 16 * half + 8 * (e / 2) + 4 * h + 2 * (e % 2);
+                    p[e] = (key <= row.token ? E::kOne : 0u) | (key + 1 <= row.token ? E::kOne << 16 : 0u);
+                }
+            }
+#pragma unroll
+            for (int dd = 0; dd < A::kVd; ++dd) {
+                if (dd + 1 < A::kVd) load_values(half, dd + 1);
+                else if (half + 1 < 2 * kBlocks) load_values(half + 1, 0);
+                __builtin_amdgcn_sched_barrier(0x7);
+                u32x4 w = vt[dd & 1];
+                if constexpr (!ordinary)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = pass_word<E>(w[e], pass);
+                state.o[dd] = mfma32<E>(w, p, state.o[dd]);
+            }
+        }
+        state.l_run += sum;
+    };
+    // The next tile on its way while this one is worked on: its buffer was read before
+    // the barrier.
+    state.start();
+    for (int tile = 0;;) {
+        all_landed();
+        if (tile + 1 < tiles) stage(tile + 1, k1, v1);
+        compute(tile, k0, v0, std::true_type{}, kOrdinary);
+        if (++tile >= tiles) break;
+        all_landed();
+        if (tile + 1 < tiles) stage(tile + 1, k0, v0);
+        compute(tile, k1, v1, std::true_type{}, kOrdinary);
+        if (++tile >= tiles) break;
+    }
+    const bool fine = __all(state.finite());
+    if (!fine && lane == 0) odd = 1;
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(odd)) {
+        uint64_t up = 0, down = 0;
+#pragma unroll 1
+        for (int pass = kCountUp; pass <= kFinite; ++pass) {
+            state.start();
+#pragma unroll 1
+            for (int tile = 0; tile < tiles; ++tile) {
+                stage(tile, k0, v0);
+                all_landed();
+                compute(tile, k0, v0, std::false_type{}, (Pass)pass);
+                __syncthreads();
+            }
+            if (pass == kCountUp) up = state.marks();
+            if (pass == kCountDown) down = state.marks();
+        }
+        state.mark(up, down);
+    }
+
+    const float l_wave = halves_sum(state.l_run);
+    uint16_t* to = a.out + (int64_t)(s.begin + row.token) * a.out_row + row.head * a.out_head + 4 * h;
+    if constexpr (kSplit == 1) {
+        if (!row.live) return;
+        const float inv = 1.0f / l_wave;
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; ++dd)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(u32x2*)(to + 32 * dd + 2 * i) = u32x2{E::pack(state.o[dd][i] * inv, state.o[dd][i + 1] * inv),
+                                                        E::pack(state.o[dd][i + 2] * inv, state.o[dd][i + 3] * inv)};
+    } else {
+        // The waves' sums meet in LDS, register i of product dd at (16 dd + i) * 64 + lane,
+        // and each wave adds up 16 / kSplit registers of every product.
+        constexpr int kSums = 64 * 16 * A::kVd, kEach = kWaves / 4;  // floats of a wave; waves in a buffer
+        static_assert(T::kBytes >= kEach * kSums * (int)sizeof(float), "the waves' sums fit the tiles");
+        auto sums_of = [&](int w) {
+            const int at = w / kEach;
+            return (float*)(at < 2 ? (at ? v0 : k0) : (at > 2 ? v1 : k1)) + w % kEach * kSums;
+        };
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; ++dd)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums_of(wave)[(16 * dd + i) * 64 + lane] = state.o[dd][i];
+        // (-inf: no key in the wave's parts)
+        stats[wave][lane] = float2v{row.token >= 32 * kBlocks * part ? state.m_run : -INFINITY, l_wave};
+        __syncthreads();
+        if (!row.live) return;
+        const int first = wave - part;
+        float top = -INFINITY, l = 0.0f, sum[16 / kSplit][A::kVd] = {};
+#pragma unroll
+        for (int w = 0; w < kSplit; ++w) top = fmaxf(top, stats[first + w][lane][0]);
+#pragma unroll
+        for (int w = 0; w < kSplit; ++w) {
+            const float2v st = stats[first + w][lane];
+            const float f = __builtin_amdgcn_exp2f(st[0] - top);
+            const float* from = sums_of(first + w) + 16 / kSplit * part * 64 + lane;
+            if (f != 0.0f) {
+                l = fmaf(st[1], f, l);
+#pragma unroll
+                for (int i = 0; i < 16 / kSplit; ++i)
+#pragma unroll
+                    for (int dd = 0; dd < A::kVd; ++dd) sum[i][dd] = fmaf(from[(16 * dd + i) * 64], f, sum[i][dd]);
+            } else if (st[0] > -INFINITY) {
+                // keys of no weight beside the others': nothing, unless a value that the row
+                // sees was not finite
+                if (st[1] != st[1]) l = st[1];
+#pragma unroll
+                for (int i = 0; i < 16 / kSplit; ++i)
+#pragma unroll
+                    for (int dd = 0; dd < A::kVd; ++dd) add_odd(sum[i][dd], from[(16 * dd + i) * 64]);
+            }
+        }
+        const float inv = 1.0f / l;
+        to += 2 * (16 / kSplit) * part;
+#pragma unroll
+        for (int dd = 0; dd < A::kVd; ++dd)
+#pragma unroll
+            for (int i = 0; i < 16 / kSplit; i += 4)
+                *(u32x2*)(to + 32 * dd + 2 * i) = u32x2{E::pack(sum[i][dd] * inv, sum[i + 1][dd] * inv),
+                                                        E::pack(sum[i + 2][dd] * inv, sum[i + 3][dd] * inv)};
+    }
 }
 
+// (waves per SIMD: two with 256 registers each, where LDS holds as much)
+template <class E, int D, int kWaves, int kSplit, int kBlocks>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 && kSplit == 4 && D == 128 ? 1 : 2) void packed_attention_kernel(PackedArgs a) {
+    attend_piece<E, D, kWaves, kSplit, kBlocks>(a);
+}
+
+// The forms of a call's workgroups.
+enum Form { kLong, kSplit2, kSplit4, kSplit4Tall };
+int tile_rows(Form f) { return f == kLong ? 128 : f == kSplit4 ? 32 : 64; }
+
 template <class E, int D>
-hipError_t launch_packed_attention(const PackedArgs& a, int64_t workgroups, hipStream_t stream) {
-    hipLaunchKernelGGL((packed_attention_kernel<E, D>), dim3((unsigned)workgroups), dim3(kThreads), 0, stream, a);
+hipError_t launch_packed_attention(const PackedArgs& a, Form form, int64_t workgroups, hipStream_t stream) {
+    const dim3 grid((unsigned)workgroups);
+    if (form == kLong) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 1, 2>), grid, dim3(256), 0, stream, a);
+    else if (form == kSplit2) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 2, 1>), grid, dim3(256), 0, stream, a);
+    else if (form == kSplit4) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 4, 1>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((packed_attention_kernel<E, D, 8, 4, 1>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
+}
+
+// The form of a call.  A workgroup's time is that of its keys one tile after the other,
+// so long as the chip holds all of them at once; then what counts is the products'
+// rate, which the fewest waves per row give.  us a call, kLong / kSplit2 / kSplit4 /
+// kSplit4Tall, 12/2 heads of 128: one prompt of 37 tokens 7.1 / 6.7 / 7.3 / 8.5, 512 15.3 /
+// 12.3 / 11.1 / 12.1, 1024 24.6 / 19.2 / 19.6 / 17.3, 2048 43 / 34 / 50 / 30, 3000 62 / 50 /
+// 94 / 58, 16384 795 / 908 / 1991 / 1019; four of 512 16.9 / 15.5 / 28 / 21, eight 20 / 24 / 54 / 33;
+// 16/16 heads of 64: eight of 60 5.2 / 5.6 / 5.8 / 6.6, one of 1000 17.1 / 13.4 / 10.6 / 11.8, two 18.4 /
+// 15.4 / 19.5 / 18.1.  The lengths are on the GPU: it goes by the sequences' average.
+Form form_of(int64_t rows, int64_t sequences, int64_t group, int64_t kv_heads, int64_t head_dim) {
+    const int64_t usual = rows / sequences, few = head_dim == 128 ? 288 : 576, half = head_dim == 128 ? 256 : 512;
+    auto tiles = [&](int64_t size) { return sequences * ((usual * group + size - 1) / size) * kv_heads; };
+    if (usual * group <= 64) return kLong;  // (a smaller tile would hold the same rows)
+    if (usual > 128) {
+        if (tiles(32) <= few) return kSplit4;
+        if (tiles(64) <= 256 || (tiles(64) <= half * 3 / 2 && usual >= 1024)) return kSplit4Tall;
+    }
+    return tiles(64) <= 512 || (tiles(64) <= 800 && usual >= 2048) ? kSplit2 : kLong;
 }
 
 }  // namespace
@@ -430,11 +576,14 @@ extern "C" int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, 
         if (!r || !r->data || ((uintptr_t)r->data & 15) || r->row % 8 || r->head % 8)
             return set_error(W4G64_STATUS_INVALID_VALUE,
                              "q, k, v and out must be non-null, 16-byte aligned, with strides that are multiples of 8 elements");
+    if (k->row > (1 << 24) || v->row > (1 << 24) || k->row < 0 || v->row < 0)
+        return set_error(W4G64_STATUS_UNSUPPORTED, "k and v rows must be at most 2^24 elements apart");
     if (!cu_rows || ((uintptr_t)cu_rows & 3))
         return set_error(W4G64_STATUS_INVALID_VALUE, "cu_rows must be a non-null, 4-byte aligned device pointer");
     const int64_t group = heads / kv_heads, sequences = batch < rows ? batch : rows;
+    const Form form = form_of(rows, sequences, group, kv_heads, head_dim);
     // (every sequence may end inside a tile; the empty ones have none)
-    const int64_t workgroups = (rows * group / kNarrowRows + sequences) * kv_heads;
+    const int64_t workgroups = (rows * group / tile_rows(form) + sequences) * kv_heads;
     if (rows * heads > 0x7FF00000 || workgroups > 0xFFFFFF)
         return set_error(W4G64_STATUS_UNSUPPORTED, "packed_attention call is too large: %lld workgroups", (long long)workgroups);
     PackedArgs a{};
@@ -453,9 +602,9 @@ extern "C" int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, 
     const hipStream_t s = (hipStream_t)stream;
     hipError_t err;
     if (dtype == W4G64_DTYPE_BF16)
-        err = head_dim == 128 ? launch_packed_attention<Bf16, 128>(a, workgroups, s) : launch_packed_attention<Bf16, 64>(a, workgroups, s);
+        err = head_dim == 128 ? launch_packed_attention<Bf16, 128>(a, form, workgroups, s) : launch_packed_attention<Bf16, 64>(a, form, workgroups, s);
     else
-        err = head_dim == 128 ? launch_packed_attention<F16, 128>(a, workgroups, s) : launch_packed_attention<F16, 64>(a, workgroups, s);
+        err = head_dim == 128 ? launch_packed_attention<F16, 128>(a, form, workgroups, s) : launch_packed_attention<F16, 64>(a, form, workgroups, s);
     if (err != hipSuccess) return set_error(W4G64_STATUS_HIP_ERROR, "packed_attention launch failed: %s", hipGetErrorString(err));
     return clear_error();
 }

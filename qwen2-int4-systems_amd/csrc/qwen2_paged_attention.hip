@@ -110,18 +110,6 @@ __device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
     return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p + i);
 }
 
-// Running sums over the wave (shifts within rows of 16 lanes, then their last lanes
-// passed on).
-__device__ __forceinline__ int running_sum(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 // Rows of a segment from which wide tiles are taken.  Main kernel, us, narrow /
 // wide, 12/2 heads of 128: a prefix of 1 K by 96 rows 10.0 / 12.1, by 240 17.4 / 15.1,
 // of 4 K by 96 17.3 / 22.3, by 192 16.0 / 15.2, by 240 31.0 / 25.0.  The bound is the

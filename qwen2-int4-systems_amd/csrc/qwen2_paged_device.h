@@ -53,6 +53,18 @@ inline Divisor divisor(int64_t d) {
     return r;
 }
 
+// Running sums over the wave (shifts within rows of 16 lanes, then their last lanes
+// passed on).
+__device__ __forceinline__ int running_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 // Exponents of probabilities.  bf16: they reach 2^kLazy before the sums are
 // rescaled, and stay at one or below with 2^-kLazy for the reference, so that values
 // add up as far as fp32 holds the keys' number times their size.  fp16 ends at

@@ -30,10 +30,18 @@ float16 product32(const V& a, const V& b, const float16& c) {
     return d;
 }
 
+// c plus both halves (the second operand is ones).
+template <bool kBf16>
+float pair_sum(uint32_t w, float c) {
+    return c + (as_float((uint16_t)w, kBf16) + as_float((uint16_t)(w >> 16), kBf16));
+}
+
 }  // namespace lanes
 
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) lanes::product32<true>(a, b, c)
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) lanes::product32<false>(a, b, c)
+#define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) lanes::pair_sum<true>(__builtin_bit_cast(uint32_t, a), c)
+#define __builtin_amdgcn_fdot2(a, b, c, clamp) lanes::pair_sum<false>(__builtin_bit_cast(uint32_t, a), c)
 #define __hip_atomic_load(p, order, scope) (*(p))
 
 // (one lane runs at a time)

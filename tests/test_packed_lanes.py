@@ -150,6 +150,7 @@ PROMPTS = [
     ([70], 6, 1, 128, BF16),
     ([33, 1, 5], 3, 3, 128, F16),
     ([140], 1, 1, 64, BF16),
+    ([260], 40, 40, 128, F16),
 ]
 
 
