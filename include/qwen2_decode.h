@@ -300,7 +300,8 @@ int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, const qwen2
  * that has to be given up leaves its state whole.  All is bounded on the device: no
  * access leaves the buffers whatever lengths, entries and parents hold.  Whole
  * numbers alone decide, in a fixed order.  batch (and children) at most 2^20, num_pages
- * at most 2^24, batch * table_width below 2^31.  Workspaces are 4-byte aligned; nothing
+ * at most 2^24, batch * table_width below 2^31.  Workspaces (none where few pages and
+ * entries are, then NULL may be given) are 4-byte aligned; nothing
  * in one survives a call, and calls that share one must be ordered on one stream.
  * ------------------------------------------------------------------------- */
 
@@ -347,7 +348,7 @@ typedef struct qwen2_page_pool {
  *   missing[i] = 1 where a copy found no free page (its entry is -1), else 0.
  * Replaces: nothing of the reference's: its batches decode greedily
  *           (src/qwen_int4/generation.py:10-115). */
-int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t num_pages);
+int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t table_width, int64_t num_pages);
 int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride, const int32_t* lengths,
                      const int32_t* page_users, const int32_t* parents, int32_t* new_table, int32_t* new_lengths,
                      int32_t* new_users, int32_t* missing, int64_t batch, int64_t children, int64_t table_width,
@@ -360,7 +361,7 @@ int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int
  *   page_users[p], 0 for all others.
  * Pages behind the first n keep what they hold, and may be given back.
  * Replaces: nothing of the reference's (one cache per batch). */
-int64_t qwen2_paged_compact_workspace_bytes(int64_t num_pages);
+int64_t qwen2_paged_compact_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages);
 int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride,
                         const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* moved_to, int64_t batch,
                         int64_t table_width, void* workspace, int64_t workspace_bytes, void* stream);

@@ -98,11 +98,12 @@ PyObject* host_paged_resize(PyObject*, PyObject* const* args, Py_ssize_t count) 
         const at::Tensor new_table = at::empty({batch, width}, options), new_users = at::empty({pages}, options);
         const at::Tensor missing = at::empty({batch}, options);
         const int64_t need = qwen2_paged_resize_workspace_bytes(batch, width, pages);
-        const at::Tensor workspace = at::empty({need}, options.dtype(at::kByte));
+        at::Tensor workspace;
+        if (need) workspace = at::empty({need}, options.dtype(at::kByte));
         const hipStream_t stream = current_stream(device);
         released([&] {
             return qwen2_paged_resize(data(t), t.stride(0), data(n), data(u), data(new_table), data(new_users),
-                                      data(missing), batch, width, pages, page_size, workspace.mutable_data_ptr(), need,
+                                      data(missing), batch, width, pages, page_size, need ? workspace.mutable_data_ptr() : nullptr, need,
                                       stream);
         });
         return tuple_of({new_table, new_users, missing});
@@ -133,13 +134,14 @@ PyObject* host_paged_fork(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const auto options = users.options().requires_grad(false);
         const at::Tensor new_table = at::empty({children, width}, options), new_lengths = at::empty({children}, options);
         const at::Tensor new_users = at::empty({pools.c.num_pages}, options), missing = at::empty({children}, options);
-        const int64_t need = qwen2_paged_fork_workspace_bytes(batch, children, pools.c.num_pages);
-        const at::Tensor workspace = at::empty({need}, options.dtype(at::kByte));
+        const int64_t need = qwen2_paged_fork_workspace_bytes(batch, children, width, pools.c.num_pages);
+        at::Tensor workspace;
+        if (need) workspace = at::empty({need}, options.dtype(at::kByte));
         const hipStream_t stream = current_stream(device);
         released([&] {
             return qwen2_paged_fork(&pools.c, data(t), t.stride(0), data(n), data(u), data(p), data(new_table),
                                     data(new_lengths), data(new_users), data(missing), batch, children, width,
-                                    workspace.mutable_data_ptr(), need, stream);
+                                    need ? workspace.mutable_data_ptr() : nullptr, need, stream);
         });
         written(pools.k), written(pools.v);
         return tuple_of({new_table, new_lengths, new_users, missing});
@@ -167,12 +169,13 @@ PyObject* host_paged_compact(PyObject*, PyObject* const* args, Py_ssize_t count)
         const auto options = users.options().requires_grad(false);
         const at::Tensor new_table = at::empty({batch, width}, options);
         const at::Tensor new_users = at::empty({pages}, options), moved_to = at::empty({pages}, options);
-        const int64_t need = qwen2_paged_compact_workspace_bytes(pages);
-        const at::Tensor workspace = at::empty({need}, options.dtype(at::kByte));
+        const int64_t need = qwen2_paged_compact_workspace_bytes(batch, width, pages);
+        at::Tensor workspace;
+        if (need) workspace = at::empty({need}, options.dtype(at::kByte));
         const hipStream_t stream = current_stream(device);
         released([&] {
             return qwen2_paged_compact(&pools.c, data(t), t.stride(0), data(u), data(new_table), data(new_users),
-                                       data(moved_to), batch, width, workspace.mutable_data_ptr(), need, stream);
+                                       data(moved_to), batch, width, need ? workspace.mutable_data_ptr() : nullptr, need, stream);
         });
         written(pools.k), written(pools.v);
         return tuple_of({new_table, new_users, moved_to});

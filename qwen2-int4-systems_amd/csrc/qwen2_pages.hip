@@ -5,8 +5,9 @@
 // page that moves goes to the i-th hole.  Pages are counted in groups of kGroup (four
 // ballots of a wave, whose bits are ranks within the group), the groups' counts are
 // summed up, and a second look at the pages writes the lists.
-//   few     one workgroup does all of that, with barriers between: up to kFewPages
-//           pages and kFewEntries table entries;
+//   few     one launch, every workgroup of which works all of that out for itself, in
+//           LDS, and then does its part of what follows: a launch costs a caller 3.6 us,
+//           more than the 64 KB that each workgroup reads at most;
 //   many    one launch counts, one lists, one applies.
 // Answers go to new arrays: what a kernel reads nobody changes, and the only atomics
 // are whole numbers' sums, so that the same inputs give the same answer.  Keys and
@@ -18,8 +19,8 @@
 #include <hip/hip_runtime.h>
 
 #include "qwen2_decode.h"
+#include "qwen2_paged_device.h"
 #include "qwen2_pages.h"
-#include "w4g64_device.h"
 #include "w4g64_internal.h"
 
 namespace w4g64 {
@@ -28,47 +29,48 @@ namespace {
 constexpr int kThreads = 1024;           // of the workgroups that count, list and plan
 constexpr int kWaves = kThreads / 64;
 constexpr int kGroup = 256;              // pages counted together, by one wave
-constexpr int kFewPages = 1 << 16;
+constexpr int kFewPages = 1 << 14;
+constexpr int kFewRows = kThreads;       // (one of a thread)
 constexpr int kFewEntries = 1 << 15;
 constexpr int64_t kMostPages = 1 << 24;  // (a workgroup sums up the counts before its own)
-constexpr int kCopyThreads = 256;
+constexpr int kMostCopyThreads = 256;
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-__device__ __forceinline__ int bits_before(uint64_t mask, int lane) {
-    return __popcll(mask & ((uint64_t(1) << lane) - 1));
+// Bits of the lanes before this one.
+__device__ __forceinline__ int bits_before(uint64_t mask) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// Sum over the workgroup's threads, the same in all of them; `meet` holds kWaves words.
-__device__ __forceinline__ int block_sum(int v, int* meet) {
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+
+// Sum over the waves before this one of what each brings (the same in its lanes), and
+// over all; `meet` holds kWaves words.
+__device__ __forceinline__ int waves_before(int v, int* meet, int& all) {
     const int lane = lane_id(), wave = wave_id();
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
     __syncthreads();
     if (lane == 0) meet[wave] = v;
     __syncthreads();
-    int sum = 0;
-    for (int w = 0; w < kWaves; ++w) sum += meet[w];
-    return sum;
+    const int upto = running_sum(lane < kWaves ? meet[lane] : 0);
+    all = last_lane(upto);
+    return __builtin_amdgcn_readlane(upto, wave) - v;
 }
-
-// Sum over the threads before this one, and over all.
+// Over the threads before this one, and over all.
 __device__ __forceinline__ int block_before(int v, int* meet, int& all) {
-    const int lane = lane_id(), wave = wave_id();
-    int upto = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int other = __shfl_up(upto, d);
-        if (lane >= d) upto += other;
-    }
-    __syncthreads();
-    if (lane == 63) meet[wave] = upto;
-    __syncthreads();
-    int before = 0;
-    all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        before += w < wave ? meet[w] : 0;
-        all += meet[w];
-    }
-    return before + upto - v;
+    const int upto = running_sum(v);
+    return waves_before(last_lane(upto), meet, all) + upto - v;
+}
+// How many threads before this one say yes, and how many do.
+__device__ __forceinline__ int block_rank(bool yes, int* meet, int& all) {
+    const uint64_t mask = __ballot(yes);
+    const int before = waves_before(__popcll(mask), meet, all);
+    return before + bits_before(mask);
+}
+// Sum over the workgroup's threads, the same in all of them.
+__device__ __forceinline__ int block_sum(int v, int* meet) {
+    int all;
+    waves_before(last_lane(running_sum(v)), meet, all);
+    return all;
 }
 
 // One group of pages as a wave sees it: bit l of free[i] is page 256 g + 64 i + l.
@@ -88,6 +90,16 @@ struct Group {
     __device__ __forceinline__ int count() const {
         return __popcll(free[0]) + __popcll(free[1]) + __popcll(free[2]) + __popcll(free[3]);
     }
+    // Free ones among the first n.
+    __device__ __forceinline__ int count_below(int n) const {
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int edge = n - 64 * i;  // bits below it count
+            sum += __popcll(free[i] & (edge <= 0 ? 0 : edge >= 64 ? ~uint64_t(0) : (uint64_t(1) << edge) - 1));
+        }
+        return sum;
+    }
 };
 
 // Writes the free pages of rank below `limit` to list[rank]; `before`: the rank of the
@@ -96,26 +108,9 @@ __device__ __forceinline__ void list_group(const Group& g, int group, int before
     const int lane = lane_id();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int rank = before + bits_before(g.free[i], lane);
+        const int rank = before + bits_before(g.free[i]);
         if (g.there[i] == 0 && rank < limit) list[rank] = group * kGroup + 64 * i + lane;
         before += __popcll(g.free[i]);
-    }
-}
-
-// The free pages' counts of all groups (one workgroup): counts[g]; with `copy`, the
-// users besides.
-__device__ __forceinline__ void count_groups(const int32_t* users, int pages, int32_t* counts, int32_t* copy) {
-    const int groups = (pages + kGroup - 1) / kGroup;
-    for (int g = wave_id(); g < groups; g += kWaves) {
-        Group x;
-        x.load(users, pages, g);
-        if (lane_id() == 0) counts[g] = x.count();
-        if (copy)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int p = g * kGroup + 64 * i + lane_id();
-                if (p < pages) copy[p] = x.there[i];
-            }
     }
 }
 
@@ -146,6 +141,54 @@ __device__ __forceinline__ void list_free(const int32_t* users, int pages, const
     }
 }
 
+// Few: all groups of the pool, wave w's being w, w + kWaves, ...
+struct Groups {
+    static constexpr int kMost = kFewPages / kGroup, kEach = kMost / kWaves;
+    static_assert(kMost == 64, "one of a lane");
+    Group x[kEach];
+    int upto;  // lane g: free pages up to and with group g
+    __device__ __forceinline__ void load(const int32_t* users, int pages) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            x[k] = Group{{}, {-1, -1, -1, -1}};
+            if (group(k) * kGroup < pages) x[k].load(users, pages, group(k));
+        }
+    }
+    // (before a barrier; sum() after it)
+    __device__ __forceinline__ void tell(int* counts) const {
+        const int wave = wave_id();
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (lane_id() == 0) counts[wave + kWaves * k] = x[k].count();
+    }
+    __device__ __forceinline__ int sum(const int* counts) {
+        upto = running_sum(counts[lane_id()]);
+        return last_lane(upto);
+    }
+    __device__ __forceinline__ int group(int k) const { return wave_id() + kWaves * k; }
+    __device__ __forceinline__ int before(int k) const { return __builtin_amdgcn_readlane(upto, group(k)) - x[k].count(); }
+    // The free pages of ranks below `limit`, in order.
+    __device__ __forceinline__ void list(int limit, int32_t* to) const {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int first = before(k);
+            if (x[k].count() && first < limit) list_group(x[k], group(k), first, limit, to);
+        }
+    }
+};
+
+// The sum of counts[first .. at), fewer than 64 (one wave).
+__device__ __forceinline__ int sum_between(const int32_t* counts, int first, int at) {
+    return last_lane(running_sum(first + lane_id() < at ? counts[first + lane_id()] : 0));
+}
+
+// The sum of counts[0 .. n) by one workgroup.
+__device__ __forceinline__ int sum_of(const int32_t* counts, int n, int* meet) {
+    int sum = 0;
+    for (int i = (int)threadIdx.x; i < n; i += kThreads) sum += counts[i];
+    return block_sum(sum, meet);
+}
+
 // ---- resize ----
 
 struct ResizeArgs {
@@ -155,97 +198,182 @@ struct ResizeArgs {
     int32_t* new_table;
     int32_t* new_users;
     int32_t* missing;
-    int32_t* want;    // [batch]: pages that a row gets
+    // many:
+    int32_t* want;    // [batch]: pages that a row lacks
+    int32_t* start;   // [batch]: those of the rows before it
+    int32_t* free;    // [1]: free pages, no more than the list holds
     int32_t* counts;  // [groups]
     int32_t* list;    // free pages in order
     int64_t table_stride;
     int batch, width, pages, page_shift, most;  // most: entries of the list
-    int row_blocks;
+    int list_blocks;
+    Divisor by_width;
 };
 
-// A row's entries in [0, upto) that name no page (one wave).
-__device__ __forceinline__ int lacking(const ResizeArgs& a, int b) {
-    const int upto = pages_wanted(a.lengths[b], a.page_shift, a.width);
-    const int32_t* row = a.table + b * a.table_stride;
-    int lacks = 0;
-    for (int c0 = 0; c0 < upto; c0 += 256) {
-        int entry[4];
+// 256 columns of a row from c0, below `end`, by one wave.
+struct Columns {
+    int entry[4];
+    __device__ __forceinline__ void load(const int32_t* row, int c0, int end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 64 * i + lane_id();
-            entry[i] = c < upto ? row[c] : 0;
-        }
+        for (int i = 0; i < 4; ++i) entry[i] = c0 + 64 * i + lane_id() < end ? row[c0 + 64 * i + lane_id()] : -1;
+    }
+};
+
+// Entries in [from, upto) that name no page (one wave); `x`: the first 256 columns.
+__device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, int from, int upto, Columns x) {
+    int lacks = 0;
+    for (int c0 = from; c0 < upto; c0 += 256) {
+        if (c0 > from) x.load(row, c0, upto);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            lacks += __popcll(__ballot(c0 + 64 * i + lane_id() < upto && !names_page(entry[i], a.pages)));
+            lacks += __popcll(__ballot(c0 + 64 * i + lane_id() < upto && !names_page(x.entry[i], a.pages)));
     }
     return lacks;
 }
 
-// A row's new entries (one wave): free pages from rank `start` on where one is wanted
-// (there are `free` in the list), pages given up where none is.
-__device__ __forceinline__ void resize_row(const ResizeArgs& a, int b, int64_t start, int free) {
-    const int need = pages_needed(a.lengths[b], a.page_shift);
-    const int upto = min(need, a.width);
+// The new entries of columns [from, end) of row b (one wave): free pages from rank
+// `start` on where one is wanted (list[rank], below `free`), none behind the length.
+// With kCount the users of pages given and given up change besides.  `x`: the first of
+// the columns.  Returns how many entries name a page.
+template <bool kCount>
+__device__ __forceinline__ int resize_columns(const ResizeArgs& a, int b, int from, int end, int64_t start, int free,
+                                              const int32_t* list, int length, Columns x) {
+    const int upto = pages_wanted(length, a.page_shift, a.width);
     const int32_t* row = a.table + b * a.table_stride;
     int32_t* to = a.new_table + (int64_t)b * a.width;
     int held = 0;
-    for (int c0 = 0; c0 < a.width; c0 += 256) {
-        int entry[4];
+    for (int c0 = from; c0 < end; c0 += 256) {
+        if (c0 > from) x.load(row, c0, end);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = c0 + 64 * i + lane_id();
-            entry[i] = c < a.width ? row[c] : -1;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 64 * i + lane_id();
-            const bool named = names_page(entry[i], a.pages);
-            const uint64_t wants = __ballot(c < upto && !named);
-            int e = named ? entry[i] : -1;
+            const bool named = names_page(x.entry[i], a.pages);
+            const uint64_t wants = __ballot(c < min(upto, end) && !named);
+            int e = named ? x.entry[i] : -1;
             if (c >= upto) {
-                if (named) atomicAdd(a.new_users + e, -1);
+                if (kCount && named) atomicAdd(a.new_users + e, -1);
                 e = -1;
-            } else if (!named) {
-                const int64_t rank = start + bits_before(wants, lane_id());
+            } else if (!named && c < end) {
+                const int64_t rank = start + bits_before(wants);
                 if (rank < free) {
-                    e = a.list[rank];
-                    atomicAdd(a.new_users + e, 1);
+                    e = list[rank];
+                    if (kCount) atomicAdd(a.new_users + e, 1);
                 }
             }
-            if (c < a.width) to[c] = e;
+            if (c < end) to[c] = e;
             held += __popcll(__ballot(e >= 0));
             start += __popcll(wants);
         }
     }
-    if (lane_id() == 0) a.missing[b] = need - held;
+    return held;
 }
 
-__global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
-    __shared__ int meet[kWaves];
-    count_groups(a.users, a.pages, a.counts, a.new_users);
-    for (int b = wave_id(); b < a.batch; b += kWaves) {
-        const int lacks = lacking(a, b);
-        if (lane_id() == 0) a.want[b] = lacks;
+// Few: use(b, c, length of b, entry) for all entries of the table, by one workgroup;
+// eight loads of a thread on their way at once.
+template <class Args, class F>
+__device__ __forceinline__ void each_entry(const Args& a, int entries, F use) {
+    constexpr int kAtOnce = 8;
+    for (int base = 0; base < entries; base += kAtOnce * kThreads) {
+        int row[kAtOnce], column[kAtOnce], length[kAtOnce], entry[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int at = base + i * kThreads + (int)threadIdx.x;
+            row[i] = a.by_width(min(at, entries - 1)), column[i] = at - row[i] * a.width;
+            length[i] = a.lengths[row[i]];
+            entry[i] = column[i] < a.width ? a.table[row[i] * a.table_stride + column[i]] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (column[i] < a.width) use(row[i], column[i], length[i], entry[i]);
     }
-    __syncthreads();
-    const int wanted = sum_groups(a.want, a.batch, meet);
-    const int free = min(sum_groups(a.counts, (a.pages + kGroup - 1) / kGroup, meet), wanted);
-    list_free(a.users, a.pages, a.counts, free, a.list);
-    __syncthreads();
-    for (int b = wave_id(); b < a.batch; b += kWaves) resize_row(a, b, a.want[b], free);
 }
 
-// Many: rows' wants by the first workgroups, pages' counts by the others.
-__global__ __launch_bounds__(kThreads) void resize_count_kernel(ResizeArgs a) {
-    if ((int)blockIdx.x < a.row_blocks) {
-        const int b = (int)blockIdx.x * kWaves + wave_id();
-        if (b >= a.batch) return;
-        const int lacks = lacking(a, b);
-        if (lane_id() == 0) a.want[b] = lacks;
+// Few.  The first workgroup writes the users, every other one kWaves rows.
+__global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
+    __shared__ int counts[Groups::kMost], want[kFewRows], given[kFewPages];
+    const int tid = (int)threadIdx.x;
+    // what this wave's row needs at the end is on its way from the start
+    const int b = ((int)blockIdx.x - 1) * kWaves + wave_id();
+    const bool mine = blockIdx.x > 0 && b < a.batch;
+    Columns row{};
+    if (mine) row.load(a.table + b * a.table_stride, 0, a.width);
+    const int row_length = mine ? a.lengths[b] : 0;
+    Groups free_pages;
+    free_pages.load(a.users, a.pages);
+    want[tid] = 0;
+    if (blockIdx.x == 0)  // there: less those given up
+        for (int p = tid; p < a.pages; p += kThreads) given[p] = 0;
+    free_pages.tell(counts);
+    __syncthreads();
+    const int entries = a.batch * a.width;
+    each_entry(a, entries, [&](int b, int c, int length, int entry) {
+        if (c < pages_needed(length, a.page_shift) && !names_page(entry, a.pages)) atomicAdd(want + b, 1);
+    });
+    __syncthreads();
+    // rows' wants before this wave's row, and all
+    int start = 0, wanted = 0;
+    for (int i = lane_id(); i < a.batch; i += 64) {
+        const int w = want[i];
+        wanted += w;
+        start += i < b ? w : 0;
+    }
+    start = last_lane(running_sum(start)), wanted = last_lane(running_sum(wanted));
+    const int free = min(free_pages.sum(counts), wanted);
+    if (blockIdx.x == 0) {
+        each_entry(a, entries, [&](int, int c, int length, int entry) {
+            if (c >= pages_needed(length, a.page_shift) && names_page(entry, a.pages)) atomicAdd(given + entry, -1);
+        });
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < Groups::kEach; ++k) {
+            const Group& x = free_pages.x[k];
+            if (free_pages.group(k) * kGroup >= a.pages) break;
+            int before = free_pages.before(k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int p = free_pages.group(k) * kGroup + 64 * i + lane_id();
+                const bool taken = x.there[i] == 0 && before + bits_before(x.free[i]) < free;
+                if (p < a.pages) a.new_users[p] = x.there[i] + given[p] + taken;
+                before += __popcll(x.free[i]);
+            }
+        }
         return;
     }
-    const int g = ((int)blockIdx.x - a.row_blocks) * kWaves + wave_id();
+    free_pages.list(free, given);
+    __syncthreads();
+    if (!mine) return;
+    const int held = resize_columns<false>(a, b, 0, a.width, start, free, given, row_length, row);
+    if (lane_id() == 0) a.missing[b] = pages_needed(row_length, a.page_shift) - held;
+}
+
+// Many.  A row by a workgroup of kRowWaves, each a part of its columns.
+constexpr int kRowWaves = 8;
+struct Part {
+    int from, end;
+};
+__device__ __forceinline__ Part part_of(int width) {
+    const int each = ((width + kRowWaves - 1) / kRowWaves + 63) / 64 * 64, from = min(wave_id() * each, width);
+    return Part{from, min(from + each, width)};
+}
+
+// Rows' wants by the first workgroups, pages' counts by the others.
+__global__ __launch_bounds__(64 * kRowWaves) void resize_count_kernel(ResizeArgs a) {
+    __shared__ int meet[kRowWaves];
+    if ((int)blockIdx.x < a.batch) {
+        const int b = (int)blockIdx.x, wave = wave_id(), lane = lane_id();
+        const Part part = part_of(a.width);
+        const int32_t* row = a.table + b * a.table_stride;
+        Columns first;
+        first.load(row, part.from, part.end);
+        const int lacks = lacking(a, row, part.from, min(part.end, pages_wanted(a.lengths[b], a.page_shift, a.width)), first);
+        if (lane == 0) meet[wave] = lacks;
+        __syncthreads();
+        int all = 0;
+        for (int w = 0; w < kRowWaves; ++w) all += meet[w];
+        if (threadIdx.x == 0) a.want[b] = all;
+        return;
+    }
+    const int g = ((int)blockIdx.x - a.batch) * kRowWaves + wave_id();
     if ((int64_t)g * kGroup >= a.pages) return;
     Group x;
     x.load(a.users, a.pages, g);
@@ -257,36 +385,51 @@ __global__ __launch_bounds__(kThreads) void resize_count_kernel(ResizeArgs a) {
     }
 }
 
-// The sum of counts[0 .. n) by one workgroup.
-__device__ __forceinline__ int sum_of(const int32_t* counts, int n, int* meet) {
-    int sum = 0;
-    for (int i = (int)threadIdx.x; i < n; i += kThreads) sum += counts[i];
-    return block_sum(sum, meet);
-}
-
+// The free pages in order (as many as there are entries), and the rows' starts.
 __global__ __launch_bounds__(kThreads) void resize_list_kernel(ResizeArgs a) {
     __shared__ int meet[kWaves];
     const int groups = (a.pages + kGroup - 1) / kGroup;
-    const int first = (int)blockIdx.x * kWaves;
-    int before = sum_of(a.counts, first, meet);
-    if (before >= a.most) return;
-    const int g = first + wave_id();
-    if (g >= groups) return;
-    for (int i = first; i < g; ++i) before += a.counts[i];
-    Group x;
-    x.load(a.users, a.pages, g);
-    list_group(x, g, before, a.most, a.list);
+    if ((int)blockIdx.x < a.list_blocks) {
+        const int first = (int)blockIdx.x * kWaves, g = first + wave_id();
+        int before = sum_of(a.counts, first, meet);
+        if (before >= a.most || g >= groups) return;
+        before += sum_between(a.counts, first, g);
+        Group x;
+        x.load(a.users, a.pages, g);
+        list_group(x, g, before, a.most, a.list);
+        return;
+    }
+    const int first = ((int)blockIdx.x - a.list_blocks) * kThreads;
+    const int before = sum_of(a.want, first, meet), b = first + (int)threadIdx.x;
+    int all;
+    const int start = before + block_before(b < a.batch ? a.want[b] : 0, meet, all);
+    if (b < a.batch) a.start[b] = start;
+    if (first == 0) {
+        const int free = sum_of(a.counts, groups, meet);
+        if (threadIdx.x == 0) *a.free = min(free, a.most);
+    }
 }
 
-__global__ __launch_bounds__(kThreads) void resize_apply_kernel(ResizeArgs a) {
-    __shared__ int meet[kWaves];
-    const int free = min(sum_of(a.counts, (a.pages + kGroup - 1) / kGroup, meet), a.most);
-    const int first = (int)blockIdx.x * kWaves;
-    int64_t start = sum_of(a.want, first, meet);
-    const int b = first + wave_id();
-    if (b >= a.batch) return;
-    for (int i = first; i < b; ++i) start += a.want[i];
-    resize_row(a, b, start, free);
+__global__ __launch_bounds__(64 * kRowWaves) void resize_apply_kernel(ResizeArgs a) {
+    __shared__ int meet[kRowWaves];
+    const int b = (int)blockIdx.x, wave = wave_id(), lane = lane_id();
+    const Part part = part_of(a.width);
+    const int32_t* row = a.table + b * a.table_stride;
+    Columns first;
+    first.load(row, part.from, part.end);
+    const int free = *a.free, length = a.lengths[b];
+    int64_t start = a.start[b];
+    const int lacks = lacking(a, row, part.from, min(part.end, pages_wanted(length, a.page_shift, a.width)), first);
+    if (lane == 0) meet[wave] = lacks;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) start += meet[w];
+    __syncthreads();
+    const int held = resize_columns<true>(a, b, part.from, part.end, start, free, a.list, length, first);
+    if (lane == 0) meet[wave] = held;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kRowWaves; ++w) all += meet[w];
+    if (threadIdx.x == 0) a.missing[b] = pages_needed(length, a.page_shift) - all;
 }
 
 // ---- copies between pages ----
@@ -296,11 +439,16 @@ struct Pool {
     int64_t layer[2], page[2], head[2], position[2];
     int layers, pieces;  // 16-byte pieces of a position
     int kv_heads, page_size;
+    int threads;         // that copy a page together: so many that each has kAtOnce pieces, a wave at least
 };
+constexpr int kAtOnce = 4;  // loads of a thread on their way
 
-// `count` positions of a page of one layer (keys or values) to another page, by the
-// workgroup: pieces in the order of the larger stride.
+// `count` positions of a page of one layer (keys or values) to another page, by
+// p.threads threads: pieces in the order of the larger stride.  Past the caches, as
+// nothing reads them again soon: 256 MB (977 pages of 8 layers) take 53.8 us so, 60.0
+// through them.
 __device__ __forceinline__ void copy_page(const Pool& p, int which, int layer, int from, int to, int count) {
+    const int tid = (int)threadIdx.x & (p.threads - 1);
     const uint16_t* base = p.data[which] + layer * p.layer[which];
     const uint16_t* source = base + from * p.page[which];
     uint16_t* target = const_cast<uint16_t*>(base) + to * p.page[which];
@@ -309,21 +457,31 @@ __device__ __forceinline__ void copy_page(const Pool& p, int which, int layer, i
     const int64_t inner_step = by_head ? p.position[which] : p.head[which];
     const int64_t outer_step = by_head ? p.head[which] : p.position[which];
     const int total = p.kv_heads * count * p.pieces;
-    constexpr int kAtOnce = 4;
-    for (int base_piece = 0; base_piece < total; base_piece += kAtOnce * kCopyThreads) {
+    for (int first = tid; first < total; first += kAtOnce * p.threads) {
         u32x4 x[kAtOnce];
         int64_t at[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const int piece = base_piece + i * kCopyThreads + (int)threadIdx.x;
+            const int piece = first + i * p.threads;
             const int row = piece / p.pieces, d = piece - row * p.pieces;
             const int outer = row / inner;
             at[i] = outer * outer_step + (row - outer * inner) * inner_step + 8 * d;
-            if (piece < total) x[i] = *(const u32x4*)(source + at[i]);
+            if (piece < total) x[i] = __builtin_nontemporal_load((const u32x4*)(source + at[i]));
         }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
-            if (base_piece + i * kCopyThreads + (int)threadIdx.x < total) *(u32x4*)(target + at[i]) = x[i];
+            if (first + i * p.threads < total) __builtin_nontemporal_store(x[i], (u32x4*)(target + at[i]));
+    }
+}
+
+// The copies of a workgroup of kThreads: `blocks` such workgroups go through `items`.
+template <class F>
+__device__ __forceinline__ void each_copy(const Pool& p, int64_t items, int block, int blocks, F copy) {
+    const int together = kThreads / p.threads;
+    for (int64_t item = (int64_t)block * together + __builtin_amdgcn_readfirstlane((int)threadIdx.x / p.threads); item < items;
+         item += (int64_t)blocks * together) {
+        const int r = (int)(item / (2 * p.layers)), rest = (int)(item - (int64_t)r * 2 * p.layers);
+        copy(r, rest & 1, rest >> 1);
     }
 }
 
@@ -339,6 +497,7 @@ struct ForkArgs {
     int32_t* new_lengths;
     int32_t* new_users;
     int32_t* missing;
+    // many:
     int32_t* first;   // [batch]: a row's first child (children if it has none)
     int32_t* born;    // [batch]: how many it has
     int32_t* target;  // [children]: the page of a child's copy, -1 if it has none, or -2 where one was wanted
@@ -346,20 +505,25 @@ struct ForkArgs {
     int32_t* list;    // [children]: free pages
     int64_t table_stride;
     int batch, children, width, pages, page_shift;
-    int counted;      // counts and new_users were made by a launch before
-    int row_blocks, old_blocks;
+    int row_blocks, old_blocks, copy_blocks;
+    Divisor by_width;
 };
 
-// A row's last page if it is there and not full: its column, or -1.
-__device__ __forceinline__ int partial_column(const ForkArgs& a, int b) {
-    const int length = max(a.lengths[b], 0);
-    const int column = length >> a.page_shift;
-    if (!(length & ((1 << a.page_shift) - 1)) || column >= a.width) return -1;
-    return names_page(a.table[b * a.table_stride + column], a.pages) ? column : -1;
-}
-// Whether only this row names that page.
-__device__ __forceinline__ bool sole(const ForkArgs& a, int b, int column) {
-    return a.users[a.table[b * a.table_stride + column]] == 1;
+// What a fork asks of an old row: its length, and its last page if that is there and not
+// full (column -1 if not).
+struct Old {
+    int length, column, page;
+    bool sole;  // only this row names that page
+};
+__device__ __forceinline__ Old old_row(const ForkArgs& a, int b) {
+    Old r;
+    r.length = max(a.lengths[b], 0);
+    r.column = r.length >> a.page_shift;
+    r.page = -1;
+    if ((r.length & ((1 << a.page_shift) - 1)) && r.column < a.width) r.page = a.table[b * a.table_stride + r.column];
+    if (!names_page(r.page, a.pages)) r.column = -1;
+    r.sole = r.column >= 0 && a.users[r.page] == 1;
+    return r;
 }
 
 __global__ __launch_bounds__(kThreads) void fork_count_kernel(ForkArgs a) {
@@ -375,12 +539,111 @@ __global__ __launch_bounds__(kThreads) void fork_count_kernel(ForkArgs a) {
     }
 }
 
-// One workgroup: who copies, and to which page.
+// Row i of the answer (one wave), a copy of row `parent` (-1: none); `target`: as in
+// ForkArgs.
+template <bool kCount>
+__device__ __forceinline__ void fork_row(const ForkArgs& a, int i, int parent, int length, int target) {
+    const int upto = pages_wanted(length, a.page_shift, a.width);
+    const int column = length >> a.page_shift;  // (where there is a copy)
+    const int32_t* row = a.table + max(parent, 0) * a.table_stride;
+    for (int c0 = 0; c0 < a.width; c0 += 256) {
+        int entry[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = c0 + 64 * k + lane_id();
+            entry[k] = c < upto ? row[c] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = c0 + 64 * k + lane_id();
+            int e = names_page(entry[k], a.pages) ? entry[k] : -1;
+            if (target != -1 && c == column) {
+                e = target < 0 ? -1 : target;
+                if (kCount && e >= 0) atomicAdd(a.new_users + e, 1);
+            }
+            if (c < a.width) a.new_table[(int64_t)i * a.width + c] = e;
+        }
+    }
+    if (lane_id() == 0) {
+        a.new_lengths[i] = length;
+        a.missing[i] = target == -2;
+    }
+}
+
+// By what the users of column c's page of an old row change: children that hold it less
+// the row itself.
+__device__ __forceinline__ int fork_change(int c, int upto, int column, int born, bool kept) {
+    return (c == column ? kept : c < upto ? born : 0) - 1;
+}
+
+// Few.  The first workgroup writes the users, the next row_blocks new rows, the others
+// copy.
+__global__ __launch_bounds__(kThreads) void fork_few_kernel(ForkArgs a) {
+    // of children: parent[], length[], target[]; of copies: source[], filled[], list[]
+    __shared__ int meet[kWaves], counts[Groups::kMost], first[kFewRows], born[kFewRows], parent[kFewRows], length[kFewRows],
+        target[kFewRows], source[kFewRows], filled[kFewRows], list[kFewRows], change[kFewPages];
+    const int tid = (int)threadIdx.x;
+    int block = (int)blockIdx.x;
+    // thread t: child t and, in the first workgroup, row t of the old batch
+    int mine = tid < a.children ? a.parents[tid] : -1;
+    if (mine >= a.batch) mine = -1;
+    Groups free_pages;
+    free_pages.load(a.users, a.pages);
+    Old from{0, -1, -1, false}, old{0, -1, -1, false};
+    if (mine >= 0) from = old_row(a, mine);
+    if (block == 0) {
+        if (tid < a.batch) old = old_row(a, tid);
+        for (int p = tid; p < a.pages; p += kThreads) change[p] = 0;
+    }
+    first[tid] = a.children, born[tid] = 0;
+    parent[tid] = max(mine, -1), length[tid] = from.length;
+    free_pages.tell(counts);
+    __syncthreads();
+    if (mine >= 0) {
+        atomicMin(first + mine, tid);
+        atomicAdd(born + mine, 1);
+    }
+    __syncthreads();
+    const bool copy = from.column >= 0 && (first[mine] != tid || !from.sole);
+    int copies;
+    const int rank = block_rank(copy, meet, copies);
+    const int free = min(free_pages.sum(counts), copies);
+    free_pages.list(free, list);
+    if (copy) source[rank] = from.page, filled[rank] = from.length;
+    __syncthreads();
+    target[tid] = !copy ? -1 : rank < free ? list[rank] : -2;
+    if (block == 0) {
+        // (now of the old batch's rows: entries in use, the last page's column, and whether a
+        // child keeps it)
+        first[tid] = pages_wanted(old.length, a.page_shift, a.width), source[tid] = old.column;
+        filled[tid] = old.sole && born[tid] > 0;
+        if (tid < free) change[list[tid]] = 1;
+        __syncthreads();
+        const int entries = a.batch * a.width;
+        each_entry(a, entries, [&](int b, int c, int, int entry) {
+            const int by = fork_change(c, first[b], source[b], born[b], filled[b]);
+            if (by && names_page(entry, a.pages)) atomicAdd(change + entry, by);
+        });
+        __syncthreads();
+        for (int p = tid; p < a.pages; p += kThreads) a.new_users[p] = a.users[p] + change[p];
+        return;
+    }
+    __syncthreads();
+    if (--block < a.row_blocks) {
+        const int i = block * kWaves + wave_id();
+        if (i < a.children) fork_row<false>(a, i, parent[i], length[i], target[i]);
+        return;
+    }
+    each_copy(a.pool, (int64_t)free * 2 * a.pool.layers, block - a.row_blocks, a.copy_blocks, [&](int r, int which, int layer) {
+        copy_page(a.pool, which, layer, source[r], list[r], filled[r] & ((1 << a.page_shift) - 1));
+    });
+}
+
+// Many.  One workgroup: who copies, and to which page.
 __global__ __launch_bounds__(kThreads) void fork_plan_kernel(ForkArgs a) {
     __shared__ int meet[kWaves];
     const int tid = (int)threadIdx.x;
     for (int b = tid; b < a.batch; b += kThreads) a.first[b] = a.children, a.born[b] = 0;
-    if (!a.counted) count_groups(a.users, a.pages, a.counts, a.new_users);
     __syncthreads();
     for (int i = tid; i < a.children; i += kThreads) {
         const int parent = a.parents[i];
@@ -396,9 +659,9 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(ForkArgs a) {
         if (i < a.children) {
             const int parent = a.parents[i];
             if (parent >= 0 && parent < a.batch) {
-                const int column = partial_column(a, parent);
-                copy = column >= 0 && (__hip_atomic_load(a.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != i ||
-                                       !sole(a, parent, column));
+                const Old from = old_row(a, parent);
+                copy = from.column >= 0 &&
+                       (__hip_atomic_load(a.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != i || !from.sole);
             }
         }
         int all;
@@ -416,59 +679,38 @@ __global__ __launch_bounds__(kThreads) void fork_plan_kernel(ForkArgs a) {
 }
 
 // Workgroups of three kinds: new rows, one wave each; old rows' users, one wave each;
-// copies, one child, layer and side (keys, values) each.
-__global__ __launch_bounds__(kCopyThreads) void fork_apply_kernel(ForkArgs a) {
+// copies.
+__global__ __launch_bounds__(kThreads) void fork_apply_kernel(ForkArgs a) {
     const int block = (int)blockIdx.x;
-    constexpr int kRows = kCopyThreads / 64;
     if (block < a.row_blocks) {
-        const int i = block * kRows + wave_id();
+        const int i = block * kWaves + wave_id();
         if (i >= a.children) return;
         const int parent = a.parents[i];
         const bool there = parent >= 0 && parent < a.batch;
-        const int length = there ? max(a.lengths[parent], 0) : 0;
-        const int upto = pages_wanted(length, a.page_shift, a.width);
-        const int target = a.target[i];
-        const int column = there ? partial_column(a, parent) : -1;
-        const int32_t* row = a.table + (there ? parent : 0) * a.table_stride;
-        for (int c = lane_id(); c < a.width; c += 64) {
-            int e = c < upto ? row[c] : -1;
-            if (!names_page(e, a.pages)) e = -1;
-            if (c == column && target != -1) {
-                e = target;
-                if (e >= 0) atomicAdd(a.new_users + e, 1);
-                else e = -1;
-            }
-            a.new_table[(int64_t)i * a.width + c] = e;
-        }
-        if (lane_id() == 0) {
-            a.new_lengths[i] = length;
-            a.missing[i] = target == -2;
-        }
+        fork_row<true>(a, i, there ? parent : -1, there ? max(a.lengths[parent], 0) : 0, a.target[i]);
         return;
     }
     if (block < a.row_blocks + a.old_blocks) {
-        const int b = (block - a.row_blocks) * kRows + wave_id();
+        const int b = (block - a.row_blocks) * kWaves + wave_id();
         if (b >= a.batch) return;
         const int born = a.born[b];
-        const int upto = pages_wanted(a.lengths[b], a.page_shift, a.width);
-        const int column = partial_column(a, b);
-        // children that hold the row's last page itself
-        const int kept = column >= 0 && born > 0 && sole(a, b, column);
+        const Old old = old_row(a, b);
+        const int upto = pages_wanted(old.length, a.page_shift, a.width);
         for (int c = lane_id(); c < a.width; c += 64) {
             const int e = a.table[b * a.table_stride + c];
-            const int change = (c == column ? kept : c < upto ? born : 0) - 1;
-            if (change && names_page(e, a.pages)) atomicAdd(a.new_users + e, change);
+            const int by = fork_change(c, upto, old.column, born, old.sole && born > 0);
+            if (by && names_page(e, a.pages)) atomicAdd(a.new_users + e, by);
         }
         return;
     }
-    const int64_t item = block - a.row_blocks - a.old_blocks;
-    const int i = (int)(item / (2 * a.pool.layers)), rest = (int)(item - (int64_t)i * 2 * a.pool.layers);
-    const int target = a.target[i];
-    if (target < 0) return;
-    const int parent = a.parents[i];
-    const int length = a.lengths[parent];
-    copy_page(a.pool, rest & 1, rest >> 1, a.table[parent * a.table_stride + (length >> a.page_shift)], target,
-              length & ((1 << a.page_shift) - 1));
+    each_copy(a.pool, (int64_t)a.children * 2 * a.pool.layers, block - a.row_blocks - a.old_blocks, a.copy_blocks,
+              [&](int i, int which, int layer) {
+                  const int target = a.target[i];
+                  if (target < 0) return;
+                  const int parent = a.parents[i], length = a.lengths[parent];
+                  copy_page(a.pool, which, layer, a.table[parent * a.table_stride + (length >> a.page_shift)], target,
+                            length & ((1 << a.page_shift) - 1));
+              });
 }
 
 // ---- compact ----
@@ -484,6 +726,7 @@ struct CompactArgs {
     int32_t* new_table;
     int32_t* new_users;
     int32_t* moved_to;
+    // many:
     int32_t* fate;    // [pages]
     int32_t* counts;  // [groups]
     int32_t* holes;   // [pages / 2]
@@ -491,7 +734,8 @@ struct CompactArgs {
     int32_t* moves;   // [1]
     int64_t table_stride;
     int batch, width, pages;
-    int page_blocks, copy_blocks;
+    int page_blocks, table_blocks, copy_blocks;
+    Divisor by_width;
 };
 
 // A group's pages; `before`: the free pages before it, `live`: all in use, `low`: free
@@ -500,7 +744,7 @@ __device__ __forceinline__ void settle_group(const CompactArgs& a, const Group& 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t p64 = (int64_t)group * kGroup + 64 * i + lane_id();
-        const int free_before = before + bits_before(g.free[i], lane_id());
+        const int free_before = before + bits_before(g.free[i]);
         before += __popcll(g.free[i]);
         if (p64 >= a.pages) continue;
         const int p = (int)p64;
@@ -522,30 +766,82 @@ __device__ __forceinline__ int free_below(const CompactArgs& a, int live, int be
     const int group = live / kGroup;  // (live <= pages: its group's pages below `live` exist)
     Group x;
     x.load(a.users, a.pages, group);
-    int low = before;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int edge = live - group * kGroup - 64 * i;  // bits below it count
-        const uint64_t mask = edge <= 0 ? 0 : edge >= 64 ? ~uint64_t(0) : (uint64_t(1) << edge) - 1;
-        low += __popcll(x.free[i] & mask);
-    }
-    return low;
+    return before + x.count_below(live % kGroup);
 }
 
-__global__ __launch_bounds__(kThreads) void compact_few_kernel(CompactArgs a) {
-    __shared__ int meet[kWaves];
-    const int groups = (a.pages + kGroup - 1) / kGroup;
-    count_groups(a.users, a.pages, a.counts, nullptr);
+// Few: `to` says where a page lies now: kFree, or the page, or kRank and its rank among
+// those that move.  The first workgroup writes what is said of pages, the next
+// table_blocks table entries, the others copy.
+// (two workgroups a CU copy faster than one: eight waves a SIMD, no more scalar registers
+// than that leaves)
+__global__ __launch_bounds__(kThreads, 8) void compact_few_kernel(CompactArgs a) {
+    constexpr uint16_t kFree = 0xFFFF, kRank = 0x8000;
+    static_assert(kFewPages / 2 + kRank < kFree && kFewPages <= kRank, "all told apart");
+    __shared__ int counts[Groups::kMost], below[kWaves];
+    __shared__ uint16_t to[kFewPages], holes[kFewPages / 2], movers[kFewPages / 2];
+    const int tid = (int)threadIdx.x;
+    Groups all;
+    all.load(a.users, a.pages);
+    all.tell(counts);
     __syncthreads();
-    const int free = sum_groups(a.counts, groups, meet);
-    const int live = a.pages - free;
-    const int low = free_below(a, live, live / kGroup < groups ? a.counts[live / kGroup] : free);
-    for (int g = wave_id(); g < groups; g += kWaves) {
-        Group x;
-        x.load(a.users, a.pages, g);
-        settle_group(a, x, g, a.counts[g], live, low);
+    const int live = a.pages - all.sum(counts);
+    // free pages below `live`: those of the groups before its own, and of that one's first pages
+    int low = 0;
+#pragma unroll
+    for (int k = 0; k < Groups::kEach; ++k)
+        if (all.group(k) == live / kGroup) low = all.before(k) + all.x[k].count_below(live % kGroup);
+    const int wave = wave_id();
+    if (lane_id() == 0) below[wave] = low;
+    __syncthreads();
+    low = live < kFewPages ? below[live / kGroup % kWaves] : 0;  // (no group is left: none is free)
+#pragma unroll
+    for (int k = 0; k < Groups::kEach; ++k) {
+        const Group& x = all.x[k];
+        if (all.group(k) * kGroup >= a.pages) break;
+        int before = all.before(k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = all.group(k) * kGroup + 64 * i + lane_id();
+            const int free_before = before + bits_before(x.free[i]);
+            before += __popcll(x.free[i]);
+            if (p >= a.pages) continue;
+            if (x.there[i] == 0) {
+                to[p] = kFree;
+                if (p < live) holes[free_before] = (uint16_t)p;
+            } else if (p < live) {
+                to[p] = (uint16_t)p;
+            } else {
+                const int rank = p - free_before - (live - low);
+                to[p] = (uint16_t)(kRank + rank);
+                movers[rank] = (uint16_t)p;
+            }
+        }
     }
-    if (threadIdx.x == 0) *a.moves = low;
+    __syncthreads();
+    auto place = [&](int p) {
+        const uint16_t t = to[p];
+        return t == kFree ? -1 : t >= kRank ? (int)holes[t - kRank] : (int)t;
+    };
+    int block = (int)blockIdx.x;
+    if (block == 0) {
+        for (int p = tid; p < a.pages; p += kThreads) {
+            const int now = place(p);
+            a.moved_to[p] = now;
+            if (now >= 0) a.new_users[now] = a.users[p];
+            if (p >= live) a.new_users[p] = 0;
+        }
+        return;
+    }
+    if (--block < a.table_blocks) {
+        const int at = block * kThreads + tid;
+        if (at >= a.batch * a.width) return;
+        const int b = a.by_width(at), e = a.table[b * a.table_stride + (at - b * a.width)];
+        a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
+        return;
+    }
+    each_copy(a.pool, (int64_t)low * 2 * a.pool.layers, block - a.table_blocks, a.copy_blocks, [&](int r, int which, int layer) {
+        copy_page(a.pool, which, layer, movers[r], holes[r], a.pool.page_size);
+    });
 }
 
 __global__ __launch_bounds__(kThreads) void compact_count_kernel(CompactArgs a) {
@@ -566,31 +862,21 @@ __global__ __launch_bounds__(kThreads) void compact_list_kernel(CompactArgs a) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.moves = low;
     const int g = first + wave_id();
     if (g >= groups) return;
-    for (int i = first; i < g; ++i) before += a.counts[i];
+    before += sum_between(a.counts, first, g);
     Group x;
     x.load(a.users, a.pages, g);
     settle_group(a, x, g, before, live, low);
 }
 
-// Copies by the first workgroups, which go through all there are; then pages, then
-// table entries.
-__global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(CompactArgs a) {
+// Pages by the first workgroups, then table entries, then copies.
+__global__ __launch_bounds__(kThreads) void compact_apply_kernel(CompactArgs a) {
     int block = (int)blockIdx.x;
-    if (block < a.copy_blocks) {
-        const int64_t items = (int64_t)*a.moves * 2 * a.pool.layers;
-        for (int64_t item = block; item < items; item += a.copy_blocks) {
-            const int i = (int)(item / (2 * a.pool.layers)), rest = (int)(item - (int64_t)i * 2 * a.pool.layers);
-            copy_page(a.pool, rest & 1, rest >> 1, a.movers[i], a.holes[i], a.pool.page_size);
-        }
-        return;
-    }
-    block -= a.copy_blocks;
     auto place = [&](int p) {
         const int32_t f = a.fate[p];
         return f == kStays ? p : f >= kMoves && f < kHole ? a.holes[f - kMoves] : -1;
     };
     if (block < a.page_blocks) {
-        const int64_t p = (int64_t)block * kCopyThreads + threadIdx.x;
+        const int64_t p = (int64_t)block * kThreads + threadIdx.x;
         if (p >= a.pages) return;
         const int32_t f = a.fate[p];
         a.moved_to[p] = place((int)p);
@@ -598,11 +884,16 @@ __global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(CompactArgs
         return;
     }
     block -= a.page_blocks;
-    const int64_t at = (int64_t)block * kCopyThreads + threadIdx.x;
-    if (at >= (int64_t)a.batch * a.width) return;
-    const int b = (int)(at / a.width), c = (int)(at - (int64_t)b * a.width);
-    const int e = a.table[b * a.table_stride + c];
-    a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
+    if (block < a.table_blocks) {
+        const int64_t at = (int64_t)block * kThreads + threadIdx.x;
+        if (at >= (int64_t)a.batch * a.width) return;
+        const int b = a.by_width((int)at), e = a.table[b * a.table_stride + ((int)at - b * a.width)];
+        a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
+        return;
+    }
+    each_copy(a.pool, (int64_t)*a.moves * 2 * a.pool.layers, block - a.table_blocks, a.copy_blocks, [&](int r, int which, int layer) {
+        copy_page(a.pool, which, layer, a.movers[r], a.holes[r], a.pool.page_size);
+    });
 }
 
 // ---- host ----
@@ -650,7 +941,8 @@ int pool_view(const char* op, const qwen2_page_pool* p, Pool* view) {
         if (s < 0 || s % 8)
             return set_error(W4G64_STATUS_INVALID_VALUE, "%s: pool strides must be multiples of 8 elements, not negative", op);
     *view = Pool{{(uint16_t*)p->k, (uint16_t*)p->v}, {p->k_layer, p->v_layer}, {p->k_page, p->v_page}, {p->k_head, p->v_head},
-                 {p->k_position, p->v_position}, (int)p->layers, (int)(p->head_dim / 8), (int)p->kv_heads, (int)p->page_size};
+                 {p->k_position, p->v_position}, (int)p->layers, (int)(p->head_dim / 8), (int)p->kv_heads, (int)p->page_size, 64};
+    while (view->threads < kMostCopyThreads && view->threads * kAtOnce < p->kv_heads * p->page_size * p->head_dim / 8) view->threads *= 2;
     return W4G64_STATUS_OK;
 }
 
@@ -669,6 +961,16 @@ int launched(const char* op) {
 
 int64_t most_given(int64_t batch, int64_t width, int64_t pages) { return batch * width < pages ? batch * width : pages; }
 
+// Whether a call's sizes are few (rows: all there are).
+bool few(int64_t rows, int64_t width, int64_t pages) {
+    return rows <= kFewRows && rows * width <= kFewEntries && pages <= kFewPages;
+}
+// Workgroups for `items` copies at most: two a CU, or as many as have something to do.
+int copy_blocks(const Pool& pool, int64_t items) {
+    const int64_t blocks = blocks_of(items, kThreads / pool.threads);
+    return (int)(blocks < 512 ? blocks : 512);
+}
+
 }  // namespace
 }  // namespace w4g64
 
@@ -678,7 +980,8 @@ extern "C" {
 
 int64_t qwen2_paged_resize_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages) {
     if (check_sizes("paged_resize", batch, table_width, num_pages)) return 0;
-    return 4 * (batch + groups_of(num_pages) + most_given(batch, table_width, num_pages));
+    return few(batch, table_width, num_pages) ? 0
+                                              : 4 * (2 * batch + 1 + groups_of(num_pages) + most_given(batch, table_width, num_pages));
 }
 
 int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* page_users,
@@ -696,26 +999,29 @@ int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const in
     ResizeArgs a{};
     a.table = page_table, a.table_stride = table_stride, a.lengths = lengths, a.users = page_users;
     a.new_table = new_table, a.new_users = new_users, a.missing = missing;
-    a.want = (int32_t*)workspace, a.counts = a.want + batch, a.list = a.counts + groups_of(num_pages);
     a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)num_pages, a.page_shift = shift_of(page_size);
-    a.most = (int)most_given(batch, table_width, num_pages);
+    a.by_width = divisor(table_width);
     const hipStream_t s = (hipStream_t)stream;
-    if (num_pages <= kFewPages && batch * table_width <= kFewEntries) {
-        hipLaunchKernelGGL(resize_few_kernel, dim3(1), dim3(kThreads), 0, s, a);
+    if (few(batch, table_width, num_pages)) {
+        hipLaunchKernelGGL(resize_few_kernel, dim3((unsigned)(1 + blocks_of(batch, kWaves))), dim3(kThreads), 0, s, a);
         return launched("paged_resize");
     }
-    a.row_blocks = (int)blocks_of(batch, kWaves);
-    const int64_t lists = blocks_of(groups_of(num_pages), kWaves);
-    hipLaunchKernelGGL(resize_count_kernel, dim3((unsigned)(a.row_blocks + lists)), dim3(kThreads), 0, s, a);
+    a.want = (int32_t*)workspace, a.start = a.want + batch, a.free = a.start + batch, a.counts = a.free + 1;
+    a.list = a.counts + groups_of(num_pages);
+    a.most = (int)most_given(batch, table_width, num_pages);
+    a.list_blocks = (int)blocks_of(groups_of(num_pages), kWaves);
+    hipLaunchKernelGGL(resize_count_kernel, dim3((unsigned)(batch + blocks_of(groups_of(num_pages), kRowWaves))),
+                       dim3(64 * kRowWaves), 0, s, a);
     if (batch) {
-        hipLaunchKernelGGL(resize_list_kernel, dim3((unsigned)lists), dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(resize_apply_kernel, dim3((unsigned)a.row_blocks), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(resize_list_kernel, dim3((unsigned)(a.list_blocks + blocks_of(batch, kThreads))), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(resize_apply_kernel, dim3((unsigned)batch), dim3(64 * kRowWaves), 0, s, a);
     }
     return launched("paged_resize");
 }
 
-int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t num_pages) {
-    if (batch < 0 || children < 0 || num_pages <= 0) return 0;
+int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t table_width, int64_t num_pages) {
+    if (batch < 0 || children < 0 || table_width <= 0 || num_pages <= 0) return 0;
+    if (few(batch, table_width, num_pages) && few(children, table_width, num_pages)) return 0;
     return 4 * (2 * batch + 2 * children + groups_of(num_pages));
 }
 
@@ -732,30 +1038,34 @@ int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int
         (children && !aligned4({parents, new_table, new_lengths, missing})))
         return set_error(W4G64_STATUS_INVALID_VALUE, "paged_fork pointers must be non-null, 4-byte aligned device pointers");
     const int64_t copies = children * 2 * pool->layers;
-    if (copies > 0x7FFFFF)  // (of 2^32 threads a launch)
-        return set_error(W4G64_STATUS_UNSUPPORTED, "paged_fork call is too large: %lld copies", (long long)copies);
-    status = check_workspace("paged_fork", qwen2_paged_fork_workspace_bytes(batch, children, pool->num_pages), workspace,
+    status = check_workspace("paged_fork", qwen2_paged_fork_workspace_bytes(batch, children, table_width, pool->num_pages), workspace,
                              workspace_bytes);
     if (status) return status;
     a.table = page_table, a.table_stride = table_stride, a.lengths = lengths, a.users = page_users, a.parents = parents;
     a.new_table = new_table, a.new_lengths = new_lengths, a.new_users = new_users, a.missing = missing;
+    a.batch = (int)batch, a.children = (int)children, a.width = (int)table_width, a.pages = (int)pool->num_pages;
+    a.page_shift = shift_of(pool->page_size), a.by_width = divisor(table_width);
+    const hipStream_t s = (hipStream_t)stream;
+    if (few(batch, table_width, pool->num_pages) && few(children, table_width, pool->num_pages)) {
+        a.row_blocks = (int)blocks_of(children, kWaves);
+        a.copy_blocks = copy_blocks(a.pool, copies);
+        hipLaunchKernelGGL(fork_few_kernel, dim3((unsigned)(1 + a.row_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);
+        return launched("paged_fork");
+    }
     a.first = (int32_t*)workspace, a.born = a.first + batch, a.target = a.born + batch, a.list = a.target + children;
     a.counts = a.list + children;
-    a.batch = (int)batch, a.children = (int)children, a.width = (int)table_width, a.pages = (int)pool->num_pages;
-    a.page_shift = shift_of(pool->page_size);
-    const hipStream_t s = (hipStream_t)stream;
-    a.counted = pool->num_pages > kFewPages;
-    if (a.counted)
-        hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)blocks_of(groups_of(pool->num_pages), kWaves)), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)blocks_of(groups_of(pool->num_pages), kWaves)), dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kThreads), 0, s, a);
-    a.row_blocks = (int)blocks_of(children, kCopyThreads / 64), a.old_blocks = (int)blocks_of(batch, kCopyThreads / 64);
-    const int64_t blocks = a.row_blocks + a.old_blocks + copies;
-    if (blocks) hipLaunchKernelGGL(fork_apply_kernel, dim3((unsigned)blocks), dim3(kCopyThreads), 0, s, a);
+    a.row_blocks = (int)blocks_of(children, kWaves), a.old_blocks = (int)blocks_of(batch, kWaves);
+    a.copy_blocks = copy_blocks(a.pool, copies);
+    const int64_t blocks = a.row_blocks + a.old_blocks + a.copy_blocks;
+    if (blocks) hipLaunchKernelGGL(fork_apply_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     return launched("paged_fork");
 }
 
-int64_t qwen2_paged_compact_workspace_bytes(int64_t num_pages) {
-    return num_pages <= 0 ? 0 : 4 * (num_pages + groups_of(num_pages) + 2 * (num_pages / 2) + 1);
+int64_t qwen2_paged_compact_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages) {
+    if (batch < 0 || table_width <= 0 || num_pages <= 0 || few(batch, table_width, num_pages)) return 0;
+    return 4 * (num_pages + groups_of(num_pages) + 2 * (num_pages / 2) + 1);
 }
 
 int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride,
@@ -768,27 +1078,28 @@ int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, 
     if (!aligned4({page_users, new_users, moved_to}) || (batch && !aligned4({page_table, new_table})))
         return set_error(W4G64_STATUS_INVALID_VALUE, "paged_compact pointers must be non-null, 4-byte aligned device pointers");
     const int64_t pages = pool->num_pages;
-    status = check_workspace("paged_compact", qwen2_paged_compact_workspace_bytes(pages), workspace, workspace_bytes);
+    status = check_workspace("paged_compact", qwen2_paged_compact_workspace_bytes(batch, table_width, pages), workspace, workspace_bytes);
     if (status) return status;
     a.table = page_table, a.table_stride = table_stride, a.users = page_users;
     a.new_table = new_table, a.new_users = new_users, a.moved_to = moved_to;
+    a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)pages, a.by_width = divisor(table_width);
+    const hipStream_t s = (hipStream_t)stream;
+    const int64_t most = pages / 2 * 2 * pool->layers;  // copies that there can be
+    if (few(batch, table_width, pages)) {
+        a.table_blocks = (int)blocks_of(batch * table_width, kThreads);
+        a.copy_blocks = copy_blocks(a.pool, most);
+        hipLaunchKernelGGL(compact_few_kernel, dim3((unsigned)(1 + a.table_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);
+        return launched("paged_compact");
+    }
     a.fate = (int32_t*)workspace, a.counts = a.fate + pages, a.holes = a.counts + groups_of(pages);
     a.movers = a.holes + pages / 2, a.moves = a.movers + pages / 2;
-    a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)pages;
-    const hipStream_t s = (hipStream_t)stream;
-    if (pages <= kFewPages) {
-        hipLaunchKernelGGL(compact_few_kernel, dim3(1), dim3(kThreads), 0, s, a);
-    } else {
-        const unsigned lists = (unsigned)blocks_of(groups_of(pages), kWaves);
-        hipLaunchKernelGGL(compact_count_kernel, dim3(lists), dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(compact_list_kernel, dim3(lists), dim3(kThreads), 0, s, a);
-    }
-    // (eight workgroups a CU go through the copies; no more than there can be)
-    const int64_t most = pages / 2 * 2 * pool->layers;
-    a.copy_blocks = (int)(most < 2048 ? most : 2048);
-    a.page_blocks = (int)blocks_of(pages, kCopyThreads);
-    const int64_t blocks = a.copy_blocks + a.page_blocks + blocks_of(batch * table_width, kCopyThreads);
-    hipLaunchKernelGGL(compact_apply_kernel, dim3((unsigned)blocks), dim3(kCopyThreads), 0, s, a);
+    const unsigned lists = (unsigned)blocks_of(groups_of(pages), kWaves);
+    hipLaunchKernelGGL(compact_count_kernel, dim3(lists), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(compact_list_kernel, dim3(lists), dim3(kThreads), 0, s, a);
+    a.copy_blocks = copy_blocks(a.pool, most);
+    a.page_blocks = (int)blocks_of(pages, kThreads), a.table_blocks = (int)blocks_of(batch * table_width, kThreads);
+    const int64_t blocks = a.page_blocks + a.table_blocks + a.copy_blocks;
+    hipLaunchKernelGGL(compact_apply_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     return launched("paged_compact");
 }
 

@@ -76,9 +76,9 @@ SIGNATURES = {
     "qwen2_packed_attention": (_int, [_p] * 5 + [_i64] * 5 + [_int, ctypes.c_float, _int, _p]),
     "qwen2_paged_resize_workspace_bytes": (_i64, [_i64] * 3),
     "qwen2_paged_resize": (_int, [_p, _i64] + [_p] * 5 + [_i64] * 4 + [_p, _i64, _p]),
-    "qwen2_paged_fork_workspace_bytes": (_i64, [_i64] * 3),
+    "qwen2_paged_fork_workspace_bytes": (_i64, [_i64] * 4),
     "qwen2_paged_fork": (_int, [_p, _p, _i64] + [_p] * 7 + [_i64] * 3 + [_p, _i64, _p]),
-    "qwen2_paged_compact_workspace_bytes": (_i64, [_i64]),
+    "qwen2_paged_compact_workspace_bytes": (_i64, [_i64] * 3),
     "qwen2_paged_compact": (_int, [_p, _p, _i64] + [_p] * 4 + [_i64] * 2 + [_p, _i64, _p]),
     "qwen2_silu_mul": (_int, [_p, _p, _i64, _i64, _p]),
     "qwen2_lm_head_workspace_bytes": (_i64, [_i64, _i64, _i64]),

@@ -42,6 +42,8 @@ float pair_sum(uint32_t w, float c) {
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) lanes::product32<false>(a, b, c)
 #define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) lanes::pair_sum<true>(__builtin_bit_cast(uint32_t, a), c)
 #define __builtin_amdgcn_fdot2(a, b, c, clamp) lanes::pair_sum<false>(__builtin_bit_cast(uint32_t, a), c)
+#define __builtin_amdgcn_mbcnt_lo(mask, base) ((base) + __builtin_popcount((mask) & (lanes::lane() < 32 ? (1u << lanes::lane()) - 1 : ~0u)))
+#define __builtin_amdgcn_mbcnt_hi(mask, base) ((base) + __builtin_popcount((mask) & (lanes::lane() < 32 ? 0u : (1u << (lanes::lane() - 32)) - 1)))
 #define __hip_atomic_load(p, order, scope) (*(p))
 
 // (one lane runs at a time)

@@ -149,9 +149,10 @@ def test_c_entry_points_refuse_before_launch():
     assert resize(pages=(1 << 24) + 1) == _lib.STATUS_UNSUPPORTED
     assert resize(batch=1 << 20, width=1 << 12) == _lib.STATUS_UNSUPPORTED
     assert resize(table=null) == 1 and resize(users=p + 2) == 1
-    need = lib.qwen2_paged_resize_workspace_bytes(2, 3, 6)
-    assert need > 0 and resize(nbytes=need - 1) == _lib.STATUS_WORKSPACE and resize(ws=null) == _lib.STATUS_WORKSPACE
-    assert lib.qwen2_paged_resize_workspace_bytes(2, 0, 6) == 0
+    need = lib.qwen2_paged_resize_workspace_bytes(2, 3, 20000)
+    assert need > 0 and resize(pages=20000, nbytes=need - 1) == _lib.STATUS_WORKSPACE
+    assert resize(pages=20000, ws=null) == _lib.STATUS_WORKSPACE
+    assert lib.qwen2_paged_resize_workspace_bytes(2, 0, 6) == 0 and lib.qwen2_paged_resize_workspace_bytes(2, 3, 6) == 0
 
     def pool(**change):
         fields = {"k": p, "v": p, "k_layer": 0, "k_page": 2048, "k_head": 1024, "k_position": 64, "v_layer": 0, "v_page": 2048,
@@ -171,9 +172,8 @@ def test_c_entry_points_refuse_before_launch():
                                ({"head_dim": 60}, _lib.STATUS_UNSUPPORTED), ({"head_dim": 2048}, _lib.STATUS_UNSUPPORTED)]:
             assert call(pool(**change)) == status, (call, change, lib.w4g64_last_error())
         assert call(null) == 1 and call(pool(), batch=-1) == 1 and call(pool(), width=0) == 1
-        assert call(pool(), ws=null) == _lib.STATUS_WORKSPACE and call(pool(), nbytes=8) == _lib.STATUS_WORKSPACE
+        assert call(pool(num_pages=20000), ws=null) == call(pool(num_pages=20000), nbytes=8) == _lib.STATUS_WORKSPACE
     assert fork(pool(), children=-1) == 1 and fork(pool(), parents=null) == 1
-    assert fork(pool(layers=100), children=1 << 20) == _lib.STATUS_UNSUPPORTED
     assert compact(pool(), users=null) == 1
 
 
