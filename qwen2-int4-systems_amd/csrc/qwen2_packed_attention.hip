@@ -97,42 +97,53 @@ struct Piece {
     int kvh;
 };
 
-// Piece `index`.  Up to 64 sequences: tiles in the order of their keys' number, the most
-// first (a tile's place in its sequence goes by it), so that no workgroup begins a long
-// one when the others are done.  More: sequence after sequence, the last tile first.
-template <int kRows>
-__device__ __forceinline__ bool find_piece(const PackedArgs& a, int index, int lane, Piece& s) {
+// The piece of workgroup `item`.  Up to 64 sequences: tiles in the order of their keys'
+// number, the most first (a tile's place in its sequence goes by it), so that no
+// workgroup begins a long one when the others are done; with kPairs, where a CU holds two
+// workgroups, the second one of each of the 256 CUs takes the shortest, as the longest
+// tiles are what a call waits for and two of them on a CU slow each other (eight prompts
+// of 1000 tokens 44.3 us in order, 41.3 so; one workgroup a CU, a prompt of 2048 31.8 and
+// 36.3).  More sequences: one after the other, the last tile first.
+template <int kRows, bool kPairs>
+__device__ __forceinline__ bool find_piece(const PackedArgs& a, int item, int lane, Piece& s) {
+    const int end = rows_end(a.cu_rows, a.batch, a.rows);
     int before = 0;
     for (int base = 0; base < a.batch; base += 64) {
         const int b = base + lane;
         // (both bounds and the last one on their way together)
-        const PackedRows r = packed_rows(a.cu_rows, min(b, a.batch - 1), rows_end(a.cu_rows, a.batch, a.rows));
+        const PackedRows r = packed_rows(a.cu_rows, min(b, a.batch - 1), end);
         const int count = b < a.batch ? (r.end - r.begin) * a.group : 0;
         const int tiles = (count + kRows - 1) / kRows;
+        const int upto = a.batch == 1 ? tiles : running_sum(tiles);
+        const int sum = a.batch == 1 ? __builtin_amdgcn_readfirstlane(tiles) : __builtin_amdgcn_readlane(upto, 63);
         int at = 0;
-        if (a.batch == 1) {
-            s.tile = __builtin_amdgcn_readfirstlane(tiles) - 1 - index;
-            if (s.tile < 0) return false;
-        } else {
-            const int upto = running_sum(tiles), sum = __builtin_amdgcn_readlane(upto, 63);
+        if (a.batch > 64) {
+            const int index = a.by_kv_heads(item);
             if (index >= before + sum) {
                 before += sum;
                 continue;
             }
-            if (a.batch > 64) {
-                at = __ffsll((unsigned long long)__ballot(before + upto > index)) - 1;
-                s.tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - index;
-            } else {
-                // more than `index` tiles have the place `low` in their sequence or a later one,
-                // `fewer`, and not more, the place `high`
-                int low = 0, high = (a.rows * a.group + kRows - 1) / kRows, fewer = 0;
-                while (high - low > 1) {
-                    const int mid = (low + high) / 2;
-                    const int from = __builtin_amdgcn_readlane(running_sum(max(tiles - mid, 0)), 63);
-                    if (from > index) low = mid;
-                    else high = mid, fewer = from;
-                }
-                s.tile = low;
+            s.kvh = item - index * a.kv_heads;
+            at = __ffsll((unsigned long long)__ballot(before + upto > index)) - 1;
+            s.tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - index;
+        } else {
+            constexpr int kCUs = 256;
+            const int all = sum * a.kv_heads, seconds = min(kCUs, all - kCUs);
+            if (item >= all) return false;
+            if (kPairs && item >= kCUs) item = item < kCUs + seconds ? all - 1 - (item - kCUs) : item - seconds;
+            const int index = a.by_kv_heads(item);
+            s.kvh = item - index * a.kv_heads;
+            // more than `index` tiles have the place `low` in their sequence or a later one,
+            // `fewer`, and not more, the place `high`
+            int low = a.batch == 1 ? sum - 1 - index : 0, high = a.batch == 1 ? 0 : (a.rows * a.group + kRows - 1) / kRows, fewer = 0;
+            while (high - low > 1) {
+                const int mid = (low + high) / 2;
+                const int from = __builtin_amdgcn_readlane(running_sum(max(tiles - mid, 0)), 63);
+                if (from > index) low = mid;
+                else high = mid, fewer = from;
+            }
+            s.tile = low;
+            if (a.batch > 1) {
                 const int has = tiles > low, rank = running_sum(has);  // (of all lanes)
                 at = __ffsll((unsigned long long)__ballot(has && rank == index - fewer + 1)) - 1;
             }
@@ -294,9 +305,7 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
                 *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
     }
     Piece s;
-    const int index = a.by_kv_heads((int)blockIdx.x);
-    s.kvh = (int)blockIdx.x - index * a.kv_heads;
-    if (!find_piece<kRows>(a, index, lane, s)) return;
+    if (!find_piece<kRows, 4 * T::kBytes <= 80 << 10 && kWaves == 4>(a, (int)blockIdx.x, lane, s)) return;
 
     const int part = wave % kSplit;  // of every tile's keys
     const int m0 = s.tile * kRows + kWaveRows * (wave / kSplit);

@@ -306,8 +306,14 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
     free_pages.tell(counts);
     __syncthreads();
     const int entries = a.batch * a.width;
+    const bool first = blockIdx.x == 0;
     each_entry(a, entries, [&](int b, int c, int length, int entry) {
-        if (c < pages_needed(length, a.page_shift) && !names_page(entry, a.pages)) atomicAdd(want + b, 1);
+        const bool named = names_page(entry, a.pages);
+        if (c < pages_needed(length, a.page_shift)) {
+            if (!named) atomicAdd(want + b, 1);
+        } else if (first && named) {
+            atomicAdd(given + entry, -1);
+        }
     });
     __syncthreads();
     // rows' wants before this wave's row, and all
@@ -319,11 +325,7 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
     }
     start = last_lane(running_sum(start)), wanted = last_lane(running_sum(wanted));
     const int free = min(free_pages.sum(counts), wanted);
-    if (blockIdx.x == 0) {
-        each_entry(a, entries, [&](int, int c, int length, int entry) {
-            if (c >= pages_needed(length, a.page_shift) && names_page(entry, a.pages)) atomicAdd(given + entry, -1);
-        });
-        __syncthreads();
+    if (first) {
 #pragma unroll
         for (int k = 0; k < Groups::kEach; ++k) {
             const Group& x = free_pages.x[k];
