@@ -6,12 +6,11 @@
 
 namespace w4g64 {
 
-// A sequence's rows, bounded by [0, rows_end()] whatever cu_rows holds.
+// A sequence's rows from its two bounds, within [0, rows_end()] whatever they are.
 struct PackedRows {
     int begin, end;
 };
-__host__ __device__ inline PackedRows packed_rows(const int32_t* cu_rows, int sequence, int rows) {
-    const int begin = cu_rows[sequence], end = cu_rows[sequence + 1];
+__host__ __device__ inline PackedRows packed_rows(int begin, int end, int rows) {
     PackedRows s;
     s.begin = begin < 0 ? 0 : (begin > rows ? rows : begin);
     s.end = end < s.begin ? s.begin : (end > rows ? rows : end);

@@ -97,59 +97,92 @@ struct Piece {
     int kvh;
 };
 
-// The piece of workgroup `item`.  Up to 64 sequences: tiles in the order of their keys'
+// The piece of workgroup `item`, up to 64 sequences: tiles in the order of their keys'
 // number, the most first (a tile's place in its sequence goes by it), so that no
 // workgroup begins a long one when the others are done; with kPairs, where a CU holds two
 // workgroups, the second one of each of the 256 CUs takes the shortest, as the longest
 // tiles are what a call waits for and two of them on a CU slow each other (eight prompts
 // of 1000 tokens 44.3 us in order, 41.3 so; one workgroup a CU, a prompt of 2048 31.8 and
-// 36.3).  More sequences: one after the other, the last tile first.
+// 36.3).
 template <int kRows, bool kPairs>
-__device__ __forceinline__ bool find_piece(const PackedArgs& a, int item, int lane, Piece& s) {
+__device__ __forceinline__ bool find_longest(const PackedArgs& a, int item, int lane, Piece& s) {
+    // (both bounds and the last one on their way together)
+    const int b = min(lane, a.batch - 1);
     const int end = rows_end(a.cu_rows, a.batch, a.rows);
-    int before = 0;
-    for (int base = 0; base < a.batch; base += 64) {
-        const int b = base + lane;
-        // (both bounds and the last one on their way together)
-        const PackedRows r = packed_rows(a.cu_rows, min(b, a.batch - 1), end);
-        const int count = b < a.batch ? (r.end - r.begin) * a.group : 0;
-        const int tiles = (count + kRows - 1) / kRows;
-        const int upto = a.batch == 1 ? tiles : running_sum(tiles);
-        const int sum = a.batch == 1 ? __builtin_amdgcn_readfirstlane(tiles) : __builtin_amdgcn_readlane(upto, 63);
-        int at = 0;
-        if (a.batch > 64) {
-            const int index = a.by_kv_heads(item);
-            if (index >= before + sum) {
-                before += sum;
-                continue;
-            }
-            s.kvh = item - index * a.kv_heads;
-            at = __ffsll((unsigned long long)__ballot(before + upto > index)) - 1;
-            s.tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - index;
-        } else {
-            constexpr int kCUs = 256;
-            const int all = sum * a.kv_heads, seconds = min(kCUs, all - kCUs);
-            if (item >= all) return false;
-            if (kPairs && item >= kCUs) item = item < kCUs + seconds ? all - 1 - (item - kCUs) : item - seconds;
-            const int index = a.by_kv_heads(item);
-            s.kvh = item - index * a.kv_heads;
-            // more than `index` tiles have the place `low` in their sequence or a later one,
-            // `fewer`, and not more, the place `high`
-            int low = a.batch == 1 ? sum - 1 - index : 0, high = a.batch == 1 ? 0 : (a.rows * a.group + kRows - 1) / kRows, fewer = 0;
-            while (high - low > 1) {
-                const int mid = (low + high) / 2;
-                const int from = __builtin_amdgcn_readlane(running_sum(max(tiles - mid, 0)), 63);
-                if (from > index) low = mid;
-                else high = mid, fewer = from;
-            }
-            s.tile = low;
-            if (a.batch > 1) {
-                const int has = tiles > low, rank = running_sum(has);  // (of all lanes)
-                at = __ffsll((unsigned long long)__ballot(has && rank == index - fewer + 1)) - 1;
-            }
+    const PackedRows r = packed_rows(a.cu_rows[b], a.cu_rows[b + 1], end);
+    const int count = lane < a.batch ? (r.end - r.begin) * a.group : 0;
+    const int tiles = (count + kRows - 1) / kRows;
+    const int sum = a.batch == 1 ? __builtin_amdgcn_readfirstlane(tiles) : __builtin_amdgcn_readlane(running_sum(tiles), 63);
+    constexpr int kCUs = 256;
+    const int all = sum * a.kv_heads, seconds = min(kCUs, all - kCUs);
+    if (item >= all) return false;
+    if (kPairs && item >= kCUs) item = item < kCUs + seconds ? all - 1 - (item - kCUs) : item - seconds;
+    const int index = a.by_kv_heads(item);
+    s.kvh = item - index * a.kv_heads;
+    int at = 0;
+    if (a.batch == 1) {
+        s.tile = sum - 1 - index;
+    } else {
+        // more than `index` tiles have the place `low` in their sequence or a later one,
+        // `fewer`, and not more, the place `high`
+        int low = 0, high = (a.rows * a.group + kRows - 1) / kRows, fewer = 0;
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            const int from = __builtin_amdgcn_readlane(running_sum(max(tiles - mid, 0)), 63);
+            if (from > index) low = mid;
+            else high = mid, fewer = from;
         }
-        s.begin = __builtin_amdgcn_readlane(r.begin, at);
-        s.count = __builtin_amdgcn_readlane(count, at);
+        s.tile = low;
+        const int has = tiles > low, rank = running_sum(has);  // (of all lanes)
+        at = __ffsll((unsigned long long)__ballot(has && rank == index - fewer + 1)) - 1;
+    }
+    s.begin = __builtin_amdgcn_readlane(r.begin, at);
+    s.count = __builtin_amdgcn_readlane(count, at);
+    return true;
+}
+
+// More sequences: one after the other, the last tile first; 256 are looked through at a
+// time, four of a lane.
+template <int kRows>
+__device__ __forceinline__ bool find_in_turn(const PackedArgs& a, int item, int lane, Piece& s) {
+    const int end = rows_end(a.cu_rows, a.batch, a.rows);
+    const int index = a.by_kv_heads(item);
+    s.kvh = item - index * a.kv_heads;
+    int before = 0, next[5];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) next[i] = a.cu_rows[min(base + 4 * lane + i, a.batch)];
+    };
+    load(0);
+    for (int base = 0; base < a.batch; base += 256) {
+        int bound[5], count[4], tiles[4];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) bound[i] = next[i];
+        load(base + 256);  // (its end over and over, past it)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const PackedRows r = packed_rows(bound[i], bound[i + 1], end);
+            bound[i] = r.begin, count[i] = base + 4 * lane + i < a.batch ? (r.end - r.begin) * a.group : 0;
+            tiles[i] = (count[i] + kRows - 1) / kRows;
+        }
+        const int mine = tiles[0] + tiles[1] + tiles[2] + tiles[3];
+        const int upto = running_sum(mine), sum = __builtin_amdgcn_readlane(upto, 63);
+        if (index >= before + sum) {
+            before += sum;
+            continue;
+        }
+        const int at = __ffsll((unsigned long long)__ballot(before + upto > index)) - 1;
+        int left = index - (before + __builtin_amdgcn_readlane(upto - mine, at));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int here = __builtin_amdgcn_readlane(tiles[i], at);
+            if (left >= 0 && left < here) {
+                s.begin = __builtin_amdgcn_readlane(bound[i], at);
+                s.count = __builtin_amdgcn_readlane(count[i], at);
+                s.tile = here - 1 - left;
+            }
+            left -= here;
+        }
         return true;
     }
     return false;
@@ -305,7 +338,9 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
                 *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
     }
     Piece s;
-    if (!find_piece<kRows, 4 * T::kBytes <= 80 << 10 && kWaves == 4>(a, (int)blockIdx.x, lane, s)) return;
+    constexpr bool kPairs = kWaves == 4 && 4 * T::kBytes <= 80 << 10;  // two workgroups a CU
+    if (a.batch <= 64 ? !find_longest<kRows, kPairs>(a, (int)blockIdx.x, lane, s) : !find_in_turn<kRows>(a, (int)blockIdx.x, lane, s))
+        return;
 
     const int part = wave % kSplit;  // of every tile's keys
     const int m0 = s.tile * kRows + kWaveRows * (wave / kSplit);

@@ -248,6 +248,8 @@ PROMPTS = [
     ([b % 97 for b in range(80)], {"heads": 16, "kv_heads": 16, "dim": 64, "dtype": F16}),
     ([(37 * b) % 150 for b in range(64)], {"heads": 12, "dim": 128}),
     ([1] * 200, {"heads": 6, "kv_heads": 2, "dim": 128}),
+    ([b % 4 for b in range(700)], {"heads": 2, "dim": 64}),
+    ([0] * 300 + [5, 130] + [0] * 250 + [1], {"heads": 8, "kv_heads": 2, "dim": 128, "dtype": F16}),
     ([1900, 600], {"heads": 40, "kv_heads": 8, "dim": 128, "dtype": F16}),
 ]
 

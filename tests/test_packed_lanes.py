@@ -151,6 +151,7 @@ PROMPTS = [
     ([33, 1, 5], 3, 3, 128, F16),
     ([140], 1, 1, 64, BF16),
     ([260], 40, 40, 128, F16),
+    ([1 + b % 2 for b in range(270)], 2, 1, 64, BF16),
 ]
 
 
