@@ -250,6 +250,8 @@ PROMPTS = [
     ([1] * 200, {"heads": 6, "kv_heads": 2, "dim": 128}),
     ([b % 4 for b in range(700)], {"heads": 2, "dim": 64}),
     ([0] * 300 + [5, 130] + [0] * 250 + [1], {"heads": 8, "kv_heads": 2, "dim": 128, "dtype": F16}),
+    ([3, 150], {"heads": 64, "kv_heads": 1, "dim": 64}),
+    ([90, 1], {"heads": 1, "kv_heads": 1, "dim": 128}),
     ([1900, 600], {"heads": 40, "kv_heads": 8, "dim": 128, "dtype": F16}),
 ]
 
@@ -551,7 +553,8 @@ def test_resize_of_strided_tables_and_of_nothing():
 @pytest.mark.parametrize("sizes, more", [(sizes, {}) for sizes in POOLS] + [
     ((20, 70, 700, 16), {"token_major": True}), ((20, 70, 700, 16), {"flat": True, "dtype": F16, "dim": 128}),
     ((6, 3, 40, 64), {"layers": 5, "heads": 3, "dim": 72, "token_major": True}), ((3, 600, 70000, 16), {"layers": 1, "heads": 1}),
-    ((1, 2, 9, 1024), {"heads": 8, "dim": 128})])
+    ((1, 2, 9, 1024), {"heads": 8, "dim": 128}), ((700, 2, 3000, 16), {"layers": 1, "dim": 8}),
+    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8})])
 def test_fork_is_the_definition(sizes, more, wild):
     batch, width, pages, page = sizes
     gen = torch.Generator().manual_seed(2)
@@ -578,7 +581,8 @@ def test_fork_is_the_definition(sizes, more, wild):
 @pytest.mark.parametrize("sizes, more", [(sizes, {}) for sizes in POOLS] + [
     ((20, 70, 700, 16), {"token_major": True}), ((20, 70, 700, 16), {"flat": True, "dtype": F16, "dim": 128}),
     ((6, 3, 40, 64), {"layers": 5, "heads": 3, "dim": 72, "token_major": True}), ((3, 600, 70000, 16), {"layers": 1, "heads": 1}),
-    ((1, 2, 9, 1024), {"heads": 8, "dim": 128})])
+    ((1, 2, 9, 1024), {"heads": 8, "dim": 128}), ((1100, 2, 3000, 16), {"layers": 1, "dim": 8}),
+    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8})])
 def test_compact_is_the_definition(sizes, more, wild):
     batch, width, pages, page = sizes
     for turn in range(6):
@@ -668,6 +672,51 @@ def test_page_operators_in_one_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(answers, want))
         assert torch.equal(p.k, pools[0]) and torch.equal(p.v, pools[1])
+
+
+@gpu
+def test_many_children_of_one_row():
+    """More of them than free pages: the last ones lack theirs."""
+    p = Pool(1, 2, 3, 1500, 16, layers=1, heads=1, dim=8)
+    p.table, p.lengths = [[0, 1, -1], [2, -1, -1]], [20, 16]
+    p.users = [1, 1, 1] + [0] * 1400 + [1] * 97
+    for children in (900, 1700):
+        parents = [0] * children + [1, 1]
+        k = p.k.clone()
+        got = paged_fork_hip(k, p.v.clone(), *p.indices(), ints(parents))
+        *want, copies = forked(p.table, p.lengths, p.users, parents, 16)
+        assert _lists(*got) == tuple(want) and sum(want[3]) == max(0, children - 1401)
+        for source, target, count in copies:
+            assert torch.equal(k[:, target, :, :count], p.k[:, source, :, :count])
+            assert torch.equal(k[:, target, :, count:], p.k[:, target, :, count:])
+
+
+@gpu
+def test_page_operators_on_other_streams_and_side_by_side():
+    """Keys and values in one buffer; calls on two streams at once; indices in strides."""
+    p = Pool(2, 20, 70, 700, 16, layers=3, token_major=True)
+    both = torch.stack((p.k, p.v), 1)
+    k, v = both.unbind(1)
+    table, lengths, users = p.indices()
+    parents = list(range(20)) + [3, 3, 7]
+    *want, copies = forked(p.table, p.lengths, p.users, parents, 16)
+    other = resized(p.table, [9] * 20, p.users, 16)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    wide = torch.stack((table, table), 2)[:, :, 1]
+    for stream in (a, b):
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(a):
+            got = paged_fork_hip(k, v, wide, lengths, users, ints(parents))
+        with torch.cuda.stream(b):
+            cut = paged_resize_hip(table, ints([9] * 20), users, page_size=16)
+            cut_too = paged_resize_hip(table.expand(1, 20, 70)[0], ints([9] * 20), users, page_size=16)
+        torch.cuda.synchronize()
+        assert _lists(*got) == tuple(want) and _lists(*cut) == other and _lists(*cut_too) == other
+    for source, target, count in copies:
+        assert torch.equal(both[:, :, target, :, :count], both[:, :, source, :, :count])
+    with torch.inference_mode():
+        assert _lists(*paged_resize_hip(table, ints([9] * 20), users, page_size=16)) == other
 
 
 @gpu
