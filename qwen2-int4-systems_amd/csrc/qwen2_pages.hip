@@ -6,8 +6,13 @@
 // ballots of a wave, whose bits are ranks within the group), the groups' counts are
 // summed up, and a second look at the pages writes the lists.
 //   few     one launch, every workgroup of which works all of that out for itself, in
-//           LDS, and then does its part of what follows: a launch costs a caller 3.6 us,
-//           more than the 64 KB that each workgroup reads at most;
+//           LDS, and then does its part of what follows: a launch costs a caller 3.6 us.
+//           Each goes through up to 64 KB of users and, but for a compaction, the old
+//           table (of a fork, the first one does).  us of a resize of empty rows, few /
+//           many, a call by itself (as part of a graph): 64 x 80 entries 7.4 / 12.7 (7.9 /
+//           8.6), 128 x 64 9.0 / 12.3 (9.5 / 8.7), 256 x 64 14.3 / 12.8 (15.0 / 8.9); of a
+//           fork to as many rows 128 x 64 8.7 / 14.1 (9.1 / 10.0), 192 x 64 12.4 / 14.1 (13.0
+//           / 9.9);
 //   many    one launch counts, one lists, one applies.
 // Answers go to new arrays: what a kernel reads nobody changes, and the only atomics
 // are whole numbers' sums, so that the same inputs give the same answer.  Keys and
@@ -31,7 +36,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kGroup = 256;              // pages counted together, by one wave
 constexpr int kFewPages = 1 << 14;
 constexpr int kFewRows = kThreads;       // (one of a thread)
-constexpr int kFewEntries = 1 << 15;
+constexpr int kFewResize = 1 << 13, kFewFork = 3 << 12;  // entries of the old table
 constexpr int64_t kMostPages = 1 << 24;  // (a workgroup sums up the counts before its own)
 constexpr int kMostCopyThreads = 256;
 
@@ -111,33 +116,6 @@ __device__ __forceinline__ void list_group(const Group& g, int group, int before
         const int rank = before + bits_before(g.free[i]);
         if (g.there[i] == 0 && rank < limit) list[rank] = group * kGroup + 64 * i + lane;
         before += __popcll(g.free[i]);
-    }
-}
-
-// Counts to sums before (in place, one workgroup); returns the sum of all.
-__device__ __forceinline__ int sum_groups(int32_t* counts, int groups, int* meet) {
-    int sum = 0;
-    for (int base = 0; base < groups; base += kThreads) {
-        const int g = base + (int)threadIdx.x;
-        int all;
-        const int before = block_before(g < groups ? counts[g] : 0, meet, all);
-        if (g < groups) counts[g] = sum + before;
-        sum += all;
-    }
-    __syncthreads();
-    return sum;
-}
-
-// The first `limit` free pages in order, by one workgroup, from the sums of
-// sum_groups().
-__device__ __forceinline__ void list_free(const int32_t* users, int pages, const int32_t* sums, int limit, int32_t* list) {
-    const int groups = (pages + kGroup - 1) / kGroup;
-    for (int g = wave_id(); g < groups; g += kWaves) {
-        const int before = sums[g];
-        if (before >= limit) break;
-        Group x;
-        x.load(users, pages, g);
-        list_group(x, g, before, limit, list);
     }
 }
 
@@ -502,12 +480,15 @@ struct ForkArgs {
     // many:
     int32_t* first;   // [batch]: a row's first child (children if it has none)
     int32_t* born;    // [batch]: how many it has
-    int32_t* target;  // [children]: the page of a child's copy, -1 if it has none, or -2 where one was wanted
+    int32_t* rank;    // [children]: of a child's copy among those of its kThreads children, -1 if it has none
+    int32_t* copies;  // [children / kThreads]
+    int32_t* free;    // [1]: free pages, no more than the list holds
     int32_t* counts;  // [groups]
     int32_t* list;    // [children]: free pages
     int64_t table_stride;
     int batch, children, width, pages, page_shift;
-    int row_blocks, old_blocks, copy_blocks;
+    int chunks;       // of 256 columns in a row
+    int list_blocks, row_blocks, old_blocks, copy_blocks;
     Divisor by_width;
 };
 
@@ -528,45 +509,26 @@ __device__ __forceinline__ Old old_row(const ForkArgs& a, int b) {
     return r;
 }
 
-__global__ __launch_bounds__(kThreads) void fork_count_kernel(ForkArgs a) {
-    const int g = (int)blockIdx.x * kWaves + wave_id();
-    if ((int64_t)g * kGroup >= a.pages) return;
-    Group x;
-    x.load(a.users, a.pages, g);
-    if (lane_id() == 0) a.counts[g] = x.count();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t p = (int64_t)g * kGroup + 64 * i + lane_id();
-        if (p < a.pages) a.new_users[p] = x.there[i];
-    }
-}
-
-// Row i of the answer (one wave), a copy of row `parent` (-1: none); `target`: as in
-// ForkArgs.
+// A chunk of row i of the answer, columns from c0 (one wave), a copy of row `parent` (-1:
+// none); `target`: the page of its copy, -1 if it has none, -2 where none was free.
 template <bool kCount>
-__device__ __forceinline__ void fork_row(const ForkArgs& a, int i, int parent, int length, int target) {
+__device__ __forceinline__ void fork_chunk(const ForkArgs& a, int i, int c0, int parent, int length, int target) {
     const int upto = pages_wanted(length, a.page_shift, a.width);
     const int column = length >> a.page_shift;  // (where there is a copy)
     const int32_t* row = a.table + max(parent, 0) * a.table_stride;
-    for (int c0 = 0; c0 < a.width; c0 += 256) {
-        int entry[4];
+    Columns x;
+    x.load(row, c0, upto);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int c = c0 + 64 * k + lane_id();
-            entry[k] = c < upto ? row[c] : -1;
+    for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 64 * k + lane_id();
+        int e = names_page(x.entry[k], a.pages) ? x.entry[k] : -1;
+        if (target != -1 && c == column) {
+            e = target < 0 ? -1 : target;
+            if (kCount && e >= 0) atomicAdd(a.new_users + e, 1);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int c = c0 + 64 * k + lane_id();
-            int e = names_page(entry[k], a.pages) ? entry[k] : -1;
-            if (target != -1 && c == column) {
-                e = target < 0 ? -1 : target;
-                if (kCount && e >= 0) atomicAdd(a.new_users + e, 1);
-            }
-            if (c < a.width) a.new_table[(int64_t)i * a.width + c] = e;
-        }
+        if (c < a.width) a.new_table[(int64_t)i * a.width + c] = e;
     }
-    if (lane_id() == 0) {
+    if (c0 == 0 && lane_id() == 0) {
         a.new_lengths[i] = length;
         a.missing[i] = target == -2;
     }
@@ -632,8 +594,8 @@ __global__ __launch_bounds__(kThreads) void fork_few_kernel(ForkArgs a) {
     }
     __syncthreads();
     if (--block < a.row_blocks) {
-        const int i = block * kWaves + wave_id();
-        if (i < a.children) fork_row<false>(a, i, parent[i], length[i], target[i]);
+        const int item = block * kWaves + wave_id(), i = item / a.chunks;
+        if (i < a.children) fork_chunk<false>(a, i, 256 * (item - i * a.chunks), parent[i], length[i], target[i]);
         return;
     }
     each_copy(a.pool, (int64_t)free * 2 * a.pool.layers, block - a.row_blocks, a.copy_blocks, [&](int r, int which, int layer) {
@@ -641,73 +603,119 @@ __global__ __launch_bounds__(kThreads) void fork_few_kernel(ForkArgs a) {
     });
 }
 
-// Many.  One workgroup: who copies, and to which page.
-__global__ __launch_bounds__(kThreads) void fork_plan_kernel(ForkArgs a) {
-    __shared__ int meet[kWaves];
-    const int tid = (int)threadIdx.x;
+// Many.  Rows' children by the first workgroup, pages' counts by the others.
+__global__ __launch_bounds__(kThreads) void fork_count_kernel(ForkArgs a) {
+    const int tid = (int)threadIdx.x, lane = lane_id();
+    if (blockIdx.x > 0) {
+        const int g = ((int)blockIdx.x - 1) * kWaves + wave_id();
+        if ((int64_t)g * kGroup >= a.pages) return;
+        Group x;
+        x.load(a.users, a.pages, g);
+        if (lane == 0) a.counts[g] = x.count();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t p = (int64_t)g * kGroup + 64 * i + lane;
+            if (p < a.pages) a.new_users[p] = x.there[i];
+        }
+        return;
+    }
     for (int b = tid; b < a.batch; b += kThreads) a.first[b] = a.children, a.born[b] = 0;
     __syncthreads();
-    for (int i = tid; i < a.children; i += kThreads) {
-        const int parent = a.parents[i];
-        if (parent < 0 || parent >= a.batch) continue;
-        atomicMin(a.first + parent, i);
-        atomicAdd(a.born + parent, 1);
-    }
-    __syncthreads();
-    int copies = 0;
-    for (int base = 0; base < a.children; base += kThreads) {
-        const int i = base + tid;
-        bool copy = false;
-        if (i < a.children) {
-            const int parent = a.parents[i];
-            if (parent >= 0 && parent < a.batch) {
-                const Old from = old_row(a, parent);
-                copy = from.column >= 0 &&
-                       (__hip_atomic_load(a.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != i || !from.sole);
+    for (int base = 0; base < a.children; base += 8 * kThreads) {
+        int parent[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = base + k * kThreads + tid;
+            parent[k] = i < a.children ? a.parents[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool there = parent[k] >= 0 && parent[k] < a.batch;
+            const uint64_t all = __ballot(there);
+            if (!all) continue;
+            // (children of one row side by side go as one: 100000 of one row take 2800 us otherwise)
+            const int head = __ffsll((unsigned long long)all) - 1;
+            const bool alike = __ballot(there && parent[k] != __builtin_amdgcn_readlane(parent[k], head)) == 0;
+            if (alike ? lane == head : there) {
+                atomicMin(a.first + parent[k], base + k * kThreads + tid);
+                atomicAdd(a.born + parent[k], alike ? __popcll(all) : 1);
             }
         }
-        int all;
-        const int rank = copies + block_before(copy, meet, all);
-        if (i < a.children) a.target[i] = copy ? rank : -1;
-        copies += all;
-    }
-    const int free = min(sum_groups(a.counts, (a.pages + kGroup - 1) / kGroup, meet), copies);
-    list_free(a.users, a.pages, a.counts, free, a.list);
-    __syncthreads();
-    for (int i = tid; i < a.children; i += kThreads) {
-        const int rank = a.target[i];
-        if (rank >= 0) a.target[i] = rank < free ? a.list[rank] : -2;
     }
 }
 
-// Workgroups of three kinds: new rows, one wave each; old rows' users, one wave each;
-// copies.
-__global__ __launch_bounds__(kThreads) void fork_apply_kernel(ForkArgs a) {
-    const int block = (int)blockIdx.x;
-    if (block < a.row_blocks) {
-        const int i = block * kWaves + wave_id();
-        if (i >= a.children) return;
-        const int parent = a.parents[i];
-        const bool there = parent >= 0 && parent < a.batch;
-        fork_row<true>(a, i, there ? parent : -1, there ? max(a.lengths[parent], 0) : 0, a.target[i]);
+// Which children copy, and the free pages in order (as many as there are children).
+__global__ __launch_bounds__(kThreads) void fork_list_kernel(ForkArgs a) {
+    __shared__ int meet[kWaves];
+    const int groups = (a.pages + kGroup - 1) / kGroup;
+    if ((int)blockIdx.x < a.list_blocks) {
+        const int first = (int)blockIdx.x * kWaves, g = first + wave_id();
+        int before = sum_of(a.counts, first, meet);
+        if (before >= a.children || g >= groups) return;
+        before += sum_between(a.counts, first, g);
+        Group x;
+        x.load(a.users, a.pages, g);
+        list_group(x, g, before, a.children, a.list);
         return;
     }
+    const int block = (int)blockIdx.x - a.list_blocks, i = block * kThreads + (int)threadIdx.x;
+    bool copy = false;
+    if (i < a.children) {
+        const int parent = a.parents[i];
+        if (parent >= 0 && parent < a.batch) {
+            const Old from = old_row(a, parent);
+            copy = from.column >= 0 && (a.first[parent] != i || !from.sole);
+        }
+    }
+    int copies;
+    const int rank = block_rank(copy, meet, copies);
+    if (i < a.children) a.rank[i] = copy ? rank : -1;
+    if (threadIdx.x == 0) a.copies[block] = copies;
+    if (block == 0) {
+        const int free = sum_of(a.counts, groups, meet);
+        if (threadIdx.x == 0) *a.free = min(free, a.children);
+    }
+}
+
+// The page of child i's copy, as fork_chunk() takes it (one wave).
+__device__ __forceinline__ int target_of(const ForkArgs& a, int i) {
+    const int mine = a.rank[i], free = *a.free;
+    if (mine < 0) return -1;
+    int before = 0;
+    for (int b = lane_id(); b < i / kThreads; b += 64) before += a.copies[b];
+    const int rank = last_lane(running_sum(before)) + mine;
+    return rank < free ? a.list[rank] : -2;
+}
+
+// Workgroups of three kinds: new rows, a chunk a wave; old rows' users, so too; copies.
+__global__ __launch_bounds__(kThreads) void fork_apply_kernel(ForkArgs a) {
+    const int block = (int)blockIdx.x;
     if (block < a.row_blocks + a.old_blocks) {
-        const int b = (block - a.row_blocks) * kWaves + wave_id();
-        if (b >= a.batch) return;
-        const int born = a.born[b];
-        const Old old = old_row(a, b);
+        const int item = (block < a.row_blocks ? block : block - a.row_blocks) * kWaves + wave_id();
+        const int i = item / a.chunks, c0 = 256 * (item - i * a.chunks);
+        if (block < a.row_blocks) {
+            if (i >= a.children) return;
+            const int parent = a.parents[i];
+            const bool there = parent >= 0 && parent < a.batch;
+            fork_chunk<true>(a, i, c0, there ? parent : -1, there ? max(a.lengths[parent], 0) : 0, target_of(a, i));
+            return;
+        }
+        if (i >= a.batch) return;
+        Columns x;
+        x.load(a.table + i * a.table_stride, c0, a.width);
+        const int born = a.born[i];
+        const Old old = old_row(a, i);
         const int upto = pages_wanted(old.length, a.page_shift, a.width);
-        for (int c = lane_id(); c < a.width; c += 64) {
-            const int e = a.table[b * a.table_stride + c];
-            const int by = fork_change(c, upto, old.column, born, old.sole && born > 0);
-            if (by && names_page(e, a.pages)) atomicAdd(a.new_users + e, by);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int by = fork_change(c0 + 64 * k + lane_id(), upto, old.column, born, old.sole && born > 0);
+            if (by && names_page(x.entry[k], a.pages)) atomicAdd(a.new_users + x.entry[k], by);
         }
         return;
     }
     each_copy(a.pool, (int64_t)a.children * 2 * a.pool.layers, block - a.row_blocks - a.old_blocks, a.copy_blocks,
               [&](int i, int which, int layer) {
-                  const int target = a.target[i];
+                  const int target = target_of(a, i);
                   if (target < 0) return;
                   const int parent = a.parents[i], length = a.lengths[parent];
                   copy_page(a.pool, which, layer, a.table[parent * a.table_stride + (length >> a.page_shift)], target,
@@ -835,9 +843,9 @@ __global__ __launch_bounds__(kThreads, 8) void compact_few_kernel(CompactArgs a)
         return;
     }
     if (--block < a.table_blocks) {
-        const int at = block * kThreads + tid;
-        if (at >= a.batch * a.width) return;
-        const int b = a.by_width(at), e = a.table[b * a.table_stride + (at - b * a.width)];
+        const int64_t at = (int64_t)block * kThreads + tid;
+        if (at >= (int64_t)a.batch * a.width) return;
+        const int b = a.by_width((int)at), e = a.table[b * a.table_stride + ((int)at - b * a.width)];
         a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
         return;
     }
@@ -963,9 +971,9 @@ int launched(const char* op) {
 
 int64_t most_given(int64_t batch, int64_t width, int64_t pages) { return batch * width < pages ? batch * width : pages; }
 
-// Whether a call's sizes are few (rows: all there are).
-bool few(int64_t rows, int64_t width, int64_t pages) {
-    return rows <= kFewRows && rows * width <= kFewEntries && pages <= kFewPages;
+// Whether a resize's or fork's sizes are few; a compaction's are where the pages are.
+bool few(int64_t rows, int64_t width, int64_t pages, int64_t entries) {
+    return rows <= kFewRows && rows * width <= entries && pages <= kFewPages;
 }
 // Workgroups for `items` copies at most: two a CU, or as many as have something to do.
 int copy_blocks(const Pool& pool, int64_t items) {
@@ -982,7 +990,7 @@ extern "C" {
 
 int64_t qwen2_paged_resize_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages) {
     if (check_sizes("paged_resize", batch, table_width, num_pages)) return 0;
-    return few(batch, table_width, num_pages) ? 0
+    return few(batch, table_width, num_pages, kFewResize) ? 0
                                               : 4 * (2 * batch + 1 + groups_of(num_pages) + most_given(batch, table_width, num_pages));
 }
 
@@ -1004,7 +1012,7 @@ int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const in
     a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)num_pages, a.page_shift = shift_of(page_size);
     a.by_width = divisor(table_width);
     const hipStream_t s = (hipStream_t)stream;
-    if (few(batch, table_width, num_pages)) {
+    if (few(batch, table_width, num_pages, kFewResize)) {
         hipLaunchKernelGGL(resize_few_kernel, dim3((unsigned)(1 + blocks_of(batch, kWaves))), dim3(kThreads), 0, s, a);
         return launched("paged_resize");
     }
@@ -1023,8 +1031,8 @@ int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const in
 
 int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t table_width, int64_t num_pages) {
     if (batch < 0 || children < 0 || table_width <= 0 || num_pages <= 0) return 0;
-    if (few(batch, table_width, num_pages) && few(children, table_width, num_pages)) return 0;
-    return 4 * (2 * batch + 2 * children + groups_of(num_pages));
+    if (few(batch, table_width, num_pages, kFewFork) && children <= kFewRows) return 0;
+    return 4 * (2 * batch + 2 * children + blocks_of(children, kThreads) + 1 + groups_of(num_pages));
 }
 
 int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int64_t table_stride, const int32_t* lengths,
@@ -1047,26 +1055,27 @@ int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int
     a.new_table = new_table, a.new_lengths = new_lengths, a.new_users = new_users, a.missing = missing;
     a.batch = (int)batch, a.children = (int)children, a.width = (int)table_width, a.pages = (int)pool->num_pages;
     a.page_shift = shift_of(pool->page_size), a.by_width = divisor(table_width);
+    a.chunks = (int)blocks_of(table_width, 256);
+    a.row_blocks = (int)blocks_of(children * a.chunks, kWaves), a.old_blocks = (int)blocks_of(batch * a.chunks, kWaves);
+    a.copy_blocks = copy_blocks(a.pool, copies);
     const hipStream_t s = (hipStream_t)stream;
-    if (few(batch, table_width, pool->num_pages) && few(children, table_width, pool->num_pages)) {
-        a.row_blocks = (int)blocks_of(children, kWaves);
-        a.copy_blocks = copy_blocks(a.pool, copies);
+    if (few(batch, table_width, pool->num_pages, kFewFork) && children <= kFewRows) {
         hipLaunchKernelGGL(fork_few_kernel, dim3((unsigned)(1 + a.row_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);
         return launched("paged_fork");
     }
-    a.first = (int32_t*)workspace, a.born = a.first + batch, a.target = a.born + batch, a.list = a.target + children;
-    a.counts = a.list + children;
-    hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)blocks_of(groups_of(pool->num_pages), kWaves)), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kThreads), 0, s, a);
-    a.row_blocks = (int)blocks_of(children, kWaves), a.old_blocks = (int)blocks_of(batch, kWaves);
-    a.copy_blocks = copy_blocks(a.pool, copies);
+    const int64_t child_blocks = blocks_of(children, kThreads);
+    a.list_blocks = (int)blocks_of(groups_of(pool->num_pages), kWaves);
+    a.first = (int32_t*)workspace, a.born = a.first + batch, a.rank = a.born + batch, a.list = a.rank + children;
+    a.copies = a.list + children, a.free = a.copies + child_blocks, a.counts = a.free + 1;
+    hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)(1 + a.list_blocks)), dim3(kThreads), 0, s, a);
+    if (children) hipLaunchKernelGGL(fork_list_kernel, dim3((unsigned)(a.list_blocks + child_blocks)), dim3(kThreads), 0, s, a);
     const int64_t blocks = a.row_blocks + a.old_blocks + a.copy_blocks;
     if (blocks) hipLaunchKernelGGL(fork_apply_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     return launched("paged_fork");
 }
 
 int64_t qwen2_paged_compact_workspace_bytes(int64_t batch, int64_t table_width, int64_t num_pages) {
-    if (batch < 0 || table_width <= 0 || num_pages <= 0 || few(batch, table_width, num_pages)) return 0;
+    if (batch < 0 || table_width <= 0 || num_pages <= kFewPages) return 0;
     return 4 * (num_pages + groups_of(num_pages) + 2 * (num_pages / 2) + 1);
 }
 
@@ -1087,7 +1096,7 @@ int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, 
     a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)pages, a.by_width = divisor(table_width);
     const hipStream_t s = (hipStream_t)stream;
     const int64_t most = pages / 2 * 2 * pool->layers;  // copies that there can be
-    if (few(batch, table_width, pages)) {
+    if (pages <= kFewPages) {
         a.table_blocks = (int)blocks_of(batch * table_width, kThreads);
         a.copy_blocks = copy_blocks(a.pool, most);
         hipLaunchKernelGGL(compact_few_kernel, dim3((unsigned)(1 + a.table_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);

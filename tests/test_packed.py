@@ -582,7 +582,7 @@ def test_fork_is_the_definition(sizes, more, wild):
     ((20, 70, 700, 16), {"token_major": True}), ((20, 70, 700, 16), {"flat": True, "dtype": F16, "dim": 128}),
     ((6, 3, 40, 64), {"layers": 5, "heads": 3, "dim": 72, "token_major": True}), ((3, 600, 70000, 16), {"layers": 1, "heads": 1}),
     ((1, 2, 9, 1024), {"heads": 8, "dim": 128}), ((1100, 2, 3000, 16), {"layers": 1, "dim": 8}),
-    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8})])
+    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8}), ((1100, 2, 17000, 16), {"layers": 1, "heads": 1, "dim": 8})])
 def test_compact_is_the_definition(sizes, more, wild):
     batch, width, pages, page = sizes
     for turn in range(6):
@@ -689,6 +689,28 @@ def test_many_children_of_one_row():
         for source, target, count in copies:
             assert torch.equal(k[:, target, :, :count], p.k[:, source, :, :count])
             assert torch.equal(k[:, target, :, count:], p.k[:, target, :, count:])
+
+
+@gpu
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("batch, width, pages", [(50, 4, 2000), (1500, 3, 6000), (3, 300, 40000)])
+def test_more_children_than_a_workgroup_has_threads(batch, width, pages, spare):
+    """Copies are counted by parts of the children; without spare pages some find none."""
+    page = 16
+    p = Pool(8, batch, width, pages, page, layers=1, heads=1, dim=8, spare=spare and pages // 4)
+    table, lengths, users = p.indices()
+    gen = torch.Generator().manual_seed(4)
+    for parents in (torch.randint(-1, batch + 1, (5000,), generator=gen).tolist(), [batch - 1] * 2049,
+                    [i // 3 if i % 64 else -1 for i in range(3 * batch)]):
+        want_k, want_v = p.k.clone(), p.v.clone()
+        k, v = p.k.clone(), p.v.clone()
+        got = paged_fork_hip(k, v, table, lengths, users, ints(parents))
+        *want, copies = forked(p.table, p.lengths, p.users, parents, page)
+        assert _lists(*got) == tuple(want)
+        for source, target, count in copies:
+            want_k[:, target, :, :count] = want_k[:, source, :, :count]
+            want_v[:, target, :, :count] = want_v[:, source, :, :count]
+        assert torch.equal(k, want_k) and torch.equal(v, want_v)
 
 
 @gpu

@@ -371,7 +371,26 @@ def _many(kernels, name):
     assert torch.equal(k[:, to[moved]], want_k[:, moved])
 
 
-CHECKS = {"prompts": _prompts, "bounds": _bounds, "resize": _resize, "fork": _fork, "compact": _compact, "many": _many}
+def _children(kernels, name):
+    """Children by several workgroups; a row of several chunks."""
+    for seed, (batch, width, pages, page) in enumerate([(5, 3, 1500, 16), (3, 600, 17000, 16)]):
+        table, lengths, users = state_of(seed, batch, width, pages, page, spare=9, wild=seed == 0)
+        gen = torch.Generator().manual_seed(seed)
+        for parents in (torch.randint(-1, batch + 1, (1100 if seed == 0 else 40,), generator=gen).tolist(), [1] * 1030, []):
+            if seed and len(parents) > 100:
+                continue
+            k, v = _pages_of(kernels, pages, page, seed, layers=1, heads=1)
+            want_k = k.clone()
+            got = kernels.fork(k, v, kernels.ints(table), kernels.ints(lengths), kernels.ints(users), kernels.ints(parents))
+            *want, copies = forked(table, lengths, users, parents, page)
+            assert _lists(*got) == tuple(want)
+            for source, target, count in copies:
+                want_k[:, target, :, :count] = want_k[:, source, :, :count]
+            assert torch.equal(k, want_k)
+
+
+CHECKS = {"prompts": _prompts, "bounds": _bounds, "resize": _resize, "fork": _fork, "compact": _compact, "many": _many,
+          "children": _children}
 
 
 @pytest.mark.parametrize("side", ["end", "start"])
