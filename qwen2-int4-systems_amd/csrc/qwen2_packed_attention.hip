@@ -345,7 +345,8 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
     const int part = wave % kSplit;  // of every tile's keys
     const int m0 = s.tile * kRows + kWaveRows * (wave / kSplit);
     // the wave's rows, then the workgroup's (rows past the last one are that one again)
-    const int least = a.by_group(min(m0, s.count - 1)), most = a.by_group(min(m0 + kWaveRows, s.count) - 1);
+    const int least = a.by_group(min(m0, s.count - 1));
+    const int most = m0 < s.count ? a.by_group(min(m0 + kWaveRows, s.count) - 1) : -1;  // (a wave without rows has no keys)
     const int all_most = a.by_group(min((s.tile + 1) * kRows, s.count) - 1);
     const int tiles = all_most / kKeys + 1;
 
@@ -564,35 +565,40 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 && kSplit == 4 && D == 128
 }
 
 // The forms of a call's workgroups.
-enum Form { kLong, kSplit2, kSplit4, kSplit4Tall };
+enum Form { kShort, kLong, kSplit2, kSplit4, kSplit4Tall };
 int tile_rows(Form f) { return f == kLong ? 128 : f == kSplit4 ? 32 : 64; }
 
 template <class E, int D>
 hipError_t launch_packed_attention(const PackedArgs& a, Form form, int64_t workgroups, hipStream_t stream) {
     const dim3 grid((unsigned)workgroups);
-    if (form == kLong) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 1, 2>), grid, dim3(256), 0, stream, a);
+    if (form == kShort) hipLaunchKernelGGL((packed_attention_kernel<E, D, 2, 1, 1>), grid, dim3(128), 0, stream, a);
+    else if (form == kLong) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 1, 2>), grid, dim3(256), 0, stream, a);
     else if (form == kSplit2) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 2, 1>), grid, dim3(256), 0, stream, a);
     else if (form == kSplit4) hipLaunchKernelGGL((packed_attention_kernel<E, D, 4, 4, 1>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((packed_attention_kernel<E, D, 8, 4, 1>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
 }
 
-// The form of a call.  A workgroup's time is that of its keys one tile after the other,
-// so long as the chip holds all of them at once; then what counts is the products'
-// rate, which the fewest waves per row give.  us a call, kLong / kSplit2 / kSplit4 /
-// kSplit4Tall, 12/2 heads of 128: one prompt of 37 tokens 7.1 / 6.7 / 7.3 / 8.5, 512 15.3 /
-// 12.3 / 11.1 / 12.1, 1024 24.6 / 19.2 / 19.6 / 17.3, 2048 43 / 34 / 50 / 30, 3000 62 / 50 /
-// 94 / 58, 16384 795 / 908 / 1991 / 1019; four of 512 16.9 / 15.5 / 28 / 21, eight 20 / 24 / 54 / 33;
-// 16/16 heads of 64: eight of 60 5.2 / 5.6 / 5.8 / 6.6, one of 1000 17.1 / 13.4 / 10.6 / 11.8, two 18.4 /
-// 15.4 / 19.5 / 18.1.  The lengths are on the GPU: it goes by the sequences' average.
+// The form of a call.  Prompts of a tile or two want small workgroups, of which a CU holds
+// many (kShort, tiles of 32 keys).  A longer one's time is that of its keys one tile
+// after the other, so long as the chip holds all workgroups at once; then what counts is
+// the products' rate, which the fewest waves per row give.  The lengths are on the GPU: it
+// goes by the sequences' average.
+// us a call, 12/2 heads of 128, kShort / best of the others: one prompt of 16 tokens
+// 5.3 / 6.7, 64 6.1 / 7.1, 128 7.4 / 7.6, 256 10.1 / 8.7; 96 of 10 6.1 / 6.8; sixteen of
+// 128 10.4 / 11.3, 200 13.2 / 14.1, 300 17.6 / 17.6; 32 of 200 20.4 / 23.6, 500 55.9 /
+// 50.4; 16/16 heads of 64, 200 of 30 15.4 / 21.7; four of 200 7.6 / 7.1, 16 of 200 10.4 / 11.7; one
+// prompt of 2000 among 40 of 16 tokens, on the other hand, 49 / 33.
+// kLong / kSplit2 / kSplit4 / kSplit4Tall: one of 512 15.3 / 12.3 / 11.1 / 12.1, 1024 24.6 / 19.2 /
+// 19.6 / 17.3, 2048 43 / 34 / 50 / 30, 3000 62 / 50 / 94 / 58, 16384 795 / 908 / 1991 / 1019;
+// four of 512 16.9 / 15.5 / 28 / 21, eight 20 / 24 / 54 / 33; 16/16 heads of 64: one of 1000 17.1 /
+// 13.4 / 10.6 / 11.8, two 18.4 / 15.4 / 19.5 / 18.1.
 Form form_of(int64_t rows, int64_t sequences, int64_t group, int64_t kv_heads, int64_t head_dim) {
     const int64_t usual = rows / sequences, few = head_dim == 128 ? 288 : 576, half = head_dim == 128 ? 256 : 512;
     auto tiles = [&](int64_t size) { return sequences * ((usual * group + size - 1) / size) * kv_heads; };
-    if (usual * group <= 64) return kLong;  // (a smaller tile would hold the same rows)
-    if (usual > 128) {
-        if (tiles(32) <= few) return kSplit4;
-        if (tiles(64) <= 256 || (tiles(64) <= half * 3 / 2 && usual >= 1024)) return kSplit4Tall;
-    }
+    if (usual <= 128 || (usual <= 256 && tiles(64) > 512)) return kShort;
+    if (tiles(32) <= few) return kSplit4;
+    if (tiles(64) <= 256 || (tiles(64) <= half * 3 / 2 && usual >= 1024)) return kSplit4Tall;
     return tiles(64) <= 512 || (tiles(64) <= 800 && usual >= 2048) ? kSplit2 : kLong;
 }
 

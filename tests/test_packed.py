@@ -253,6 +253,9 @@ PROMPTS = [
     ([3, 150], {"heads": 64, "kv_heads": 1, "dim": 64}),
     ([90, 1], {"heads": 1, "kv_heads": 1, "dim": 128}),
     ([1900, 600], {"heads": 40, "kv_heads": 8, "dim": 128, "dtype": F16}),
+    ([30 + 3 * b for b in range(66)], {"heads": 12, "dim": 128}),
+    ([260] * 40, {"heads": 12, "dim": 64}),
+    ([1200] + [20] * 30, {"heads": 8, "kv_heads": 1, "dim": 128}),
 ]
 
 
@@ -314,7 +317,7 @@ def test_rows_behind_the_last_sequence(lengths):
 @gpu
 @pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 64)])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("lengths, heads", [([20, 30], 4), ([5, 400, 70], 4), ([300], 40), ([130] * 30, 12)])
+@pytest.mark.parametrize("lengths, heads", [([20, 30], 4), ([5, 400, 70], 4), ([300], 40), ([130] * 30, 12), ([290] * 30, 12)])
 def test_values_that_are_not_finite(dtype, dim, bad, lengths, heads):
     """Whole values at one position: the rows before it and the other sequences are
     unmoved, those from it on are what the formula says; then one element alone, then two

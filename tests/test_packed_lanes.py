@@ -155,9 +155,14 @@ PROMPTS = [
 ]
 
 
-def _prompts(kernels, name):
-    for lengths, heads, kv_heads, dim, dtype in PROMPTS:
-        q, k, v, cu = args = _packed(kernels, lengths, heads, kv_heads, dim, dtype, tail=2)
+def _forms(kernels, name):
+    """Prompts that only the rows behind them make long ones of many tiles."""
+    _prompts(kernels, name, [([131, 90], 8, 8, 128, F16, 600), ([131, 90], 8, 8, 128, F16, 1900), ([150], 2, 1, 64, BF16, 17000)])
+
+
+def _prompts(kernels, name, prompts=[(*case, 2) for case in PROMPTS]):
+    for lengths, heads, kv_heads, dim, dtype, tail in prompts:
+        q, k, v, cu = args = _packed(kernels, lengths, heads, kv_heads, dim, dtype, tail)
         out = kernels.attention(*args)
         # (a half step of the output and of each probability, values of a few units)
         assert float((out.double() - formula(*args)).abs().amax()) < 4 * torch.finfo(dtype).eps, (lengths, dim)
@@ -390,7 +395,7 @@ def _children(kernels, name):
 
 
 CHECKS = {"prompts": _prompts, "bounds": _bounds, "resize": _resize, "fork": _fork, "compact": _compact, "many": _many,
-          "children": _children}
+          "children": _children, "forms": _forms}
 
 
 @pytest.mark.parametrize("side", ["end", "start"])
