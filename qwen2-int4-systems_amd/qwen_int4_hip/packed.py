@@ -33,8 +33,9 @@ def packed_attention_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_r
     ``scale`` is head_dim ** -0.5 unless given.
 
     Keys and values that a row does not see take no part, whatever they hold; an
-    infinity or NaN that it sees reaches it, however small the key's weight (such rows
-    take some ten times as long).  Rows behind the last sequence are left as they are in
+    infinity or NaN that it sees reaches it, however small the key's weight (a call full
+    of such rows takes three to seventeen times as long: 23 us instead of 6.5 for 37
+    tokens, 400 instead of 42 for eight prompts of 1000).  Rows behind the last sequence are left as they are in
     ``out``, and zeros in a new tensor.  Scores, softmax and sums are fp32, in a fixed
     order: the same inputs give the same bits.  A probability is rounded once to the
     tensors' type before it meets its value, and the sum that divides is the rounded
