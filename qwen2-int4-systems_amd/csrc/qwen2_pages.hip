@@ -29,6 +29,8 @@
 // used; what names no page is left out.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "qwen2_decode.h"
 #include "qwen2_paged_device.h"
 #include "qwen2_pages.h"
@@ -849,10 +851,10 @@ __global__ __launch_bounds__(kThreads, 8) void compact_few_kernel(CompactArgs a)
         return;
     }
     if (--block < a.table_blocks) {
-        const int64_t at = (int64_t)block * kThreads + tid;
-        if (at >= (int64_t)a.batch * a.width) return;
-        const int b = a.by_width((int)at), e = a.table[b * a.table_stride + ((int)at - b * a.width)];
-        a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
+        for (int64_t at = (int64_t)block * kThreads + tid; at < (int64_t)a.batch * a.width; at += (int64_t)a.table_blocks * kThreads) {
+            const int b = a.by_width((int)at), e = a.table[b * a.table_stride + ((int)at - b * a.width)];
+            a.new_table[at] = names_page(e, a.pages) ? place(e) : -1;
+        }
         return;
     }
     each_copy(a.pool, (int64_t)low * 2 * a.pool.layers, block - a.table_blocks, a.copy_blocks, [&](int r, int which, int layer) {
@@ -981,6 +983,10 @@ int64_t most_given(int64_t batch, int64_t width, int64_t pages) { return batch *
 bool few(int64_t rows, int64_t width, int64_t pages, int64_t entries) {
     return rows <= kFewRows && rows * width <= entries && pages <= kFewPages;
 }
+// (and a fork's new rows keep no more workgroups busy than run at once: each plans)
+bool few_fork(int64_t batch, int64_t children, int64_t width, int64_t pages) {
+    return few(batch, width, pages, kFewFork) && children <= kFewRows && children * blocks_of(width, 256) <= 256 * kWaves;
+}
 // Workgroups for `items` copies at most: two a CU, or as many as have something to do.
 int copy_blocks(const Pool& pool, int64_t items) {
     const int64_t blocks = blocks_of(items, kThreads / pool.threads);
@@ -1037,7 +1043,7 @@ int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const in
 
 int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t table_width, int64_t num_pages) {
     if (batch < 0 || children < 0 || table_width <= 0 || num_pages <= 0) return 0;
-    if (few(batch, table_width, num_pages, kFewFork) && children <= kFewRows) return 0;
+    if (few_fork(batch, children, table_width, num_pages)) return 0;
     return 4 * (2 * batch + 2 * children + blocks_of(children, kThreads) + 1 + groups_of(num_pages));
 }
 
@@ -1065,7 +1071,7 @@ int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int
     a.row_blocks = (int)blocks_of(children * a.chunks, kWaves), a.old_blocks = (int)blocks_of(batch * a.chunks, kWaves);
     a.copy_blocks = copy_blocks(a.pool, copies);
     const hipStream_t s = (hipStream_t)stream;
-    if (few(batch, table_width, pool->num_pages, kFewFork) && children <= kFewRows) {
+    if (few_fork(batch, children, table_width, pool->num_pages)) {
         hipLaunchKernelGGL(fork_few_kernel, dim3((unsigned)(1 + a.row_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);
         return launched("paged_fork");
     }
@@ -1103,7 +1109,7 @@ int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, 
     const hipStream_t s = (hipStream_t)stream;
     const int64_t most = pages / 2 * 2 * pool->layers;  // copies that there can be
     if (pages <= kFewPages) {
-        a.table_blocks = (int)blocks_of(batch * table_width, kThreads);
+        a.table_blocks = (int)std::min<int64_t>(blocks_of(batch * table_width, kThreads), 512);  // (each plans: as many as run at once)
         a.copy_blocks = copy_blocks(a.pool, most);
         hipLaunchKernelGGL(compact_few_kernel, dim3((unsigned)(1 + a.table_blocks + a.copy_blocks)), dim3(kThreads), 0, s, a);
         return launched("paged_compact");

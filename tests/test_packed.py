@@ -585,7 +585,8 @@ def test_fork_is_the_definition(sizes, more, wild):
     ((20, 70, 700, 16), {"token_major": True}), ((20, 70, 700, 16), {"flat": True, "dtype": F16, "dim": 128}),
     ((6, 3, 40, 64), {"layers": 5, "heads": 3, "dim": 72, "token_major": True}), ((3, 600, 70000, 16), {"layers": 1, "heads": 1}),
     ((1, 2, 9, 1024), {"heads": 8, "dim": 128}), ((1100, 2, 3000, 16), {"layers": 1, "dim": 8}),
-    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8}), ((1100, 2, 17000, 16), {"layers": 1, "heads": 1, "dim": 8})])
+    ((30, 1200, 9000, 16), {"layers": 1, "dim": 8}), ((1100, 2, 17000, 16), {"layers": 1, "heads": 1, "dim": 8}),
+    ((700, 800, 3000, 16), {"layers": 1, "heads": 1, "dim": 8})])
 def test_compact_is_the_definition(sizes, more, wild):
     batch, width, pages, page = sizes
     for turn in range(6):
