@@ -577,9 +577,12 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
     }
 }
 
-// (waves per SIMD: two with 256 registers each, where LDS holds as much)
+// (waves per SIMD: two with 256 registers each, where LDS holds as much; short prompts of
+// 64 dimensions four, for which nine registers are put away during the counting passes
+// alone: 200 of 30 15.7 -> 14.3 us, 32 of 200 18.0 -> 16.7, 96 of 1 to 119 15.7 -> 15.9)
 template <class E, int D, int kWaves, int kSplit, int kBlocks>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 4 && kSplit == 4 && D == 128 ? 1 : 2) void packed_attention_kernel(PackedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 && kSplit == 4 && D == 128 ? 1 : kWaves == 2 && D == 64 ? 4 : 2)
+void packed_attention_kernel(PackedArgs a) {
     attend_piece<E, D, kWaves, kSplit, kBlocks>(a);
 }
 
