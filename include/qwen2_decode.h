@@ -313,6 +313,11 @@ int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, const qwen2
  *   new_table [batch, table_width], new_users[p] = page_users[p] - entries given up
  *   + entries given, missing[b] = pages that row b still lacks (its table's width or
  *   the pool too small; the last columns of the last rows go without first).
+ * _cached: cached[b] (NULL: none) positions of row b hold keys and values already.  Of
+ * the entries that hold them, c < ceil(cached[b] / page_size), one that names no page is
+ * lost: no page is given there, for it would hold what another sequence left in it, but
+ * the entry is -1 and counts as missing at every call until the row's length (or cached[b])
+ * is brought below it.
  * page_table's rows lie table_stride apart.  page_size: a power of two in [16, 2^20].
  * Replaces: the growth of the cache in QwenAttention.forward (model.py:83-90),
  *           where keys and values lie in pages. */
@@ -320,6 +325,10 @@ int64_t qwen2_paged_resize_workspace_bytes(int64_t batch, int64_t table_width, i
 int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* page_users,
                        int32_t* new_table, int32_t* new_users, int32_t* missing, int64_t batch, int64_t table_width,
                        int64_t num_pages, int64_t page_size, void* workspace, int64_t workspace_bytes, void* stream);
+int qwen2_paged_resize_cached(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* cached,
+                              const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* missing,
+                              int64_t batch, int64_t table_width, int64_t num_pages, int64_t page_size, void* workspace,
+                              int64_t workspace_bytes, void* stream);
 
 /* Pools of `layers` layers whose pages one table names: the key of page p, position
  * t, head h of layer l is k + l * k_layer + p * k_page + h * k_head + t * k_position, v
@@ -345,7 +354,9 @@ typedef struct qwen2_page_pool {
  * behind their length; those are free from the next call on.
  *   new_table [children, table_width], new_lengths [children],
  *   new_users[p] = page_users[p] - entries of page_table + entries of new_table,
- *   missing[i] = 1 where a copy found no free page (its entry is -1), else 0.
+ *   missing[i] = 1 where a copy found no free page (its entry is -1), else 0.  Such a
+ * row keeps its length, and what its last page held is lost to it: a resize that is to
+ * grow it has to know (qwen2_paged_resize_cached), or would give it a page unwritten.
  * Replaces: nothing of the reference's: its batches decode greedily
  *           (src/qwen_int4/generation.py:10-115). */
 int64_t qwen2_paged_fork_workspace_bytes(int64_t batch, int64_t children, int64_t table_width, int64_t num_pages);

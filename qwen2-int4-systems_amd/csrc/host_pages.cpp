@@ -77,23 +77,27 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> all) {
 
 }  // namespace
 
-// (page_table, lengths, page_users, page_size) -> (table, users, missing)
+// (page_table, lengths, page_users, page_size, cached or None) -> (table, users, missing)
 PyObject* host_paged_resize(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return guarded([&]() -> PyObject* {
         const char* op = "paged_resize_hip";
-        check_count(op, count, 4);
+        check_count(op, count, 5);
         check_state(op);
         const at::Tensor& table = indices(args[0], op, "page_table", 2);
         const at::Tensor& lengths = indices(args[1], op, "lengths", 1);
         const at::Tensor& users = indices(args[2], op, "page_users", 1);
         const int64_t page_size = whole(args[3], "page_size");
+        const at::Tensor* cached = args[4] == Py_None ? nullptr : &indices(args[4], op, "cached", 1);
         const int64_t batch = table.size(0), width = table.size(1), pages = users.size(0);
         check_shape(lengths, "lengths", {batch});
+        if (cached) check_shape(*cached, "cached", {batch});
         if (!width) refuse(PyExc_ValueError, "page_table must have at least one column");
         if (!pages) refuse(PyExc_ValueError, "page_users must have at least one entry");
-        const c10::Device device = device_of({{&table, "page_table"}, {&lengths, "lengths"}, {&users, "page_users"}});
+        const c10::Device device = device_of({{&table, "page_table"}, {&lengths, "lengths"}, {&users, "page_users"},
+            {cached ? cached : &users, "cached"}});
         const c10::DeviceGuard guard(device);
         const at::Tensor t = rows_contiguous(table), n = contiguous(lengths), u = contiguous(users);
+        const at::Tensor held = cached ? contiguous(*cached) : at::Tensor();
         const auto options = users.options().requires_grad(false);
         const at::Tensor new_table = at::empty({batch, width}, options), new_users = at::empty({pages}, options);
         const at::Tensor missing = at::empty({batch}, options);
@@ -102,9 +106,9 @@ PyObject* host_paged_resize(PyObject*, PyObject* const* args, Py_ssize_t count) 
         if (need) workspace = at::empty({need}, options.dtype(at::kByte));
         const hipStream_t stream = current_stream(device);
         released([&] {
-            return qwen2_paged_resize(data(t), t.stride(0), data(n), data(u), data(new_table), data(new_users),
-                                      data(missing), batch, width, pages, page_size, need ? workspace.mutable_data_ptr() : nullptr, need,
-                                      stream);
+            return qwen2_paged_resize_cached(data(t), t.stride(0), data(n), cached ? data(held) : nullptr, data(u),
+                                             data(new_table), data(new_users), data(missing), batch, width, pages, page_size,
+                                             need ? workspace.mutable_data_ptr() : nullptr, need, stream);
         });
         return tuple_of({new_table, new_users, missing});
     });

@@ -180,6 +180,7 @@ __device__ __forceinline__ int sum_of(const int32_t* counts, int n, int* meet) {
 struct ResizeArgs {
     const int32_t* table;
     const int32_t* lengths;
+    const int32_t* cached;  // may be null
     const int32_t* users;
     int32_t* new_table;
     int32_t* new_users;
@@ -196,6 +197,12 @@ struct ResizeArgs {
     Divisor by_width;
 };
 
+// The first column of row b that may be given a page: those before it hold cached
+// positions, and a page given there would hold what another sequence left in it.
+__device__ __forceinline__ int first_given(const ResizeArgs& a, int b) {
+    return a.cached ? pages_needed(a.cached[b], a.page_shift) : 0;
+}
+
 // 256 columns of a row from c0, below `end`, by one wave.
 struct Columns {
     int entry[4];
@@ -205,25 +212,29 @@ struct Columns {
     }
 };
 
-// Entries in [from, upto) that name no page (one wave); `x`: the first 256 columns.
-__device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, int from, int upto, Columns x) {
+// Entries in [from, upto), of column `given` or a later one, that name no page (one
+// wave); `x`: the first 256 columns.
+__device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, int from, int upto, int given, Columns x) {
     int lacks = 0;
     for (int c0 = from; c0 < upto; c0 += 256) {
         if (c0 > from) x.load(row, c0, upto);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            lacks += __popcll(__ballot(c0 + 64 * i + lane_id() < upto && !names_page(x.entry[i], a.pages)));
+        for (int i = 0; i < 4; ++i) {
+            const int c = c0 + 64 * i + lane_id();
+            lacks += __popcll(__ballot(c >= given && c < upto && !names_page(x.entry[i], a.pages)));
+        }
     }
     return lacks;
 }
 
 // The new entries of columns [from, end) of row b (one wave): free pages from rank
-// `start` on where one is wanted (list[rank], below `free`), none behind the length.
+// `start` on where one is wanted (list[rank], below `free`; from column `given` on), none
+// behind the length.
 // With kCount the users of pages given and given up change besides.  `x`: the first of
 // the columns.  Returns how many entries name a page.
 template <bool kCount>
 __device__ __forceinline__ int resize_columns(const ResizeArgs& a, int b, int from, int end, int64_t start, int free,
-                                              const int32_t* list, int length, Columns x) {
+                                              const int32_t* list, int length, int given, Columns x) {
     const int upto = pages_wanted(length, a.page_shift, a.width);
     const int32_t* row = a.table + b * a.table_stride;
     int32_t* to = a.new_table + (int64_t)b * a.width;
@@ -234,12 +245,12 @@ __device__ __forceinline__ int resize_columns(const ResizeArgs& a, int b, int fr
         for (int i = 0; i < 4; ++i) {
             const int c = c0 + 64 * i + lane_id();
             const bool named = names_page(x.entry[i], a.pages);
-            const uint64_t wants = __ballot(c < min(upto, end) && !named);
+            const uint64_t wants = __ballot(c >= given && c < min(upto, end) && !named);
             int e = named ? x.entry[i] : -1;
             if (c >= upto) {
                 if (kCount && named) atomicAdd(a.new_users + e, -1);
                 e = -1;
-            } else if (!named && c < end) {
+            } else if (!named && c >= given && c < end) {
                 const int64_t rank = start + bits_before(wants);
                 if (rank < free) {
                     e = list[rank];
@@ -283,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
     const bool mine = blockIdx.x > 0 && b < a.batch;
     Columns row{};
     if (mine) row.load(a.table + b * a.table_stride, 0, a.width);
-    const int row_length = mine ? a.lengths[b] : 0;
+    const int row_length = mine ? a.lengths[b] : 0, row_given = mine ? first_given(a, b) : 0;
     Groups free_pages;
     free_pages.load(a.users, a.pages);
     want[tid] = 0;
@@ -296,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
     each_entry(a, entries, [&](int b, int c, int length, int entry) {
         const bool named = names_page(entry, a.pages);
         if (c < pages_needed(length, a.page_shift)) {
-            if (!named) atomicAdd(want + b, 1);
+            if (!named && c >= first_given(a, b)) atomicAdd(want + b, 1);
         } else if (first && named) {
             atomicAdd(given + entry, -1);
         }
@@ -330,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
     free_pages.list(free, given);
     __syncthreads();
     if (!mine) return;
-    const int held = resize_columns<false>(a, b, 0, a.width, start, free, given, row_length, row);
+    const int held = resize_columns<false>(a, b, 0, a.width, start, free, given, row_length, row_given, row);
     if (lane_id() == 0) a.missing[b] = pages_needed(row_length, a.page_shift) - held;
 }
 
@@ -353,7 +364,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void resize_count_kernel(ResizeArgs
         const int32_t* row = a.table + b * a.table_stride;
         Columns first;
         first.load(row, part.from, part.end);
-        const int lacks = lacking(a, row, part.from, min(part.end, pages_wanted(a.lengths[b], a.page_shift, a.width)), first);
+        const int upto = min(part.end, pages_wanted(a.lengths[b], a.page_shift, a.width));
+        const int lacks = lacking(a, row, part.from, upto, first_given(a, b), first);
         if (lane == 0) meet[wave] = lacks;
         __syncthreads();
         int all = 0;
@@ -405,14 +417,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void resize_apply_kernel(ResizeArgs
     const int32_t* row = a.table + b * a.table_stride;
     Columns first;
     first.load(row, part.from, part.end);
-    const int free = *a.free, length = a.lengths[b];
+    const int free = *a.free, length = a.lengths[b], given = first_given(a, b);
     int64_t start = a.start[b];
-    const int lacks = lacking(a, row, part.from, min(part.end, pages_wanted(length, a.page_shift, a.width)), first);
+    const int lacks = lacking(a, row, part.from, min(part.end, pages_wanted(length, a.page_shift, a.width)), given, first);
     if (lane == 0) meet[wave] = lacks;
     __syncthreads();
     for (int w = 0; w < wave; ++w) start += meet[w];
     __syncthreads();
-    const int held = resize_columns<true>(a, b, part.from, part.end, start, free, a.list, length, first);
+    const int held = resize_columns<true>(a, b, part.from, part.end, start, free, a.list, length, given, first);
     if (lane == 0) meet[wave] = held;
     __syncthreads();
     int all = 0;
@@ -1009,17 +1021,26 @@ int64_t qwen2_paged_resize_workspace_bytes(int64_t batch, int64_t table_width, i
 int qwen2_paged_resize(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* page_users,
                        int32_t* new_table, int32_t* new_users, int32_t* missing, int64_t batch, int64_t table_width,
                        int64_t num_pages, int64_t page_size, void* workspace, int64_t workspace_bytes, void* stream) {
+    return qwen2_paged_resize_cached(page_table, table_stride, lengths, nullptr, page_users, new_table, new_users, missing, batch,
+                                     table_width, num_pages, page_size, workspace, workspace_bytes, stream);
+}
+
+int qwen2_paged_resize_cached(const int32_t* page_table, int64_t table_stride, const int32_t* lengths, const int32_t* cached,
+                              const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* missing,
+                              int64_t batch, int64_t table_width, int64_t num_pages, int64_t page_size, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
     int status = check_sizes("paged_resize", batch, table_width, num_pages);
     if (status) return status;
     if (shift_of(page_size) < 0)
         return set_error(W4G64_STATUS_INVALID_VALUE, "page_size must be a power of two in [16, 2^20], got %lld", (long long)page_size);
-    if (!aligned4({page_users, new_users}) || (batch && !aligned4({page_table, lengths, new_table, missing})))
-        return set_error(W4G64_STATUS_INVALID_VALUE, "paged_resize pointers must be non-null, 4-byte aligned device pointers");
+    if (!aligned4({page_users, new_users}) || (batch && !aligned4({page_table, lengths, new_table, missing})) ||
+        ((uintptr_t)cached & 3))
+        return set_error(W4G64_STATUS_INVALID_VALUE, "paged_resize pointers (`cached` alone may be null) must be non-null, 4-byte aligned device pointers");
     status = check_workspace("paged_resize", qwen2_paged_resize_workspace_bytes(batch, table_width, num_pages), workspace,
                              workspace_bytes);
     if (status) return status;
     ResizeArgs a{};
-    a.table = page_table, a.table_stride = table_stride, a.lengths = lengths, a.users = page_users;
+    a.table = page_table, a.table_stride = table_stride, a.lengths = lengths, a.cached = cached, a.users = page_users;
     a.new_table = new_table, a.new_users = new_users, a.missing = missing;
     a.batch = (int)batch, a.width = (int)table_width, a.pages = (int)num_pages, a.page_shift = shift_of(page_size);
     a.by_width = divisor(table_width);

@@ -76,6 +76,7 @@ SIGNATURES = {
     "qwen2_packed_attention": (_int, [_p] * 5 + [_i64] * 5 + [_int, ctypes.c_float, _int, _p]),
     "qwen2_paged_resize_workspace_bytes": (_i64, [_i64] * 3),
     "qwen2_paged_resize": (_int, [_p, _i64] + [_p] * 5 + [_i64] * 4 + [_p, _i64, _p]),
+    "qwen2_paged_resize_cached": (_int, [_p, _i64] + [_p] * 6 + [_i64] * 4 + [_p, _i64, _p]),
     "qwen2_paged_fork_workspace_bytes": (_i64, [_i64] * 4),
     "qwen2_paged_fork": (_int, [_p, _p, _i64] + [_p] * 7 + [_i64] * 3 + [_p, _i64, _p]),
     "qwen2_paged_compact_workspace_bytes": (_i64, [_i64] * 3),

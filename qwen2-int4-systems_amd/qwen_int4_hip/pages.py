@@ -5,7 +5,7 @@ The reference keeps one growing cache per batch (src/qwen_int4/generation.py:10-
 and has no pages.  Here a step's lengths are on the GPU (``verify_drafts_hip`` decides
 there how many tokens stand), so the pages are dealt out there too:
 
-    table, users, missing = paged_resize_hip(table, lengths, users, page_size=16)
+    table, users, missing = paged_resize_hip(table, lengths + drafts, users, page_size=16, cached=lengths)
     table, lengths, users, missing = paged_fork_hip(k_pages, v_pages, table, lengths, users, parents)
     table, users, moved_to = paged_compact_hip(k_pages, v_pages, table, users)
 
@@ -44,7 +44,7 @@ from . import paged
 
 
 def paged_resize_hip(page_table: torch.Tensor, lengths: torch.Tensor, page_users: torch.Tensor, *,
-                     page_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                     page_size: int, cached: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Give every sequence the pages that its length needs, and take the others.
 
     Row b's first ``ceil(lengths[b] / page_size)`` entries keep the pages that they
@@ -57,9 +57,19 @@ def paged_resize_hip(page_table: torch.Tensor, lengths: torch.Tensor, page_users
     without) or its table's width was too small; ``paged_append_hip`` does not write
     there, ``paged_attention_hip`` gives NaN.
 
+    ``cached`` (int32 [B]): how many positions of each row hold keys and values already.
+    A page that such a position should lie in and that the table does not name is lost (a
+    resize or a fork found none free): a page given there now would hold what another
+    sequence left in it.  With ``cached`` it is not given; the row goes on missing it, and
+    giving NaN, at every call until its length is set below it (0 frees the row) or it is
+    filled anew and ``cached`` says so.  Without ``cached`` every missing page is given,
+    which is right only where none of a row's positions at such pages counts as cached: a
+    row that an earlier ``missing`` names is then to be freed, or that step redone from the state
+    before it.
+
     A sequence that is cut back into a page which something else names must be passed
     through ``paged_fork_hip`` (with itself as its parent) before it is written again."""
-    return paged._calls().paged_resize(page_table, lengths, page_users, page_size)
+    return paged._calls().paged_resize(page_table, lengths, page_users, page_size, cached)
 
 
 def paged_fork_hip(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -76,7 +86,9 @@ def paged_fork_hip(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
     and all give up the pages behind their length.
 
     Returns (table [C, W], lengths [C], page_users, missing [C]): ``missing`` is 1 where
-    a copy found no free page (its entry is -1)."""
+    a copy found no free page (its entry is -1).  Such a row keeps its length without the
+    positions of its last page: free it, redo the fork from the state before it, or give the
+    next ``paged_resize_hip`` these lengths as ``cached``, which then goes on calling it missing."""
     return paged._calls().paged_fork(k_pages, v_pages, page_table, lengths, page_users, parents)
 
 

@@ -1,0 +1,225 @@
+"""More of the packed prompt attention and the page operators: pages that a row has lost.
+
+Checks of the kernels' sources on the CPU run in processes of their own, as in
+test_packed_lanes."""
+
+from __future__ import annotations
+
+import ctypes
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+
+from test_packed_lanes import POOLS, Kernels, lanes_library, state_of  # noqa: E402, F401
+
+BF16, F16, I32 = torch.bfloat16, torch.float16, torch.int32
+WILD = [2 ** 31 - 1, -(2 ** 31)]
+
+
+def _lists(*tensors):
+    return tuple(t.tolist() for t in tensors)
+
+
+def resized_cached(table, lengths, users, page, cached):
+    """The resize's answers, entry by entry: one that holds cached positions is given no page."""
+    table, users, missing = [list(r) for r in table], list(users), []
+    free = iter([p for p, n in enumerate(users) if n == 0])
+    for row, length, filled in zip(table, lengths, cached):
+        need = -(-max(length, 0) // page)
+        for c, e in enumerate(row):
+            named = 0 <= e < len(users)
+            if c >= need:
+                if named:
+                    users[e] -= 1
+                row[c] = -1
+            elif not named:
+                row[c] = -1 if c * page < filled else next(free, -1)
+                if row[c] >= 0:
+                    users[row[c]] += 1
+        missing.append(need - sum(e >= 0 for e in row))
+    return table, users, missing
+
+
+def _lengths(seed, batch, most):
+    return torch.randint(0, most + 1, (batch,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def cached_cases(sizes, wild, spare):
+    """(table, users, [(lengths, cached), ...]) of rows some of whose entries name no page."""
+    batch, width, pages, page = sizes
+    table, lengths, users = state_of(11, *sizes, spare=spare, wild=wild)
+    for b in range(0, batch, 2):  # an entry is lost here and there
+        c = (7 * b) % width
+        if 0 <= table[b][c] < pages:
+            users[table[b][c]] -= 1
+            table[b][c] = -1
+    most = width * page + 20
+    return table, users, [(_lengths(1, batch, most), lengths), (_lengths(2, batch, most), _lengths(3, batch, most)),
+                          ([width * page] * batch, [page * (width // 2) + b % 3 for b in range(batch)]),
+                          (lengths, [(0, -5, *WILD)[b % 4] for b in range(batch)])]
+
+
+# ---------------------------------------------------------------------------
+# On the CPU, in the process of a check
+# ---------------------------------------------------------------------------
+
+class MoreKernels(Kernels):
+    def resize_cached(self, table, lengths, users, page, cached):
+        (batch, width), pages = table.shape, len(users)
+        answers = self.empty(batch, width), self.empty(pages), self.empty(batch)
+        need = self.lib.qwen2_paged_resize_workspace_bytes(batch, width, pages)
+        workspace = self.memory(torch.full((need,), 0xA5, dtype=torch.uint8))
+        self.check(self.lib.qwen2_paged_resize_cached(
+            table.data_ptr(), width, lengths.data_ptr(), cached.data_ptr(), users.data_ptr(),
+            *(t.data_ptr() for t in answers), batch, width, pages, page, workspace.data_ptr(), need, None))
+        return answers
+
+
+def _lost(kernels):
+    """A fork finds no free page for its second child while a sequence ends and gives one up:
+    the next resize does not pass that one off as the child's."""
+    k, v = (kernels.memory(torch.zeros(1, 3, 1, 16, 8, dtype=BF16)) for _ in range(2))
+    table, lengths, users, missing = kernels.fork(k, v, kernels.ints([[0, 1, -1], [2, -1, -1]]), kernels.ints([20, 16]),
+                                                  kernels.ints([1, 1, 1]), kernels.ints([0, 0]))
+    assert _lists(table, lengths, users, missing) == ([[0, 1, -1], [0, -1, -1]], [20, 20], [2, 1, 0], [0, 1])
+    for _ in range(2):  # at every call, as the row grows
+        table, users, missing = kernels.resize_cached(table, kernels.ints([20, 21]), users, 16, lengths)
+        assert _lists(table, users, missing) == ([[0, 1, -1], [0, -1, -1]], [2, 1, 0], [0, 1])
+        lengths = kernels.ints([20, 21])
+    # a new page behind the lost one is given; freed, the row starts anew
+    grown = kernels.resize_cached(table, kernels.ints([20, 40]), users, 16, lengths)
+    assert _lists(*grown) == ([[0, 1, -1], [0, -1, 2]], [2, 1, 1], [0, 1])
+    table, users, missing = kernels.resize_cached(table, kernels.ints([20, 0]), users, 16, lengths)
+    assert _lists(table, users, missing) == ([[0, 1, -1], [-1, -1, -1]], [1, 1, 0], [0, 0])
+    anew = kernels.resize_cached(table, kernels.ints([20, 5]), users, 16, kernels.ints([20, 0]))
+    assert _lists(*anew) == ([[0, 1, -1], [2, -1, -1]], [1, 1, 1], [0, 0])
+
+
+def _cached(kernels):
+    for sizes in [s for s in POOLS if s[2] < 400] + [(3, 20, 16500, 16), (2, 4200, 500, 16)]:
+        for wild in (False, True):
+            table, users, calls = cached_cases(sizes, wild, min(sizes[2] // 7, 9))
+            for lengths, cached in calls:
+                got = kernels.resize_cached(kernels.ints(table), kernels.ints(lengths), kernels.ints(users), sizes[3],
+                                            kernels.ints(cached))
+                assert _lists(*got) == resized_cached(table, lengths, users, sizes[3], cached), (sizes, wild)
+
+
+CHECKS = {"lost": _lost, "cached": _cached}
+
+
+@pytest.mark.parametrize("side", ["end", "start"])
+@pytest.mark.parametrize("name", CHECKS)
+def test_on_the_cpu(lanes_library, name, side):  # noqa: F811
+    result = subprocess.run([sys.executable, __file__, str(lanes_library), name, side], capture_output=True, text=True,
+                            timeout=600)
+    assert result.returncode == 0 and result.stdout.endswith("done\n"), (result.returncode, result.stderr[-2000:])
+
+
+if __name__ == "__main__":
+    torch.set_num_threads(1)
+    CHECKS[sys.argv[2]](MoreKernels(sys.argv[1], sys.argv[3]))
+    print("done")
+    sys.exit(0)
+
+
+from test_packed import Pool, built, gpu, ints  # noqa: E402
+
+from qwen_int4_hip import (  # noqa: E402
+    _lib, paged_append_hip, paged_attention_hip, paged_fork_hip, paged_resize_hip)
+
+
+# ---------------------------------------------------------------------------
+# Refusals
+# ---------------------------------------------------------------------------
+
+@built
+def test_cached_is_refused_before_launch():
+    table, lengths, users = torch.zeros(2, 3, dtype=I32), torch.zeros(2, dtype=I32), torch.zeros(6, dtype=I32)
+    for cached, error, said in [(lengths.long(), TypeError, "cached must have dtype torch.int32"),
+                                (torch.zeros(3, dtype=I32), ValueError, r"cached must have shape \[2\]"),
+                                (table, ValueError, "cached must have 1 dimensions"), ([0, 0], TypeError, "must be a torch.Tensor"),
+                                (lengths, ValueError, "must be a GPU tensor")]:
+        with pytest.raises(error, match=said):
+            paged_resize_hip(table, lengths, users, page_size=16, cached=cached)
+    buffer = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buffer) + 15) & ~15
+    call = _lib.load().qwen2_paged_resize_cached
+    assert call(p, 3, p, p + 2, p, p, p, p, 2, 3, 6, 16, None, 0, None) == 1
+    assert call(p, 3, p, p, p, p, p, p, 2, 3, 6, 24, None, 0, None) == 1
+
+
+# ---------------------------------------------------------------------------
+# On the GPU
+# ---------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("wild", [False, True])
+@pytest.mark.parametrize("sizes", POOLS + [(300, 40, 5000, 16), (9, 5000, 70000, 32), (1100, 7, 3000, 16)])
+def test_resize_gives_no_page_to_cached_positions(sizes, wild):
+    page = sizes[3]
+    table, users, calls = cached_cases(sizes, wild, min(sizes[2] // 7, 9))
+    device = ints(table).view(sizes[0], -1), ints(users)
+    for lengths, cached in calls:
+        got = paged_resize_hip(device[0], ints(lengths), device[1], page_size=page, cached=ints(cached))
+        assert _lists(*got) == resized_cached(table, lengths, users, page, cached)
+        strided = torch.stack((ints(cached), ints(cached)), 1)[:, 1]
+        assert _lists(*paged_resize_hip(device[0], ints(lengths), device[1], page_size=page, cached=strided)) == _lists(*got)
+        none = paged_resize_hip(device[0], ints(lengths), device[1], page_size=page, cached=ints([0] * sizes[0]))
+        assert _lists(*none) == _lists(*paged_resize_hip(device[0], ints(lengths), device[1], page_size=page))
+
+
+@gpu
+def test_a_lost_page_stays_missing_in_a_graph():
+    p = Pool(12, 12, 9, 150, 16, layers=1)
+    table, _, users = p.indices()
+    table[3, 0] = -1
+    lengths, cached = ints(p.lengths), ints(p.lengths)
+    paged_resize_hip(table, lengths, users, page_size=16, cached=cached)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = paged_resize_hip(table, lengths, users, page_size=16, cached=cached)
+    for turn in range(4):
+        lengths.copy_(ints(_lengths(turn, 12, 9 * 16)))
+        cached.copy_(ints(_lengths(turn + 9, 12, 9 * 16)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _lists(*got) == resized_cached(table.tolist(), lengths.tolist(), users.tolist(), 16, cached.tolist())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_row_that_lost_a_page_is_not_served_from_another_one(dtype):
+    """Two sequences, one forked into three children while the other ends and no page is free: the
+    pages that the ended one gave up go to no lost place, so that the children without a copy
+    attend NaN at every step, and the one that kept its page what the formula says."""
+    heads, kv_heads, dim, page = 4, 2, 64, 16
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k_pages, v_pages = (torch.randn(5, kv_heads, page, dim, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    users, table, lengths = ints([1, 1, 1, 1, 1]), ints([[4, 1, 2, -1], [3, 0, -1, -1]]), ints([37, 30])
+    keys, values = (torch.cat([t[p].transpose(0, 1) for p in (4, 1, 2)])[:37].clone() for t in (k_pages, v_pages))
+    table, lengths, users, lost = paged_fork_hip(k_pages, v_pages, table, lengths, users, ints([0, 0, 0]))
+    assert lost.tolist() == [0, 1, 1] and users.tolist() == [0, 3, 1, 0, 3]
+    cu = ints([0, 1, 2, 3])
+    for step in range(11):  # to the end of the last page
+        table, users, missing = paged_resize_hip(table, lengths + 1, users, page_size=page, cached=lengths)
+        lengths = lengths + 1
+        assert missing.tolist() == [0, 1, 1] and table[1:, 2].tolist() == [-1, -1]
+        q, k, v = (torch.randn(3, n, dim, generator=gen, device="cuda").to(dtype) for n in (heads, kv_heads, kv_heads))
+        rotated = paged_append_hip(q, k, v, k_pages, v_pages, table, cu, lengths, None)
+        got = paged_attention_hip(rotated, k_pages, v_pages, table, cu, lengths).double()
+        assert bool(got[1:].isnan().all())
+        keys, values = torch.cat((keys, k[:1])), torch.cat((values, v[:1]))
+        for h in range(heads):
+            w = torch.softmax(keys[:, h // 2].double() @ q[0, h].double() * dim ** -0.5, 0)
+            want = w @ values[:, h // 2].double()
+            # (a half step of the result, values of a few units, and one of each probability's two terms)
+            assert float((got[0, h] - want).abs().amax()) < 4 * torch.finfo(dtype).eps
+    lengths[1:] = 0
+    table, users, missing = paged_resize_hip(table, lengths, users, page_size=page, cached=lengths)
+    assert not missing.any() and sorted(users.tolist()) == [0, 0, 1, 1, 1] and bool((table[1:] == -1).all())
