@@ -20,4 +20,15 @@ __host__ __device__ inline int pages_wanted(int length, int page_shift, int widt
     return need < width ? need : width;
 }
 
+// The columns of a row that part `part` of `parts` sees to: as many 64s as each needs at
+// most, from the first on (worked out without a sign: a part's end may pass 2^31 - 1).
+struct ColumnPart {
+    int from, end;
+};
+__host__ __device__ inline ColumnPart column_part(int width, int part, int parts) {
+    const uint32_t columns = (uint32_t)width, least = 64 * (uint32_t)parts, each = (columns + least - 1) / least * 64;
+    const uint32_t from = (uint32_t)part * each, end = from + each;
+    return ColumnPart{(int)(from < columns ? from : columns), (int)(end < columns ? end : columns)};
+}
+
 }  // namespace w4g64

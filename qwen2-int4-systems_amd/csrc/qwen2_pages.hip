@@ -203,24 +203,29 @@ __device__ __forceinline__ int first_given(const ResizeArgs& a, int b) {
     return a.cached ? pages_needed(a.cached[b], a.page_shift) : 0;
 }
 
-// 256 columns of a row from c0, below `end`, by one wave.
+// 256 columns of a row from c0, below `end`, by one wave.  (Columns go up to 2^31 - 1, and
+// the ones looked at past the last go by: they are counted in 32 bits without a sign.)
 struct Columns {
     int entry[4];
-    __device__ __forceinline__ void load(const int32_t* row, int c0, int end) {
+    __device__ __forceinline__ void load(const int32_t* row, uint32_t c0, uint32_t end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) entry[i] = c0 + 64 * i + lane_id() < end ? row[c0 + 64 * i + lane_id()] : -1;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t c = c0 + 64 * i + lane_id();
+            entry[i] = c < end ? row[c] : -1;
+        }
     }
 };
 
 // Entries in [from, upto), of column `given` or a later one, that name no page (one
 // wave); `x`: the first 256 columns.
-__device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, int from, int upto, int given, Columns x) {
+__device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, uint32_t from, uint32_t upto, uint32_t given,
+                                       Columns x) {
     int lacks = 0;
-    for (int c0 = from; c0 < upto; c0 += 256) {
+    for (uint32_t c0 = from; c0 < upto; c0 += 256) {
         if (c0 > from) x.load(row, c0, upto);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 64 * i + lane_id();
+            const uint32_t c = c0 + 64 * i + lane_id();
             lacks += __popcll(__ballot(c >= given && c < upto && !names_page(x.entry[i], a.pages)));
         }
     }
@@ -233,19 +238,19 @@ __device__ __forceinline__ int lacking(const ResizeArgs& a, const int32_t* row, 
 // With kCount the users of pages given and given up change besides.  `x`: the first of
 // the columns.  Returns how many entries name a page.
 template <bool kCount>
-__device__ __forceinline__ int resize_columns(const ResizeArgs& a, int b, int from, int end, int64_t start, int free,
-                                              const int32_t* list, int length, int given, Columns x) {
-    const int upto = pages_wanted(length, a.page_shift, a.width);
+__device__ __forceinline__ int resize_columns(const ResizeArgs& a, int b, uint32_t from, uint32_t end, int64_t start, int free,
+                                              const int32_t* list, int length, uint32_t given, Columns x) {
+    const uint32_t upto = pages_wanted(length, a.page_shift, a.width), reach = upto < end ? upto : end;
     const int32_t* row = a.table + b * a.table_stride;
     int32_t* to = a.new_table + (int64_t)b * a.width;
     int held = 0;
-    for (int c0 = from; c0 < end; c0 += 256) {
+    for (uint32_t c0 = from; c0 < end; c0 += 256) {
         if (c0 > from) x.load(row, c0, end);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 64 * i + lane_id();
+            const uint32_t c = c0 + 64 * i + lane_id();
             const bool named = names_page(x.entry[i], a.pages);
-            const uint64_t wants = __ballot(c >= given && c < min(upto, end) && !named);
+            const uint64_t wants = __ballot(c >= given && c < reach && !named);
             int e = named ? x.entry[i] : -1;
             if (c >= upto) {
                 if (kCount && named) atomicAdd(a.new_users + e, -1);
@@ -347,20 +352,12 @@ __global__ __launch_bounds__(kThreads) void resize_few_kernel(ResizeArgs a) {
 
 // Many.  A row by a workgroup of kRowWaves, each a part of its columns.
 constexpr int kRowWaves = 8;
-struct Part {
-    int from, end;
-};
-__device__ __forceinline__ Part part_of(int width) {
-    const int each = ((width + kRowWaves - 1) / kRowWaves + 63) / 64 * 64, from = min(wave_id() * each, width);
-    return Part{from, min(from + each, width)};
-}
-
 // Rows' wants by the first workgroups, pages' counts by the others.
 __global__ __launch_bounds__(64 * kRowWaves) void resize_count_kernel(ResizeArgs a) {
     __shared__ int meet[kRowWaves];
     if ((int)blockIdx.x < a.batch) {
         const int b = (int)blockIdx.x, wave = wave_id(), lane = lane_id();
-        const Part part = part_of(a.width);
+        const ColumnPart part = column_part(a.width, wave, kRowWaves);
         const int32_t* row = a.table + b * a.table_stride;
         Columns first;
         first.load(row, part.from, part.end);
@@ -413,7 +410,7 @@ __global__ __launch_bounds__(kThreads) void resize_list_kernel(ResizeArgs a) {
 __global__ __launch_bounds__(64 * kRowWaves) void resize_apply_kernel(ResizeArgs a) {
     __shared__ int meet[kRowWaves];
     const int b = (int)blockIdx.x, wave = wave_id(), lane = lane_id();
-    const Part part = part_of(a.width);
+    const ColumnPart part = column_part(a.width, wave, kRowWaves);
     const int32_t* row = a.table + b * a.table_stride;
     Columns first;
     first.load(row, part.from, part.end);

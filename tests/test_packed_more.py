@@ -1,4 +1,5 @@
-"""More of the packed prompt attention and the page operators: pages that a row has lost.
+"""More of the packed prompt attention and the page operators: pages that a row has lost,
+tables of the greatest width.
 
 Checks of the kernels' sources on the CPU run in processes of their own, as in
 test_packed_lanes."""
@@ -15,7 +16,7 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parent))
 
-from test_packed_lanes import POOLS, Kernels, lanes_library, state_of  # noqa: E402, F401
+from test_packed_lanes import CSRC, LANES, MORE, POOLS, REPO, Kernels, _compiler, lanes_library, state_of  # noqa: E402, F401
 
 BF16, F16, I32 = torch.bfloat16, torch.float16, torch.int32
 WILD = [2 ** 31 - 1, -(2 ** 31)]
@@ -110,13 +111,58 @@ def _cached(kernels):
                 assert _lists(*got) == resized_cached(table, lengths, users, sizes[3], cached), (sizes, wild)
 
 
-CHECKS = {"lost": _lost, "cached": _cached}
+def _ends(kernels):
+    """The last 640 columns of rows as wide as can be: kept, given up, and (by a page size that makes
+    a length need them) given."""
+    call = kernels.lib.ends_resize
+    call.restype, call.argtypes = None, [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 4
+    pages, count = 700, 640
+    for width in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 63, 2 ** 31 - 64, 2 ** 31 - 300, 2 ** 30, 1000):
+        start = width - count
+        for length, shift in ((2 ** 31 - 1, 0), (start + 5, 0), (0, 4)):
+            row = [(7 * c) % pages if c % 3 else -1 for c in range(count)]
+            table, new_table, said = kernels.ints(row), kernels.empty(count), kernels.empty(2)
+            users, spare = kernels.ints([1] * pages), [pages - 1 - c for c in range(100)]
+            call(table.data_ptr(), new_table.data_ptr(), users.data_ptr(), kernels.ints(spare).data_ptr(), said.data_ptr(),
+                 width, start, pages, 100, length, shift)
+            upto, want, after, given = min(length, width) - start if length else 0, [], [1] * pages, iter(spare)
+            for c, e in enumerate(row):
+                if c >= upto:
+                    if e >= 0:
+                        after[e] -= 1
+                    e = -1
+                elif e < 0:
+                    e = next(given, -1)
+                    if e >= 0:
+                        after[e] += 1
+                want.append(e)
+            assert new_table.tolist() == want and users.tolist() == after, (width, length)
+            assert said.tolist() == [sum(e < 0 for e in row[:max(upto, 0)]), sum(e >= 0 for e in want)]
+
+
+CHECKS = {"lost": _lost, "cached": _cached, "ends": _ends}
+
+
+@pytest.fixture(scope="module")
+def more_library(lanes_library):  # noqa: F811
+    """The library of test_packed_lanes, with the drivers of lanes_more in it."""
+    root = lanes_library.parent
+    library = root / "more.so"
+    drivers = [(source, root / f"more_{source.stem}.o") for source in sorted(MORE.glob("*.cpp"))]
+    for source, made in drivers:
+        subprocess.run([_compiler(), "-std=c++17", "-O2", "-fPIC", "-ffp-contract=off", "-mf16c", "-mfma", "-w", f"-I{LANES}",
+                        f"-I{root}", f"-I{REPO / 'include'}", f"-I{MORE}", "-include", str(MORE / "more.h"), "-x", "c++", "-c",
+                        str(source), "-o", str(made)], check=True)
+    # (a driver brings its kernels' source with it: their entry points come once)
+    rest = [made for made in root.glob("*.o") if made.name != "qwen2_pages.o"]
+    subprocess.run([_compiler(), "-shared", *map(str, rest), "-o", str(library)], check=True)
+    return library
 
 
 @pytest.mark.parametrize("side", ["end", "start"])
 @pytest.mark.parametrize("name", CHECKS)
-def test_on_the_cpu(lanes_library, name, side):  # noqa: F811
-    result = subprocess.run([sys.executable, __file__, str(lanes_library), name, side], capture_output=True, text=True,
+def test_on_the_cpu(more_library, name, side):
+    result = subprocess.run([sys.executable, __file__, str(more_library), name, side], capture_output=True, text=True,
                             timeout=600)
     assert result.returncode == 0 and result.stdout.endswith("done\n"), (result.returncode, result.stderr[-2000:])
 
@@ -128,10 +174,44 @@ if __name__ == "__main__":
     sys.exit(0)
 
 
+PARTS_PROGRAM = r"""
+#define __host__
+#define __device__
+#include "qwen2_pages.h"
+#include <cstdio>
+using namespace w4g64;
+int main() {
+    const int64_t spans[][2] = {{1, 1100}, {1 << 30, (1 << 30) + 1}, {2147483648ll - 1100, 2147483648ll}};
+    for (const auto& span : spans)
+        for (int64_t w = span[0]; w < span[1]; ++w)
+            for (int p = 0; p < 8; ++p) {
+                const ColumnPart part = column_part((int)w, p, 8);
+                printf("%d %d %d\n", (int)w, part.from, part.end);
+            }
+}
+"""
+
+
+def test_the_parts_of_a_row_cover_it(tmp_path):
+    """At every width one after the other, without a gap, from multiples of 64 on."""
+    source, program = tmp_path / "parts.cpp", tmp_path / "parts"
+    source.write_text(PARTS_PROGRAM)
+    subprocess.run(["g++", "-std=c++17", f"-I{CSRC}", str(source), "-o", str(program)], check=True)
+    said = [tuple(map(int, line.split())) for line in subprocess.run([str(program)], check=True, capture_output=True,
+                                                                     text=True).stdout.splitlines()]
+    assert len(said) == 8 * (1099 + 1 + 1100)
+    for at in range(0, len(said), 8):
+        width, reached = said[at][0], 0
+        for w, begin, end in said[at:at + 8]:
+            assert w == width and begin == reached and end >= begin and (begin % 64 == 0 or begin == width)
+            reached = end
+        assert reached == width
+
+
 from test_packed import Pool, built, gpu, ints  # noqa: E402
 
 from qwen_int4_hip import (  # noqa: E402
-    _lib, paged_append_hip, paged_attention_hip, paged_fork_hip, paged_resize_hip)
+    _lib, paged_append_hip, paged_attention_hip, paged_compact_hip, paged_fork_hip, paged_resize_hip)
 
 
 # ---------------------------------------------------------------------------
@@ -223,3 +303,28 @@ def test_a_row_that_lost_a_page_is_not_served_from_another_one(dtype):
     lengths[1:] = 0
     table, users, missing = paged_resize_hip(table, lengths, users, page_size=page, cached=lengths)
     assert not missing.any() and sorted(users.tolist()) == [0, 0, 1, 1, 1] and bool((table[1:] == -1).all())
+
+
+@gpu
+def test_page_operators_over_a_row_as_wide_as_can_be():
+    """2^31 - 1 columns, more than any length needs; pages named in the last of them are given up
+    (resize, fork) or renamed (compact)."""
+    width, pages = 2 ** 31 - 1, 100
+    table = torch.full((1, width), -1, dtype=I32, device="cuda")
+    last = [0, 1, 5, width // 2, width - 700, width - 513, width - 512, width - 257, width - 64, width - 2, width - 1]
+    table[0, last] = ints(range(20, 20 + len(last)))
+    users = torch.zeros(pages, dtype=I32, device="cuda")
+    users[20:20 + len(last)] = 1
+    got = paged_resize_hip(table, ints([40]), users, page_size=16)
+    assert got[0].shape == (1, width) and got[0][0, :4].tolist() == [20, 21, 0, -1] and int((got[0] >= 0).sum()) == 3
+    assert int((got[0] == -1).sum()) == width - 3 and got[2].tolist() == [0]
+    assert got[1].tolist() == [int(p in (0, 20, 21)) for p in range(pages)]
+    del got
+    pools = [torch.zeros(pages, 1, 16, 8, dtype=BF16, device="cuda") for _ in range(2)]
+    got = paged_fork_hip(*pools, table, ints([32]), users, ints([0]))
+    assert got[0][0, :3].tolist() == [20, 21, -1] and int((got[0] == -1).sum()) == width - 2
+    assert got[1].tolist() == [32] and got[3].tolist() == [0] and got[2].tolist() == [int(p in (20, 21)) for p in range(pages)]
+    del got
+    got = paged_compact_hip(*pools, table, users)
+    assert got[0][0, last].tolist() == list(range(len(last))) and int((got[0] == -1).sum()) == width - len(last)
+    assert got[1].tolist() == [int(p < len(last)) for p in range(pages)]
