@@ -276,8 +276,8 @@ int qwen2_verify_drafts(const void* target, int64_t target_batch, int64_t target
  * head_dim], k, v [rows, kv_heads, head_dim]: parts of a fused projection are read in
  * place.  Scores, softmax and sums in fp32; a probability is rounded once to dtype
  * before it meets its value, and it is the rounded ones that the sum adds up; the result
- * is rounded once.  Rows behind the last sequence are left as they are, or zeroed with
- * zero_rest.  Keys and values that a row does not see take no part, whatever they hold;
+ * is rounded once.  Rows of no sequence (behind the last one, or before cu_rows[0]) are
+ * left as they are, or zeroed with zero_rest.  Keys and values that a row does not see take no part, whatever they hold;
  * an infinity or NaN among the values that it sees reaches it, however small the key's
  * weight.  (Values are summed before the sum is divided: the keys' number times the
  * values' size has to stay in fp32.)

@@ -17,4 +17,16 @@ __host__ __device__ inline PackedRows packed_rows(int begin, int end, int rows) 
     return s;
 }
 
+// Rows of no sequence, those before the first one's and those behind the last one's, none
+// twice whatever the bounds are: how many there are, and the i-th.
+struct FreeRows {
+    int before, end;
+};
+__host__ __device__ inline FreeRows free_rows(const int32_t* cu_rows, int batch, int rows) {
+    const int end = rows_end(cu_rows, batch, rows), first = cu_rows[0];
+    return FreeRows{first < 0 ? 0 : first < end ? first : end, end};
+}
+__host__ __device__ inline int free_count(const FreeRows& f, int rows) { return f.before + (rows - f.end); }
+__host__ __device__ inline int free_row(const FreeRows& f, int i) { return i < f.before ? i : f.end + (i - f.before); }
+
 }  // namespace w4g64

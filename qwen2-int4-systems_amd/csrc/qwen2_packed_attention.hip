@@ -352,9 +352,12 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
     const int j = lane & 31;
     const int h = lane >> 5;
     if (a.zero_rest) {
-        for (int64_t r = rest_row(a.cu_rows, a.batch, a.rows, blockIdx.x); r < a.rows; r += gridDim.x)
+        const FreeRows rest = free_rows(a.cu_rows, a.batch, a.rows);
+        for (int64_t i = blockIdx.x, n = free_count(rest, a.rows); i < n; i += gridDim.x) {
+            const int64_t r = free_row(rest, (int)i);
             for (int d = 8 * tid; d < a.heads * D; d += 8 * kThreads)
                 *(u32x4*)(a.out + r * a.out_row + (d / D) * a.out_head + d % D) = u32x4{0u, 0u, 0u, 0u};
+        }
     }
     Piece s;
     constexpr bool kPairs = kWaves == 4 && 4 * T::kBytes <= 80 << 10;  // two workgroups a CU

@@ -35,12 +35,13 @@ def packed_attention_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_r
     Keys and values that a row does not see take no part, whatever they hold; an
     infinity or NaN that it sees reaches it, however small the key's weight (a call full
     of such rows takes three to seventeen times as long: 23 us instead of 6.5 for 37
-    tokens, 400 instead of 42 for eight prompts of 1000).  Rows behind the last sequence are left as they are in
-    ``out``, and zeros in a new tensor.  Scores, softmax and sums are fp32, in a fixed
-    order: the same inputs give the same bits.  A probability is rounded once to the
-    tensors' type before it meets its value, and the sum that divides is the rounded
-    ones'; values are summed before the division: the keys' number times the values'
-    size has to stay in fp32.  The result is rounded once.
+    tokens, 400 instead of 42 for eight prompts of 1000).  Rows of no sequence (behind
+    the last one, or before ``cu_rows[0]``) are left as they are in ``out``, and zeros in
+    a new tensor.  Scores, softmax and sums are fp32, in a fixed order: the same inputs
+    give the same bits.  A probability is rounded once to the tensors' type before it
+    meets its value, and the sum that divides is the rounded ones'; values are summed
+    before the division: the keys' number times the values' size has to stay in fp32.
+    The result is rounded once.
 
     Launches on torch's current stream of the tensors' device; raises before anything is
     launched: TypeError for a dtype, ValueError for shapes, strides, devices and memory

@@ -1,5 +1,5 @@
 """More of the packed prompt attention and the page operators: pages that a row has lost,
-tables of the greatest width.
+tables of the greatest width, rows before the first sequence.
 
 Checks of the kernels' sources on the CPU run in processes of their own, as in
 test_packed_lanes."""
@@ -16,7 +16,12 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parent))
 
-from test_packed_lanes import CSRC, LANES, MORE, POOLS, REPO, Kernels, _compiler, lanes_library, state_of  # noqa: E402, F401
+from test_packed_lanes import (  # noqa: E402, F401
+    CSRC, LANES, MORE, POOLS, REPO, Kernels, _compiler, _packed, formula, lanes_library, state_of)
+from test_packed import Pool, Prompts, built, gpu, ints, near  # noqa: E402
+
+from qwen_int4_hip import (  # noqa: E402
+    _lib, packed_attention_hip, paged_append_hip, paged_attention_hip, paged_compact_hip, paged_fork_hip, paged_resize_hip)
 
 BF16, F16, I32 = torch.bfloat16, torch.float16, torch.int32
 WILD = [2 ** 31 - 1, -(2 ** 31)]
@@ -140,7 +145,26 @@ def _ends(kernels):
             assert said.tolist() == [sum(e < 0 for e in row[:max(upto, 0)]), sum(e >= 0 for e in want)]
 
 
-CHECKS = {"lost": _lost, "cached": _cached, "ends": _ends}
+def _before(kernels):
+    """Sequences that begin behind the first row: the rows before them are as those behind the last."""
+    for first, lengths, tail in ((1, [2, 0, 3], 0), (3, [40, 7], 2), (70, [33], 1), (5, [1 + b % 2 for b in range(100)], 3)):
+        rows = first + sum(lengths)
+        q, k, v, _ = _packed(kernels, [rows], 4, 2, 64, tail=tail)
+        cu = kernels.ints([first + sum(lengths[:b]) for b in range(len(lengths) + 1)])
+        want = formula(q, k, v, cu)
+        for zero_rest, rest in ((1, 0.0), (0, 7.0)):
+            out = kernels.attention(q, k, v, cu, zero_rest, fill=7.0)
+            assert bool((out[:first] == rest).all()) and bool((out[rows:] == rest).all()), (first, zero_rest)
+            # (a half step of the output and of each probability, values of a few units)
+            assert float((out.double() - want)[first:rows].abs().amax()) < 4 * torch.finfo(BF16).eps
+    for values in [[5, 2], [9, 9], [2 ** 31 - 1, 3], [4, -1], [-3, 2]]:  # rows of 8
+        q, k, v, _ = _packed(kernels, [8], 4, 2, 64)
+        out = kernels.attention(q, k, v, kernels.ints(values), fill=7.0)
+        end = min(max(values[1], 0), 8)
+        assert not out[:min(max(values[0], 0), end)].any() and not out[end:].any(), values
+
+
+CHECKS = {"lost": _lost, "cached": _cached, "ends": _ends, "before": _before}
 
 
 @pytest.fixture(scope="module")
@@ -165,13 +189,6 @@ def test_on_the_cpu(more_library, name, side):
     result = subprocess.run([sys.executable, __file__, str(more_library), name, side], capture_output=True, text=True,
                             timeout=600)
     assert result.returncode == 0 and result.stdout.endswith("done\n"), (result.returncode, result.stderr[-2000:])
-
-
-if __name__ == "__main__":
-    torch.set_num_threads(1)
-    CHECKS[sys.argv[2]](MoreKernels(sys.argv[1], sys.argv[3]))
-    print("done")
-    sys.exit(0)
 
 
 PARTS_PROGRAM = r"""
@@ -206,12 +223,6 @@ def test_the_parts_of_a_row_cover_it(tmp_path):
             assert w == width and begin == reached and end >= begin and (begin % 64 == 0 or begin == width)
             reached = end
         assert reached == width
-
-
-from test_packed import Pool, built, gpu, ints  # noqa: E402
-
-from qwen_int4_hip import (  # noqa: E402
-    _lib, paged_append_hip, paged_attention_hip, paged_compact_hip, paged_fork_hip, paged_resize_hip)
 
 
 # ---------------------------------------------------------------------------
@@ -328,3 +339,28 @@ def test_page_operators_over_a_row_as_wide_as_can_be():
     got = paged_compact_hip(*pools, table, users)
     assert got[0][0, last].tolist() == list(range(len(last))) and int((got[0] == -1).sum()) == width - len(last)
     assert got[1].tolist() == [int(p < len(last)) for p in range(pages)]
+
+
+@gpu
+@pytest.mark.parametrize("first, lengths, more", [
+    (1, [2, 0, 1], {}), (70, [200, 9], {"heads": 6}), (3, [600], {"heads": 12, "dim": 128}),
+    (400, [1300, 40], {"heads": 12, "dim": 128, "dtype": F16}), (37, [1 + b % 9 for b in range(90)], {})])
+def test_rows_before_the_first_sequence(first, lengths, more):
+    p = Prompts([first, *lengths], tail=2, **more)
+    want, slack = p.reference()
+    want[:first] = 0
+    bounds = p.cu[1:].clone()
+    torch.full_like(p.q, 7.0)  # (what an answer's memory held)
+    got = packed_attention_hip(p.q, p.k, p.v, bounds)
+    near(got, want, slack)
+    assert not got[:first].any() and not got[p.total:].any()
+    out = torch.full_like(got, 7.0)
+    packed_attention_hip(p.q, p.k, p.v, bounds, out=out)
+    assert torch.equal(out[first:p.total], got[first:p.total])
+    assert bool((out[:first] == 7.0).all()) and bool((out[p.total:] == 7.0).all())
+
+
+if __name__ == "__main__":
+    torch.set_num_threads(1)
+    CHECKS[sys.argv[2]](MoreKernels(sys.argv[1], sys.argv[3]))
+    print("done")
