@@ -1,5 +1,6 @@
 """More of the packed prompt attention and the page operators: pages that a row has lost,
-tables of the greatest width, rows before the first sequence.
+tables of the greatest width, rows before the first sequence, bounds of many sequences
+that fall or lead out, keys that are not finite.
 
 Checks of the kernels' sources on the CPU run in processes of their own, as in
 test_packed_lanes."""
@@ -7,6 +8,7 @@ test_packed_lanes."""
 from __future__ import annotations
 
 import ctypes
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -164,7 +166,64 @@ def _before(kernels):
         assert not out[:min(max(values[0], 0), end)].any() and not out[end:].any(), values
 
 
-CHECKS = {"lost": _lost, "cached": _cached, "ends": _ends, "before": _before}
+def wild_bounds(batch, rows):
+    """Row bounds of `batch` sequences that no program should have."""
+    even = [rows * b // batch for b in range(batch + 1)]
+    gen = torch.Generator().manual_seed(batch)
+    anywhere = torch.randint(-3, rows + 4, (batch + 1,), generator=gen).tolist()
+    return [even[::-1], [rows] * (batch + 1), [0, rows] * (batch // 2) + [0] * (batch % 2 + 1), [WILD[0]] * (batch + 1),
+            [WILD[1]] * (batch + 1), [WILD[b % 2] for b in range(batch + 1)], anywhere, [*anywhere[:-1], rows],
+            [*anywhere[:-1], -1], [*even[:batch // 2], WILD[0], *even[batch // 2 + 1:]], [0] * batch + [rows],
+            [0] * (batch - 1) + [rows, 2]]
+
+
+def _many_bounds(kernels):
+    for batch in (65, 256, 257, 300):
+        rows = 70
+        q, k, v, _ = _packed(kernels, [rows], 2, 1, 64)
+        for values in wild_bounds(batch, rows):
+            end = min(max(values[-1], 0), rows)
+            out = kernels.attention(q, k, v, kernels.ints(values), 0, fill=7.0)
+            assert bool((out[end:] == 7.0).all()), (batch, values[:5])
+            out = kernels.attention(q, k, v, kernels.ints(values), 1, fill=7.0)
+            assert not out[end:].any(), (batch, values[:5])
+
+
+def pieces(bounds, rows, group, kv_heads, tile_rows):
+    """(first row, (token, head) rows, tile, head) of every workgroup, sequences in order, last tiles first."""
+    end = min(max(bounds[-1], 0), rows)
+    found = []
+    for first, last in zip(bounds, bounds[1:]):
+        first = min(max(first, 0), end)
+        count = (min(max(last, first), end) - first) * group
+        found += [(first, count, tile, head) for tile in reversed(range(-(-count // tile_rows))) for head in range(kv_heads)]
+    return found
+
+
+def _finds(kernels):
+    """Every workgroup's place, and that those past the last one have none."""
+    call = kernels.lib.finds
+    call.restype, call.argtypes = None, [ctypes.c_void_p] * 2 + [ctypes.c_int] * 7
+    for batch, rows, group, kv_heads, tile_rows in ((1, 300, 6, 2, 64), (2, 90, 1, 1, 32), (63, 400, 7, 1, 32), (64, 5000, 6, 2, 128),
+                                                    (65, 500, 3, 2, 64), (256, 900, 1, 1, 32), (257, 2000, 2, 1, 64),
+                                                    (300, 600, 6, 2, 128), (1100, 3000, 1, 3, 64)):
+        for values in [[rows * b // batch for b in range(batch + 1)]] + (wild_bounds(batch, rows) if batch > 1 else []):
+            want = pieces(values, rows, group, kv_heads, tile_rows)
+            if len(want) > 3000:
+                continue
+            some = len(want) + 3
+            for longest in ((1, 2) if batch <= 64 else (0,)):
+                said = kernels.empty(some, 5)
+                call(kernels.ints(values).data_ptr(), said.data_ptr(), batch, rows, group, kv_heads, tile_rows, longest, some)
+                got = said.tolist()
+                assert [g[0] for g in got] == [1] * len(want) + [0] * 3, (batch, values[:5])
+                got = [tuple(g[1:]) for g in got[:len(want)]]
+                assert got == want if longest == 0 else sorted(got) == sorted(want), (batch, longest, values[:5])
+                if longest == 1:  # (the most keys first)
+                    assert [g[2] for g in got] == sorted((g[2] for g in got), reverse=True)
+
+
+CHECKS = {"lost": _lost, "cached": _cached, "ends": _ends, "before": _before, "many_bounds": _many_bounds, "finds": _finds}
 
 
 @pytest.fixture(scope="module")
@@ -178,7 +237,7 @@ def more_library(lanes_library):  # noqa: F811
                         f"-I{root}", f"-I{REPO / 'include'}", f"-I{MORE}", "-include", str(MORE / "more.h"), "-x", "c++", "-c",
                         str(source), "-o", str(made)], check=True)
     # (a driver brings its kernels' source with it: their entry points come once)
-    rest = [made for made in root.glob("*.o") if made.name != "qwen2_pages.o"]
+    rest = [made for made in root.glob("*.o") if made.name not in ("qwen2_pages.o", "qwen2_packed_attention.o")]
     subprocess.run([_compiler(), "-shared", *map(str, rest), "-o", str(library)], check=True)
     return library
 
@@ -339,6 +398,48 @@ def test_page_operators_over_a_row_as_wide_as_can_be():
     got = paged_compact_hip(*pools, table, users)
     assert got[0][0, last].tolist() == list(range(len(last))) and int((got[0] == -1).sum()) == width - len(last)
     assert got[1].tolist() == [int(p < len(last)) for p in range(pages)]
+
+
+@gpu
+@pytest.mark.parametrize("batch", [65, 256, 257, 300])
+def test_bounds_of_many_sequences_stay_in_the_buffers(batch):
+    rows = 700
+    p = Prompts([rows], heads=6)
+    for values in wild_bounds(batch, rows):
+        p.cu = ints(values)
+        out = torch.full_like(p.q, 7.0)
+        p.attention(out=out)
+        end = min(max(values[-1], 0), rows)
+        assert bool((out[end:] == 7.0).all()) and not p.attention()[end:].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("lengths, heads", [([20, 30], 4), ([5, 400, 70], 4), ([300], 40), ([130] * 30, 12), ([290] * 30, 12),
+                                            ([25] * 80, 4)])
+def test_keys_that_are_not_finite(dtype, dim, bad, lengths, heads):
+    """Infinite elements of two keys: a score of +inf leaves its row NaN, one of -inf leaves its key
+    out (and a row that sees no other one NaN); whole keys besides, whose scores have no sum."""
+    at, half = lengths[0] if len(lengths) > 1 else 0, torch.finfo(dtype).eps / 2
+    for whole in (False, True):
+        p = Prompts(lengths, heads=heads, kv_heads=2, dim=dim, dtype=dtype)
+        for spot in (at, at + 11):
+            p.k[spot, :, slice(None) if whole else 5] = bad
+        want, begin = torch.zeros(p.q.shape, dtype=torch.float64, device="cuda"), 0
+        slack = want.clone()
+        for n in lengths:
+            x, y, z = (t[begin:begin + n].double().transpose(0, 1).repeat_interleave(heads // t.shape[1], 0) for t in (p.q, p.k, p.v))
+            hidden = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+            w = torch.softmax((x @ y.transpose(1, 2) * dim ** -0.5).masked_fill(hidden, -math.inf), dim=-1)
+            part, size = w @ z, w @ z.abs()
+            # as Prompts.reference() bounds it, by the scores that are finite
+            big = (x.abs() @ y.abs().nan_to_num(posinf=0).transpose(1, 2)).amax() * dim ** -0.5
+            off = 2.0 ** -24 * (2 * (dim + 8) * big + n / 4 + 64) * size + half * (1 + 2 * half) * (size + part.abs())
+            want[begin:begin + n] = part.transpose(0, 1)
+            slack[begin:begin + n] = (off + n * 2.0 ** -36 * z.abs().amax()).transpose(0, 1)
+            begin += n
+        near(p.attention(), want, slack)
 
 
 @gpu
