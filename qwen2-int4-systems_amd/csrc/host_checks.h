@@ -22,7 +22,7 @@
 #include <cstdarg>
 #include <string>
 
-#include "../../include/qwen2_decode.h"
+#include "serving_sizes.h"
 
 namespace {
 

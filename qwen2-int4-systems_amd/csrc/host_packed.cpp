@@ -29,16 +29,19 @@ PyObject* host_packed_attention(PyObject*, PyObject* const* args, Py_ssize_t cou
         if (given && (!apart(*given, q) || !apart(*given, k) || !apart(*given, v) || overlap(*given, cu)))
             refuse(PyExc_ValueError, "out must share no memory with q, k, v and cu_rows");
         const c10::DeviceGuard guard(device);
+        const int64_t batch = cu.size(0) - 1;
+        const int code = q.scalar_type() == at::kHalf ? W4G64_DTYPE_F16 : W4G64_DTYPE_BF16;
+        // (before anything is copied or filled)
+        auto row_step = [&](const at::Tensor& t) { return readable(t) ? step(t, 0) : kv_heads * dim; };
+        check_status(w4g64::packed_attention_sizes(batch, rows, heads, kv_heads, dim, row_step(k), row_step(v), code, (float)scale));
         const at::Tensor qs = usable(q), ks = usable(k), vs = usable(v), bounds = contiguous(cu);
-        const int64_t batch = bounds.size(0) - 1;
-        const bool none = !batch || !rows;  // (the call still checks the sizes)
+        const bool none = !batch || !rows;
         const at::Tensor out = given ? *given : none ? at::zeros(q.sizes(), q.options().requires_grad(false))
                                                      : at::empty(q.sizes(), q.options().requires_grad(false));
         auto rows_of = [](const at::Tensor& t) {
             return qwen2_rows{const_cast<void*>(t.const_data_ptr()), step(t, 0), step(t, 1)};
         };
         const qwen2_rows rq = rows_of(qs), rk = rows_of(ks), rv = rows_of(vs), ro = rows_of(out);
-        const int code = q.scalar_type() == at::kHalf ? W4G64_DTYPE_F16 : W4G64_DTYPE_BF16;
         const hipStream_t stream = current_stream(device);
         released([&] {
             return qwen2_packed_attention(&rq, &rk, &rv, &ro, (const int32_t*)bounds.const_data_ptr(), batch, rows, heads,

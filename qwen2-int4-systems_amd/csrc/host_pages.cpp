@@ -96,6 +96,7 @@ PyObject* host_paged_resize(PyObject*, PyObject* const* args, Py_ssize_t count) 
         const c10::Device device = device_of({{&table, "page_table"}, {&lengths, "lengths"}, {&users, "page_users"},
             {cached ? cached : &users, "cached"}});
         const c10::DeviceGuard guard(device);
+        check_status(w4g64::paged_resize_sizes(batch, width, pages, page_size));  // (before anything is copied)
         const at::Tensor t = rows_contiguous(table), n = contiguous(lengths), u = contiguous(users);
         const at::Tensor held = cached ? contiguous(*cached) : at::Tensor();
         const auto options = users.options().requires_grad(false);
@@ -134,6 +135,7 @@ PyObject* host_paged_fork(PyObject*, PyObject* const* args, Py_ssize_t count) {
         pools.apart_from({{&table, "page_table"}, {&lengths, "lengths"}, {&users, "page_users"}, {&parents, "parents"}});
         const c10::DeviceGuard guard(device);
         pools.bind();
+        check_status(w4g64::paged_fork_sizes(&pools.c, batch, children, width));
         const at::Tensor t = rows_contiguous(table), n = contiguous(lengths), u = contiguous(users), p = contiguous(parents);
         const auto options = users.options().requires_grad(false);
         const at::Tensor new_table = at::empty({children, width}, options), new_lengths = at::empty({children}, options);
@@ -169,6 +171,7 @@ PyObject* host_paged_compact(PyObject*, PyObject* const* args, Py_ssize_t count)
         pools.apart_from({{&table, "page_table"}, {&users, "page_users"}});
         const c10::DeviceGuard guard(device);
         pools.bind();
+        check_status(w4g64::paged_compact_sizes(&pools.c, batch, width));
         const at::Tensor t = rows_contiguous(table), u = contiguous(users);
         const auto options = users.options().requires_grad(false);
         const at::Tensor new_table = at::empty({batch, width}, options);

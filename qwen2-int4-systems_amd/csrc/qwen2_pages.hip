@@ -34,6 +34,7 @@
 #include "qwen2_decode.h"
 #include "qwen2_paged_device.h"
 #include "qwen2_pages.h"
+#include "serving_sizes.h"
 #include "w4g64_internal.h"
 
 namespace w4g64 {
@@ -1005,6 +1006,28 @@ int copy_blocks(const Pool& pool, int64_t items) {
 }
 
 }  // namespace
+
+int paged_resize_sizes(int64_t batch, int64_t table_width, int64_t num_pages, int64_t page_size) {
+    const int status = check_sizes("paged_resize", batch, table_width, num_pages);
+    if (status) return status;
+    if (shift_of(page_size) < 0)
+        return set_error(W4G64_STATUS_INVALID_VALUE, "page_size must be a power of two in [16, 2^20], got %lld", (long long)page_size);
+    return clear_error();
+}
+
+int paged_fork_sizes(const qwen2_page_pool* pool, int64_t batch, int64_t children, int64_t table_width) {
+    Pool view;
+    int status = pool_view("paged_fork", pool, &view);
+    if (!status) status = check_sizes("paged_fork", batch, table_width, pool->num_pages);
+    return status ? status : check_sizes("paged_fork", children, table_width, pool->num_pages);
+}
+
+int paged_compact_sizes(const qwen2_page_pool* pool, int64_t batch, int64_t table_width) {
+    Pool view;
+    const int status = pool_view("paged_compact", pool, &view);
+    return status ? status : check_sizes("paged_compact", batch, table_width, pool->num_pages);
+}
+
 }  // namespace w4g64
 
 using namespace w4g64;
@@ -1028,10 +1051,8 @@ int qwen2_paged_resize_cached(const int32_t* page_table, int64_t table_stride, c
                               const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* missing,
                               int64_t batch, int64_t table_width, int64_t num_pages, int64_t page_size, void* workspace,
                               int64_t workspace_bytes, void* stream) {
-    int status = check_sizes("paged_resize", batch, table_width, num_pages);
+    int status = paged_resize_sizes(batch, table_width, num_pages, page_size);
     if (status) return status;
-    if (shift_of(page_size) < 0)
-        return set_error(W4G64_STATUS_INVALID_VALUE, "page_size must be a power of two in [16, 2^20], got %lld", (long long)page_size);
     if (!aligned4({page_users, new_users}) || (batch && !aligned4({page_table, lengths, new_table, missing})) ||
         ((uintptr_t)cached & 3))
         return set_error(W4G64_STATUS_INVALID_VALUE, "paged_resize pointers (`cached` alone may be null) must be non-null, 4-byte aligned device pointers");
@@ -1074,10 +1095,9 @@ int qwen2_paged_fork(const qwen2_page_pool* pool, const int32_t* page_table, int
                      int32_t* new_users, int32_t* missing, int64_t batch, int64_t children, int64_t table_width,
                      void* workspace, int64_t workspace_bytes, void* stream) {
     ForkArgs a{};
-    int status = pool_view("paged_fork", pool, &a.pool);
-    if (!status) status = check_sizes("paged_fork", batch, table_width, pool->num_pages);
-    if (!status) status = check_sizes("paged_fork", children, table_width, pool->num_pages);
+    int status = paged_fork_sizes(pool, batch, children, table_width);
     if (status) return status;
+    pool_view("paged_fork", pool, &a.pool);
     if (!aligned4({page_users, new_users}) || (batch && !aligned4({page_table, lengths})) ||
         (children && !aligned4({parents, new_table, new_lengths, missing})))
         return set_error(W4G64_STATUS_INVALID_VALUE, "paged_fork pointers must be non-null, 4-byte aligned device pointers");
@@ -1117,9 +1137,9 @@ int qwen2_paged_compact(const qwen2_page_pool* pool, const int32_t* page_table, 
                         const int32_t* page_users, int32_t* new_table, int32_t* new_users, int32_t* moved_to, int64_t batch,
                         int64_t table_width, void* workspace, int64_t workspace_bytes, void* stream) {
     CompactArgs a{};
-    int status = pool_view("paged_compact", pool, &a.pool);
-    if (!status) status = check_sizes("paged_compact", batch, table_width, pool->num_pages);
+    int status = paged_compact_sizes(pool, batch, table_width);
     if (status) return status;
+    pool_view("paged_compact", pool, &a.pool);
     if (!aligned4({page_users, new_users, moved_to}) || (batch && !aligned4({page_table, new_table})))
         return set_error(W4G64_STATUS_INVALID_VALUE, "paged_compact pointers must be non-null, 4-byte aligned device pointers");
     const int64_t pages = pool->num_pages;

@@ -26,7 +26,8 @@ leads outside its table or the pool is not written (``paged_append_hip``) or
 gives NaN (``paged_attention_hip``).
 
 Every function launches on torch's current stream of its tensors' device and
-raises before anything is launched: TypeError for a dtype, ValueError for shapes,
+raises before any of its kernels is launched (what is not laid out as they read it may
+have been copied by then): TypeError for a dtype, ValueError for shapes,
 strides, devices and memory that overlaps, RuntimeError where a gradient would be
 due (they have none), under a dispatch mode, trace or function transform, and
 without the built library.

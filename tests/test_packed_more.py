@@ -309,6 +309,36 @@ def test_cached_is_refused_before_launch():
 # ---------------------------------------------------------------------------
 
 @gpu
+def test_refusals_come_before_any_copy():
+    """Arguments that a good call would copy (unaligned rows, strided indices) are not when it is refused."""
+    def odd(*shape):
+        return torch.zeros(2 * math.prod(shape) + 3, dtype=BF16, device="cuda")[3:3 + math.prod(shape)].view(shape)
+
+    cu, one = torch.zeros(3, 2, dtype=I32, device="cuda")[:, 0], torch.zeros(5, 2, 64, dtype=BF16, device="cuda")
+    far = torch.zeros(2, 1 << 25, dtype=BF16, device="cuda")[:, :128].view(2, 2, 64)
+    table, lengths = torch.zeros(2, 6, dtype=I32, device="cuda")[:, ::2], torch.zeros(2, 2, dtype=I32, device="cuda")[:, 0]
+    users, pool = torch.zeros(6, 2, dtype=I32, device="cuda")[:, 0], torch.zeros(2, 6, 2, 24, 64, dtype=BF16, device="cuda")
+    heads = [odd(5, 4, 48), odd(5, 2, 48), odd(5, 2, 48)]
+    calls = [
+        (ValueError, "head_dim of 64 or 128", packed_attention_hip, (*heads, cu), {}),
+        (ValueError, "head_dim of 64 or 128", packed_attention_hip, (*heads, cu[:1]), {}),
+        (ValueError, "multiple of kv_heads", packed_attention_hip, (odd(5, 3, 64), one, one, cu), {}),
+        (ValueError, "multiple of kv_heads", packed_attention_hip, (odd(5, 3, 64)[:0], one[:0], one[:0], cu), {}),
+        (ValueError, "finite", packed_attention_hip, (odd(5, 4, 64), one, one, cu), {"scale": math.nan}),
+        (ValueError, "2\\^24 elements apart", packed_attention_hip, (odd(2, 4, 64), far, far, cu), {}),
+        (ValueError, "power of two", paged_resize_hip, (table, lengths, users), {"page_size": 24}),
+        (ValueError, "power of two", paged_resize_hip, (table, lengths, users), {"page_size": 24, "cached": lengths}),
+        (ValueError, "power of two", paged_fork_hip, (pool[0], pool[1], table, lengths, users, lengths), {}),
+        (ValueError, "power of two", paged_compact_hip, (pool[0], pool[1], table, users), {}),
+    ]
+    for error, said, call, args, more in calls:
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        with pytest.raises(error, match=said):
+            call(*args, **more)
+        assert torch.cuda.memory_stats()["allocation.all.allocated"] == before, (call, said)
+
+
+@gpu
 @pytest.mark.parametrize("wild", [False, True])
 @pytest.mark.parametrize("sizes", POOLS + [(300, 40, 5000, 16), (9, 5000, 70000, 32), (1100, 7, 3000, 16)])
 def test_resize_gives_no_page_to_cached_positions(sizes, wild):
