@@ -31,11 +31,13 @@ PyObject* host_packed_attention(PyObject*, PyObject* const* args, Py_ssize_t cou
         const c10::DeviceGuard guard(device);
         const int64_t batch = cu.size(0) - 1;
         const int code = q.scalar_type() == at::kHalf ? W4G64_DTYPE_F16 : W4G64_DTYPE_BF16;
-        // (before anything is copied or filled)
-        auto row_step = [&](const at::Tensor& t) { return readable(t) ? step(t, 0) : kv_heads * dim; };
-        check_status(w4g64::packed_attention_sizes(batch, rows, heads, kv_heads, dim, row_step(k), row_step(v), code, (float)scale));
-        const at::Tensor qs = usable(q), ks = usable(k), vs = usable(v), bounds = contiguous(cu);
         const bool none = !batch || !rows;
+        // (before anything is copied or filled; where nothing is, the library's call asks the same)
+        if (none || !readable(q) || !readable(k) || !readable(v) || !cu.is_contiguous()) {
+            auto row_step = [&](const at::Tensor& t) { return readable(t) ? step(t, 0) : kv_heads * dim; };
+            check_status(w4g64::packed_attention_sizes(batch, rows, heads, kv_heads, dim, row_step(k), row_step(v), code, (float)scale));
+        }
+        const at::Tensor qs = usable(q), ks = usable(k), vs = usable(v), bounds = contiguous(cu);
         const at::Tensor out = given ? *given : none ? at::zeros(q.sizes(), q.options().requires_grad(false))
                                                      : at::empty(q.sizes(), q.options().requires_grad(false));
         auto rows_of = [](const at::Tensor& t) {

@@ -628,15 +628,13 @@ Form form_of(int64_t rows, int64_t sequences, int64_t group, int64_t kv_heads, i
     return tiles(64) <= 512 || (tiles(64) <= 800 && usual >= 2048) ? kSplit2 : kLong;
 }
 
-// (every sequence may end inside a tile; the empty ones have none)
-int64_t workgroups_of(Form form, int64_t rows, int64_t sequences, int64_t group, int64_t kv_heads) {
-    return (rows * group / tile_rows(form) + sequences) * kv_heads;
-}
-
-}  // namespace
-
-int packed_attention_sizes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t k_row,
-                           int64_t v_row, int dtype, float scale) {
+// How a call is cut up, if its sizes are any (a status if not).
+struct PackedPlan {
+    Form form;
+    int64_t group, workgroups;
+};
+int packed_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t k_row, int64_t v_row,
+                int dtype, float scale, PackedPlan* plan) {
     if (dtype != W4G64_DTYPE_BF16 && dtype != W4G64_DTYPE_F16)
         return set_error(W4G64_STATUS_INVALID_DTYPE, "packed_attention dtype must be bf16 or fp16, got code %d", dtype);
     if (head_dim != 64 && head_dim != 128)
@@ -652,10 +650,21 @@ int packed_attention_sizes(int64_t batch, int64_t rows, int64_t heads, int64_t k
     if (k_row > (1 << 24) || v_row > (1 << 24) || k_row < 0 || v_row < 0)
         return set_error(W4G64_STATUS_UNSUPPORTED, "k and v rows must be at most 2^24 elements apart");
     const int64_t group = heads / kv_heads, sequences = batch < rows ? batch : rows;
-    const int64_t workgroups = workgroups_of(form_of(rows, sequences, group, kv_heads, head_dim), rows, sequences, group, kv_heads);
+    const Form form = form_of(rows, sequences, group, kv_heads, head_dim);
+    // (every sequence may end inside a tile; the empty ones have none)
+    const int64_t workgroups = (rows * group / tile_rows(form) + sequences) * kv_heads;
     if (rows * heads > 0x7FF00000 || workgroups > 0xFFFFFF)
         return set_error(W4G64_STATUS_UNSUPPORTED, "packed_attention call is too large: %lld workgroups", (long long)workgroups);
+    *plan = PackedPlan{form, group, workgroups};
     return clear_error();
+}
+
+}  // namespace
+
+int packed_attention_sizes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t k_row,
+                           int64_t v_row, int dtype, float scale) {
+    PackedPlan plan;
+    return packed_plan(batch, rows, heads, kv_heads, head_dim, k_row, v_row, dtype, scale, &plan);
 }
 
 }  // namespace w4g64
@@ -665,18 +674,16 @@ using namespace w4g64;
 extern "C" int qwen2_packed_attention(const qwen2_rows* q, const qwen2_rows* k, const qwen2_rows* v, const qwen2_rows* out,
                                       const int32_t* cu_rows, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
                                       int64_t head_dim, int dtype, float scale, int zero_rest, void* stream) {
-    const bool none = rows == 0 || batch == 0;
-    const int status = packed_attention_sizes(batch, rows, heads, kv_heads, head_dim, k ? k->row : 0, v ? v->row : 0, dtype, scale);
-    if (status || none) return status;
+    PackedPlan plan;
+    const int status = packed_plan(batch, rows, heads, kv_heads, head_dim, k ? k->row : 0, v ? v->row : 0, dtype, scale, &plan);
+    if (status || rows == 0 || batch == 0) return status;
     for (const qwen2_rows* r : {q, k, v, out})
         if (!r || !r->data || ((uintptr_t)r->data & 15) || r->row % 8 || r->head % 8)
             return set_error(W4G64_STATUS_INVALID_VALUE,
                              "q, k, v and out must be non-null, 16-byte aligned, with strides that are multiples of 8 elements");
     if (!cu_rows || ((uintptr_t)cu_rows & 3))
         return set_error(W4G64_STATUS_INVALID_VALUE, "cu_rows must be a non-null, 4-byte aligned device pointer");
-    const int64_t group = heads / kv_heads, sequences = batch < rows ? batch : rows;
-    const Form form = form_of(rows, sequences, group, kv_heads, head_dim);
-    const int64_t workgroups = workgroups_of(form, rows, sequences, group, kv_heads);
+    const auto [form, group, workgroups] = plan;
     PackedArgs a{};
     a.q = (const uint16_t*)q->data, a.q_row = q->row, a.q_head = q->head;
     a.k = (const uint16_t*)k->data, a.k_row = k->row, a.k_head = k->head;
