@@ -32,10 +32,12 @@
 // 32 products (535 ns) and, a lane, 32 exponentials (164 ns) with some 96 other vector
 // instructions (236 ns); alone a wave takes 1.2 us for such a tile, two waves 2.0.  12/2
 // heads of 128, bf16: one prompt
-// of 16384 tokens 779 to 817 us (two cards; 1060 and 1010 TFLOP/s of the 1206 that a
-// product of 8192^3 reaches on the first; matrix unit busy 53 % of the cycles, vector unit
-// 43 %, no LDS bank conflicts); three of 1003, 4001 and 6999, 32/8 heads, fp16, 567 (950).
-// Eight of 400 to 1600: 46 us (620): the longest prompt's last tiles.  Short ones: loads
+// of 16384 tokens 759 to 830 us (by the card; 1090 to 1000 TFLOP/s, a product of 8192^3
+// reaching 1206; on the slowest one the matrix unit is busy for 55 % of the shader engines'
+// cycles, the vector unit for 44 %, no LDS bank conflicts); three of 1003, 4001 and 6999,
+// 32/8 heads, fp16, 559 to 601 (967 to 900).  Heads of 64, half the products for the same
+// exponentials: 16384 tokens, 16/16 heads, 645 (852).  Eight of 400 to 1600: 46 us (620): the
+// longest prompt's last tiles.  Short ones: loads
 // that depend on each other (bounds, then rows, then the output) and the launch: 37
 // tokens 5.1, 512 10.6.
 // What else was measured, us for 16384 tokens against 780: products of the next tile
@@ -583,7 +585,7 @@ __device__ __forceinline__ void attend_piece(const PackedArgs& a) {
 
 // (waves per SIMD: two with 256 registers each, where LDS holds as much; short prompts of
 // 64 dimensions four, for which nine registers are put away during the counting passes
-// alone: 200 of 30 15.7 -> 14.3 us, 32 of 200 18.0 -> 16.7, 96 of 1 to 119 15.7 -> 15.9)
+// alone: 200 of 30 15.1 -> 13.4 us, 32 of 200 17.6 -> 16.2, 96 of 1 to 119 14.0 -> 14.3)
 template <class E, int D, int kWaves, int kSplit, int kBlocks>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 4 && kSplit == 4 && D == 128 ? 1 : kWaves == 2 && D == 64 ? 4 : 2)
 void packed_attention_kernel(PackedArgs a) {

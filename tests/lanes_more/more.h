@@ -44,7 +44,6 @@ float pair_sum(uint32_t w, float c) {
 #define __builtin_amdgcn_fdot2(a, b, c, clamp) lanes::pair_sum<false>(__builtin_bit_cast(uint32_t, a), c)
 #define __builtin_amdgcn_mbcnt_lo(mask, base) ((base) + __builtin_popcount((mask) & (lanes::lane() < 32 ? (1u << lanes::lane()) - 1 : ~0u)))
 #define __builtin_amdgcn_mbcnt_hi(mask, base) ((base) + __builtin_popcount((mask) & (lanes::lane() < 32 ? 0u : (1u << (lanes::lane() - 32)) - 1)))
-#define __hip_atomic_load(p, order, scope) (*(p))
 
 // (one lane runs at a time)
 inline int atomicAdd(int* p, int v) {
