@@ -31,15 +31,13 @@
 // time of two waves and overlap only in part.  64 keys by 32 rows of 128 dimensions are
 // 32 products (535 ns) and, a lane, 32 exponentials (164 ns) with some 96 other vector
 // instructions (236 ns); alone a wave takes 1.2 us for such a tile, two waves 2.0.  12/2
-// heads of 128, bf16: one prompt
-// of 16384 tokens 759 to 830 us (by the card; 1090 to 1000 TFLOP/s, a product of 8192^3
-// reaching 1206; on the slowest one the matrix unit is busy for 55 % of the shader engines'
-// cycles, the vector unit for 44 %, no LDS bank conflicts); three of 1003, 4001 and 6999,
-// 32/8 heads, fp16, 559 to 601 (967 to 900).  Heads of 64, half the products for the same
-// exponentials: 16384 tokens, 16/16 heads, 645 (852).  Eight of 400 to 1600: 46 us (620): the
-// longest prompt's last tiles.  Short ones: loads
-// that depend on each other (bounds, then rows, then the output) and the launch: 37
-// tokens 5.1, 512 10.6.
+// heads of 128, bf16: one prompt of 16384 tokens 759 to 830 us (by the card; 1090 to 1000
+// TFLOP/s, a product of 8192^3 reaching 1206; on the slowest one the matrix unit is busy for
+// 55 % of the shader engines' cycles, the vector unit for 44 %, no LDS bank conflicts); three
+// of 1003, 4001 and 6999, 32/8 heads, fp16, 559 to 601 (967 to 900).  Heads of 64, half the
+// products for the same exponentials: 16384 tokens, 16/16 heads, 645 (852).  Eight of 400 to
+// 1600: 46 us (620): the longest prompt's last tiles.  Short ones: loads that depend on each
+// other (bounds, then rows, then the output) and the launch: 37 tokens 5.1 to 5.4, 512 10.6.
 // What else was measured, us for 16384 tokens against 780: products of the next tile
 // between the exponentials of this one by hand 970 to 1300 (registers); a ring of 32-key
 // tiles 975 to 1050; one wave a SIMD with more rows 970 to 1240; two groups of waves in
