@@ -23,7 +23,7 @@
 // kernel).  Copies of pages: memory; 977 pages of 8 layers moved, 256 MB read and
 // written, take 51.7 of a compaction's 53 us (4.95 TB/s; a large copy 5.18).  A resize of
 // 511 rows of up to 2048 pages, a ninth of them given up and a ninth cut back: 3.2 + 4.6 +
-// 10.7 us, 5.5 of it atomics on the users of some 90000 pages.
+// 10.5 us, 5.5 of it atomics on the users of some 90000 pages.
 //
 // Indices from device memory (entries, lengths, parents) are bounded before they are
 // used; what names no page is left out.
